@@ -7,6 +7,10 @@ and one code-generation guard:
   -mllvm -disable-promote-alloca-to-lds  the AMDGPU pass that moves small private arrays into LDS
       (256 lanes x the array) fires or not depending on register pressure; in kd_bin_count it
       turned the 8-float cull array into 8 KB of LDS traffic per workgroup (30 -> 51 us)
+and one for the results:
+  -target-feature -packed-fp32-ops  no packed fp32 instructions (v_pk_add / mul / fma_f32), which
+      -O3 forms from ordinary scalar code and some forms of which have given wrong results now and
+      then on these cards (the host pass does not know the feature and says so)
 """
 import concurrent.futures
 import os
@@ -31,6 +35,7 @@ ARCH = os.environ.get('KAOLIN_AMD_ARCH', 'gfx950')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 FLAGS = ['-O3', '-std=c++17', '-fPIC', '-ffp-contract=off', f'--offload-arch={ARCH}',
          '-mllvm', '-disable-promote-alloca-to-lds',
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
          '-Wall', '-Wno-unused-function', '-Wno-unused-result']
 
 # per-source flags, each measured on one box against the default scheduler (tools/ab_variant.sh +
