@@ -656,6 +656,100 @@ int kd_deftet_sparse_render_backward_f64(int batch, int64_t num_pixels, int64_t 
                                          const double *fvi, const double *feat, float eps,
                                          double *grad_fvi, double *grad_feat, void *stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * surface_embedding: a table of embeddings with a row per face or vertex, looked up at n indices
+ * (any order; int64): out (n, D) = scale * embeddings[index], 0 where index lies outside
+ * [0, rows).  batch > 1: embeddings (batch, rows, D) and the indices in batch equal blocks, each
+ * looked up in its own table.  The backward writes every row of grad_embeddings (batch, rows, D):
+ * scale * the sum of its indices' rows of grad_out (n, D), added in a fixed order (no atomics).
+ * Limits: n < 2^31, batch * rows < 2^31, D <= 2^20.  The pointers are f32, f64, f16 or bf16 data
+ * by the suffix; element_size is 4, 8 or 2.
+ * ------------------------------------------------------------------------------------------- */
+size_t kd_surface_embedding_workspace_size(int64_t num_indices, int64_t batch, int64_t rows,
+                                           int channels, int element_size);
+int kd_surface_embedding_forward_f32(int64_t num_indices, int64_t batch, int64_t rows, int channels,
+                                      const int64_t *index, const void *embeddings, double scale,
+                                      void *out, void *stream);
+int kd_surface_embedding_backward_f32(int64_t num_indices, int64_t batch, int64_t rows, int channels,
+                                       const int64_t *index, const void *grad_out, double scale,
+                                       void *grad_embeddings, void *workspace,
+                                       size_t workspace_bytes, void *stream);
+int kd_surface_embedding_forward_f64(int64_t num_indices, int64_t batch, int64_t rows, int channels,
+                                      const int64_t *index, const void *embeddings, double scale,
+                                      void *out, void *stream);
+int kd_surface_embedding_backward_f64(int64_t num_indices, int64_t batch, int64_t rows, int channels,
+                                       const int64_t *index, const void *grad_out, double scale,
+                                       void *grad_embeddings, void *workspace,
+                                       size_t workspace_bytes, void *stream);
+int kd_surface_embedding_forward_f16(int64_t num_indices, int64_t batch, int64_t rows, int channels,
+                                      const int64_t *index, const void *embeddings, double scale,
+                                      void *out, void *stream);
+int kd_surface_embedding_backward_f16(int64_t num_indices, int64_t batch, int64_t rows, int channels,
+                                       const int64_t *index, const void *grad_out, double scale,
+                                       void *grad_embeddings, void *workspace,
+                                       size_t workspace_bytes, void *stream);
+int kd_surface_embedding_forward_bf16(int64_t num_indices, int64_t batch, int64_t rows, int channels,
+                                      const int64_t *index, const void *embeddings, double scale,
+                                      void *out, void *stream);
+int kd_surface_embedding_backward_bf16(int64_t num_indices, int64_t batch, int64_t rows, int channels,
+                                       const int64_t *index, const void *grad_out, double scale,
+                                       void *grad_embeddings, void *workspace,
+                                       size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * surface_cross_entropy: softmax cross entropy of features (n, D) against embeddings (rows, D),
+ * logits = scale * features . embeddings, at labels (n) int64; a pixel whose label lies outside
+ * [0, rows) takes no part.  reduction: 0 a loss per pixel (n), 1 the mean over the pixels that
+ * take part, 2 the sum.  loss is fp32 whatever the data's type (f32, f16, bf16 by the suffix).
+ * need_features / need_embeddings say which gradients a backward call may ask for; `state` (at
+ * least kd_surface_xent_state_size bytes) carries what it needs and is written by the forward and
+ * only read by the backward, `scratch` is free after each call.  The backward takes the loss's
+ * gradient (a scalar, or (n) for reduction 0; fp32, device) and writes grad_features (n, D) and
+ * grad_embeddings (rows, D); NULL skips one.  Limits: 1 <= D <= 256, 1 <= rows < 2^31 - 256,
+ * n < 2^31 - 256, |scale| < 1e30.
+ * ------------------------------------------------------------------------------------------- */
+size_t kd_surface_xent_state_size(int64_t num_pixels, int64_t rows, int channels,
+                                  int element_size, int need_features, int need_embeddings);
+size_t kd_surface_xent_scratch_size(int64_t num_pixels, int64_t rows, int channels,
+                                    int element_size, int need_features, int need_embeddings,
+                                    int backward);
+int kd_surface_xent_forward_f32(int64_t num_pixels, int64_t rows, int channels,
+                                 const void *features, const void *embeddings,
+                                 const int64_t *labels, double scale, int reduction,
+                                 int need_features, int need_embeddings, float *loss, void *state,
+                                 size_t state_bytes, void *scratch, size_t scratch_bytes,
+                                 void *stream);
+int kd_surface_xent_backward_f32(int64_t num_pixels, int64_t rows, int channels,
+                                  const int64_t *labels, double scale, int reduction,
+                                  int need_features, int need_embeddings, const float *grad_loss,
+                                  void *grad_features, void *grad_embeddings, void *state,
+                                  size_t state_bytes, void *scratch, size_t scratch_bytes,
+                                  void *stream);
+int kd_surface_xent_forward_f16(int64_t num_pixels, int64_t rows, int channels,
+                                 const void *features, const void *embeddings,
+                                 const int64_t *labels, double scale, int reduction,
+                                 int need_features, int need_embeddings, float *loss, void *state,
+                                 size_t state_bytes, void *scratch, size_t scratch_bytes,
+                                 void *stream);
+int kd_surface_xent_backward_f16(int64_t num_pixels, int64_t rows, int channels,
+                                  const int64_t *labels, double scale, int reduction,
+                                  int need_features, int need_embeddings, const float *grad_loss,
+                                  void *grad_features, void *grad_embeddings, void *state,
+                                  size_t state_bytes, void *scratch, size_t scratch_bytes,
+                                  void *stream);
+int kd_surface_xent_forward_bf16(int64_t num_pixels, int64_t rows, int channels,
+                                 const void *features, const void *embeddings,
+                                 const int64_t *labels, double scale, int reduction,
+                                 int need_features, int need_embeddings, float *loss, void *state,
+                                 size_t state_bytes, void *scratch, size_t scratch_bytes,
+                                 void *stream);
+int kd_surface_xent_backward_bf16(int64_t num_pixels, int64_t rows, int channels,
+                                  const int64_t *labels, double scale, int reduction,
+                                  int need_features, int need_embeddings, const float *grad_loss,
+                                  void *grad_features, void *grad_embeddings, void *state,
+                                  size_t state_bytes, void *scratch, size_t scratch_bytes,
+                                  void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,6 +15,7 @@ Extra entry points (used by kaolin_amd.render.mesh's autograd functions, not in 
 ``rasterize_forward_fused``, ``rasterize_backward_autograd``, ``dibr_soft_mask_forward_fused``,
 ``dibr_soft_mask_backward_binned``.
 """
+import math
 import types
 
 import torch
@@ -744,6 +745,161 @@ def texture_mapping_backward(grad_out, coords, tex, mode, need_coords=True, need
 
 
 # -------------------------------------------------------------------------------------------
+# a learned table of embeddings, one row per face or vertex: lookup and softmax cross entropy
+# -------------------------------------------------------------------------------------------
+_SFX16 = {torch.float32: 'f32', torch.float64: 'f64', torch.float16: 'f16',
+          torch.bfloat16: 'bf16'}
+
+
+def _sfx16(t, fname, double=True):
+    sfx = _SFX16.get(t.dtype)
+    if sfx is None or (sfx == 'f64' and not double):
+        raise RuntimeError(f'"{fname}" not implemented for \'{t.dtype}\'')
+    return sfx
+
+
+def _check_index(fname, name, t):
+    if t.dtype != torch.int64:
+        raise RuntimeError(f'{fname}: expected {name} to have dtype torch.int64, got {t.dtype}')
+
+
+def _number(fname, name, x):
+    if isinstance(x, torch.Tensor) or isinstance(x, bool):
+        raise RuntimeError(f'{fname}: {name} must be a number, got {type(x).__name__}')
+    x = float(x)
+    if not math.isfinite(x) or abs(x) >= 1e30:
+        raise RuntimeError(f'{fname}: {name} must be finite and below 1e30, got {x}')
+    return x
+
+
+def _bytes(nb, dev):
+    return torch.empty((max(int(nb), 1),), dtype=torch.uint8, device=dev)
+
+
+def _embedding_args(fn, index, shape, scale):
+    """(tokens, batch, rows, channels, scale) of a lookup in a table of `shape`."""
+    _check_index(fn, 'index', index)
+    if len(shape) not in (2, 3):
+        raise RuntimeError(f'{fn}: embeddings must be (rows, channels) or (batch, rows, channels), '
+                           f'got {list(shape)}')
+    batch = 1
+    if len(shape) == 3:
+        batch = shape[0]
+        if index.dim() < 1 or index.shape[0] != batch:
+            raise RuntimeError(f'{fn}: a table per batch entry needs index of shape '
+                               f'({batch}, ...), got {list(index.shape)}')
+    rows, D = shape[-2:]
+    if index.numel() >= 2 ** 31 or batch * rows >= 2 ** 31 or D > 2 ** 20:
+        raise RuntimeError(f'{fn}: needs fewer than 2^31 indices, 2^31 embeddings and at most '
+                           f'2^20 channels')
+    return index.numel(), max(batch, 1), rows, D, _number(fn, 'scale', scale)
+
+
+def surface_embedding_forward(index, embeddings, scale):
+    """index (...) int64, embeddings (N, D) or (B, N, D) with index (B, ...) -> (..., D):
+    scale * embeddings[index], 0 where the index lies outside [0, N)."""
+    fn = 'surface_embedding'
+    dev = _check_same_gpu(fn, index=index, embeddings=embeddings)
+    sfx = _sfx16(embeddings, fn)
+    n, B, N, D, scale = _embedding_args(fn, index, embeddings.shape, scale)
+    index, embeddings = index.contiguous(), embeddings.contiguous()
+    out = torch.empty((*index.shape, D), device=dev, dtype=embeddings.dtype)
+    if out.numel():
+        with torch.cuda.device(dev):
+            _lib.call(f'kd_surface_embedding_forward_{sfx}', n, B, N, D, _ptr(index),
+                      _ptr(embeddings), scale, _ptr(out), _stream(dev))
+    return out
+
+
+def surface_embedding_backward(grad_out, index, shape, scale):
+    """The gradient of a table of `shape`: scale * the sum of the rows of grad_out (..., D) that
+    each table row was looked up for, added in the indices' order."""
+    fn = 'surface_embedding_backward'
+    dev = _check_same_gpu(fn, grad_out=grad_out, index=index)
+    sfx = _sfx16(grad_out, fn)
+    n, B, N, D, scale = _embedding_args(fn, index, shape, scale)
+    _check_size(fn, 'grad_out', grad_out, (*index.shape, D))
+    index, grad_out = index.contiguous(), grad_out.contiguous()
+    grad = torch.empty(tuple(shape), device=dev, dtype=grad_out.dtype)
+    if grad.numel():
+        nb = int(_lib.load().kd_surface_embedding_workspace_size(n, B, N, D,
+                                                                 grad_out.element_size()))
+        ws = _bytes(nb, dev)
+        with torch.cuda.device(dev):
+            _lib.call(f'kd_surface_embedding_backward_{sfx}', n, B, N, D, _ptr(index),
+                      _ptr(grad_out), scale, _ptr(grad), _ptr(ws), nb, _stream(dev))
+    return grad
+
+
+_REDUCTIONS = {'none': 0, 'mean': 1, 'sum': 2}
+XENT_MAX_CHANNELS = 256
+
+
+def surface_xent_forward(features, embeddings, labels, scale, reduction, need_features=False,
+                         need_embeddings=False):
+    """features (..., D), embeddings (N, D), labels (...) int64 -> (loss, state): the softmax
+    cross entropy of scale * features @ embeddings.T at the labels in [0, N), in 32 bits, and what
+    surface_xent_backward needs for the gradients asked for."""
+    fn = 'surface_cross_entropy'
+    dev = _check_same_gpu(fn, features=features, embeddings=embeddings, labels=labels)
+    sfx = _sfx16(features, fn, double=False)
+    _check_dtype(fn, features, embeddings=embeddings)
+    _check_index(fn, 'labels', labels)
+    if embeddings.dim() != 2:
+        raise RuntimeError(f'{fn}: embeddings must be (rows, channels), got '
+                           f'{list(embeddings.shape)}')
+    N, D = embeddings.shape
+    _check_size(fn, 'features', features, (*labels.shape, D))
+    if reduction not in _REDUCTIONS:
+        raise RuntimeError(f'{fn}: reduction must be "none", "mean" or "sum", got {reduction!r}')
+    n = labels.numel()
+    if not 1 <= D <= XENT_MAX_CHANNELS:
+        raise RuntimeError(f'{fn}: needs 1 to {XENT_MAX_CHANNELS} channels, got {D}')
+    if N < 1 or N >= 2 ** 31 - 256 or n >= 2 ** 31 - 256:
+        raise RuntimeError(f'{fn}: needs at least one embedding, and fewer than 2^31 - 256 '
+                           f'embeddings and pixels, got {N} and {n}')
+    scale = _number(fn, 'scale', scale)
+    features, embeddings, labels = (features.contiguous(), embeddings.contiguous(),
+                                    labels.contiguous())
+    loss = torch.empty(labels.shape if reduction == 'none' else (), device=dev,
+                       dtype=torch.float32)
+    lib, esize = _lib.load(), features.element_size()
+    nx, ne = 1 if need_features else 0, 1 if need_embeddings else 0
+    ns = int(lib.kd_surface_xent_state_size(n, N, D, esize, nx, ne))
+    nw = int(lib.kd_surface_xent_scratch_size(n, N, D, esize, nx, ne, 0))
+    state, scratch = _bytes(ns, dev), _bytes(nw, dev)
+    with torch.cuda.device(dev):
+        _lib.call(f'kd_surface_xent_forward_{sfx}', n, N, D, _ptr(features), _ptr(embeddings),
+                  _ptr(labels), scale, _REDUCTIONS[reduction], nx, ne, _ptr(loss), _ptr(state), ns,
+                  _ptr(scratch), nw, _stream(dev))
+    return loss, state
+
+
+def surface_xent_backward(grad_loss, labels, shape, dtype, scale, reduction, state,
+                          need_features=True, need_embeddings=True, features=True,
+                          embeddings=True):
+    """(grad_features or None, grad_embeddings or None) from the forward's state; need_* as in
+    the forward call, `features` / `embeddings` the gradients wanted now."""
+    dev = labels.device
+    N, D = shape
+    n = labels.numel()
+    labels = labels.contiguous()
+    g = grad_loss.to(torch.float32).contiguous()
+    gx = torch.empty((*labels.shape, D), device=dev, dtype=dtype) if features else None
+    ge = torch.empty((N, D), device=dev, dtype=dtype) if embeddings else None
+    nx, ne = 1 if need_features else 0, 1 if need_embeddings else 0
+    esize = 4 if dtype == torch.float32 else 2
+    nw = int(_lib.load().kd_surface_xent_scratch_size(n, N, D, esize, nx, 1 if embeddings else 0,
+                                                      1))
+    scratch = _bytes(nw, dev)
+    with torch.cuda.device(dev):
+        _lib.call(f'kd_surface_xent_backward_{_SFX16[dtype]}', n, N, D, _ptr(labels), float(scale),
+                  _REDUCTIONS[reduction], nx, ne, _ptr(g), _ptr(gx), _ptr(ge), _ptr(state),
+                  state.numel(), _ptr(scratch), nw, _stream(dev))
+    return gx, ge
+
+
+# -------------------------------------------------------------------------------------------
 # nvdiffrast_fwd compatibility (rasterization.py:145-241), SURVEY §8 f4
 # -------------------------------------------------------------------------------------------
 def rast_interpolate(rast, face_features):
@@ -911,6 +1067,10 @@ render = types.SimpleNamespace(mesh=types.SimpleNamespace(
     deftet_sparse_render_backward=deftet_sparse_render_backward,
     deftet_sparse_render_forward_cuda=deftet_sparse_render_forward_cuda,
     deftet_sparse_render_backward_cuda=deftet_sparse_render_backward_cuda,
+    surface_embedding_forward=surface_embedding_forward,
+    surface_embedding_backward=surface_embedding_backward,
 ))
 metrics = types.SimpleNamespace(mask_iou_forward=mask_iou_forward,
-                                mask_iou_backward=mask_iou_backward)
+                                mask_iou_backward=mask_iou_backward,
+                                surface_xent_forward=surface_xent_forward,
+                                surface_xent_backward=surface_xent_backward)

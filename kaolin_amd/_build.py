@@ -29,7 +29,8 @@ OBJDIR_DIAG = os.path.join(PKG, 'build_diag')
 
 SOURCES = ['kd_capi.cpp', 'kd_binning.hip', 'kd_raster.hip', 'kd_softmask.hip', 'kd_softpair.hip',
            'kd_prepare.hip', 'kd_dibr.hip', 'kd_metrics.hip', 'kd_texture.hip',
-           'kd_rastcompat.hip', 'kd_deftet.hip']
+           'kd_rastcompat.hip', 'kd_deftet.hip', 'kd_embedding.hip',
+           'kd_xent_f32.hip', 'kd_xent_f16.hip', 'kd_xent_bf16.hip']
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith('.hpp'))  # every source depends on all
 ARCH = os.environ.get('KAOLIN_AMD_ARCH', 'gfx950')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')

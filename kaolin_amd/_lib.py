@@ -97,6 +97,21 @@ _SIGS = {
                                           c_int, c_p, c_p, c_p, c_p, c_size, c_p],
 }
 
+# the surface-embedding entry points: one per element type, with that type as suffix
+_TYPED_SIGS = {
+    'kd_surface_embedding_forward': (('f32', 'f64', 'f16', 'bf16'),
+                                     [c_i64, c_i64, c_i64, c_int, c_p, c_p, c_double, c_p, c_p]),
+    'kd_surface_embedding_backward': (('f32', 'f64', 'f16', 'bf16'),
+                                      [c_i64, c_i64, c_i64, c_int, c_p, c_p, c_double, c_p, c_p,
+                                       c_size, c_p]),
+    'kd_surface_xent_forward': (('f32', 'f16', 'bf16'),
+                                [c_i64, c_i64, c_int, c_p, c_p, c_p, c_double, c_int, c_int, c_int,
+                                 c_p, c_p, c_size, c_p, c_size, c_p]),
+    'kd_surface_xent_backward': (('f32', 'f16', 'bf16'),
+                                 [c_i64, c_i64, c_int, c_p, c_double, c_int, c_int, c_int, c_p,
+                                  c_p, c_p, c_p, c_size, c_p, c_size, c_p]),
+}
+
 
 def load():
     """Load (once) and return the ctypes library; raises if it is not built."""
@@ -164,6 +179,18 @@ def load():
                     fn = getattr(lib, f'{base}_{sfx}')
                     fn.argtypes = sig
                     fn.restype = c_int
+            for base, (types, sig) in _TYPED_SIGS.items():
+                for sfx in types:
+                    fn = getattr(lib, f'{base}_{sfx}')
+                    fn.argtypes = sig
+                    fn.restype = c_int
+            lib.kd_surface_embedding_workspace_size.argtypes = [c_i64, c_i64, c_i64, c_int, c_int]
+            lib.kd_surface_embedding_workspace_size.restype = c_size
+            lib.kd_surface_xent_state_size.argtypes = [c_i64, c_i64, c_int, c_int, c_int, c_int]
+            lib.kd_surface_xent_state_size.restype = c_size
+            lib.kd_surface_xent_scratch_size.argtypes = [c_i64, c_i64, c_int, c_int, c_int, c_int,
+                                                         c_int]
+            lib.kd_surface_xent_scratch_size.restype = c_size
             _lib = lib
     return _lib
 

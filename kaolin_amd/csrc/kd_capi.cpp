@@ -115,7 +115,8 @@ const char *kNames[K_NUM_KERNELS] = {
     "kd_prepare_fwd", "kd_prepare_bwd", "kd_tile_order", "kd_iou_partial", "kd_iou_bwd",
     "kd_tex_fwd", "kd_tex_bwd", "kd_rast_interp", "kd_dt_bin",
     "kd_dt_fwd", "kd_dibr_bwd", "kd_dibr_fwd", "kd_soft_ovf_fwd", "kd_soft_ovf_bwd",
-    "kd_dt_bwd"};
+    "kd_dt_bwd", "kd_embed_gather", "kd_embed_bwd", "kd_xent_fwd",
+    "kd_xent_bwd"};
 }  // namespace
 
 ProfScope::ProfScope(int id_, hipStream_t s) : id(id_), stream(s), on(g_prof.load()) {

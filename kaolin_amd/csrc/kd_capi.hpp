@@ -42,6 +42,10 @@ enum KernelId {
   K_SOFT_OVF_FWD,
   K_SOFT_OVF_BWD,
   K_DT_BWD,
+  K_EMBED_FWD,
+  K_EMBED_BWD,
+  K_XENT_FWD,
+  K_XENT_BWD,
   K_NUM_KERNELS
 };
 

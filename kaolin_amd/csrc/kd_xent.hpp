@@ -1,0 +1,929 @@
+// kd_xent.hpp -- surface_cross_entropy: softmax cross entropy of pixel features against every row
+// of a table of embeddings, without keeping the logits, and both gradients.
+//
+//   z_iv = scale x_i . e_v,   loss_i = log sum_v exp z_iv - z_iy,   y = labels[i]
+// over the rows i whose label names a row of the table (0 <= y < V); the others take no part.
+// Everything is written with the label's own term left out of the sums:
+//   L'_i = log sum_{v != y} exp z_iv,   w_i = 1 - p_iy = sigmoid(L'_i - z_iy)
+//   loss_i = softplus(L'_i - z_iy)
+//   dX_i = g_i scale w_i (m_i - e_y),   m_i = sum_{v != y} exp(z_iv - L'_i) e_v
+//   dE_v = scale sum_i g_i q_iv x_i,    q_iv = p_iv (v != y),  -w_i (v = y)
+// so that nothing cancels where p_iy is next to 1 (a trained network), in the loss or in p - 1.
+//
+// Forward: rows with a label are listed (in order) and packed with the table into the matrix
+// instructions' operand layout; kd_xent_rows holds a block of rows in registers and walks the
+// table once: 32 x 32 logits at a time, a running maximum and sum (32 bits), and, if dX is wanted,
+// the weighted sum of the table's rows (32 bits) -- the logits never leave registers.  When there
+// are few rows the table is split over workgroups and kd_xent_combine joins the parts.
+// Backward: kd_xent_table holds a block of table rows and walks the pixels; the logits are computed
+// again from the packed operands with the saved log sums, split over the pixels when the table is
+// small and joined in a fixed order.  No atomics on values: results do not depend on timing.
+//
+// 16-bit data multiply exactly into 32-bit sums.  The probabilities enter their product with the
+// table (or the features) rounded to the data's type, at most 2^-8 (bf16) or 2^-11 (fp16, scaled so that
+// small ones stay normal) of each term, like the operands themselves; the sums L' use the
+// unrounded values.  32-bit data are split by truncation into three bf16 parts (8 + 8 + 8 bits, the
+// whole significand) and multiplied as the six products above 2^-24: the fp32 matrix instructions
+// run at 1/16 of the bf16 rate, six bf16 products at 1/6.
+#pragma once
+
+#include "kd_capi.hpp"
+#include "kd_common.hpp"
+#include "kd_float16.hpp"
+
+#include <algorithm>
+
+namespace kd {
+namespace xent {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef half_t half8 __attribute__((ext_vector_type(8)));
+typedef bfloat_t bfloat8 __attribute__((ext_vector_type(8)));
+
+// How data of type T are multiplied: the operand type H, its 8-vector, the number of parts
+// (planes), and the power of two by which probabilities are scaled in the products.
+template <typename T>
+struct Form;
+template <>
+struct Form<bfloat_t> {
+  using H = bfloat_t;
+  using H8 = bfloat8;
+  static constexpr int np = 1;
+  static constexpr float shift = 0.f, slack = 8.f, shift_table = 0.f;
+};
+template <>
+struct Form<half_t> {
+  using H = half_t;
+  using H8 = half8;
+  static constexpr int np = 1;
+  // exp2(z - max + shift) <= 2^(shift + slack) stays below 65504
+  static constexpr float shift = 10.f, slack = 5.f, shift_table = 14.f;
+};
+template <>
+struct Form<float> {
+  using H = bfloat_t;
+  using H8 = bfloat8;
+  static constexpr int np = 3;
+  static constexpr float shift = 0.f, slack = 8.f, shift_table = 0.f;
+};
+
+__device__ __forceinline__ f32x16 mfma(half8 a, half8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma(bfloat8 a, bfloat8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// x as three bf16 by truncation (exact: 8 + 8 + 8 significand bits)
+__device__ __forceinline__ void split3(float x, uint16_t &a, uint16_t &b, uint16_t &c) {
+  const uint32_t u = __float_as_uint(x);
+  a = (uint16_t)(u >> 16);
+  const float r = x - __uint_as_float(u & 0xffff0000u);
+  const uint32_t v = __float_as_uint(r);
+  b = (uint16_t)(v >> 16);
+  c = (uint16_t)(__float_as_uint(r - __uint_as_float(v & 0xffff0000u)) >> 16);
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kRowPad = 256;  // packed rows are padded with zeros to a multiple of this
+constexpr int kMapChunk = 2048;
+
+// The work of one call.  Packed operands of a matrix M (rows padded to kRowPad, channels to DP),
+// in tiles of 32 rows, each tile NP planes, 16 bytes a lane:
+//   straight   [tile][plane][k step of 16 channels][lane][8] = M[lane % 32][16 step + 8 (lane / 32) + j]
+//   transposed [tile][plane][row half s][32 channels t][lane][8] =
+//       M[16 s + 8 (j / 4) + 4 (lane / 32) + j % 4][32 t + lane % 32]
+// The transposed order of rows is the order in which a 32 x 32 product leaves its result in a
+// lane's registers, so a block of probabilities goes into the next product as it stands.
+struct Args {
+  int64_t n, npad;  // pixels, padded
+  int V, vpad, D, dp;
+  float c2;         // |scale| log2(e)
+  float scale;
+  int reduction;    // 0 none, 1 mean, 2 sum
+  int rsplit, tsplit;
+  // state kept from forward to backward
+  int *count;       // pixels with a label
+  int *rowid, *lab; // listed pixel -> pixel, its label
+  float *lse, *w;   // log2 of the whole sum, 1 - p_y
+  uint16_t *xs, *xt, *es;
+  float *raw;       // (n, D): w (m - e_y)
+  // scratch
+  int *blk;
+  uint16_t *et;
+  float *pm, *pl, *po;
+  float *lrow;
+  double *part;
+  float *grow, *pe;
+  uint32_t *gmax;
+};
+
+// ------------------------------------------------------------------------------------------------
+// listing the pixels with a label
+// ------------------------------------------------------------------------------------------------
+static __global__ __launch_bounds__(kBlock) void kd_xent_count(int64_t n, int64_t V,
+                                                        const int64_t *__restrict__ labels,
+                                                        int *__restrict__ blk) {
+  __shared__ int s_c[kBlock / kWave];
+  const int64_t b = (int64_t)blockIdx.x * kMapChunk;
+  int c = 0;
+#pragma unroll
+  for (int k = 0; k < kMapChunk / kBlock; ++k) {
+    const int64_t i = b + k * kBlock + threadIdx.x;
+    const int64_t y = i < n ? labels[i] : -1;
+    c += __popcll(__ballot(y >= 0 && y < V));
+  }
+  if ((threadIdx.x & 63) == 0) s_c[threadIdx.x >> 6] = c;
+  __syncthreads();
+  if (threadIdx.x == 0) blk[blockIdx.x] = s_c[0] + s_c[1] + s_c[2] + s_c[3];
+}
+
+static __global__ __launch_bounds__(kBlock) void kd_xent_scan(int nblk, int *__restrict__ blk,
+                                                       int *__restrict__ count) {
+  __shared__ int s_w[kBlock / kWave];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int run = 0;
+  for (int b = 0; b < nblk; b += kBlock) {
+    const int i = b + threadIdx.x;
+    const int c = i < nblk ? blk[i] : 0;
+    int x = c;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int y = __shfl_up(x, d);
+      if (lane >= d) x += y;
+    }
+    if (lane == 63) s_w[w] = x;
+    __syncthreads();
+    int off = 0, tot = 0;
+#pragma unroll
+    for (int k = 0; k < kBlock / kWave; ++k) {
+      if (k < w) off += s_w[k];
+      tot += s_w[k];
+    }
+    __syncthreads();
+    if (i < nblk) blk[i] = run + off + x - c;
+    run += tot;
+  }
+  if (threadIdx.x == 0) *count = run;
+}
+
+static __global__ __launch_bounds__(kBlock) void kd_xent_map(int64_t n, int64_t V,
+                                                      const int64_t *__restrict__ labels,
+                                                      const int *__restrict__ blk,
+                                                      int *__restrict__ rowid,
+                                                      int *__restrict__ lab) {
+  __shared__ int s_c[4];
+  const int64_t b = (int64_t)blockIdx.x * kMapChunk;
+  int run = blk[blockIdx.x];
+  for (int k = 0; k < kMapChunk / kBlock; ++k) {
+    const int64_t i = b + k * kBlock + threadIdx.x;
+    const int64_t y = i < n ? labels[i] : -1;
+    int total;
+    const int p = wg_compact(y >= 0 && y < V, s_c, total);
+    if (p >= 0) {
+      rowid[run + p] = (int)i;
+      lab[run + p] = (int)y;
+    }
+    run += total;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// packing
+// ------------------------------------------------------------------------------------------------
+template <typename T, int DP>
+__global__ __launch_bounds__(kBlock) void kd_xent_pack(Args a, int xtiles,
+                                                       const T *__restrict__ features,
+                                                       const T *__restrict__ table) {
+  using F = Form<T>;
+  constexpr int kPitch = DP + 4 / (int)sizeof(T);  // odd in words: columns spread over the banks
+  __shared__ T s_m[32 * kPitch];
+  const bool is_x = (int)blockIdx.x < xtiles;
+  const int tile = is_x ? (int)blockIdx.x : (int)blockIdx.x - xtiles;
+  const int count = *a.count;
+  const int64_t r0 = (int64_t)tile * 32;
+  if (is_x && r0 >= ((int64_t)count + kRowPad - 1) / kRowPad * kRowPad) return;
+  const bool flip = is_x && a.scale < 0.f;
+  for (int e = threadIdx.x; e < 32 * DP; e += kBlock) {
+    const int r = e / DP, d = e % DP;
+    const int64_t i = r0 + r;
+    T x = (T)0.f;
+    if (d < a.D) {
+      if (is_x) {
+        if (i < count) x = features[(int64_t)a.rowid[i] * a.D + d];
+      } else if (i < a.V) {
+        x = table[i * a.D + d];
+      }
+    }
+    s_m[r * kPitch + d] = flip ? (T)(-(float)x) : x;
+  }
+  if (is_x && threadIdx.x < 32 && r0 + threadIdx.x >= count) {
+    a.lab[r0 + threadIdx.x] = -1;
+    a.lse[r0 + threadIdx.x] = INFINITY;  // its probabilities are 0
+    a.w[r0 + threadIdx.x] = 0.f;
+  }
+  __syncthreads();
+  constexpr int kGroups = 32 * DP / 8;  // 16-byte groups per plane and layout
+  uint16_t *straight = (is_x ? a.xs : a.es) + (int64_t)tile * F::np * 32 * DP;
+  uint16_t *transposed = is_x ? a.xt : a.et;
+  if (transposed) transposed += (int64_t)tile * F::np * 32 * DP;
+  for (int q = threadIdx.x; q < 2 * kGroups; q += kBlock) {
+    const bool tr = q >= kGroups;
+    if (tr && !transposed) break;
+    const int g = tr ? q - kGroups : q;
+    const int lane = g & 63, blkid = g >> 6;
+    Pack<uint16_t, 8> o[F::np];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      int r, d;
+      if (!tr) {
+        r = lane & 31;
+        d = 16 * blkid + 8 * (lane >> 5) + j;
+      } else {
+        constexpr int kT = DP / 32;
+        r = 16 * (blkid / kT) + 8 * (j >> 2) + 4 * (lane >> 5) + (j & 3);
+        d = 32 * (blkid % kT) + (lane & 31);
+      }
+      const T x = s_m[r * kPitch + d];
+      if constexpr (F::np == 1) {
+        o[0].v[j] = __builtin_bit_cast(uint16_t, x);
+      } else {
+        split3(x, o[0].v[j], o[1].v[j], o[2].v[j]);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < F::np; ++p)
+      *(Pack<uint16_t, 8> *)((tr ? transposed : straight) + (int64_t)p * 32 * DP + g * 8) = o[p];
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// shared pieces of the two walks
+// ------------------------------------------------------------------------------------------------
+// acc += a . b over the planes' products, the small ones first
+template <int NP, typename H8>
+__device__ __forceinline__ f32x16 mfma_planes(const H8 *a, const H8 *b, f32x16 c) {
+  if constexpr (NP == 3) {
+    c = mfma(a[0], b[2], c);
+    c = mfma(a[2], b[0], c);
+    c = mfma(a[1], b[1], c);
+    c = mfma(a[0], b[1], c);
+    c = mfma(a[1], b[0], c);
+  }
+  return mfma(a[0], b[0], c);
+}
+
+// 16 probabilities of a lane as the two B operands (row halves) of the next product
+template <typename T>
+__device__ __forceinline__ void pack_probs(const float *p, typename Form<T>::H8 (*o)[2]) {
+  using H = typename Form<T>::H;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (Form<T>::np == 1) {
+        o[0][s][j] = (H)p[8 * s + j];
+      } else {
+        uint16_t b[3];
+        split3(p[8 * s + j], b[0], b[1], b[2]);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) o[q][s][j] = __builtin_bit_cast(H, b[q]);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void stage(uint4 *dst, const uint16_t *src, int bytes) {
+  const uint4 *s = (const uint4 *)src;
+  for (int i = threadIdx.x; i < bytes / 16; i += kBlock) dst[i] = s[i];
+}
+
+// rows a wave holds (32 each): two blocks double the products per operand read from LDS; the
+// registers of wide or split operands allow one
+template <typename T, int DP>
+struct Blocks {
+  static constexpr int rb = Form<T>::np == 1 && DP <= 128 ? 2 : 1;
+  static constexpr int rows = 4 * 32 * rb;  // per workgroup
+};
+
+// ------------------------------------------------------------------------------------------------
+// the walk over the table
+// ------------------------------------------------------------------------------------------------
+template <typename T, int DP, bool SUM>
+__global__ __launch_bounds__(kBlock) void kd_xent_rows(Args a) {
+  using F = Form<T>;
+  using H8 = typename F::H8;
+  constexpr int NP = F::np, RB = Blocks<T, DP>::rb, KS = DP / 16, DT = DP / 32;
+  constexpr int kTileBytes = NP * 32 * DP * 2;
+  __shared__ uint4 s_e[kTileBytes / 16];
+  __shared__ uint4 s_t[SUM ? kTileBytes / 16 : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int64_t row0 = ((int64_t)blockIdx.x * 4 + wave) * (32 * RB);
+  if ((int64_t)blockIdx.x * Blocks<T, DP>::rows >= *a.count) return;
+  H8 x[RB][KS][NP];
+  int lab[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    lab[b] = a.lab[row0 + 32 * b + (lane & 31)];
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+        x[b][k][p] = *(const H8 *)(a.xs + ((((row0 >> 5) + b) * NP + p) * KS + k) * 512 + lane * 8);
+  }
+  f32x16 o[RB][DT];
+  float m[RB], l[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    m[b] = -1e30f;
+    l[b] = 0.f;
+    if constexpr (SUM)
+#pragma unroll
+      for (int t = 0; t < DT; ++t) o[b][t] = (f32x16)(0.f);
+  }
+  const int ntile = (a.V + 31) / 32;
+  const int t0 = (int)((int64_t)ntile * blockIdx.y / gridDim.y);
+  const int t1 = (int)((int64_t)ntile * (blockIdx.y + 1) / gridDim.y);
+  for (int t = t0; t < t1; ++t) {
+    __syncthreads();
+    stage(s_e, a.es + (int64_t)t * (kTileBytes / 2), kTileBytes);
+    if constexpr (SUM) stage(s_t, a.et + (int64_t)t * (kTileBytes / 2), kTileBytes);
+    __syncthreads();
+    const int v0 = t * 32;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      f32x16 s = (f32x16)(0.f);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        H8 e[NP];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) e[p] = *(const H8 *)&s_e[(p * KS + k) * 64 + lane];
+        s = mfma_planes<NP>(e, x[b][k], s);
+      }
+      // the label's own column and the table's padding take no part
+      uint32_t off = 0;
+      const bool edge = v0 + 32 > a.V;
+      const uint32_t rel = (uint32_t)(lab[b] - v0);
+      if (edge || __any(rel < 32u)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int v = 8 * (i >> 2) + 4 * half + (i & 3);
+          if (rel == (uint32_t)v || v0 + v >= a.V) {
+            off |= 1u << i;
+            s[i] = -3e38f;
+          }
+        }
+      }
+      float top = fmaxf(s[0], s[1]);
+#pragma unroll
+      for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(top, s[i]), s[i + 1]);
+      top *= a.c2;
+      if (__any(top > m[b] + F::slack)) {  // the maximum moves: rarely after the first tiles
+        const float mn = fmaxf(m[b], fmaxf(top, __shfl_xor(top, 32)));
+        const float f = __builtin_amdgcn_exp2f(m[b] - mn);
+        m[b] = mn;
+        l[b] *= f;
+        if constexpr (SUM)
+#pragma unroll
+          for (int t2 = 0; t2 < DT; ++t2)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[b][t2][i] *= f;
+      }
+      float p[16];
+      const float shift = F::shift - m[b];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c2, shift));
+      if (edge || __any(off != 0)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] = (off >> i) & 1u ? 0.f : p[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) l[b] += p[i];
+      if constexpr (SUM) {
+        H8 q[NP][2];
+        pack_probs<T>(p, q);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          H8 pb[NP];
+#pragma unroll
+          for (int pl = 0; pl < NP; ++pl) pb[pl] = q[pl][h];
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            H8 e[NP];
+#pragma unroll
+            for (int pl = 0; pl < NP; ++pl)
+              e[pl] = *(const H8 *)&s_t[((pl * 2 + h) * DT + d) * 64 + lane];
+            o[b][d] = mfma_planes<NP>(e, pb, o[b][d]);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int64_t r = (int64_t)blockIdx.y * a.npad + row0 + 32 * b + (lane & 31);
+    l[b] += __shfl_xor(l[b], 32);
+    if (half == 0) {
+      a.pm[r] = m[b] - F::shift;
+      a.pl[r] = l[b];
+    }
+    if constexpr (SUM) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f32x4 v;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = o[b][d][4 * i + j];
+          *(f32x4 *)(a.po + r * DP + 32 * d + 8 * i + 4 * half) = v;
+        }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// joining the parts: a wave per listed pixel
+// ------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__restrict__ features,
+                                                          const T *__restrict__ table,
+                                                          float *__restrict__ loss) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * (kBlock / kWave) + (threadIdx.x >> 6);
+  if (r >= *a.count) return;
+  const int64_t i = a.rowid[r], y = a.lab[r];
+  float z = 0.f;
+  for (int d = lane; d < a.D; d += kWave)
+    z = fmaf((float)features[i * a.D + d], (float)table[y * a.D + d], z);
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) z += __shfl_xor(z, s);
+  const float z2 = z * (a.scale * kLog2e);
+  float m = -1e30f;
+  for (int s = lane; s < a.rsplit; s += kWave) m = fmaxf(m, a.pm[(int64_t)s * a.npad + r]);
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+  float l = 0.f;
+  for (int s = lane; s < a.rsplit; s += kWave) {
+    const int64_t q = (int64_t)s * a.npad + r;
+    l += a.pl[q] * __builtin_amdgcn_exp2f(a.pm[q] - m);
+  }
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) l += __shfl_xor(l, s);
+  const float u = (m + log2f(l) - z2) * kLn2;  // -inf when the label is the only row
+  const float t = expf(-fabsf(u));
+  const float value = fmaxf(u, 0.f) + log1pf(t);
+  const float w = u >= 0.f ? 1.f / (1.f + t) : t / (1.f + t);
+  const float wn = u != u ? u : w;
+  const float out = u != u ? u : value;
+  if (lane == 0) {
+    a.lse[r] = z2 + out * kLog2e;
+    a.w[r] = wn;
+    if (a.reduction == 0)
+      loss[i] = out;
+    else
+      a.lrow[r] = out;
+  }
+  if (!a.raw) return;
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  for (int d = lane; d < a.D; d += kWave) {
+    float o = 0.f;
+    for (int s = 0; s < a.rsplit; ++s) {
+      const int64_t q = (int64_t)s * a.npad + r;
+      o += a.po[q * a.dp + d] * __builtin_amdgcn_exp2f(a.pm[q] - m);
+    }
+    a.raw[i * a.D + d] = wn * (o * inv - (float)table[y * a.D + d]);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// the loss
+// ------------------------------------------------------------------------------------------------
+constexpr int kReduceBlocks = 256;
+
+__device__ __forceinline__ double wg_sum(double x, double *s_x) {
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) x += __shfl_xor(x, s);
+  if ((threadIdx.x & 63) == 0) s_x[threadIdx.x >> 6] = x;
+  __syncthreads();
+  return s_x[0] + s_x[1] + s_x[2] + s_x[3];
+}
+
+static __global__ __launch_bounds__(kBlock) void kd_xent_sum(Args a) {
+  __shared__ double s_x[kBlock / kWave];
+  const int count = *a.count;
+  double x = 0.0;
+  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < count;
+       i += (int64_t)kReduceBlocks * kBlock)
+    x += (double)a.lrow[i];
+  x = wg_sum(x, s_x);
+  if (threadIdx.x == 0) a.part[blockIdx.x] = x;
+}
+
+static __global__ __launch_bounds__(kBlock) void kd_xent_finish(Args a, float *__restrict__ loss) {
+  __shared__ double s_x[kBlock / kWave];
+  const double x = wg_sum(a.part[threadIdx.x], s_x);
+  if (threadIdx.x == 0) {
+    const int count = *a.count;
+    *loss = (float)(a.reduction == 1 ? x / (double)(count > 0 ? count : 1) : x);
+  }
+}
+
+static __global__ __launch_bounds__(kBlock) void kd_xent_zero(int64_t n, float *__restrict__ p) {
+  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n;
+       i += (int64_t)gridDim.x * kBlock)
+    p[i] = 0.f;
+}
+
+// ------------------------------------------------------------------------------------------------
+// backward
+// ------------------------------------------------------------------------------------------------
+// the listed pixels' gradients of a loss per pixel, and the largest of their sizes (its bits as a
+// whole number: the order of the maxima does not matter)
+static __global__ __launch_bounds__(kBlock) void kd_xent_rowgrad(Args a, const float *__restrict__ grad) {
+  const int64_t r = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  const int count = *a.count;
+  float g = 0.f;
+  if (r < count) g = grad[a.rowid[r]];
+  if (r < a.npad) a.grow[r] = g;
+  uint32_t b = __float_as_uint(fabsf(g));
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) b = max(b, (uint32_t)__shfl_xor((int)b, s));
+  if ((threadIdx.x & 63) == 0 && b) atomicMax(a.gmax, b);
+}
+
+// the power of two that brings the largest gradient into [1, 2): the products' operands stay in
+// range whatever the incoming gradient's scale
+__device__ __forceinline__ float grad_unit(const uint32_t *gmax) {
+  const uint32_t e = *gmax >> 23;
+  return e == 0 || e >= 254 ? 1.f : __uint_as_float((254u - e) << 23);
+}
+
+template <typename T, int DP, bool ROWG>
+__global__ __launch_bounds__(kBlock) void kd_xent_table(Args a) {
+  using F = Form<T>;
+  using H8 = typename F::H8;
+  constexpr int NP = F::np, RB = Blocks<T, DP>::rb, KS = DP / 16, DT = DP / 32;
+  constexpr int kTileBytes = NP * 32 * DP * 2;
+  __shared__ uint4 s_x[kTileBytes / 16], s_t[kTileBytes / 16];
+  __shared__ float s_lse[32], s_w[32], s_g[32];
+  __shared__ int s_lab[32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int v0 = ((int)blockIdx.x * 4 + wave) * (32 * RB);
+  H8 e[RB][KS][NP];
+#pragma unroll
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+        e[b][k][p] =
+            *(const H8 *)(a.es + ((((int64_t)(v0 >> 5) + b) * NP + p) * KS + k) * 512 + lane * 8);
+  f32x16 o[RB][DT];
+#pragma unroll
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[b][t] = (f32x16)(0.f);
+  const int ntile = (*a.count + 31) / 32;
+  const int t0 = (int)((int64_t)ntile * blockIdx.y / gridDim.y);
+  const int t1 = (int)((int64_t)ntile * (blockIdx.y + 1) / gridDim.y);
+  const float unit = ROWG ? grad_unit(a.gmax) : 1.f;
+  const float top = exp2f(F::shift_table);
+  for (int t = t0; t < t1; ++t) {
+    __syncthreads();
+    stage(s_x, a.xs + (int64_t)t * (kTileBytes / 2), kTileBytes);
+    stage(s_t, a.xt + (int64_t)t * (kTileBytes / 2), kTileBytes);
+    if (threadIdx.x < 32) {
+      const int64_t r = (int64_t)t * 32 + threadIdx.x;
+      s_lse[threadIdx.x] = F::shift_table - a.lse[r];
+      s_w[threadIdx.x] = -a.w[r] * top;
+      s_lab[threadIdx.x] = a.lab[r];
+      if (ROWG) s_g[threadIdx.x] = a.grow[r] * unit;
+    }
+    __syncthreads();
+    const int y = s_lab[lane & 31];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      f32x16 s = (f32x16)(0.f);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        H8 x[NP];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) x[p] = *(const H8 *)&s_x[(p * KS + k) * 64 + lane];
+        s = mfma_planes<NP>(x, e[b][k], s);
+      }
+      float p[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = 8 * (i >> 2) + 4 * half + (i & 3);
+        p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c2, s_lse[r]));
+      }
+      const int vb = v0 + 32 * b;
+      if (__any((uint32_t)(y - vb) < 32u)) {  // pixels labelled with one of these rows
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int r = 8 * (i >> 2) + 4 * half + (i & 3);
+          if (s_lab[r] == vb + (lane & 31)) p[i] = s_w[r];
+        }
+      }
+      if (ROWG) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] *= s_g[8 * (i >> 2) + 4 * half + (i & 3)];
+      }
+      H8 q[NP][2];
+      pack_probs<T>(p, q);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        H8 pb[NP];
+#pragma unroll
+        for (int pl = 0; pl < NP; ++pl) pb[pl] = q[pl][h];
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          H8 xt[NP];
+#pragma unroll
+          for (int pl = 0; pl < NP; ++pl)
+            xt[pl] = *(const H8 *)&s_t[((pl * 2 + h) * DT + d) * 64 + lane];
+          o[b][d] = mfma_planes<NP>(xt, pb, o[b][d]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int64_t v = (int64_t)blockIdx.y * a.vpad + v0 + 32 * b + (lane & 31);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f32x4 c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[j] = o[b][d][4 * i + j];
+        *(f32x4 *)(a.pe + v * DP + 32 * d + 8 * i + 4 * half) = c;
+      }
+  }
+}
+
+// The gradient's common factor: the incoming scalar, over the count for the mean.
+__device__ __forceinline__ float grad_factor(const Args &a, const float *grad) {
+  float g = *grad;
+  if (a.reduction == 1) {
+    const int count = *a.count;
+    g /= (float)(count > 0 ? count : 1);
+  }
+  return g;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kBlock) void kd_xent_table_join(Args a, const float *__restrict__ grad,
+                                                             T *__restrict__ out) {
+  const int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if (q >= (int64_t)a.V * a.D) return;
+  const int64_t v = q / a.D;
+  const int d = (int)(q - v * a.D);
+  float x = 0.f;
+  for (int s = 0; s < a.tsplit; ++s) x += a.pe[((int64_t)s * a.vpad + v) * a.dp + d];
+  const float f = a.reduction == 0 ? 1.f / grad_unit(a.gmax) : grad_factor(a, grad);
+  out[q] = (T)(x * exp2f(-Form<T>::shift_table) * fabsf(a.scale) * f);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kBlock) void kd_xent_grad_features(Args a,
+                                                                const int64_t *__restrict__ labels,
+                                                                const float *__restrict__ grad,
+                                                                T *__restrict__ out) {
+  const int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if (q >= a.n * a.D) return;
+  const int64_t i = q / a.D;
+  const int64_t y = labels[i];
+  T v = (T)0.f;
+  if (y >= 0 && y < a.V) {
+    const float g = a.reduction == 0 ? grad[i] : grad_factor(a, grad);
+    v = (T)(a.raw[q] * (a.scale * g));
+  }
+  out[q] = v;
+}
+
+// ------------------------------------------------------------------------------------------------
+// host
+// ------------------------------------------------------------------------------------------------
+inline int padded_channels(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+
+struct Space {
+  char *base;
+  size_t used;
+  template <typename U>
+  U *take(size_t n) {
+    U *p = base ? (U *)(base + used) : nullptr;
+    used += (n * sizeof(U) + 255) & ~(size_t)255;
+    return p;
+  }
+};
+
+// rows a workgroup holds, and into how many parts the other matrix is cut so that the grid fills
+// the chip when there are few rows to hold
+inline int held_rows(int np, int dp) { return 128 * (np == 1 && dp <= 128 ? 2 : 1); }
+inline int parts(int64_t held, int per, int64_t walked) {
+  const int64_t gx = (held + per - 1) / per, tiles = (walked + 31) / 32;
+  int64_t s = (1024 + gx - 1) / (gx > 0 ? gx : 1);
+  if (s > tiles) s = tiles;
+  return (int)(s < 1 ? 1 : (s > 1024 ? 1024 : s));
+}
+
+inline Args shape(int64_t n, int64_t V, int D, int np, double scale, int reduction) {
+  Args a = {};
+  a.n = n;
+  a.npad = (n + kRowPad - 1) / kRowPad * kRowPad;
+  a.V = (int)V;
+  a.vpad = (int)((V + kRowPad - 1) / kRowPad * kRowPad);
+  a.D = D;
+  a.dp = padded_channels(D);
+  a.scale = (float)scale;
+  a.c2 = (float)(fabs(scale) * 1.4426950408889634);
+  a.reduction = reduction;
+  a.rsplit = parts(n, held_rows(np, a.dp), V);
+  a.tsplit = parts(V, held_rows(np, a.dp), n);
+  return a;
+}
+
+inline size_t lay_state(Args &a, int np, bool need_x, bool need_e, void *base) {
+  Space s{(char *)base, 0};
+  const size_t xe = (size_t)a.npad * a.dp * np, ee = (size_t)a.vpad * a.dp * np;
+  a.count = s.take<int>(64);
+  a.rowid = s.take<int>(a.npad);
+  a.lab = s.take<int>(a.npad);
+  a.lse = s.take<float>(a.npad);
+  a.w = s.take<float>(a.npad);
+  a.xs = s.take<uint16_t>(xe);
+  a.xt = need_e ? s.take<uint16_t>(xe) : nullptr;
+  a.es = s.take<uint16_t>(ee);
+  a.raw = need_x ? s.take<float>((size_t)a.n * a.D) : nullptr;
+  return s.used;
+}
+
+inline size_t lay_forward(Args &a, int np, bool need_x, void *base) {
+  Space s{(char *)base, 0};
+  a.blk = s.take<int>((size_t)((a.n + kMapChunk - 1) / kMapChunk));
+  a.et = need_x ? s.take<uint16_t>((size_t)a.vpad * a.dp * np) : nullptr;
+  a.pm = s.take<float>((size_t)a.rsplit * a.npad);
+  a.pl = s.take<float>((size_t)a.rsplit * a.npad);
+  a.po = need_x ? s.take<float>((size_t)a.rsplit * a.npad * a.dp) : nullptr;
+  a.lrow = s.take<float>(a.npad);
+  a.part = s.take<double>(kReduceBlocks);
+  return s.used;
+}
+
+inline size_t lay_backward(Args &a, bool need_e, void *base) {
+  Space s{(char *)base, 0};
+  a.gmax = s.take<uint32_t>(64);
+  a.grow = s.take<float>(a.npad);
+  a.pe = need_e ? s.take<float>((size_t)a.tsplit * a.vpad * a.dp) : nullptr;
+  return s.used;
+}
+
+inline int check(int64_t n, int64_t V, int D, double scale, int reduction) {
+  KD_CHECK_ARG(n >= 0 && n < ((int64_t)1 << 31) - kRowPad,
+               "surface_cross_entropy: need 0 <= pixels < 2^31 - 256");
+  KD_CHECK_ARG(V >= 1 && V < ((int64_t)1 << 31) - kRowPad,
+               "surface_cross_entropy: need 1 <= embeddings < 2^31 - 256");
+  KD_CHECK_ARG(D >= 1 && D <= 256, "surface_cross_entropy: need 1 <= channels <= 256");
+  KD_CHECK_ARG(scale - scale == 0.0 && fabs(scale) < 1e30,
+               "surface_cross_entropy: scale must be finite");
+  KD_CHECK_ARG(reduction >= 0 && reduction <= 2, "surface_cross_entropy: unknown reduction");
+  return KD_OK;
+}
+
+template <typename T, int DP>
+void launch_forward(const Args &a, bool need_x, const T *features, const T *table,
+                    hipStream_t stream) {
+  const int xtiles = (int)(a.npad / 32), etiles = a.vpad / 32;
+  hipLaunchKernelGGL((kd_xent_pack<T, DP>), dim3((unsigned)(xtiles + etiles)), dim3(kBlock), 0,
+                     stream, a, xtiles, features, table);
+  constexpr int rows = Blocks<T, DP>::rows;
+  const dim3 grid((unsigned)((a.n + rows - 1) / rows), (unsigned)a.rsplit);
+  if (need_x)
+    hipLaunchKernelGGL((kd_xent_rows<T, DP, true>), grid, dim3(kBlock), 0, stream, a);
+  else
+    hipLaunchKernelGGL((kd_xent_rows<T, DP, false>), grid, dim3(kBlock), 0, stream, a);
+}
+
+template <typename T, int DP>
+void launch_table(const Args &a, hipStream_t stream) {
+  constexpr int rows = Blocks<T, DP>::rows;
+  const dim3 grid((unsigned)((a.V + rows - 1) / rows), (unsigned)a.tsplit);
+  if (a.reduction == 0)
+    hipLaunchKernelGGL((kd_xent_table<T, DP, true>), grid, dim3(kBlock), 0, stream, a);
+  else
+    hipLaunchKernelGGL((kd_xent_table<T, DP, false>), grid, dim3(kBlock), 0, stream, a);
+}
+
+inline unsigned blocks(int64_t n) { return (unsigned)((n + kBlock - 1) / kBlock); }
+
+template <typename T>
+int forward(int64_t n, int64_t V, int D, const T *features, const T *table, const int64_t *labels,
+            double scale, int reduction, int need_x, int need_e, float *loss, void *state,
+            size_t state_bytes, void *scratch, size_t scratch_bytes, hipStream_t stream) {
+  const int rc = check(n, V, D, scale, reduction);
+  if (rc != KD_OK) return rc;
+  KD_CHECK_ARG(loss || (n == 0 && reduction == 0), "surface_cross_entropy: loss is NULL");
+  KD_CHECK_ARG(table && (n == 0 || (features && labels)), "surface_cross_entropy: NULL input");
+  Args a = shape(n, V, D, Form<T>::np, scale, reduction);
+  const size_t ns = lay_state(a, Form<T>::np, need_x, need_e, state);
+  const size_t nw = lay_forward(a, Form<T>::np, need_x, scratch);
+  if (!state || state_bytes < ns || !scratch || scratch_bytes < nw)
+    return set_error(KD_ERR_WORKSPACE, "workspace too small: %zu < %zu or %zu < %zu", state_bytes,
+                     ns, scratch_bytes, nw);
+  ProfScope prof(K_XENT_FWD, stream);
+  if (reduction == 0 && n > 0)
+    hipLaunchKernelGGL(kd_xent_zero, dim3(std::min(blocks(n), 4096u)), dim3(kBlock), 0, stream, n,
+                       loss);
+  const int nblk = (int)((n + kMapChunk - 1) / kMapChunk);
+  if (nblk > 0)
+    hipLaunchKernelGGL(kd_xent_count, dim3(nblk), dim3(kBlock), 0, stream, n, V, labels, a.blk);
+  hipLaunchKernelGGL(kd_xent_scan, dim3(1), dim3(kBlock), 0, stream, nblk, a.blk, a.count);
+  if (n > 0) {
+    hipLaunchKernelGGL(kd_xent_map, dim3(nblk), dim3(kBlock), 0, stream, n, V, labels, a.blk,
+                       a.rowid, a.lab);
+    switch (a.dp) {
+      case 32: launch_forward<T, 32>(a, need_x, features, table, stream); break;
+      case 64: launch_forward<T, 64>(a, need_x, features, table, stream); break;
+      case 128: launch_forward<T, 128>(a, need_x, features, table, stream); break;
+      default: launch_forward<T, 256>(a, need_x, features, table, stream); break;
+    }
+    hipLaunchKernelGGL(kd_xent_combine<T>, dim3((unsigned)((n + 3) / 4)), dim3(kBlock), 0, stream,
+                       a, features, table, loss);
+  }
+  if (reduction != 0) {
+    hipLaunchKernelGGL(kd_xent_sum, dim3(kReduceBlocks), dim3(kBlock), 0, stream, a);
+    hipLaunchKernelGGL(kd_xent_finish, dim3(1), dim3(kBlock), 0, stream, a, loss);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess)
+    return set_error(KD_ERR_LAUNCH, "surface_cross_entropy: %s", hipGetErrorString(e));
+  return KD_OK;
+}
+
+template <typename T>
+int backward(int64_t n, int64_t V, int D, const int64_t *labels, double scale, int reduction,
+             int need_x, int need_e, const float *grad, T *gx, T *ge, void *state,
+             size_t state_bytes, void *scratch, size_t scratch_bytes, hipStream_t stream) {
+  const int rc = check(n, V, D, scale, reduction);
+  if (rc != KD_OK) return rc;
+  KD_CHECK_ARG(grad || (n == 0 && reduction == 0), "surface_cross_entropy: grad_loss is NULL");
+  KD_CHECK_ARG(n == 0 || labels, "surface_cross_entropy: NULL input");
+  KD_CHECK_ARG((!gx || need_x) && (!ge || need_e),
+               "surface_cross_entropy: a gradient that the forward call did not prepare");
+  Args a = shape(n, V, D, Form<T>::np, scale, reduction);
+  const size_t ns = lay_state(a, Form<T>::np, need_x, need_e, state);
+  const size_t nw = lay_backward(a, ge != nullptr, scratch);
+  if (!state || state_bytes < ns || !scratch || scratch_bytes < nw)
+    return set_error(KD_ERR_WORKSPACE, "workspace too small: %zu < %zu or %zu < %zu", state_bytes,
+                     ns, scratch_bytes, nw);
+  ProfScope prof(K_XENT_BWD, stream);
+  if (gx && n > 0)
+    hipLaunchKernelGGL(kd_xent_grad_features<T>, dim3(blocks(n * D)), dim3(kBlock), 0, stream, a,
+                       labels, grad, gx);
+  if (ge) {
+    if (reduction == 0) {
+      hipLaunchKernelGGL(kd_xent_zero, dim3(1), dim3(kBlock), 0, stream, (int64_t)64,
+                         (float *)a.gmax);
+      if (n > 0)
+        hipLaunchKernelGGL(kd_xent_rowgrad, dim3(blocks(a.npad)), dim3(kBlock), 0, stream, a, grad);
+    }
+    switch (a.dp) {
+      case 32: launch_table<T, 32>(a, stream); break;
+      case 64: launch_table<T, 64>(a, stream); break;
+      case 128: launch_table<T, 128>(a, stream); break;
+      default: launch_table<T, 256>(a, stream); break;
+    }
+    hipLaunchKernelGGL(kd_xent_table_join<T>, dim3(blocks((int64_t)V * D)), dim3(kBlock), 0, stream,
+                       a, grad, ge);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess)
+    return set_error(KD_ERR_LAUNCH, "surface_cross_entropy bwd: %s", hipGetErrorString(e));
+  return KD_OK;
+}
+
+}  // namespace xent
+}  // namespace kd
+
+#define KD_XENT(SFX, T)                                                                           \
+  extern "C" int kd_surface_xent_forward_##SFX(                                                   \
+      int64_t n, int64_t rows, int channels, const void *features, const void *embeddings,        \
+      const int64_t *labels, double scale, int reduction, int need_features, int need_embeddings, \
+      float *loss, void *state, size_t state_bytes, void *scratch, size_t scratch_bytes,          \
+      void *stream) {                                                                             \
+    return kd::xent::forward<T>(n, rows, channels, (const T *)features, (const T *)embeddings,    \
+                                labels, scale, reduction, need_features, need_embeddings, loss,   \
+                                state, state_bytes, scratch, scratch_bytes, (hipStream_t)stream); \
+  }                                                                                               \
+  extern "C" int kd_surface_xent_backward_##SFX(                                                  \
+      int64_t n, int64_t rows, int channels, const int64_t *labels, double scale, int reduction,  \
+      int need_features, int need_embeddings, const float *grad_loss, void *grad_features,        \
+      void *grad_embeddings, void *state, size_t state_bytes, void *scratch,                      \
+      size_t scratch_bytes, void *stream) {                                                       \
+    return kd::xent::backward<T>(n, rows, channels, labels, scale, reduction, need_features,      \
+                                 need_embeddings, grad_loss, (T *)grad_features,                  \
+                                 (T *)grad_embeddings, state, state_bytes, scratch,               \
+                                 scratch_bytes, (hipStream_t)stream);                             \
+  }
