@@ -32,6 +32,7 @@
 #include "kd_float16.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace kd {
 namespace xent {
@@ -106,7 +107,9 @@ struct Args {
   // state kept from forward to backward
   int *count;       // pixels with a label
   int *rowid, *lab; // listed pixel -> pixel, its label
-  float *lse, *w;   // log2 of the whole sum, 1 - p_y
+  float *lse, *w;   // exponent of a probability but its logit, its complement negated (scaled)
+  float *xn;        // squared sizes of the pixels' features
+  uint32_t *emax;   // the largest squared size of the table's rows (its bits)
   uint16_t *xs, *xt, *es;
   float *raw;       // (n, D): w (m - e_y)
   // scratch
@@ -140,7 +143,8 @@ static __global__ __launch_bounds__(kBlock) void kd_xent_count(int64_t n, int64_
 }
 
 static __global__ __launch_bounds__(kBlock) void kd_xent_scan(int nblk, int *__restrict__ blk,
-                                                       int *__restrict__ count) {
+                                                       int *__restrict__ count,
+                                                       uint32_t *__restrict__ emax) {
   __shared__ int s_w[kBlock / kWave];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int run = 0;
@@ -165,7 +169,10 @@ static __global__ __launch_bounds__(kBlock) void kd_xent_scan(int nblk, int *__r
     if (i < nblk) blk[i] = run + off + x - c;
     run += tot;
   }
-  if (threadIdx.x == 0) *count = run;
+  if (threadIdx.x == 0) {
+    *count = run;
+    *emax = 0u;
+  }
 }
 
 static __global__ __launch_bounds__(kBlock) void kd_xent_map(int64_t n, int64_t V,
@@ -220,10 +227,32 @@ __global__ __launch_bounds__(kBlock) void kd_xent_pack(Args a, int xtiles,
   }
   if (is_x && threadIdx.x < 32 && r0 + threadIdx.x >= count) {
     a.lab[r0 + threadIdx.x] = -1;
-    a.lse[r0 + threadIdx.x] = INFINITY;  // its probabilities are 0
+    a.lse[r0 + threadIdx.x] = -INFINITY;  // its probabilities are 0
     a.w[r0 + threadIdx.x] = 0.f;
   }
   __syncthreads();
+  {  // squared sizes: 8 lanes a row
+    const int r = threadIdx.x >> 3;
+    float q = 0.f;
+#pragma unroll
+    for (int k = 0; k < DP / 8; ++k) {
+      const int d = (threadIdx.x & 7) + 8 * k;
+      const float x = (float)s_m[r * kPitch + d];
+      q = fmaf(x, x, q);
+    }
+#pragma unroll
+    for (int k = 4; k >= 1; k >>= 1) q += __shfl_xor(q, k);
+    if (is_x) {
+      if ((threadIdx.x & 7) == 0) a.xn[r0 + r] = q;
+    } else {
+      uint32_t u = __float_as_uint(q);
+#pragma unroll
+      for (int k = 32; k >= 8; k >>= 1) u = max(u, (uint32_t)__shfl_xor((int)u, k));
+      // the look before saves all but the few atomics that raise it: one address, many tiles
+      if ((threadIdx.x & 63) == 0 && u > __hip_atomic_load(a.emax, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+        atomicMax(a.emax, u);
+    }
+  }
   constexpr int kGroups = 32 * DP / 8;  // 16-byte groups per plane and layout
   uint16_t *straight = (is_x ? a.xs : a.es) + (int64_t)tile * F::np * 32 * DP;
   uint16_t *transposed = is_x ? a.xt : a.et;
@@ -274,159 +303,319 @@ __device__ __forceinline__ f32x16 mfma_planes(const H8 *a, const H8 *b, f32x16 c
   return mfma(a[0], b[0], c);
 }
 
-// 16 probabilities of a lane as the two B operands (row halves) of the next product
+// the upper halves of two words as one
+__device__ __forceinline__ uint32_t upper2(uint32_t lo, uint32_t hi) {
+  return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+}
+
+// 8 probabilities of a lane as a B operand of the next product
 template <typename T>
-__device__ __forceinline__ void pack_probs(const float *p, typename Form<T>::H8 (*o)[2]) {
+__device__ __forceinline__ void pack_probs(const float *p, typename Form<T>::H8 *o) {
   using H = typename Form<T>::H;
+  using H8 = typename Form<T>::H8;
+  if constexpr (Form<T>::np == 1) {
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
+    for (int j = 0; j < 8; ++j) o[0][j] = (H)p[j];
+  } else {
+    uint4 q[3];
+    uint32_t *w = (uint32_t *)q;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if constexpr (Form<T>::np == 1) {
-        o[0][s][j] = (H)p[8 * s + j];
-      } else {
-        uint16_t b[3];
-        split3(p[8 * s + j], b[0], b[1], b[2]);
+    for (int j = 0; j < 8; j += 2) {
+      uint32_t u[3][2];
 #pragma unroll
-        for (int q = 0; q < 3; ++q) o[q][s][j] = __builtin_bit_cast(H, b[q]);
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t a = __float_as_uint(p[j + k]);
+        const float r = p[j + k] - __uint_as_float(a & 0xffff0000u);
+        const uint32_t b = __float_as_uint(r);
+        u[0][k] = a;
+        u[1][k] = b;
+        u[2][k] = __float_as_uint(r - __uint_as_float(b & 0xffff0000u));
       }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) w[4 * k + j / 2] = upper2(u[k][0], u[k][1]);
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) o[k] = __builtin_bit_cast(H8, q[k]);
+  }
+}
+
+// How a walk is laid out.  rb: blocks of 32 rows that a wave holds; two double the products per
+// operand read from LDS, the registers of wide or split operands allow one.  kt: tiles of 32 rows
+// per stage in LDS.  dbl: two buffers a side, loads one stage ahead and one barrier a stage; else
+// one buffer a side and the loads one phase ahead (the straight operands arrive while the second
+// product runs and the other way round), which halves the LDS of the widest split operands.
+template <typename T, int DP>
+struct Walk {
+  static constexpr int np = Form<T>::np;
+  static constexpr int rb = np == 1 && DP <= 128 ? 2 : 1;
+  static constexpr int kt = np == 1 && DP <= 64 ? 2 : 1;
+  static constexpr bool dbl = np == 1 || DP <= 64;
+  static constexpr int ahead = np == 3 ? 1 : DP == 128 ? 2 : 2;  // operands read ahead
+  static constexpr int rows = 4 * 32 * rb;                 // held by a workgroup
+  static constexpr int waves = np == 3 && DP == 256 ? 1 : 2;  // per SIMD, at least
+  static constexpr int tile_words = np * 32 * DP / 2;      // 4-byte words of a tile's operands
+  static constexpr int stage_bytes = kt * tile_words * 4;  // a multiple of 1024
+};
+
+// acc[b] += A_n . B[n][b] over N operands A_n that are read from LDS, G at a time and one group ahead
+// of the products; the fences keep the compiler from reading more ahead than registers hold.
+// at(n) is operand n's offset, B(n, b) and C(n, b) give the other operand and the sum.
+template <typename T, int DP, int N, typename At, typename B, typename C>
+__device__ __forceinline__ void products(const uint4 *s, At at, B other, C sum) {
+  using H8 = typename Form<T>::H8;
+  constexpr int NP = Form<T>::np, RB = Walk<T, DP>::rb, G = Walk<T, DP>::ahead;
+  static_assert(N % G == 0, "whole groups");
+  const int lane = threadIdx.x & 63;
+  H8 a[2][G][NP];
+#pragma unroll
+  for (int g = -1; g < N / G; ++g) {
+    if (g + 1 < N / G) {
+#pragma unroll
+      for (int j = 0; j < G; ++j)
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          a[(g + 1) & 1][j][p] = *(const H8 *)&s[at((g + 1) * G + j, p) * 64 + lane];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (g >= 0) {
+#pragma unroll
+      for (int j = 0; j < G; ++j)
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+          f32x16 &c = sum(g * G + j, b);
+          c = mfma_planes<NP>(a[g & 1][j], other(g * G + j, b), c);
+        }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
 
-__device__ __forceinline__ void stage(uint4 *dst, const uint16_t *src, int bytes) {
-  const uint4 *s = (const uint4 *)src;
-  for (int i = threadIdx.x; i < bytes / 16; i += kBlock) dst[i] = s[i];
+// Copies `bytes` from global memory to LDS without registers: 1 KB a wave and instruction, waited
+// for with arrive().
+template <int BYTES>
+__device__ __forceinline__ void fetch(uint4 *dst, const uint16_t *src) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  static_assert(BYTES % 1024 == 0, "a wave copies 1 KB at a time");
+#pragma unroll
+  for (int c = 0; c < BYTES / 1024; c += 4) {
+    if (BYTES % 4096 != 0 && c + wave >= BYTES / 1024) break;
+    const int k = c + wave;
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) void *)(src + k * 512 + lane * 8),
+        (__attribute__((address_space(3))) void *)(dst + k * 64), 16, 0, 0);
+  }
 }
 
-// rows a wave holds (32 each): two blocks double the products per operand read from LDS; the
-// registers of wide or split operands allow one
-template <typename T, int DP>
-struct Blocks {
-  static constexpr int rb = Form<T>::np == 1 && DP <= 128 ? 2 : 1;
-  static constexpr int rows = 4 * 32 * rb;  // per workgroup
-};
+__device__ __forceinline__ void arrive() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
 
 // ------------------------------------------------------------------------------------------------
 // the walk over the table
 // ------------------------------------------------------------------------------------------------
+// exp2 of logits up to this size needs no maximum: 2^60 a term leaves room for the sum and for the
+// smallest term, 2^-60, in 32 bits (and in bf16)
+constexpr float kSafeLogit = 60.f;
+
 template <typename T, int DP, bool SUM>
-__global__ __launch_bounds__(kBlock) void kd_xent_rows(Args a) {
+struct RowsWalk {
   using F = Form<T>;
   using H8 = typename F::H8;
-  constexpr int NP = F::np, RB = Blocks<T, DP>::rb, KS = DP / 16, DT = DP / 32;
-  constexpr int kTileBytes = NP * 32 * DP * 2;
-  __shared__ uint4 s_e[kTileBytes / 16];
-  __shared__ uint4 s_t[SUM ? kTileBytes / 16 : 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int64_t row0 = ((int64_t)blockIdx.x * 4 + wave) * (32 * RB);
-  if ((int64_t)blockIdx.x * Blocks<T, DP>::rows >= *a.count) return;
+  using W = Walk<T, DP>;
+  static constexpr int NP = F::np, RB = W::rb, KS = DP / 16, DT = DP / 32;
   H8 x[RB][KS][NP];
   int lab[RB];
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    lab[b] = a.lab[row0 + 32 * b + (lane & 31)];
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int p = 0; p < NP; ++p)
-        x[b][k][p] = *(const H8 *)(a.xs + ((((row0 >> 5) + b) * NP + p) * KS + k) * 512 + lane * 8);
-  }
-  f32x16 o[RB][DT];
+  f32x16 o[SUM ? RB : 1][SUM ? DT : 1];
   float m[RB], l[RB];
+  bool online;
+  int V;
+  float c2;
+
+  // one tile of 32 table rows: the logits, and the probabilities as operands
+  template <bool ONLINE>
+  __device__ __forceinline__ void logits(const uint4 *s_e, int v0, H8 (*q)[2][NP]) {
+    const int half = (threadIdx.x & 63) >> 5;
+    f32x16 s[RB];
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    m[b] = -1e30f;
-    l[b] = 0.f;
-    if constexpr (SUM)
+    for (int b = 0; b < RB; ++b) s[b] = (f32x16)(0.f);
+    products<T, DP, KS>(
+        s_e, [](int k, int p) { return p * KS + k; }, [&](int k, int b) { return x[b][k]; },
+        [&](int, int b) -> f32x16 & { return s[b]; });
+    // the label's own column and the table's padding take no part
+    bool near = false;
 #pragma unroll
-      for (int t = 0; t < DT; ++t) o[b][t] = (f32x16)(0.f);
-  }
-  const int ntile = (a.V + 31) / 32;
-  const int t0 = (int)((int64_t)ntile * blockIdx.y / gridDim.y);
-  const int t1 = (int)((int64_t)ntile * (blockIdx.y + 1) / gridDim.y);
-  for (int t = t0; t < t1; ++t) {
-    __syncthreads();
-    stage(s_e, a.es + (int64_t)t * (kTileBytes / 2), kTileBytes);
-    if constexpr (SUM) stage(s_t, a.et + (int64_t)t * (kTileBytes / 2), kTileBytes);
-    __syncthreads();
-    const int v0 = t * 32;
+    for (int b = 0; b < RB; ++b) near |= (uint32_t)(lab[b] - v0) < 32u;
+    const bool hit = v0 + 32 > V || __any(near);
+    if (hit) {
+      int first = 4 * half;
+      asm volatile("" : "+v"(first));  // its sums stay in here and out of the loop's registers
+      first += v0;
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      f32x16 s = (f32x16)(0.f);
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        H8 e[NP];
-#pragma unroll
-        for (int p = 0; p < NP; ++p) e[p] = *(const H8 *)&s_e[(p * KS + k) * 64 + lane];
-        s = mfma_planes<NP>(e, x[b][k], s);
-      }
-      // the label's own column and the table's padding take no part
-      uint32_t off = 0;
-      const bool edge = v0 + 32 > a.V;
-      const uint32_t rel = (uint32_t)(lab[b] - v0);
-      if (edge || __any(rel < 32u)) {
+      for (int b = 0; b < RB; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int v = 8 * (i >> 2) + 4 * half + (i & 3);
-          if (rel == (uint32_t)v || v0 + v >= a.V) {
-            off |= 1u << i;
-            s[i] = -3e38f;
-          }
+          const int v = first + 8 * (i >> 2) + (i & 3);
+          s[b][i] = v == lab[b] || v >= V ? -INFINITY : s[b][i];
         }
+    }
+    if constexpr (ONLINE) {
+      float top[RB];
+      bool up = false;
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        top[b] = fmaxf(s[b][0], s[b][1]);
+#pragma unroll
+        for (int i = 2; i < 16; i += 2) top[b] = fmaxf(fmaxf(top[b], s[b][i]), s[b][i + 1]);
+        top[b] *= c2;
+        up |= top[b] > m[b] + F::slack;
       }
-      float top = fmaxf(s[0], s[1]);
+      if (__any(up)) {  // a maximum moves: rarely after the first tiles
 #pragma unroll
-      for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(top, s[i]), s[i + 1]);
-      top *= a.c2;
-      if (__any(top > m[b] + F::slack)) {  // the maximum moves: rarely after the first tiles
-        const float mn = fmaxf(m[b], fmaxf(top, __shfl_xor(top, 32)));
-        const float f = __builtin_amdgcn_exp2f(m[b] - mn);
-        m[b] = mn;
-        l[b] *= f;
-        if constexpr (SUM)
+        for (int b = 0; b < RB; ++b) {
+          const float mn = fmaxf(m[b], fmaxf(top[b], __shfl_xor(top[b], 32)));
+          const float f = __builtin_amdgcn_exp2f(m[b] - mn);
+          m[b] = mn;
+          l[b] *= f;
+          if constexpr (SUM) {
 #pragma unroll
-          for (int t2 = 0; t2 < DT; ++t2)
+            for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[b][t2][i] *= f;
-      }
-      float p[16];
-      const float shift = F::shift - m[b];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c2, shift));
-      if (edge || __any(off != 0)) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) p[i] = (off >> i) & 1u ? 0.f : p[i];
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) l[b] += p[i];
-      if constexpr (SUM) {
-        H8 q[NP][2];
-        pack_probs<T>(p, q);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          H8 pb[NP];
-#pragma unroll
-          for (int pl = 0; pl < NP; ++pl) pb[pl] = q[pl][h];
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            H8 e[NP];
-#pragma unroll
-            for (int pl = 0; pl < NP; ++pl)
-              e[pl] = *(const H8 *)&s_t[((pl * 2 + h) * DT + d) * 64 + lane];
-            o[b][d] = mfma_planes<NP>(e, pb, o[b][d]);
+              for (int i = 0; i < 16; ++i) o[b][d][i] *= f;
           }
         }
       }
     }
+    float p[RB][16];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      const float shift = ONLINE ? F::shift - m[b] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        p[b][i] = __builtin_amdgcn_exp2f(ONLINE ? fmaf(s[b][i], c2, shift) : s[b][i] * c2);
+    }
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t[i & 3] += p[b][i];
+      l[b] += (t[0] + t[1]) + (t[2] + t[3]);
+      if constexpr (SUM) {
+        pack_probs<T>(p[b], q[b][0]);
+        pack_probs<T>(p[b] + 8, q[b][1]);
+      }
+    }
   }
+
+  __device__ __forceinline__ void add(const uint4 *s_t, const H8 (*q)[2][NP]) {
+    products<T, DP, 2 * DT>(
+        s_t, [](int n, int p) { return p * 2 * DT + n; },
+        [&](int n, int b) { return q[b][n / DT]; },
+        [&](int n, int b) -> f32x16 & { return o[b][n % DT]; });
+  }
+
+  template <bool ONLINE>
+  __device__ __forceinline__ void stage(const uint4 *s_e, const uint4 *s_t, int v0) {
+#pragma unroll
+    for (int k = 0; k < W::kt; ++k) {
+      H8 q[RB][2][NP];
+      logits<ONLINE>(s_e + k * (W::tile_words / 4), v0 + 32 * k, q);
+      if constexpr (SUM) add(s_t + k * (W::tile_words / 4), q);
+    }
+  }
+};
+
+template <typename T, int DP, bool SUM>
+__global__ __launch_bounds__(kBlock, (Walk<T, DP>::waves)) void kd_xent_rows(Args a) {
+  using F = Form<T>;
+  using W = Walk<T, DP>;
+  using H8 = typename F::H8;
+  constexpr int NP = F::np, RB = W::rb, KS = DP / 16, DT = DP / 32, kBytes = W::stage_bytes;
+  __shared__ uint4 s_e0[kBytes / 16], s_t0[SUM ? kBytes / 16 : 1];
+  __shared__ uint4 s_e1[W::dbl || !SUM ? kBytes / 16 : 1], s_t1[SUM && W::dbl ? kBytes / 16 : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int64_t row0 = ((int64_t)blockIdx.x * 4 + wave) * (32 * RB);
+  if ((int64_t)blockIdx.x * W::rows >= *a.count) return;
+  RowsWalk<T, DP, SUM> w;
+  w.V = a.V;
+  w.c2 = a.c2;
+  // |logit| <= |x| |e| scale; a NaN size takes the general way
+  const float emax = __uint_as_float(*a.emax);
+  bool safe = F::shift == 0.f;
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int64_t r = row0 + 32 * b + (lane & 31);
+    w.lab[b] = a.lab[r];
+    safe &= a.c2 * sqrtf(a.xn[r]) * sqrtf(emax) < kSafeLogit;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+        w.x[b][k][p] =
+            *(const H8 *)(a.xs + ((((row0 >> 5) + b) * NP + p) * KS + k) * 512 + lane * 8);
+  }
+  w.online = !__all(safe);
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    w.m[b] = w.online ? -1e30f : 0.f;
+    w.l[b] = 0.f;
+    if constexpr (SUM) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t) w.o[b][t] = (f32x16)(0.f);
+    }
+  }
+  constexpr int kRows = 32 * W::kt;
+  constexpr int kStep2 = 2;  // stages come in pairs, for the two buffers
+  const int nst = (a.V + kStep2 * kRows - 1) / (kStep2 * kRows);
+  const int t0 = (int)((int64_t)nst * blockIdx.y / gridDim.y) * kStep2;
+  const int t1 = (int)((int64_t)nst * (blockIdx.y + 1) / gridDim.y) * kStep2;
+  const uint16_t *es = a.es, *et = a.et;
+  constexpr int64_t kStep = kBytes / 2;
+  auto walk = [&](auto online) {
+  constexpr bool ONLINE = decltype(online)::value;
+  if constexpr (W::dbl || !SUM) {
+    if (t0 < t1) {
+      fetch<kBytes>(s_e0, es + t0 * kStep);
+      if constexpr (SUM) fetch<kBytes>(s_t0, et + t0 * kStep);
+    }
+    arrive();
+    for (int t = t0; t < t1; t += 2) {
+      fetch<kBytes>(s_e1, es + (t + 1) * kStep);
+      if constexpr (SUM) fetch<kBytes>(s_t1, et + (t + 1) * kStep);
+      w.template stage<ONLINE>(s_e0, s_t0, t * kRows);
+      arrive();
+      if (t + 2 < t1) {
+        fetch<kBytes>(s_e0, es + (t + 2) * kStep);
+        if constexpr (SUM) fetch<kBytes>(s_t0, et + (t + 2) * kStep);
+      }
+      w.template stage<ONLINE>(s_e1, s_t1, (t + 1) * kRows);
+      arrive();
+    }
+  } else {
+    if (t0 < t1) fetch<kBytes>(s_e0, es + t0 * kStep);
+    arrive();
+    for (int t = t0; t < t1; ++t) {
+      H8 q[RB][2][NP];
+      fetch<kBytes>(s_t0, et + t * kStep);
+      w.template logits<ONLINE>(s_e0, t * kRows, q);
+      arrive();
+      if (t + 1 < t1) fetch<kBytes>(s_e0, es + (t + 1) * kStep);
+      w.add(s_t0, q);
+      arrive();
+    }
+  }
+  };
+  if (w.online)
+    walk(std::true_type{});
+  else
+    walk(std::false_type{});
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
     const int64_t r = (int64_t)blockIdx.y * a.npad + row0 + 32 * b + (lane & 31);
-    l[b] += __shfl_xor(l[b], 32);
+    const float l = w.l[b] + __shfl_xor(w.l[b], 32);
     if (half == 0) {
-      a.pm[r] = m[b] - F::shift;
-      a.pl[r] = l[b];
+      a.pm[r] = w.m[b] - F::shift;
+      a.pl[r] = l;
     }
     if constexpr (SUM) {
 #pragma unroll
@@ -435,7 +624,7 @@ __global__ __launch_bounds__(kBlock) void kd_xent_rows(Args a) {
         for (int i = 0; i < 4; ++i) {
           f32x4 v;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = o[b][d][4 * i + j];
+          for (int j = 0; j < 4; ++j) v[j] = w.o[b][d][4 * i + j];
           *(f32x4 *)(a.po + r * DP + 32 * d + 8 * i + 4 * half) = v;
         }
     }
@@ -477,8 +666,8 @@ __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__res
   const float wn = u != u ? u : w;
   const float out = u != u ? u : value;
   if (lane == 0) {
-    a.lse[r] = z2 + out * kLog2e;
-    a.w[r] = wn;
+    a.lse[r] = Form<T>::shift_table - (z2 + out * kLog2e);
+    a.w[r] = -wn * exp2f(Form<T>::shift_table);
     if (a.reduction == 0)
       loss[i] = out;
     else
@@ -560,104 +749,186 @@ __device__ __forceinline__ float grad_unit(const uint32_t *gmax) {
 }
 
 template <typename T, int DP, bool ROWG>
-__global__ __launch_bounds__(kBlock) void kd_xent_table(Args a) {
+struct TableWalk {
   using F = Form<T>;
   using H8 = typename F::H8;
-  constexpr int NP = F::np, RB = Blocks<T, DP>::rb, KS = DP / 16, DT = DP / 32;
-  constexpr int kTileBytes = NP * 32 * DP * 2;
-  __shared__ uint4 s_x[kTileBytes / 16], s_t[kTileBytes / 16];
-  __shared__ float s_lse[32], s_w[32], s_g[32];
-  __shared__ int s_lab[32];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int v0 = ((int)blockIdx.x * 4 + wave) * (32 * RB);
+  using W = Walk<T, DP>;
+  static constexpr int NP = F::np, RB = W::rb, KS = DP / 16, DT = DP / 32;
   H8 e[RB][KS][NP];
+  f32x16 o[RB][DT];
+  int v0;
+  float c2, unit, lunit;
+
+  // one tile of 32 pixels: the logits, and the probabilities' gradients as operands
+  __device__ __forceinline__ void logits(const uint4 *s_x, const float *s_l, const float *s_w,
+                                         const int *s_lab, const float *s_g, H8 (*q)[2][NP]) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    f32x16 s[RB];
 #pragma unroll
-  for (int b = 0; b < RB; ++b)
+    for (int b = 0; b < RB; ++b) s[b] = (f32x16)(0.f);
+    products<T, DP, KS>(
+        s_x, [](int k, int p) { return p * KS + k; }, [&](int k, int b) { return e[b][k]; },
+        [&](int, int b) -> f32x16 & { return s[b]; });
+    float p[RB][16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x4 l = *(const f32x4 *)(s_l + 8 * i + 4 * half);
+      f32x4 g;
+      if (ROWG) {
+        g = *(const f32x4 *)(s_g + 8 * i + 4 * half);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) l[j] += lunit;
+      }
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float z = __builtin_amdgcn_exp2f(fmaf(s[b][4 * i + j], c2, l[j]));
+          p[b][4 * i + j] = ROWG ? z * g[j] : z;
+        }
+    }
+    if (__any((uint32_t)(s_lab[lane & 31] - v0) < 32u * RB)) {  // pixels labelled with these rows
+      int mine = v0 + (lane & 31);
+      asm volatile("" : "+v"(mine));  // its sums stay in here and out of the loop's registers
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = 8 * (i >> 2) + 4 * half + (i & 3);
+        const int y = s_lab[r] - mine;
+        const float neg = ROWG ? s_w[r] * (s_g[r] * unit) : s_w[r];
+#pragma unroll
+        for (int b = 0; b < RB; ++b) p[b][i] = y == 32 * b ? neg : p[b][i];
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      pack_probs<T>(p[b], q[b][0]);
+      pack_probs<T>(p[b] + 8, q[b][1]);
+    }
+  }
+
+  __device__ __forceinline__ void add(const uint4 *s_t, const H8 (*q)[2][NP]) {
+    products<T, DP, 2 * DT>(
+        s_t, [](int n, int p) { return p * 2 * DT + n; },
+        [&](int n, int b) { return q[b][n / DT]; },
+        [&](int n, int b) -> f32x16 & { return o[b][n % DT]; });
+  }
+
+  __device__ __forceinline__ void stage(const uint4 *s_x, const uint4 *s_t, const uint32_t *s_m) {
+#pragma unroll
+    for (int k = 0; k < W::kt; ++k) {
+      H8 q[RB][2][NP];
+      rows(s_x + k * (W::tile_words / 4), s_m, k, q);
+      add(s_t + k * (W::tile_words / 4), q);
+    }
+  }
+
+  // s_m: the stage's [4][32 kt] exponents, complements, labels and gradients
+  __device__ __forceinline__ void rows(const uint4 *s_x, const uint32_t *s_m, int k,
+                                       H8 (*q)[2][NP]) {
+    constexpr int n = 32 * W::kt;
+    logits(s_x, (const float *)s_m + 32 * k, (const float *)s_m + n + 32 * k,
+           (const int *)s_m + 2 * n + 32 * k, (const float *)s_m + 3 * n + 32 * k, q);
+  }
+};
+
+// a stage's values per pixel: wave w brings array w
+template <int N, bool ROWG>
+__device__ __forceinline__ void fetch_rows(uint32_t *s_m, const Args &a, int64_t r) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint32_t *src = wave == 0   ? (const uint32_t *)a.lse
+                        : wave == 1 ? (const uint32_t *)a.w
+                        : wave == 2 ? (const uint32_t *)a.lab
+                                    : (const uint32_t *)a.grow;
+  if ((ROWG || wave < 3) && lane < N)
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) void *)(src + r + lane),
+        (__attribute__((address_space(3))) void *)(s_m + wave * N), 4, 0, 0);
+}
+
+template <typename T, int DP, bool ROWG>
+__global__ __launch_bounds__(kBlock, (Walk<T, DP>::waves)) void kd_xent_table(Args a) {
+  using F = Form<T>;
+  using W = Walk<T, DP>;
+  using H8 = typename F::H8;
+  constexpr int NP = F::np, RB = W::rb, KS = DP / 16, DT = DP / 32, kBytes = W::stage_bytes;
+  constexpr int kRows = 32 * W::kt;
+  __shared__ uint4 s_x0[kBytes / 16], s_t0[kBytes / 16];
+  __shared__ uint4 s_x1[W::dbl ? kBytes / 16 : 1], s_t1[W::dbl ? kBytes / 16 : 1];
+  __shared__ uint4 s_m0[kRows], s_m1[W::dbl ? kRows : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  TableWalk<T, DP, ROWG> w;
+  w.v0 = ((int)blockIdx.x * 4 + wave) * (32 * RB);
+  w.c2 = a.c2;
+  w.unit = ROWG ? grad_unit(a.gmax) : 1.f;
+  w.lunit = ROWG ? log2f(w.unit) : 0.f;  // a power of two: exact
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
 #pragma unroll
     for (int k = 0; k < KS; ++k)
 #pragma unroll
       for (int p = 0; p < NP; ++p)
-        e[b][k][p] =
-            *(const H8 *)(a.es + ((((int64_t)(v0 >> 5) + b) * NP + p) * KS + k) * 512 + lane * 8);
-  f32x16 o[RB][DT];
+        w.e[b][k][p] =
+            *(const H8 *)(a.es + ((((int64_t)(w.v0 >> 5) + b) * NP + p) * KS + k) * 512 + lane * 8);
 #pragma unroll
-  for (int b = 0; b < RB; ++b)
-#pragma unroll
-    for (int t = 0; t < DT; ++t) o[b][t] = (f32x16)(0.f);
-  const int ntile = (*a.count + 31) / 32;
-  const int t0 = (int)((int64_t)ntile * blockIdx.y / gridDim.y);
-  const int t1 = (int)((int64_t)ntile * (blockIdx.y + 1) / gridDim.y);
-  const float unit = ROWG ? grad_unit(a.gmax) : 1.f;
-  const float top = exp2f(F::shift_table);
-  for (int t = t0; t < t1; ++t) {
-    __syncthreads();
-    stage(s_x, a.xs + (int64_t)t * (kTileBytes / 2), kTileBytes);
-    stage(s_t, a.xt + (int64_t)t * (kTileBytes / 2), kTileBytes);
-    if (threadIdx.x < 32) {
-      const int64_t r = (int64_t)t * 32 + threadIdx.x;
-      s_lse[threadIdx.x] = F::shift_table - a.lse[r];
-      s_w[threadIdx.x] = -a.w[r] * top;
-      s_lab[threadIdx.x] = a.lab[r];
-      if (ROWG) s_g[threadIdx.x] = a.grow[r] * unit;
+    for (int t = 0; t < DT; ++t) w.o[b][t] = (f32x16)(0.f);
+  }
+  constexpr int kStep2 = 2;
+  const int nst = (int)(((int64_t)*a.count + kStep2 * kRows - 1) / (kStep2 * kRows));
+  const int t0 = (int)((int64_t)nst * blockIdx.y / gridDim.y) * kStep2;
+  const int t1 = (int)((int64_t)nst * (blockIdx.y + 1) / gridDim.y) * kStep2;
+  const uint16_t *xs = a.xs, *xt = a.xt;
+  constexpr int64_t kStep = kBytes / 2;
+  uint32_t *m0 = (uint32_t *)s_m0, *m1 = (uint32_t *)s_m1;
+  if constexpr (W::dbl) {
+    if (t0 < t1) {
+      fetch<kBytes>(s_x0, xs + t0 * kStep);
+      fetch<kBytes>(s_t0, xt + t0 * kStep);
+      fetch_rows<kRows, ROWG>(m0, a, (int64_t)t0 * kRows);
     }
-    __syncthreads();
-    const int y = s_lab[lane & 31];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      f32x16 s = (f32x16)(0.f);
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        H8 x[NP];
-#pragma unroll
-        for (int p = 0; p < NP; ++p) x[p] = *(const H8 *)&s_x[(p * KS + k) * 64 + lane];
-        s = mfma_planes<NP>(x, e[b][k], s);
+    arrive();
+    for (int t = t0; t < t1; t += 2) {
+      fetch<kBytes>(s_x1, xs + (t + 1) * kStep);
+      fetch<kBytes>(s_t1, xt + (t + 1) * kStep);
+      fetch_rows<kRows, ROWG>(m1, a, (int64_t)(t + 1) * kRows);
+      w.stage(s_x0, s_t0, m0);
+      arrive();
+      if (t + 2 < t1) {
+        fetch<kBytes>(s_x0, xs + (t + 2) * kStep);
+        fetch<kBytes>(s_t0, xt + (t + 2) * kStep);
+        fetch_rows<kRows, ROWG>(m0, a, (int64_t)(t + 2) * kRows);
       }
-      float p[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int r = 8 * (i >> 2) + 4 * half + (i & 3);
-        p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c2, s_lse[r]));
+      w.stage(s_x1, s_t1, m1);
+      arrive();
+    }
+  } else {
+    if (t0 < t1) {
+      fetch<kBytes>(s_x0, xs + t0 * kStep);
+      fetch_rows<kRows, ROWG>(m0, a, (int64_t)t0 * kRows);
+    }
+    arrive();
+    for (int t = t0; t < t1; ++t) {
+      H8 q[RB][2][NP];
+      fetch<kBytes>(s_t0, xt + t * kStep);
+      w.rows(s_x0, m0, 0, q);
+      arrive();
+      if (t + 1 < t1) {
+        fetch<kBytes>(s_x0, xs + (t + 1) * kStep);
+        fetch_rows<kRows, ROWG>(m0, a, (int64_t)(t + 1) * kRows);
       }
-      const int vb = v0 + 32 * b;
-      if (__any((uint32_t)(y - vb) < 32u)) {  // pixels labelled with one of these rows
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int r = 8 * (i >> 2) + 4 * half + (i & 3);
-          if (s_lab[r] == vb + (lane & 31)) p[i] = s_w[r];
-        }
-      }
-      if (ROWG) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) p[i] *= s_g[8 * (i >> 2) + 4 * half + (i & 3)];
-      }
-      H8 q[NP][2];
-      pack_probs<T>(p, q);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        H8 pb[NP];
-#pragma unroll
-        for (int pl = 0; pl < NP; ++pl) pb[pl] = q[pl][h];
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          H8 xt[NP];
-#pragma unroll
-          for (int pl = 0; pl < NP; ++pl)
-            xt[pl] = *(const H8 *)&s_t[((pl * 2 + h) * DT + d) * 64 + lane];
-          o[b][d] = mfma_planes<NP>(xt, pb, o[b][d]);
-        }
-      }
+      w.add(s_t0, q);
+      arrive();
     }
   }
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
-    const int64_t v = (int64_t)blockIdx.y * a.vpad + v0 + 32 * b + (lane & 31);
+    const int64_t v = (int64_t)blockIdx.y * a.vpad + w.v0 + 32 * b + (lane & 31);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         f32x4 c;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c[j] = o[b][d][4 * i + j];
+        for (int j = 0; j < 4; ++j) c[j] = w.o[b][d][4 * i + j];
         *(f32x4 *)(a.pe + v * DP + 32 * d + 8 * i + 4 * half) = c;
       }
   }
@@ -738,7 +1009,8 @@ inline Args shape(int64_t n, int64_t V, int D, int np, double scale, int reducti
   a.D = D;
   a.dp = padded_channels(D);
   a.scale = (float)scale;
-  a.c2 = (float)(fabs(scale) * 1.4426950408889634);
+  // never 0: a masked logit, -inf, stays -inf (a scale of 0 makes every logit next to 0 all the same)
+  a.c2 = (float)std::max(fabs(scale) * 1.4426950408889634, 1e-30);
   a.reduction = reduction;
   a.rsplit = parts(n, held_rows(np, a.dp), V);
   a.tsplit = parts(V, held_rows(np, a.dp), n);
@@ -749,10 +1021,12 @@ inline size_t lay_state(Args &a, int np, bool need_x, bool need_e, void *base) {
   Space s{(char *)base, 0};
   const size_t xe = (size_t)a.npad * a.dp * np, ee = (size_t)a.vpad * a.dp * np;
   a.count = s.take<int>(64);
+  a.emax = s.take<uint32_t>(64);
   a.rowid = s.take<int>(a.npad);
   a.lab = s.take<int>(a.npad);
   a.lse = s.take<float>(a.npad);
   a.w = s.take<float>(a.npad);
+  a.xn = s.take<float>(a.npad);
   a.xs = s.take<uint16_t>(xe);
   a.xt = need_e ? s.take<uint16_t>(xe) : nullptr;
   a.es = s.take<uint16_t>(ee);
@@ -798,7 +1072,7 @@ void launch_forward(const Args &a, bool need_x, const T *features, const T *tabl
   const int xtiles = (int)(a.npad / 32), etiles = a.vpad / 32;
   hipLaunchKernelGGL((kd_xent_pack<T, DP>), dim3((unsigned)(xtiles + etiles)), dim3(kBlock), 0,
                      stream, a, xtiles, features, table);
-  constexpr int rows = Blocks<T, DP>::rows;
+  constexpr int rows = Walk<T, DP>::rows;
   const dim3 grid((unsigned)((a.n + rows - 1) / rows), (unsigned)a.rsplit);
   if (need_x)
     hipLaunchKernelGGL((kd_xent_rows<T, DP, true>), grid, dim3(kBlock), 0, stream, a);
@@ -808,7 +1082,7 @@ void launch_forward(const Args &a, bool need_x, const T *features, const T *tabl
 
 template <typename T, int DP>
 void launch_table(const Args &a, hipStream_t stream) {
-  constexpr int rows = Blocks<T, DP>::rows;
+  constexpr int rows = Walk<T, DP>::rows;
   const dim3 grid((unsigned)((a.V + rows - 1) / rows), (unsigned)a.tsplit);
   if (a.reduction == 0)
     hipLaunchKernelGGL((kd_xent_table<T, DP, true>), grid, dim3(kBlock), 0, stream, a);
@@ -839,7 +1113,8 @@ int forward(int64_t n, int64_t V, int D, const T *features, const T *table, cons
   const int nblk = (int)((n + kMapChunk - 1) / kMapChunk);
   if (nblk > 0)
     hipLaunchKernelGGL(kd_xent_count, dim3(nblk), dim3(kBlock), 0, stream, n, V, labels, a.blk);
-  hipLaunchKernelGGL(kd_xent_scan, dim3(1), dim3(kBlock), 0, stream, nblk, a.blk, a.count);
+  hipLaunchKernelGGL(kd_xent_scan, dim3(1), dim3(kBlock), 0, stream, nblk, a.blk, a.count,
+                     a.emax);
   if (n > 0) {
     hipLaunchKernelGGL(kd_xent_map, dim3(nblk), dim3(kBlock), 0, stream, n, V, labels, a.blk,
                        a.rowid, a.lab);
