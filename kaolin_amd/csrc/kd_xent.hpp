@@ -357,6 +357,17 @@ struct Walk {
   static constexpr int stage_bytes = kt * tile_words * 4;  // a multiple of 1024
 };
 
+// The waves that share a SIMD take different priorities (by their slot): waves of the same priority
+// fall into step, all in their products and then all in their exponentials, and leave one of the two
+// pipes idle; with one ahead the other fills the pipe that it leaves free.
+__device__ __forceinline__ void stagger() {
+  const uint32_t slot = __builtin_amdgcn_s_getreg(4 | (3 << 11));  // the wave's slot in its SIMD
+  if (slot & 1)
+    __builtin_amdgcn_s_setprio(1);
+  else
+    __builtin_amdgcn_s_setprio(0);
+}
+
 // acc[b] += A_n . B[n][b] over N operands A_n that are read from LDS, G at a time and one group ahead
 // of the products; the fences keep the compiler from reading more ahead than registers hold.
 // at(n) is operand n's offset, B(n, b) and C(n, b) give the other operand and the sum.
@@ -536,6 +547,7 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP>::waves)) void kd_xent_rows(Arg
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int64_t row0 = ((int64_t)blockIdx.x * 4 + wave) * (32 * RB);
   if ((int64_t)blockIdx.x * W::rows >= *a.count) return;
+  stagger();
   RowsWalk<T, DP, SUM> w;
   w.V = a.V;
   w.c2 = a.c2;
@@ -856,6 +868,7 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP>::waves)) void kd_xent_table(Ar
   __shared__ uint4 s_x1[W::dbl ? kBytes / 16 : 1], s_t1[W::dbl ? kBytes / 16 : 1];
   __shared__ uint4 s_m0[kRows], s_m1[W::dbl ? kRows : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  stagger();
   TableWalk<T, DP, ROWG> w;
   w.v0 = ((int)blockIdx.x * 4 + wave) * (32 * RB);
   w.c2 = a.c2;
