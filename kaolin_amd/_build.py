@@ -44,6 +44,12 @@ FLAGS = ['-O3', '-std=c++17', '-fPIC', '-ffp-contract=off', f'--offload-arch={AR
 # 18.7-19.2 us at C3 and leaves the scan / scatter unchanged; on the tile kernels it changes
 # nothing (kd_dibr_fwd_tiles) or loses (kd_dibr_bwd +2.7 us)
 SOURCE_FLAGS = {'kd_binning.hip': ['-mllvm', '-amdgpu-sched-strategy=max-ilp']}
+# matrix products accumulate in ordinary registers, also where a kernel has more than 256: the
+# logits go straight to vector instructions, which cannot read the accumulation registers; and the
+# step of the widest split operands (192 products) is unrolled whole
+SOURCE_FLAGS.update({f'kd_xent_{t}.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form=1',
+                                          '-mllvm', '-pragma-unroll-threshold=131072']
+                     for t in ('f32', 'f16', 'bf16')})
 
 
 def _stale(target, deps):

@@ -290,17 +290,15 @@ __global__ __launch_bounds__(kBlock) void kd_xent_pack(Args a, int xtiles,
 // ------------------------------------------------------------------------------------------------
 // shared pieces of the two walks
 // ------------------------------------------------------------------------------------------------
-// acc += a . b over the planes' products, the small ones first
+// acc += the i-th of the planes' products of a . b, the small ones first
 template <int NP, typename H8>
-__device__ __forceinline__ f32x16 mfma_planes(const H8 *a, const H8 *b, f32x16 c) {
-  if constexpr (NP == 3) {
-    c = mfma(a[0], b[2], c);
-    c = mfma(a[2], b[0], c);
-    c = mfma(a[1], b[1], c);
-    c = mfma(a[0], b[1], c);
-    c = mfma(a[1], b[0], c);
+__device__ __forceinline__ f32x16 product(int i, const H8 *a, const H8 *b, f32x16 c) {
+  if constexpr (NP == 1) {
+    return mfma(a[0], b[0], c);
+  } else {
+    constexpr int ka[6] = {0, 2, 1, 0, 1, 0}, kb[6] = {2, 0, 1, 1, 0, 0};
+    return mfma(a[ka[i]], b[kb[i]], c);
   }
-  return mfma(a[0], b[0], c);
 }
 
 // the upper halves of two words as one
@@ -308,53 +306,48 @@ __device__ __forceinline__ uint32_t upper2(uint32_t lo, uint32_t hi) {
   return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
 }
 
-// 8 probabilities of a lane as a B operand of the next product
+// Two probabilities of a lane as elements 2 i and 2 i + 1 of an operand (its words, plane by plane).
 template <typename T>
-__device__ __forceinline__ void pack_probs(const float *p, typename Form<T>::H8 *o) {
+__device__ __forceinline__ void pack_pair(float p0, float p1, int i, uint4 *o) {
   using H = typename Form<T>::H;
-  using H8 = typename Form<T>::H8;
   if constexpr (Form<T>::np == 1) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[0][j] = (H)p[j];
+    typedef H h2 __attribute__((ext_vector_type(2)));
+    h2 v;
+    v[0] = (H)p0;
+    v[1] = (H)p1;
+    ((uint32_t *)o)[i] = __builtin_bit_cast(uint32_t, v);
   } else {
-    uint4 q[3];
-    uint32_t *w = (uint32_t *)q;
+    uint32_t u[3][2];
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      uint32_t u[3][2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t a = __float_as_uint(p[j + k]);
-        const float r = p[j + k] - __uint_as_float(a & 0xffff0000u);
-        const uint32_t b = __float_as_uint(r);
-        u[0][k] = a;
-        u[1][k] = b;
-        u[2][k] = __float_as_uint(r - __uint_as_float(b & 0xffff0000u));
-      }
-#pragma unroll
-      for (int k = 0; k < 3; ++k) w[4 * k + j / 2] = upper2(u[k][0], u[k][1]);
+    for (int k = 0; k < 2; ++k) {
+      const float p = k ? p1 : p0;
+      const uint32_t a = __float_as_uint(p);
+      const float r = p - __uint_as_float(a & 0xffff0000u);
+      const uint32_t b = __float_as_uint(r);
+      u[0][k] = a;
+      u[1][k] = b;
+      u[2][k] = __float_as_uint(r - __uint_as_float(b & 0xffff0000u));
     }
 #pragma unroll
-    for (int k = 0; k < 3; ++k) o[k] = __builtin_bit_cast(H8, q[k]);
+    for (int k = 0; k < 3; ++k) ((uint32_t *)&o[k])[i] = upper2(u[k][0], u[k][1]);
   }
 }
 
-// How a walk is laid out.  rb: blocks of 32 rows that a wave holds; two double the products per
-// operand read from LDS, the registers of wide or split operands allow one.  kt: tiles of 32 rows
-// per stage in LDS.  dbl: two buffers a side, loads one stage ahead and one barrier a stage; else
-// one buffer a side and the loads one phase ahead (the straight operands arrive while the second
-// product runs and the other way round), which halves the LDS of the widest split operands.
-template <typename T, int DP>
+// How a walk is laid out (KIND 0: over the table, loss only; 1: over the table with dX; 2: over the
+// pixels, dE).  rb: blocks of 32 rows that a wave holds; two double the products per operand read from
+// LDS, the registers of wide or split operands allow one.  waves: per SIMD, at least; one where the
+// held operands, the sums and two blocks of logits need more than 256 registers.  cs: into how many
+// column ranges the sums are cut, over workgroups that each form the logits: two where the operands
+// of all columns would not fit LDS twice.
+template <typename T, int DP, int KIND>
 struct Walk {
   static constexpr int np = Form<T>::np;
-  static constexpr int rb = np == 1 && DP <= 128 ? 2 : 1;
-  static constexpr int kt = np == 1 && DP <= 64 ? 2 : 1;
-  static constexpr bool dbl = np == 1 || DP <= 64;
-  static constexpr int ahead = np == 3 ? 1 : DP == 128 ? 2 : 2;  // operands read ahead
-  static constexpr int rows = 4 * 32 * rb;                 // held by a workgroup
-  static constexpr int waves = np == 3 && DP == 256 ? 1 : 2;  // per SIMD, at least
-  static constexpr int tile_words = np * 32 * DP / 2;      // 4-byte words of a tile's operands
-  static constexpr int stage_bytes = kt * tile_words * 4;  // a multiple of 1024
+  static constexpr int rb = np == 1 && (DP <= 64 || (DP == 128 && KIND == 0)) ? 2 : 1;
+  static constexpr int waves = (np == 1 ? DP == 256 && KIND > 0 : DP >= (KIND > 0 ? 128 : 256)) ? 1 : 2;
+  static constexpr int cs = np == 3 && DP == 256 && KIND > 0 ? 2 : 1;
+  static constexpr int rows = 4 * 32 * rb;             // held by a workgroup
+  static constexpr int tile_bytes = np * 32 * DP * 2;  // a tile's operands: a multiple of 1024
+  static constexpr int sum_bytes = tile_bytes / cs;    // of the weighted sum
 };
 
 // The waves that share a SIMD take different priorities (by their slot): waves of the same priority
@@ -366,39 +359,6 @@ __device__ __forceinline__ void stagger() {
     __builtin_amdgcn_s_setprio(1);
   else
     __builtin_amdgcn_s_setprio(0);
-}
-
-// acc[b] += A_n . B[n][b] over N operands A_n that are read from LDS, G at a time and one group ahead
-// of the products; the fences keep the compiler from reading more ahead than registers hold.
-// at(n) is operand n's offset, B(n, b) and C(n, b) give the other operand and the sum.
-template <typename T, int DP, int N, typename At, typename B, typename C>
-__device__ __forceinline__ void products(const uint4 *s, At at, B other, C sum) {
-  using H8 = typename Form<T>::H8;
-  constexpr int NP = Form<T>::np, RB = Walk<T, DP>::rb, G = Walk<T, DP>::ahead;
-  static_assert(N % G == 0, "whole groups");
-  const int lane = threadIdx.x & 63;
-  H8 a[2][G][NP];
-#pragma unroll
-  for (int g = -1; g < N / G; ++g) {
-    if (g + 1 < N / G) {
-#pragma unroll
-      for (int j = 0; j < G; ++j)
-#pragma unroll
-        for (int p = 0; p < NP; ++p)
-          a[(g + 1) & 1][j][p] = *(const H8 *)&s[at((g + 1) * G + j, p) * 64 + lane];
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    if (g >= 0) {
-#pragma unroll
-      for (int j = 0; j < G; ++j)
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
-          f32x16 &c = sum(g * G + j, b);
-          c = mfma_planes<NP>(a[g & 1][j], other(g * G + j, b), c);
-        }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
 }
 
 // Copies `bytes` from global memory to LDS without registers: 1 KB a wave and instruction, waited
@@ -417,10 +377,166 @@ __device__ __forceinline__ void fetch(uint4 *dst, const uint16_t *src) {
   }
 }
 
+// The transposed operands of a tile for the column range z (see Walk::cs).
+template <typename W>
+__device__ __forceinline__ void fetch_sum(uint4 *dst, const uint16_t *src, int z) {
+  if constexpr (W::cs == 1) {
+    fetch<W::sum_bytes>(dst, src);
+  } else {
+    constexpr int kBlocks = 2 * W::np, kPart = W::sum_bytes / kBlocks;  // per plane and row half
+#pragma unroll
+    for (int k = 0; k < kBlocks; ++k)
+      fetch<kPart>(dst + k * (kPart / 16), src + (k * W::cs + z) * (kPart / 2));
+  }
+}
+
 __device__ __forceinline__ void arrive() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
 }
+
+// One step of a walk: the matrix pipe's work on the tiles i - 1 (weighted sum) and i + 1 (logits), and
+// the vector pipe's on tile i (exponentials) in the products' shadow, so that a wave keeps both pipes
+// busy by itself.  s holds the logits of tile i and then of i + 1, q the operands of i - 1 and then
+// of i.
+template <typename T, int DP, int KIND>
+struct Step {
+  using F = Form<T>;
+  using H8 = typename F::H8;
+  using W = Walk<T, DP, KIND>;
+  static constexpr bool SUM = KIND > 0;
+  static constexpr int NP = F::np, RB = W::rb, KS = DP / 16, DT = DP / 32 / W::cs;
+  H8 held[RB][KS][NP];
+  f32x16 s[RB];
+  f32x16 o[SUM ? RB : 1][SUM ? DT : 1];
+  uint4 q[RB][2][NP];
+
+  __device__ __forceinline__ void hold(const uint16_t *packed, int64_t row0) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          held[b][k][p] =
+              *(const H8 *)(packed + ((((row0 >> 5) + b) * NP + p) * KS + k) * 512 + lane * 8);
+      if constexpr (SUM) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[b][t] = (f32x16)(0.f);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) q[b][h][p] = make_uint4(0, 0, 0, 0);
+    }
+  }
+
+  // The products of a step, one after the other, with between(i) behind the i-th: the weighted sum's
+  // (if ADD) and the logits' (if LOGITS).  Operands are read from LDS a few products ahead; the fences
+  // keep the compiler from gathering the products and the vector work apart.
+  template <bool ADD, bool LOGITS, typename Between>
+  __device__ __forceinline__ void products(const uint4 *straight, const uint4 *transposed,
+                                           f32x16 *next, Between between) {
+    constexpr int kAdd = ADD ? 2 * DT : 0, kOps = kAdd + (LOGITS ? KS : 0);
+    constexpr int kAhead = NP == 3 ? 2 : RB == 2 ? 3 : 5, kTimes = NP == 3 ? 6 : 1;
+    const int lane = threadIdx.x & 63;
+    H8 a[kOps][NP];
+    auto load = [&](int n) {
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+        a[n][p] = n < kAdd ? *(const H8 *)&transposed[(p * 2 * DT + n) * 64 + lane]
+                           : *(const H8 *)&straight[(p * KS + n - kAdd) * 64 + lane];
+    };
+#pragma unroll
+    for (int n = 0; n < (kAhead < kOps ? kAhead : kOps); ++n) load(n);
+    between(0);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (LOGITS) {
+#pragma unroll
+      for (int b = 0; b < RB; ++b) next[b] = (f32x16)(0.f);
+    }
+    int done = 1;
+#pragma unroll
+    for (int n = 0; n < kOps; ++n) {
+      if (n + kAhead < kOps) load(n + kAhead);
+#pragma unroll
+      for (int i = 0; i < kTimes; ++i)
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+          if (n < kAdd) {
+            H8 w[NP];
+#pragma unroll
+            for (int p = 0; p < NP; ++p) w[p] = __builtin_bit_cast(H8, q[b][n / DT][p]);
+            o[b][n % DT] = product<NP>(i, a[n], w, o[b][n % DT]);
+          } else {
+            next[b] = product<NP>(i, a[n], held[b][n - kAdd], next[b]);
+          }
+          between(done++);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+  }
+
+  __device__ __forceinline__ void logits(const uint4 *straight) {
+    products<false, true>(straight, straight, s, [](int) {});
+  }
+
+  __device__ __forceinline__ void add(const uint4 *transposed) {
+    products<true, false>(transposed, transposed, s, [](int) {});
+  }
+
+  // pair(b, i, z0, z1): the probabilities 2 i and 2 i + 1 of block b in place of their logits
+  template <typename Pair>
+  __device__ __forceinline__ void step(const uint4 *straight, const uint4 *transposed, Pair pair) {
+    constexpr int kSlots = (NP == 3 ? 6 : 1) * RB * (KS + (SUM ? 2 * DT : 0)) + 1;
+    constexpr int kPairs = RB * 8;
+    f32x16 next[RB];
+    uint4 fresh[RB][2][NP];
+    products<SUM, true>(straight, transposed, next, [&](int slot) {
+#pragma unroll
+      for (int k = slot * kPairs / kSlots; k < (slot + 1) * kPairs / kSlots; ++k) {
+        const int b = k / 8, i = k % 8;
+        float p0 = s[b][2 * i], p1 = s[b][2 * i + 1];
+        pair(b, i, p0, p1);
+        if constexpr (SUM) {
+          pack_pair<T>(p0, p1, i & 3, fresh[b][i >> 2]);
+          // (stays in its slot: the compiler would move it behind the products)
+#pragma unroll
+          for (int p = 0; p < NP; ++p)
+            asm volatile("" : "+v"(((uint32_t *)&fresh[b][i >> 2][p])[i & 3]));
+        }
+      }
+    });
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      s[b] = next[b];
+      if constexpr (SUM) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int p = 0; p < NP; ++p) q[b][h][p] = fresh[b][h][p];
+      }
+    }
+  }
+
+  // the sums, lane = held row, to [row][DP] from column c0 on
+  __device__ __forceinline__ void store(float *out, int64_t row0, int c0) const {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f32x4 v;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = o[b][d][4 * i + j];
+          *(f32x4 *)(out + (row0 + 32 * b + (lane & 31)) * DP + c0 + 32 * d + 8 * i + 4 * half) =
+              v;
+        }
+  }
+};
 
 // ------------------------------------------------------------------------------------------------
 // the walk over the table
@@ -430,36 +546,23 @@ __device__ __forceinline__ void arrive() {
 constexpr float kSafeLogit = 60.f;
 
 template <typename T, int DP, bool SUM>
-struct RowsWalk {
+struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
+  using B = Step<T, DP, SUM ? 1 : 0>;
   using F = Form<T>;
   using H8 = typename F::H8;
-  using W = Walk<T, DP>;
-  static constexpr int NP = F::np, RB = W::rb, KS = DP / 16, DT = DP / 32;
-  H8 x[RB][KS][NP];
+  static constexpr int NP = B::NP, RB = B::RB, DT = B::DT;
   int lab[RB];
-  f32x16 o[SUM ? RB : 1][SUM ? DT : 1];
-  float m[RB], l[RB];
-  bool online;
+  float m[RB], l[RB][2];
   int V;
   float c2;
 
-  // one tile of 32 table rows: the logits, and the probabilities as operands
-  template <bool ONLINE>
-  __device__ __forceinline__ void logits(const uint4 *s_e, int v0, H8 (*q)[2][NP]) {
-    const int half = (threadIdx.x & 63) >> 5;
-    f32x16 s[RB];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) s[b] = (f32x16)(0.f);
-    products<T, DP, KS>(
-        s_e, [](int k, int p) { return p * KS + k; }, [&](int k, int b) { return x[b][k]; },
-        [&](int, int b) -> f32x16 & { return s[b]; });
-    // the label's own column and the table's padding take no part
+  // the label's own column and the table's padding take no part
+  __device__ __forceinline__ void mask(int v0) {
     bool near = false;
 #pragma unroll
     for (int b = 0; b < RB; ++b) near |= (uint32_t)(lab[b] - v0) < 32u;
-    const bool hit = v0 + 32 > V || __any(near);
-    if (hit) {
-      int first = 4 * half;
+    if (v0 + 32 > V || __any(near)) {
+      int first = 4 * ((threadIdx.x & 63) >> 5);
       asm volatile("" : "+v"(first));  // its sums stay in here and out of the loop's registers
       first += v0;
 #pragma unroll
@@ -467,83 +570,79 @@ struct RowsWalk {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int v = first + 8 * (i >> 2) + (i & 3);
-          s[b][i] = v == lab[b] || v >= V ? -INFINITY : s[b][i];
+          this->s[b][i] = v == lab[b] || v >= V ? -INFINITY : this->s[b][i];
         }
-    }
-    if constexpr (ONLINE) {
-      float top[RB];
-      bool up = false;
-#pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        top[b] = fmaxf(s[b][0], s[b][1]);
-#pragma unroll
-        for (int i = 2; i < 16; i += 2) top[b] = fmaxf(fmaxf(top[b], s[b][i]), s[b][i + 1]);
-        top[b] *= c2;
-        up |= top[b] > m[b] + F::slack;
-      }
-      if (__any(up)) {  // a maximum moves: rarely after the first tiles
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
-          const float mn = fmaxf(m[b], fmaxf(top[b], __shfl_xor(top[b], 32)));
-          const float f = __builtin_amdgcn_exp2f(m[b] - mn);
-          m[b] = mn;
-          l[b] *= f;
-          if constexpr (SUM) {
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[b][d][i] *= f;
-          }
-        }
-      }
-    }
-    float p[RB][16];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      const float shift = ONLINE ? F::shift - m[b] : 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        p[b][i] = __builtin_amdgcn_exp2f(ONLINE ? fmaf(s[b][i], c2, shift) : s[b][i] * c2);
-    }
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      float t[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 16; ++i) t[i & 3] += p[b][i];
-      l[b] += (t[0] + t[1]) + (t[2] + t[3]);
-      if constexpr (SUM) {
-        pack_probs<T>(p[b], q[b][0]);
-        pack_probs<T>(p[b] + 8, q[b][1]);
-      }
     }
   }
 
-  __device__ __forceinline__ void add(const uint4 *s_t, const H8 (*q)[2][NP]) {
-    products<T, DP, 2 * DT>(
-        s_t, [](int n, int p) { return p * 2 * DT + n; },
-        [&](int n, int b) { return q[b][n / DT]; },
-        [&](int n, int b) -> f32x16 & { return o[b][n % DT]; });
+  // the running maximum over the new logits: a power of two apart from the last one, so that what is
+  // summed up already (q too) changes exactly
+  __device__ __forceinline__ void raise() {
+    float top[RB];
+    bool up = false;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      top[b] = fmaxf(this->s[b][0], this->s[b][1]);
+#pragma unroll
+      for (int i = 2; i < 16; i += 2)
+        top[b] = fmaxf(fmaxf(top[b], this->s[b][i]), this->s[b][i + 1]);
+      top[b] *= c2;
+      up |= top[b] > m[b] + F::slack;
+    }
+    if (__any(up)) {  // rarely after the first tiles
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        const float mn = fmaxf(m[b], ceilf(fmaxf(top[b], __shfl_xor(top[b], 32))));
+        const float f = __builtin_amdgcn_exp2f(m[b] - mn);
+        m[b] = mn;
+        l[b][0] *= f;
+        l[b][1] *= f;
+        if constexpr (SUM) {
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) this->o[b][d][i] *= f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                typename F::H *e = (typename F::H *)&this->q[b][h][p] + j;
+                *e = (typename F::H)((float)*e * f);
+              }
+        }
+      }
+    }
   }
 
   template <bool ONLINE>
-  __device__ __forceinline__ void stage(const uint4 *s_e, const uint4 *s_t, int v0) {
-#pragma unroll
-    for (int k = 0; k < W::kt; ++k) {
-      H8 q[RB][2][NP];
-      logits<ONLINE>(s_e + k * (W::tile_words / 4), v0 + 32 * k, q);
-      if constexpr (SUM) add(s_t + k * (W::tile_words / 4), q);
-    }
+  __device__ __forceinline__ void ready(int v0) {
+    mask(v0);
+    if constexpr (ONLINE) raise();
+  }
+
+  template <bool ONLINE>
+  __device__ __forceinline__ void next(const uint4 *s_e, const uint4 *s_t) {
+    B::step(s_e, s_t, [&](int b, int, float &p0, float &p1) {
+      const float shift = ONLINE ? F::shift - m[b] : 0.f;
+      p0 = __builtin_amdgcn_exp2f(ONLINE ? fmaf(p0, c2, shift) : p0 * c2);
+      p1 = __builtin_amdgcn_exp2f(ONLINE ? fmaf(p1, c2, shift) : p1 * c2);
+      l[b][0] += p0;
+      l[b][1] += p1;
+      asm volatile("" : "+v"(l[b][0]), "+v"(l[b][1]));  // (stays in its slot)
+    });
   }
 };
 
 template <typename T, int DP, bool SUM>
-__global__ __launch_bounds__(kBlock, (Walk<T, DP>::waves)) void kd_xent_rows(Args a) {
+__global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_xent_rows(Args a) {
   using F = Form<T>;
-  using W = Walk<T, DP>;
-  using H8 = typename F::H8;
-  constexpr int NP = F::np, RB = W::rb, KS = DP / 16, DT = DP / 32, kBytes = W::stage_bytes;
-  __shared__ uint4 s_e0[kBytes / 16], s_t0[SUM ? kBytes / 16 : 1];
-  __shared__ uint4 s_e1[W::dbl || !SUM ? kBytes / 16 : 1], s_t1[SUM && W::dbl ? kBytes / 16 : 1];
+  using W = Walk<T, DP, SUM ? 1 : 0>;
+  constexpr int RB = W::rb, kBytes = W::tile_bytes;
+  __shared__ uint4 s_e0[kBytes / 16], s_e1[kBytes / 16];
+  __shared__ uint4 s_t0[SUM ? W::sum_bytes / 16 : 1], s_t1[SUM ? W::sum_bytes / 16 : 1];
+  const int z = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int64_t row0 = ((int64_t)blockIdx.x * 4 + wave) * (32 * RB);
   if ((int64_t)blockIdx.x * W::rows >= *a.count) return;
@@ -551,96 +650,69 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP>::waves)) void kd_xent_rows(Arg
   RowsWalk<T, DP, SUM> w;
   w.V = a.V;
   w.c2 = a.c2;
-  // |logit| <= |x| |e| scale; a NaN size takes the general way
-  const float emax = __uint_as_float(*a.emax);
+  // |logit| <= |x| |e| scale, over the kRowPad rows about this wave's (so that the choice does not
+  // depend on how many of them a wave holds); a NaN size takes the general way
+  const float size = a.c2 * sqrtf(__uint_as_float(*a.emax));
   bool safe = F::shift == 0.f;
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const int64_t r = row0 + 32 * b + (lane & 31);
-    w.lab[b] = a.lab[r];
-    safe &= a.c2 * sqrtf(a.xn[r]) * sqrtf(emax) < kSafeLogit;
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int p = 0; p < NP; ++p)
-        w.x[b][k][p] =
-            *(const H8 *)(a.xs + ((((row0 >> 5) + b) * NP + p) * KS + k) * 512 + lane * 8);
-  }
-  w.online = !__all(safe);
+  for (int k = 0; k < kRowPad / kWave; ++k)
+    safe &= size * sqrtf(a.xn[row0 / kRowPad * kRowPad + k * kWave + lane]) < kSafeLogit;
+  const bool general = !__all(safe);
+  w.hold(a.xs, row0);
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
-    w.m[b] = w.online ? -1e30f : 0.f;
-    w.l[b] = 0.f;
-    if constexpr (SUM) {
-#pragma unroll
-      for (int t = 0; t < DT; ++t) w.o[b][t] = (f32x16)(0.f);
-    }
+    w.lab[b] = a.lab[row0 + 32 * b + (lane & 31)];
+    w.m[b] = general ? -1e30f : 0.f;
+    w.l[b][0] = w.l[b][1] = 0.f;
   }
-  constexpr int kRows = 32 * W::kt;
-  constexpr int kStep2 = 2;  // stages come in pairs, for the two buffers
-  const int nst = (a.V + kStep2 * kRows - 1) / (kStep2 * kRows);
-  const int t0 = (int)((int64_t)nst * blockIdx.y / gridDim.y) * kStep2;
-  const int t1 = (int)((int64_t)nst * (blockIdx.y + 1) / gridDim.y) * kStep2;
+  // tiles come in pairs, for the two buffers
+  const int npair = (a.V + 63) / 64;
+  const int t0 = (int)((int64_t)npair * blockIdx.y / gridDim.y) * 2;
+  const int t1 = (int)((int64_t)npair * (blockIdx.y + 1) / gridDim.y) * 2;
   const uint16_t *es = a.es, *et = a.et;
-  constexpr int64_t kStep = kBytes / 2;
+  constexpr int64_t kTile = kBytes / 2;
   auto walk = [&](auto online) {
-  constexpr bool ONLINE = decltype(online)::value;
-  if constexpr (W::dbl || !SUM) {
-    if (t0 < t1) {
-      fetch<kBytes>(s_e0, es + t0 * kStep);
-      if constexpr (SUM) fetch<kBytes>(s_t0, et + t0 * kStep);
-    }
+    constexpr bool ONLINE = decltype(online)::value;
+    fetch<kBytes>(s_e0, es + t0 * kTile);
+    arrive();
+    fetch<kBytes>(s_e1, es + (t0 + 1) * kTile);
+    if constexpr (SUM) fetch_sum<W>(s_t1, et + t0 * kTile, z);  // (times zeros)
+    w.logits(s_e0);
+    w.template ready<ONLINE>(t0 * 32);
     arrive();
     for (int t = t0; t < t1; t += 2) {
-      fetch<kBytes>(s_e1, es + (t + 1) * kStep);
-      if constexpr (SUM) fetch<kBytes>(s_t1, et + (t + 1) * kStep);
-      w.template stage<ONLINE>(s_e0, s_t0, t * kRows);
+      const int t2 = min(t + 2, t1 - 1), t3 = min(t + 3, t1 - 1);  // behind the end: not used
+      fetch<kBytes>(s_e0, es + t2 * kTile);
+      if constexpr (SUM) fetch_sum<W>(s_t0, et + t * kTile, z);
+      w.template next<ONLINE>(s_e1, s_t1);
+      w.template ready<ONLINE>((t + 1) * 32);
       arrive();
-      if (t + 2 < t1) {
-        fetch<kBytes>(s_e0, es + (t + 2) * kStep);
-        if constexpr (SUM) fetch<kBytes>(s_t0, et + (t + 2) * kStep);
-      }
-      w.template stage<ONLINE>(s_e1, s_t1, (t + 1) * kRows);
-      arrive();
-    }
-  } else {
-    if (t0 < t1) fetch<kBytes>(s_e0, es + t0 * kStep);
-    arrive();
-    for (int t = t0; t < t1; ++t) {
-      H8 q[RB][2][NP];
-      fetch<kBytes>(s_t0, et + t * kStep);
-      w.template logits<ONLINE>(s_e0, t * kRows, q);
-      arrive();
-      if (t + 1 < t1) fetch<kBytes>(s_e0, es + (t + 1) * kStep);
-      w.add(s_t0, q);
+      fetch<kBytes>(s_e1, es + t3 * kTile);
+      if constexpr (SUM) fetch_sum<W>(s_t1, et + (t + 1) * kTile, z);
+      w.template next<ONLINE>(s_e0, s_t0);
+      w.template ready<ONLINE>(t2 * 32);
       arrive();
     }
-  }
+    if constexpr (SUM) w.add(s_t1);
   };
-  if (w.online)
-    walk(std::true_type{});
-  else
-    walk(std::false_type{});
+  if (t0 < t1) {
+    if (general)
+      walk(std::true_type{});
+    else
+      walk(std::false_type{});
+  }
+  const int64_t part = (int64_t)blockIdx.y * a.npad;
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
-    const int64_t r = (int64_t)blockIdx.y * a.npad + row0 + 32 * b + (lane & 31);
-    const float l = w.l[b] + __shfl_xor(w.l[b], 32);
-    if (half == 0) {
+    const int64_t r = part + row0 + 32 * b + (lane & 31);
+    float l = w.l[b][0] + w.l[b][1];
+    l += __shfl_xor(l, 32);
+    if (half == 0 && z == 0) {
       a.pm[r] = w.m[b] - F::shift;
       a.pl[r] = l;
     }
-    if constexpr (SUM) {
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          f32x4 v;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = w.o[b][d][4 * i + j];
-          *(f32x4 *)(a.po + r * DP + 32 * d + 8 * i + 4 * half) = v;
-        }
-    }
   }
+  if constexpr (SUM) w.store(a.po, part + row0, z * (DP / W::cs));
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -760,191 +832,126 @@ __device__ __forceinline__ float grad_unit(const uint32_t *gmax) {
   return e == 0 || e >= 254 ? 1.f : __uint_as_float((254u - e) << 23);
 }
 
+// The walk over the pixels.  A lane's 16 pixels of a tile are 8 i + 4 (lane / 32) + j: their exponents
+// (and gradients) are read one step ahead.
 template <typename T, int DP, bool ROWG>
-struct TableWalk {
+struct TableWalk : Step<T, DP, 2> {
+  using B = Step<T, DP, 2>;
   using F = Form<T>;
-  using H8 = typename F::H8;
-  using W = Walk<T, DP>;
-  static constexpr int NP = F::np, RB = W::rb, KS = DP / 16, DT = DP / 32;
-  H8 e[RB][KS][NP];
-  f32x16 o[RB][DT];
-  int v0;
+  static constexpr int NP = B::NP, RB = B::RB;
+  int v0, near;  // near: this lane's pixel's label
   float c2, unit, lunit;
+  f32x4 lse[4], g[ROWG ? 4 : 1];
+  const float *plse, *pw, *pg;
+  const int *plab;
 
-  // one tile of 32 pixels: the logits, and the probabilities' gradients as operands
-  __device__ __forceinline__ void logits(const uint4 *s_x, const float *s_l, const float *s_w,
-                                         const int *s_lab, const float *s_g, H8 (*q)[2][NP]) {
-    const int lane = threadIdx.x & 63, half = lane >> 5;
-    f32x16 s[RB];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) s[b] = (f32x16)(0.f);
-    products<T, DP, KS>(
-        s_x, [](int k, int p) { return p * KS + k; }, [&](int k, int b) { return e[b][k]; },
-        [&](int, int b) -> f32x16 & { return s[b]; });
-    float p[RB][16];
+  __device__ __forceinline__ void rows(int t, f32x4 *l, f32x4 *gr, int &y) {
+    const int lane = threadIdx.x & 63;
+    const int64_t r = (int64_t)t * 32;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      f32x4 l = *(const f32x4 *)(s_l + 8 * i + 4 * half);
-      f32x4 g;
+      l[i] = *(const f32x4 *)(plse + r + 8 * i + 4 * (lane >> 5));
+      if (ROWG) gr[i] = *(const f32x4 *)(pg + r + 8 * i + 4 * (lane >> 5));
+    }
+    y = plab[r + (lane & 31)];
+  }
+
+  // tile t is stepped over, t1 the next one's values
+  __device__ __forceinline__ void next(const uint4 *s_x, const uint4 *s_t, int t, int t1) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    f32x4 l1[4], g1[ROWG ? 4 : 1];
+    int near1;
+    rows(t1, l1, g1, near1);
+    B::step(s_x, s_t, [&](int, int i, float &p0, float &p1) {
+      const f32x4 l = lse[i / 2];
+      const int j = 2 * (i & 1);
+      p0 = __builtin_amdgcn_exp2f(fmaf(p0, c2, ROWG ? l[j] + lunit : l[j]));
+      p1 = __builtin_amdgcn_exp2f(fmaf(p1, c2, ROWG ? l[j + 1] + lunit : l[j + 1]));
       if (ROWG) {
-        g = *(const f32x4 *)(s_g + 8 * i + 4 * half);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) l[j] += lunit;
+        p0 *= g[i / 2][j];
+        p1 *= g[i / 2][j + 1];
       }
+    });
+    // pixels labelled with these rows: p - 1 = -(1 - p) in the place of p
+    if (__any((uint32_t)(near - v0) < 32u * RB)) {
+      int64_t r = (int64_t)t * 32 + 4 * half;
+      asm volatile("" : "+v"(r));  // its sums stay in here and out of the loop's registers
 #pragma unroll
-      for (int b = 0; b < RB; ++b)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float z = __builtin_amdgcn_exp2f(fmaf(s[b][4 * i + j], c2, l[j]));
-          p[b][4 * i + j] = ROWG ? z * g[j] : z;
+        for (int j = 0; j < 8; ++j) {
+          const int64_t k = r + 16 * h + 8 * (j >> 2) + (j & 3);
+          const int y = plab[k] - v0 - (lane & 31);
+          const float neg = ROWG ? pw[k] * (pg[k] * unit) : pw[k];
+          uint16_t part[3] = {0, 0, 0};
+          if constexpr (NP == 1)
+            part[0] = __builtin_bit_cast(uint16_t, (typename F::H)neg);
+          else
+            split3(neg, part[0], part[1], part[2]);
+#pragma unroll
+          for (int b = 0; b < RB; ++b)
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+              uint16_t *e = (uint16_t *)&this->q[b][h][p] + j;
+              *e = y == 32 * b ? part[p] : *e;
+            }
         }
     }
-    if (__any((uint32_t)(s_lab[lane & 31] - v0) < 32u * RB)) {  // pixels labelled with these rows
-      int mine = v0 + (lane & 31);
-      asm volatile("" : "+v"(mine));  // its sums stay in here and out of the loop's registers
+    near = near1;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int r = 8 * (i >> 2) + 4 * half + (i & 3);
-        const int y = s_lab[r] - mine;
-        const float neg = ROWG ? s_w[r] * (s_g[r] * unit) : s_w[r];
-#pragma unroll
-        for (int b = 0; b < RB; ++b) p[b][i] = y == 32 * b ? neg : p[b][i];
-      }
+    for (int i = 0; i < 4; ++i) {
+      lse[i] = l1[i];
+      if (ROWG) g[i] = g1[i];
     }
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      pack_probs<T>(p[b], q[b][0]);
-      pack_probs<T>(p[b] + 8, q[b][1]);
-    }
-  }
-
-  __device__ __forceinline__ void add(const uint4 *s_t, const H8 (*q)[2][NP]) {
-    products<T, DP, 2 * DT>(
-        s_t, [](int n, int p) { return p * 2 * DT + n; },
-        [&](int n, int b) { return q[b][n / DT]; },
-        [&](int n, int b) -> f32x16 & { return o[b][n % DT]; });
-  }
-
-  __device__ __forceinline__ void stage(const uint4 *s_x, const uint4 *s_t, const uint32_t *s_m) {
-#pragma unroll
-    for (int k = 0; k < W::kt; ++k) {
-      H8 q[RB][2][NP];
-      rows(s_x + k * (W::tile_words / 4), s_m, k, q);
-      add(s_t + k * (W::tile_words / 4), q);
-    }
-  }
-
-  // s_m: the stage's [4][32 kt] exponents, complements, labels and gradients
-  __device__ __forceinline__ void rows(const uint4 *s_x, const uint32_t *s_m, int k,
-                                       H8 (*q)[2][NP]) {
-    constexpr int n = 32 * W::kt;
-    logits(s_x, (const float *)s_m + 32 * k, (const float *)s_m + n + 32 * k,
-           (const int *)s_m + 2 * n + 32 * k, (const float *)s_m + 3 * n + 32 * k, q);
   }
 };
 
-// a stage's values per pixel: wave w brings array w
-template <int N, bool ROWG>
-__device__ __forceinline__ void fetch_rows(uint32_t *s_m, const Args &a, int64_t r) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const uint32_t *src = wave == 0   ? (const uint32_t *)a.lse
-                        : wave == 1 ? (const uint32_t *)a.w
-                        : wave == 2 ? (const uint32_t *)a.lab
-                                    : (const uint32_t *)a.grow;
-  if ((ROWG || wave < 3) && lane < N)
-    __builtin_amdgcn_global_load_lds(
-        (const __attribute__((address_space(1))) void *)(src + r + lane),
-        (__attribute__((address_space(3))) void *)(s_m + wave * N), 4, 0, 0);
-}
-
 template <typename T, int DP, bool ROWG>
-__global__ __launch_bounds__(kBlock, (Walk<T, DP>::waves)) void kd_xent_table(Args a) {
-  using F = Form<T>;
-  using W = Walk<T, DP>;
-  using H8 = typename F::H8;
-  constexpr int NP = F::np, RB = W::rb, KS = DP / 16, DT = DP / 32, kBytes = W::stage_bytes;
-  constexpr int kRows = 32 * W::kt;
-  __shared__ uint4 s_x0[kBytes / 16], s_t0[kBytes / 16];
-  __shared__ uint4 s_x1[W::dbl ? kBytes / 16 : 1], s_t1[W::dbl ? kBytes / 16 : 1];
-  __shared__ uint4 s_m0[kRows], s_m1[W::dbl ? kRows : 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+__global__ __launch_bounds__(kBlock, (Walk<T, DP, 2>::waves)) void kd_xent_table(Args a) {
+  using W = Walk<T, DP, 2>;
+  constexpr int RB = W::rb, kBytes = W::tile_bytes;
+  __shared__ uint4 s_x0[kBytes / 16], s_x1[kBytes / 16];
+  __shared__ uint4 s_t0[W::sum_bytes / 16], s_t1[W::sum_bytes / 16];
+  const int z = blockIdx.z;
+  const int wave = threadIdx.x >> 6;
   stagger();
   TableWalk<T, DP, ROWG> w;
   w.v0 = ((int)blockIdx.x * 4 + wave) * (32 * RB);
   w.c2 = a.c2;
   w.unit = ROWG ? grad_unit(a.gmax) : 1.f;
   w.lunit = ROWG ? log2f(w.unit) : 0.f;  // a power of two: exact
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int p = 0; p < NP; ++p)
-        w.e[b][k][p] =
-            *(const H8 *)(a.es + ((((int64_t)(w.v0 >> 5) + b) * NP + p) * KS + k) * 512 + lane * 8);
-#pragma unroll
-    for (int t = 0; t < DT; ++t) w.o[b][t] = (f32x16)(0.f);
-  }
-  constexpr int kStep2 = 2;
-  const int nst = (int)(((int64_t)*a.count + kStep2 * kRows - 1) / (kStep2 * kRows));
-  const int t0 = (int)((int64_t)nst * blockIdx.y / gridDim.y) * kStep2;
-  const int t1 = (int)((int64_t)nst * (blockIdx.y + 1) / gridDim.y) * kStep2;
+  w.plse = a.lse;
+  w.pw = a.w;
+  w.pg = a.grow;
+  w.plab = a.lab;
+  w.hold(a.es, w.v0);
+  const int npair = (int)(((int64_t)*a.count + 63) / 64);
+  const int t0 = (int)((int64_t)npair * blockIdx.y / gridDim.y) * 2;
+  const int t1 = (int)((int64_t)npair * (blockIdx.y + 1) / gridDim.y) * 2;
   const uint16_t *xs = a.xs, *xt = a.xt;
-  constexpr int64_t kStep = kBytes / 2;
-  uint32_t *m0 = (uint32_t *)s_m0, *m1 = (uint32_t *)s_m1;
-  if constexpr (W::dbl) {
-    if (t0 < t1) {
-      fetch<kBytes>(s_x0, xs + t0 * kStep);
-      fetch<kBytes>(s_t0, xt + t0 * kStep);
-      fetch_rows<kRows, ROWG>(m0, a, (int64_t)t0 * kRows);
-    }
+  constexpr int64_t kTile = kBytes / 2;
+  if (t0 < t1) {
+    fetch<kBytes>(s_x0, xs + t0 * kTile);
+    w.rows(t0, w.lse, w.g, w.near);
+    arrive();
+    fetch<kBytes>(s_x1, xs + (t0 + 1) * kTile);
+    fetch_sum<W>(s_t1, xt + t0 * kTile, z);  // (times zeros)
+    w.logits(s_x0);
     arrive();
     for (int t = t0; t < t1; t += 2) {
-      fetch<kBytes>(s_x1, xs + (t + 1) * kStep);
-      fetch<kBytes>(s_t1, xt + (t + 1) * kStep);
-      fetch_rows<kRows, ROWG>(m1, a, (int64_t)(t + 1) * kRows);
-      w.stage(s_x0, s_t0, m0);
+      const int t2 = min(t + 2, t1 - 1), t3 = min(t + 3, t1 - 1);  // behind the end: not used
+      fetch<kBytes>(s_x0, xs + t2 * kTile);
+      fetch_sum<W>(s_t0, xt + t * kTile, z);
+      w.next(s_x1, s_t1, t, t + 1);
       arrive();
-      if (t + 2 < t1) {
-        fetch<kBytes>(s_x0, xs + (t + 2) * kStep);
-        fetch<kBytes>(s_t0, xt + (t + 2) * kStep);
-        fetch_rows<kRows, ROWG>(m0, a, (int64_t)(t + 2) * kRows);
-      }
-      w.stage(s_x1, s_t1, m1);
+      fetch<kBytes>(s_x1, xs + t3 * kTile);
+      fetch_sum<W>(s_t1, xt + (t + 1) * kTile, z);
+      w.next(s_x0, s_t0, t + 1, t2);
       arrive();
     }
-  } else {
-    if (t0 < t1) {
-      fetch<kBytes>(s_x0, xs + t0 * kStep);
-      fetch_rows<kRows, ROWG>(m0, a, (int64_t)t0 * kRows);
-    }
-    arrive();
-    for (int t = t0; t < t1; ++t) {
-      H8 q[RB][2][NP];
-      fetch<kBytes>(s_t0, xt + t * kStep);
-      w.rows(s_x0, m0, 0, q);
-      arrive();
-      if (t + 1 < t1) {
-        fetch<kBytes>(s_x0, xs + (t + 1) * kStep);
-        fetch_rows<kRows, ROWG>(m0, a, (int64_t)(t + 1) * kRows);
-      }
-      w.add(s_t0, q);
-      arrive();
-    }
+    w.add(s_t1);
   }
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const int64_t v = (int64_t)blockIdx.y * a.vpad + w.v0 + 32 * b + (lane & 31);
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f32x4 c;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c[j] = w.o[b][d][4 * i + j];
-        *(f32x4 *)(a.pe + v * DP + 32 * d + 8 * i + 4 * half) = c;
-      }
-  }
+  w.store(a.pe, (int64_t)blockIdx.y * a.vpad + w.v0, z * (DP / W::cs));
 }
 
 // The gradient's common factor: the incoming scalar, over the count for the mean.
@@ -1005,7 +1012,7 @@ struct Space {
 
 // rows a workgroup holds, and into how many parts the other matrix is cut so that the grid fills
 // the chip when there are few rows to hold
-inline int held_rows(int np, int dp) { return 128 * (np == 1 && dp <= 128 ? 2 : 1); }
+inline int held_rows(int np, int dp) { return 128 * (np == 1 && dp <= 64 ? 2 : 1); }
 inline int parts(int64_t held, int per, int64_t walked) {
   const int64_t gx = (held + per - 1) / per, tiles = (walked + 31) / 32;
   int64_t s = (1024 + gx - 1) / (gx > 0 ? gx : 1);
@@ -1085,18 +1092,21 @@ void launch_forward(const Args &a, bool need_x, const T *features, const T *tabl
   const int xtiles = (int)(a.npad / 32), etiles = a.vpad / 32;
   hipLaunchKernelGGL((kd_xent_pack<T, DP>), dim3((unsigned)(xtiles + etiles)), dim3(kBlock), 0,
                      stream, a, xtiles, features, table);
-  constexpr int rows = Walk<T, DP>::rows;
-  const dim3 grid((unsigned)((a.n + rows - 1) / rows), (unsigned)a.rsplit);
-  if (need_x)
+  if (need_x) {
+    constexpr int rows = Walk<T, DP, 1>::rows;
+    const dim3 grid((unsigned)((a.n + rows - 1) / rows), (unsigned)a.rsplit, Walk<T, DP, 1>::cs);
     hipLaunchKernelGGL((kd_xent_rows<T, DP, true>), grid, dim3(kBlock), 0, stream, a);
-  else
+  } else {
+    constexpr int rows = Walk<T, DP, 0>::rows;
+    const dim3 grid((unsigned)((a.n + rows - 1) / rows), (unsigned)a.rsplit);
     hipLaunchKernelGGL((kd_xent_rows<T, DP, false>), grid, dim3(kBlock), 0, stream, a);
+  }
 }
 
 template <typename T, int DP>
 void launch_table(const Args &a, hipStream_t stream) {
-  constexpr int rows = Walk<T, DP>::rows;
-  const dim3 grid((unsigned)((a.V + rows - 1) / rows), (unsigned)a.tsplit);
+  constexpr int rows = Walk<T, DP, 2>::rows;
+  const dim3 grid((unsigned)((a.V + rows - 1) / rows), (unsigned)a.tsplit, Walk<T, DP, 2>::cs);
   if (a.reduction == 0)
     hipLaunchKernelGGL((kd_xent_table<T, DP, true>), grid, dim3(kBlock), 0, stream, a);
   else
