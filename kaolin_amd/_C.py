@@ -772,6 +772,15 @@ def _number(fname, name, x):
     return x
 
 
+def _launch(dev, name, *args):
+    """The native call on the current stream of `dev`, which need not be the current device."""
+    if torch.cuda.current_device() == dev.index:
+        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
 def _bytes(nb, dev):
     return torch.empty((max(int(nb), 1),), dtype=torch.uint8, device=dev)
 
@@ -805,9 +814,8 @@ def surface_embedding_forward(index, embeddings, scale):
     index, embeddings = index.contiguous(), embeddings.contiguous()
     out = torch.empty((*index.shape, D), device=dev, dtype=embeddings.dtype)
     if out.numel():
-        with torch.cuda.device(dev):
-            _lib.call(f'kd_surface_embedding_forward_{sfx}', n, B, N, D, _ptr(index),
-                      _ptr(embeddings), scale, _ptr(out), _stream(dev))
+        _launch(dev, f'kd_surface_embedding_forward_{sfx}', n, B, N, D, _ptr(index),
+                _ptr(embeddings), scale, _ptr(out))
     return out
 
 
@@ -825,9 +833,8 @@ def surface_embedding_backward(grad_out, index, shape, scale):
         nb = int(_lib.load().kd_surface_embedding_workspace_size(n, B, N, D,
                                                                  grad_out.element_size()))
         ws = _bytes(nb, dev)
-        with torch.cuda.device(dev):
-            _lib.call(f'kd_surface_embedding_backward_{sfx}', n, B, N, D, _ptr(index),
-                      _ptr(grad_out), scale, _ptr(grad), _ptr(ws), nb, _stream(dev))
+        _launch(dev, f'kd_surface_embedding_backward_{sfx}', n, B, N, D, _ptr(index),
+                _ptr(grad_out), scale, _ptr(grad), _ptr(ws), nb)
     return grad
 
 
@@ -868,10 +875,9 @@ def surface_xent_forward(features, embeddings, labels, scale, reduction, need_fe
     ns = int(lib.kd_surface_xent_state_size(n, N, D, esize, nx, ne))
     nw = int(lib.kd_surface_xent_scratch_size(n, N, D, esize, nx, ne, 0))
     state, scratch = _bytes(ns, dev), _bytes(nw, dev)
-    with torch.cuda.device(dev):
-        _lib.call(f'kd_surface_xent_forward_{sfx}', n, N, D, _ptr(features), _ptr(embeddings),
-                  _ptr(labels), scale, _REDUCTIONS[reduction], nx, ne, _ptr(loss), _ptr(state), ns,
-                  _ptr(scratch), nw, _stream(dev))
+    _launch(dev, f'kd_surface_xent_forward_{sfx}', n, N, D, _ptr(features), _ptr(embeddings),
+            _ptr(labels), scale, _REDUCTIONS[reduction], nx, ne, _ptr(loss), _ptr(state), ns,
+            _ptr(scratch), nw)
     return loss, state
 
 
@@ -892,10 +898,9 @@ def surface_xent_backward(grad_loss, labels, shape, dtype, scale, reduction, sta
     nw = int(_lib.load().kd_surface_xent_scratch_size(n, N, D, esize, nx, 1 if embeddings else 0,
                                                       1))
     scratch = _bytes(nw, dev)
-    with torch.cuda.device(dev):
-        _lib.call(f'kd_surface_xent_backward_{_SFX16[dtype]}', n, N, D, _ptr(labels), float(scale),
-                  _REDUCTIONS[reduction], nx, ne, _ptr(g), _ptr(gx), _ptr(ge), _ptr(state),
-                  state.numel(), _ptr(scratch), nw, _stream(dev))
+    _launch(dev, f'kd_surface_xent_backward_{_SFX16[dtype]}', n, N, D, _ptr(labels), float(scale),
+            _REDUCTIONS[reduction], nx, ne, _ptr(g), _ptr(gx), _ptr(ge), _ptr(state),
+            state.numel(), _ptr(scratch), nw)
     return gx, ge
 
 

@@ -9,13 +9,13 @@
 // Forward: one pass, a thread per 16 bytes of output; reads 8 n bytes of indices and the rows that
 // are looked at, writes n * D * sizeof(T).
 //
-// Backward: no atomics on values, so the result does not depend on timing.  The tokens are sorted
-// by key with a stable least-significant-digit radix sort (two to four passes over 8 bytes a
-// token), so a row's tokens stand together in token order; then each group of G lanes (one row of
-// the gradient, 16 bytes a lane) walks a run of sorted tokens and adds their gradient rows in
-// registers.  Runs that cross a group's border are joined in LDS by the group in which they begin,
-// runs that cross a workgroup's border by a second launch.  The split of the walk over groups goes
-// by position and not by key, so one face that fills the image costs no more than any other.
+// Backward: no atomics on values, so the result does not depend on timing.  The tokens that name a row
+// are sorted by key with a stable least-significant-digit radix sort (8 bits a pass, 8 bytes a token),
+// so a row's tokens stand together in token order; then each group of G lanes (one row of the
+// gradient, 16 bytes a lane) walks a run of sorted tokens and adds their gradient rows in registers.
+// Runs that cross a group's border are joined in LDS by the group in which they begin, runs that cross
+// a workgroup's border by a second launch.  The split of the walk over groups goes by position and
+// not by key, so one face that fills the image costs no more than any other.
 #include "kd_capi.hpp"
 #include "kd_common.hpp"
 #include "kd_float16.hpp"
@@ -27,35 +27,54 @@ namespace kd {
 constexpr int kSortTile = 4096;             // tokens per sort workgroup (16 per thread)
 constexpr int kSortIters = kSortTile / kBlock;
 constexpr int kDigits = 256;
+constexpr int kFewTiles = 64;               // up to so many tiles the sort needs no scan launch
 constexpr int kMaxChannels = 1 << 20;
 
 // ------------------------------------------------------------------------------------------------
 // forward
 // ------------------------------------------------------------------------------------------------
-template <typename T, int VEC>
+template <typename T>
 __global__ __launch_bounds__(kBlock) void kd_embed_gather(
     int64_t n, uint32_t per_batch, int64_t rows, int D, int rows_per_block,
     const int64_t *__restrict__ index, const T *__restrict__ table, typename Wide<T>::type scale,
     T *__restrict__ out) {
-  using A = typename Wide<T>::type;
+  constexpr int V = 16 / sizeof(T);
+  constexpr int U = 4;  // in flight per thread: the index, then the row, then the store
   const int64_t r0 = (int64_t)blockIdx.x * rows_per_block;
   const uint32_t nrow = (uint32_t)min((int64_t)rows_per_block, n - r0);
-  const uint32_t vpr = (uint32_t)(D / VEC), total = nrow * vpr;
-  for (uint32_t v = threadIdx.x; v < total; v += kBlock) {
-    const uint32_t lr = v / vpr, c = (v - lr * vpr) * VEC;
-    const int64_t i = r0 + lr;
-    const int64_t k = index[i];
-    Pack<T, VEC> o;
-    if (k >= 0 && k < rows) {
-      const int64_t row = per_batch ? (int64_t)((uint32_t)i / per_batch) * rows + k : k;
-      const Pack<T, VEC> e = *(const Pack<T, VEC> *)(table + row * D + c);
+  const uint32_t vpr = (uint32_t)(D + V - 1) / V, total = nrow * vpr;
+  for (uint32_t v0 = threadIdx.x; v0 < total; v0 += U * kBlock) {
+    uint32_t lr[U], c[U];
+    int64_t k[U];
+    Pack<T, V> o[U];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) o.v[j] = from_wide<T>(to_wide(e.v[j]) * scale);
-    } else {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) o.v[j] = from_wide<T>((A)0);
+    for (int u = 0; u < U; ++u) {
+      const uint32_t v = min(v0 + u * kBlock, total - 1);
+      lr[u] = v / vpr;
+      c[u] = (v - lr[u] * vpr) * V;
+      k[u] = index[r0 + lr[u]];
     }
-    *(Pack<T, VEC> *)(out + i * D + c) = o;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (k[u] >= 0 && k[u] < rows) {
+        const int64_t row =
+            per_batch ? (int64_t)((uint32_t)(r0 + lr[u]) / per_batch) * rows + k[u] : k[u];
+        o[u] = load_pack<T, V>(table + row * D + c[u], D - (int)c[u]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[u].v[j] = (T)0.f;
+        k[u] = -1;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (v0 + u * kBlock >= total) break;
+      if (k[u] >= 0) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[u].v[j] = from_wide<T>(to_wide(o[u].v[j]) * scale);
+      }
+      store_pack<T, V>(out + (r0 + lr[u]) * D + c[u], o[u], D - (int)c[u]);
+    }
   }
 }
 
@@ -63,29 +82,58 @@ __global__ __launch_bounds__(kBlock) void kd_embed_gather(
 // stable radix sort of (key, token)
 // ------------------------------------------------------------------------------------------------
 struct SortKeys {
-  const int64_t *index;  // first pass: keys from the indices
-  const uint32_t *keys, *toks;
-  uint32_t n, per_batch, nkeys;
+  const int64_t *index;  // first pass: keys from the indices, tokens that name no row left out
+  const uint2 *pairs;    // later: (key, token)
+  const uint32_t *kept;  // later: how many
+  uint32_t n, per_batch;
   int64_t rows;
-  __device__ __forceinline__ uint32_t key(uint32_t i) const {
-    if (!index) return keys[i];
+  __device__ __forceinline__ uint32_t count() const { return index ? n : *kept; }
+  __device__ __forceinline__ bool get(uint32_t i, uint32_t m, uint2 &kt) const {
+    if (i >= m) return false;
+    if (!index) {
+      kt = pairs[i];
+      return true;
+    }
     const int64_t k = index[i];
-    if (k < 0 || k >= rows) return nkeys;  // no row: sorted behind every row
-    return (uint32_t)((per_batch ? (int64_t)(i / per_batch) * rows : 0) + k);
+    kt.x = (uint32_t)((per_batch ? (int64_t)(i / per_batch) * rows : 0) + k);
+    kt.y = i;
+    return k >= 0 && k < rows;
   }
-  __device__ __forceinline__ uint32_t tok(uint32_t i) const { return index ? i : toks[i]; }
 };
 
+// rows that no token names: zeros
+__device__ __forceinline__ void embed_fill(uint32_t block, uint32_t nblocks, int64_t bytes,
+                                           void *p) {
+  const int64_t head = min(bytes, (int64_t)((16 - ((uintptr_t)p & 15)) & 15));
+  const int64_t body = (bytes - head) / 16, i0 = (int64_t)block * kBlock + threadIdx.x;
+  uint4 *q = (uint4 *)((char *)p + head);
+  for (int64_t i = i0; i < body; i += (int64_t)nblocks * kBlock) q[i] = make_uint4(0, 0, 0, 0);
+  if (block == 0) {  // the two ends, 2 bytes at a time
+    uint16_t *a = (uint16_t *)p, *z = (uint16_t *)(q + body);
+    const int na = (int)(head / 2), nz = (int)((bytes - head - body * 16) / 2);
+    if ((int)threadIdx.x < na) a[threadIdx.x] = 0;
+    if ((int)threadIdx.x < nz) z[threadIdx.x] = 0;
+  }
+}
+
+// Per tile the count of each digit; the blocks behind the tiles clear the gradient.
 __global__ __launch_bounds__(kBlock) void kd_embed_hist(SortKeys s, int shift, uint32_t mask,
-                                                        int ntile, uint32_t *__restrict__ hist) {
+                                                        int ntile, uint32_t *__restrict__ hist,
+                                                        int64_t fill_bytes, void *fill) {
+  if ((int)blockIdx.x >= ntile) {
+    embed_fill(blockIdx.x - ntile, gridDim.x - ntile, fill_bytes, fill);
+    return;
+  }
   __shared__ uint32_t cnt[kDigits];
   cnt[threadIdx.x] = 0;
   __syncthreads();
-  const uint32_t base = blockIdx.x * (uint32_t)kSortTile;
-#pragma unroll 4
-  for (int it = 0; it < kSortIters; ++it) {
-    const uint32_t i = base + it * kBlock + threadIdx.x;
-    if (i < s.n) atomicAdd(&cnt[(s.key(i) >> shift) & mask], 1u);
+  const uint32_t base = blockIdx.x * (uint32_t)kSortTile, m = s.count();
+  if (base < m) {
+#pragma unroll 8
+    for (int it = 0; it < kSortIters; ++it) {
+      uint2 kt;
+      if (s.get(base + it * kBlock + threadIdx.x, m, kt)) atomicAdd(&cnt[(kt.x >> shift) & mask], 1u);
+    }
   }
   __syncthreads();
   if (threadIdx.x <= mask) hist[(int64_t)threadIdx.x * ntile + blockIdx.x] = cnt[threadIdx.x];
@@ -132,51 +180,75 @@ __global__ __launch_bounds__(kBlock) void kd_embed_scan(int ntile, uint32_t *__r
 // Each wave ranks its 1024 consecutive tokens 64 at a time: the lanes that hold the same digit are
 // found with one ballot per digit bit, a lane's rank is the number of lower ones among them plus
 // the wave's count of that digit so far.  The order within a digit is the tokens' order: stable.
+// Where the tiles are few (kFewTiles) each workgroup adds up the tiles' counts itself, a thread a
+// digit, and a single tile counts its own: the launches cost more than the work there.
 __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
     SortKeys s, int shift, int bits, int ntile, const uint32_t *__restrict__ hist,
-    const uint32_t *__restrict__ totals, uint32_t *__restrict__ okeys,
-    uint32_t *__restrict__ otoks) {
+    const uint32_t *__restrict__ totals, uint32_t *__restrict__ kept, uint2 *__restrict__ out,
+    int64_t fill_bytes, void *fill) {
   constexpr int kWaves = kBlock / kWave;
+  if ((int)blockIdx.x >= ntile) {
+    embed_fill(blockIdx.x - ntile, gridDim.x - ntile, fill_bytes, fill);
+    return;
+  }
   __shared__ uint32_t wcnt[kWaves][kDigits];
   __shared__ uint32_t s_w[kWaves];
-  const uint32_t mask = (1u << bits) - 1u;
+  const uint32_t mask = (1u << bits) - 1u, m = s.count();
+  if (blockIdx.x * (uint32_t)kSortTile >= m && blockIdx.x > 0) return;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
 #pragma unroll
   for (int k = 0; k < kWaves; ++k) wcnt[k][threadIdx.x] = 0;
-  // where each digit begins among all tokens
-  uint32_t tot;
-  const uint32_t mine = threadIdx.x <= mask ? totals[threadIdx.x] : 0u;
-  const uint32_t begin = wg_scan(mine, s_w, tot) - mine;  // (barriers inside)
   const uint32_t base = blockIdx.x * (uint32_t)kSortTile + w * (kSortTile / kWaves) + lane;
-  uint32_t key[kSortIters], rank[kSortIters];
+  uint2 kt[kSortIters];
+  uint32_t rank[kSortIters], in = 0;
+#pragma unroll
+  for (int it = 0; it < kSortIters; ++it)
+    if (s.get(base + it * kWave, m, kt[it])) in |= 1u << it;
+  __syncthreads();
 #pragma unroll
   for (int it = 0; it < kSortIters; ++it) {
-    const uint32_t i = base + it * kWave;
-    key[it] = i < s.n ? s.key(i) : 0u;
-  }
-#pragma unroll
-  for (int it = 0; it < kSortIters; ++it) {
-    const bool in = base + it * kWave < s.n;
-    const uint32_t d = (key[it] >> shift) & mask;
-    uint64_t same = __ballot(in);
+    const bool have = (in >> it) & 1u;
+    const uint32_t d = (kt[it].x >> shift) & mask;
+    uint64_t same = __ballot(have);
     for (int b = 0; b < bits; ++b) {
-      const uint64_t m = __ballot((d >> b) & 1u);
-      same &= ((d >> b) & 1u) ? m : ~m;
+      const uint64_t set = __ballot((d >> b) & 1u);
+      same &= ((d >> b) & 1u) ? set : ~set;
     }
     const int below = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32),
                                                 __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
     uint32_t r = 0;
-    if (in) {
+    if (have) {
       r = wcnt[w][d];
       rank[it] = r + below;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (in && below == 0) wcnt[w][d] = r + (uint32_t)__popcll(same);
+    if (have && below == 0) wcnt[w][d] = r + (uint32_t)__popcll(same);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
   __syncthreads();
+  // where each digit begins among all tokens, and this tile's part of it
+  uint32_t all = 0, before = 0, tot;
   if (threadIdx.x <= mask) {
-    uint32_t off = begin + hist[(int64_t)threadIdx.x * ntile + blockIdx.x];
+    if (ntile == 1) {
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) all += wcnt[k][threadIdx.x];
+    } else if (ntile <= kFewTiles) {
+      const uint32_t *h = hist + (int64_t)threadIdx.x * ntile;
+#pragma unroll 8
+      for (int k = 0; k < ntile; ++k) {
+        const uint32_t c = h[k];
+        before += k < (int)blockIdx.x ? c : 0u;
+        all += c;
+      }
+    } else {
+      all = totals[threadIdx.x];
+      before = hist[(int64_t)threadIdx.x * ntile + blockIdx.x];
+    }
+  }
+  const uint32_t begin = wg_scan(all, s_w, tot) - all;
+  if (blockIdx.x == 0 && threadIdx.x == 0 && kept) *kept = tot;
+  if (threadIdx.x <= mask) {
+    uint32_t off = begin + before;
 #pragma unroll
     for (int k = 0; k < kWaves; ++k) {
       const uint32_t c = wcnt[k][threadIdx.x];
@@ -186,14 +258,8 @@ __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
   }
   __syncthreads();
 #pragma unroll
-  for (int it = 0; it < kSortIters; ++it) {
-    const uint32_t i = base + it * kWave;
-    if (i < s.n) {
-      const uint32_t p = wcnt[w][(key[it] >> shift) & mask] + rank[it];
-      okeys[p] = key[it];
-      otoks[p] = s.tok(i);
-    }
-  }
+  for (int it = 0; it < kSortIters; ++it)
+    if ((in >> it) & 1u) out[wcnt[w][(kt[it].x >> shift) & mask] + rank[it]] = kt[it];
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -204,137 +270,129 @@ constexpr int kHasTail = 2;   // the last run goes on behind this range
 constexpr int kThrough = 4;   // one run covers the range and both borders (its sum is the head's)
 
 struct SegArgs {
-  uint32_t n, nkeys;
+  const uint32_t *kept;    // sorted tokens
   int D, glog, per_group;  // lanes per gradient row (log2), sorted tokens per group
-  const uint32_t *keys, *toks;
+  const uint2 *pairs;
   int *flags;              // per workgroup
 };
 
-template <typename T>
-__global__ __launch_bounds__(kBlock) void kd_embed_fill(int64_t n, T *__restrict__ p) {
-  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n;
-       i += (int64_t)gridDim.x * kBlock)
-    p[i] = (T)0;
-}
-
-template <typename T, int VEC>
+template <typename T, int V>
 __device__ __forceinline__ void embed_store(T *out, int D, uint32_t key, int col,
                                             const typename Wide<T>::type *acc,
                                             typename Wide<T>::type scale) {
-  Pack<T, VEC> o;
+  Pack<T, V> o;
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) o.v[j] = from_wide<T>(acc[j] * scale);
-  *(Pack<T, VEC> *)(out + (int64_t)key * D + col) = o;
+  for (int j = 0; j < V; ++j) o.v[j] = from_wide<T>(acc[j] * scale);
+  store_pack<T, V>(out + (int64_t)key * D + col, o, D - col);
 }
 
-template <typename T, int VEC>
+template <typename T>
 __global__ __launch_bounds__(kBlock) void kd_embed_segments(SegArgs a, const T *__restrict__ grad,
                                                             typename Wide<T>::type scale,
                                                             T *__restrict__ out,
                                                             typename Wide<T>::type *__restrict__ head,
                                                             typename Wide<T>::type *__restrict__ tail) {
   using A = typename Wide<T>::type;
-  constexpr int U = 4;  // gradient rows in flight per lane
-  __shared__ A s_head[kBlock * VEC], s_tail[kBlock * VEC];
+  constexpr int V = 16 / sizeof(T), U = 8;  // channels of a lane, gradient rows in flight
+  __shared__ A s_head[kBlock * V];
   __shared__ int s_kind[kBlock];
+  const uint32_t n = *a.kept;
   const int G = 1 << a.glog, NG = kBlock >> a.glog;
   const int g = threadIdx.x >> a.glog, gl = threadIdx.x & (G - 1);
-  const int col = ((int)blockIdx.y * G + gl) * VEC;
+  const int col = ((int)blockIdx.y * G + gl) * V;
   const bool live = col < a.D;
+  if ((uint64_t)blockIdx.x * NG * (uint64_t)a.per_group >= n) {  // behind the last token
+    if (threadIdx.x == 0 && blockIdx.y == 0) a.flags[blockIdx.x] = 0;
+    return;
+  }
   const uint64_t s64 = ((uint64_t)blockIdx.x * NG + g) * (uint64_t)a.per_group;
-  const uint32_t s = (uint32_t)min(s64, (uint64_t)a.n);
-  const uint32_t e = (uint32_t)min(s64 + a.per_group, (uint64_t)a.n);
+  const uint32_t s = (uint32_t)min(s64, (uint64_t)n);
+  const uint32_t e = (uint32_t)min(s64 + a.per_group, (uint64_t)n);
   int kind = 0;
-  A acc[VEC];
+  A acc[V];
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) acc[j] = (A)0;
+  for (int j = 0; j < V; ++j) acc[j] = (A)0;
   if (s < e) {
-    const uint32_t none = 0xffffffffu;
-    const uint32_t prev = s > 0 ? a.keys[s - 1] : none;
-    const uint32_t next = e < a.n ? a.keys[e] : none;
-    uint32_t cur = a.keys[s];
+    const uint32_t none = 0xffffffffu;  // (keys are below 2^31)
+    const uint32_t prev = s > 0 ? a.pairs[s - 1].x : none;
+    const uint32_t next = e < n ? a.pairs[e].x : none;
+    uint32_t cur = a.pairs[s].x;
     bool from_prev = cur == prev;
     for (uint32_t i = s; i < e; i += U) {
-      uint32_t k[U];
-      Pack<T, VEC> row[U];
+      uint2 kt[U];
+      Pack<T, V> row[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) kt[u] = a.pairs[min(i + u, e - 1)];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (live && i + u < e) row[u] = load_pack<T, V>(grad + (int64_t)kt[u].y * a.D + col, a.D - col);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        k[u] = i + u < e ? a.keys[i + u] : none;
-        if (k[u] < a.nkeys && live)
-          row[u] = *(const Pack<T, VEC> *)(grad + (int64_t)a.toks[i + u] * a.D + col);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (i + u >= e || cur >= a.nkeys) break;
-        if (k[u] != cur) {  // the run ends inside this group's range
+        if (i + u >= e) break;
+        if (kt[u].x != cur) {  // the run ends inside this group's range
           if (from_prev) {
             kind |= kHasHead;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s_head[threadIdx.x * VEC + j] = acc[j];
+            for (int j = 0; j < V; ++j) s_head[threadIdx.x * V + j] = acc[j];
           } else if (live) {
-            embed_store<T, VEC>(out, a.D, cur, col, acc, scale);
+            embed_store<T, V>(out, a.D, cur, col, acc, scale);
           }
-          cur = k[u];
+          cur = kt[u].x;
           from_prev = false;
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) acc[j] = (A)0;
-          if (cur >= a.nkeys) break;  // tokens without a row: nothing behind them either
+          for (int j = 0; j < V; ++j) acc[j] = (A)0;
         }
         if (live) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) acc[j] += to_wide(row[u].v[j]);
+          for (int j = 0; j < V; ++j) acc[j] += to_wide(row[u].v[j]);
         }
       }
     }
-    if (cur < a.nkeys) {
-      const bool on = next == cur;
-      if (from_prev) {
-        kind |= kHasHead | (on ? kThrough : 0);
+    const bool on = next == cur;
+    if (from_prev) {
+      kind |= kHasHead | (on ? kThrough : 0);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) s_head[threadIdx.x * VEC + j] = acc[j];
-      } else if (on) {
-        kind |= kHasTail;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s_tail[threadIdx.x * VEC + j] = acc[j];
-      } else if (live) {
-        embed_store<T, VEC>(out, a.D, cur, col, acc, scale);
-      }
+      for (int j = 0; j < V; ++j) s_head[threadIdx.x * V + j] = acc[j];
+    } else if (on) {
+      kind |= kHasTail;  // (its sum stays in registers)
+    } else if (live) {
+      embed_store<T, V>(out, a.D, cur, col, acc, scale);
     }
   }
   if (gl == 0) s_kind[g] = kind;
   __syncthreads();
-  const int64_t wcol = (int64_t)gridDim.y * G * VEC;  // a partial's channels
+  const int64_t wcol = (int64_t)gridDim.y * G * V;  // a partial's channels
   if (kind & kHasTail) {  // the run's owner: add the heads behind it
     int q = g + 1;
     bool open = true;
     for (; q < NG && open; ++q) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[j] += s_head[((q << a.glog) + gl) * VEC + j];
+      for (int j = 0; j < V; ++j) acc[j] += s_head[((q << a.glog) + gl) * V + j];
       open = s_kind[q] & kThrough;
     }
     if (!open) {
-      if (live) embed_store<T, VEC>(out, a.D, a.keys[e - 1], col, acc, scale);
+      if (live) embed_store<T, V>(out, a.D, a.pairs[e - 1].x, col, acc, scale);
     } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) tail[(int64_t)blockIdx.x * wcol + col + j] = acc[j];
+      for (int j = 0; j < V; ++j) tail[(int64_t)blockIdx.x * wcol + col + j] = acc[j];
     }
   }
   if (g == 0) {
     int f = 0;
     if (kind & kHasHead) {  // the run that began in an earlier workgroup
       f = kHasHead;
-      A h[VEC];
+      A h[V];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) h[j] = s_head[threadIdx.x * VEC + j];
+      for (int j = 0; j < V; ++j) h[j] = s_head[threadIdx.x * V + j];
       bool open = kind & kThrough;
       for (int q = 1; q < NG && open; ++q) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) h[j] += s_head[((q << a.glog) + gl) * VEC + j];
+        for (int j = 0; j < V; ++j) h[j] += s_head[((q << a.glog) + gl) * V + j];
         open = s_kind[q] & kThrough;
       }
       if (open) f |= kThrough;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) head[(int64_t)blockIdx.x * wcol + col + j] = h[j];
+      for (int j = 0; j < V; ++j) head[(int64_t)blockIdx.x * wcol + col + j] = h[j];
     }
     // a run that is open at the end of the workgroup began in it unless it runs through
     for (int q = NG - 1; q >= 0; --q) {
@@ -348,17 +406,18 @@ __global__ __launch_bounds__(kBlock) void kd_embed_segments(SegArgs a, const T *
 // The runs that cross a workgroup's border: the workgroup in which such a run begins adds up its
 // own part and the heads of the workgroups behind it, split over the groups of lanes in a fixed
 // order.
-template <typename T, int VEC>
+template <typename T>
 __global__ __launch_bounds__(kBlock) void kd_embed_join(SegArgs a, int nwg,
                                                         typename Wide<T>::type scale,
                                                         const typename Wide<T>::type *__restrict__ head,
                                                         const typename Wide<T>::type *__restrict__ tail,
                                                         T *__restrict__ out) {
   using A = typename Wide<T>::type;
+  constexpr int V = 16 / sizeof(T);
   const int w = blockIdx.x;
   if (!(a.flags[w] & kHasTail)) return;
   __shared__ int s_end;
-  __shared__ A s_sum[kBlock * VEC];
+  __shared__ A s_sum[kBlock * V];
   const int G = 1 << a.glog, NG = kBlock >> a.glog;
   const int g = threadIdx.x >> a.glog, gl = threadIdx.x & (G - 1);
   if (threadIdx.x == 0) s_end = nwg;
@@ -373,25 +432,25 @@ __global__ __launch_bounds__(kBlock) void kd_embed_join(SegArgs a, int nwg,
     if (found) break;
   }
   const int last = min(s_end, nwg - 1);
-  const int col = ((int)blockIdx.y * G + gl) * VEC;
-  const int64_t wcol = (int64_t)gridDim.y * G * VEC;
-  A acc[VEC];
+  const int col = ((int)blockIdx.y * G + gl) * V;
+  const int64_t wcol = (int64_t)gridDim.y * G * V;
+  A acc[V];
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) acc[j] = g == 0 ? tail[(int64_t)w * wcol + col + j] : (A)0;
+  for (int j = 0; j < V; ++j) acc[j] = g == 0 ? tail[(int64_t)w * wcol + col + j] : (A)0;
   for (int q = w + 1 + g; q <= last; q += NG) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] += head[(int64_t)q * wcol + col + j];
+    for (int j = 0; j < V; ++j) acc[j] += head[(int64_t)q * wcol + col + j];
   }
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) s_sum[threadIdx.x * VEC + j] = acc[j];
+  for (int j = 0; j < V; ++j) s_sum[threadIdx.x * V + j] = acc[j];
   __syncthreads();
   if (g == 0 && col < a.D) {
     for (int q = 1; q < NG; ++q) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[j] += s_sum[((q << a.glog) + gl) * VEC + j];
+      for (int j = 0; j < V; ++j) acc[j] += s_sum[((q << a.glog) + gl) * V + j];
     }
     const uint64_t end = (uint64_t)(w + 1) * NG * a.per_group;  // <= n: a run goes on behind it
-    embed_store<T, VEC>(out, a.D, a.keys[end - 1], col, acc, scale);
+    embed_store<T, V>(out, a.D, a.pairs[end - 1].x, col, acc, scale);
   }
 }
 
@@ -399,175 +458,137 @@ __global__ __launch_bounds__(kBlock) void kd_embed_join(SegArgs a, int nwg,
 // host
 // ------------------------------------------------------------------------------------------------
 struct EmbedPlan {
-  int vec, glog, gy, per_group, nwg, ntile, passes, bits;
+  int glog, gy, per_group, nwg, ntile, passes, bits;
   size_t pairs, hist, part, flags, total;  // workspace parts in bytes
 };
 
 static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-static EmbedPlan embed_plan(int64_t n, int64_t nkeys, int D, int esize, bool vec) {
+static EmbedPlan embed_plan(int64_t n, int64_t nkeys, int D, int esize) {
   EmbedPlan p;
-  p.vec = vec ? 16 / esize : 1;
-  const int cols = D / p.vec;
+  const int V = 16 / esize, cols = (D + V - 1) / V;
   p.glog = 0;
   while (p.glog < 6 && (1 << p.glog) < cols) ++p.glog;
   p.gy = (cols + (1 << p.glog) - 1) >> p.glog;
-  const int ng = kBlock >> p.glog;
-  // tokens per group: long walks read less at the borders, short ones fill the chip
+  const int64_t ng = kBlock >> p.glog;
+  // tokens per group: long walks write less at the borders, short ones fill the chip
   p.per_group = 64;
-  while (p.per_group > 8 && (n + (int64_t)ng * p.per_group - 1) / ((int64_t)ng * p.per_group) < 2048)
-    p.per_group >>= 1;
-  p.nwg = (int)((n + (int64_t)ng * p.per_group - 1) / ((int64_t)ng * p.per_group));
+  while (p.per_group > 8 && (n + ng * p.per_group - 1) / (ng * p.per_group) < 4096) p.per_group >>= 1;
+  p.nwg = (int)((n + ng * p.per_group - 1) / (ng * p.per_group));
   p.ntile = (int)((n + kSortTile - 1) / kSortTile);
   int kb = 1;
-  while (kb < 32 && (nkeys >> kb) != 0) ++kb;  // keys 0 .. nkeys
+  while (kb < 32 && ((nkeys - 1) >> kb) != 0) ++kb;  // keys 0 .. nkeys - 1
   p.passes = (kb + 7) / 8;
   p.bits = (kb + p.passes - 1) / p.passes;
   const int asize = esize == 8 ? 8 : 4;
-  p.pairs = up256(4 * (size_t)n);
-  p.hist = up256(4 * (size_t)kDigits * (size_t)p.ntile + 4 * kDigits);
-  // the workspace query does not know the pointers' alignment: the larger of both layouts
-  p.part = up256((size_t)p.nwg * (size_t)p.gy * (size_t)(p.vec << p.glog) * (size_t)asize);
+  p.pairs = up256(8 * (size_t)n);
+  p.hist = up256(4 * (size_t)kDigits * (size_t)p.ntile + 4 * kDigits + 4);
+  p.part = up256((size_t)p.nwg * (size_t)p.gy * (size_t)(V << p.glog) * (size_t)asize);
   p.flags = up256(4 * (size_t)p.nwg);
-  p.total = 4 * p.pairs + p.hist + 2 * p.part + p.flags;
+  p.total = 2 * p.pairs + p.hist + 2 * p.part + p.flags;
   return p;
 }
 
-static size_t embed_workspace(int64_t n, int64_t nkeys, int D, int esize) {
-  size_t t = embed_plan(n, nkeys, D, esize, false).total;
-  if (D % (16 / esize) == 0) t = std::max(t, embed_plan(n, nkeys, D, esize, true).total);
-  return t;
-}
-
-static bool embed_aligned(const void *p) { return ((uintptr_t)p & 15u) == 0; }
-
 static int embed_check(int64_t n, int64_t batch, int64_t rows, int D, const void *index,
-                       const void *x, const void *y) {
+                       const void *x) {
   KD_CHECK_ARG(n >= 0 && n < ((int64_t)1 << 31), "surface_embedding: need 0 <= indices < 2^31");
   KD_CHECK_ARG(batch >= 1 && rows >= 0 && rows < ((int64_t)1 << 31) &&
-                   batch * rows < ((int64_t)1 << 31),
+                   batch < ((int64_t)1 << 31) && batch * rows < ((int64_t)1 << 31),
                "surface_embedding: need batch >= 1 and batch * rows < 2^31");
   KD_CHECK_ARG(n % batch == 0, "surface_embedding: the indices do not split over the batch");
   KD_CHECK_ARG(D >= 0 && D <= kMaxChannels, "surface_embedding: need 0 <= channels <= 2^20");
   KD_CHECK_ARG(n == 0 || index, "surface_embedding: index is NULL");
   KD_CHECK_ARG(n == 0 || D == 0 || x, "surface_embedding: NULL input");
-  (void)y;
   return KD_OK;
 }
 
 template <typename T>
 static int embed_forward(int64_t n, int64_t batch, int64_t rows, int D, const int64_t *index,
                          const T *table, double scale, T *out, hipStream_t stream) {
-  const int rc = embed_check(n, batch, rows, D, index, out, nullptr);
+  const int rc = embed_check(n, batch, rows, D, index, out);
   if (rc != KD_OK) return rc;
   KD_CHECK_ARG(rows == 0 || D == 0 || n == 0 || table, "surface_embedding: embeddings is NULL");
   if (n == 0 || D == 0) return KD_OK;
   using A = typename Wide<T>::type;
   constexpr int V = 16 / (int)sizeof(T);
-  const bool vec = D % V == 0 && embed_aligned(table) && embed_aligned(out);
-  const int vpr = vec ? D / V : D;
-  const int rpb = std::max(1, kBlock * 4 / vpr);
+  const int rpb = std::max(1, kBlock * 4 / ((D + V - 1) / V));
   const unsigned grid = (unsigned)((n + rpb - 1) / rpb);
   const uint32_t pb = batch > 1 ? (uint32_t)(n / batch) : 0u;
   {
     ProfScope prof(K_EMBED_FWD, stream);
-    if (vec)
-      hipLaunchKernelGGL((kd_embed_gather<T, V>), dim3(grid), dim3(kBlock), 0, stream, n, pb, rows,
-                         D, rpb, index, table, (A)scale, out);
-    else
-      hipLaunchKernelGGL((kd_embed_gather<T, 1>), dim3(grid), dim3(kBlock), 0, stream, n, pb, rows,
-                         D, rpb, index, table, (A)scale, out);
+    hipLaunchKernelGGL(kd_embed_gather<T>, dim3(grid), dim3(kBlock), 0, stream, n, pb, rows, D, rpb,
+                       index, table, (A)scale, out);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(KD_ERR_LAUNCH, "surface_embedding: %s", hipGetErrorString(e));
   return KD_OK;
 }
 
-template <typename T, int VEC>
-static void embed_segments(const EmbedPlan &p, const SegArgs &a, const T *grad,
-                           typename Wide<T>::type scale, T *out, void *head, void *tail,
-                           hipStream_t stream) {
-  using A = typename Wide<T>::type;
-  const dim3 grid((unsigned)p.nwg, (unsigned)p.gy);
-  hipLaunchKernelGGL((kd_embed_segments<T, VEC>), grid, dim3(kBlock), 0, stream, a, grad, scale,
-                     out, (A *)head, (A *)tail);
-  if (p.nwg > 1)
-    hipLaunchKernelGGL((kd_embed_join<T, VEC>), grid, dim3(kBlock), 0, stream, a, p.nwg, scale,
-                       (const A *)head, (const A *)tail, out);
-}
-
 template <typename T>
 static int embed_backward(int64_t n, int64_t batch, int64_t rows, int D, const int64_t *index,
                           const T *grad, double scale, T *out, void *ws, size_t wsb,
                           hipStream_t stream) {
-  const int rc = embed_check(n, batch, rows, D, index, grad, nullptr);
+  const int rc = embed_check(n, batch, rows, D, index, grad);
   if (rc != KD_OK) return rc;
   const int64_t nkeys = batch * rows, nout = nkeys * D;
   if (nout == 0) return KD_OK;
   KD_CHECK_ARG(out, "surface_embedding: grad_embeddings is NULL");
   using A = typename Wide<T>::type;
-  constexpr int V = 16 / (int)sizeof(T);
-  const bool vec = D % V == 0 && embed_aligned(grad) && embed_aligned(out);
-  const EmbedPlan p = embed_plan(n, nkeys, D, (int)sizeof(T), vec);
-  if (n > 0 && (wsb < p.total || !ws))
-    return set_error(KD_ERR_WORKSPACE, "workspace too small: %zu < %zu", wsb, p.total);
+  const int64_t fill = nout * (int64_t)sizeof(T);
+  const unsigned fblocks = (unsigned)std::min<int64_t>((fill / 16 + kBlock) / kBlock, 2048);
   ProfScope prof(K_EMBED_BWD, stream);
-  {  // rows that no token names
-    const int64_t words = (nout * (int64_t)sizeof(T)) / 4;
-    const bool even = (nout * (int64_t)sizeof(T)) % 4 == 0 && ((uintptr_t)out & 3u) == 0;
-    const int64_t m = even ? words : nout;
-    const unsigned blocks = (unsigned)std::min<int64_t>((m + kBlock - 1) / kBlock, 4096);
-    if (even)
-      hipLaunchKernelGGL(kd_embed_fill<uint32_t>, dim3(blocks), dim3(kBlock), 0, stream, m,
-                         (uint32_t *)out);
-    else
-      hipLaunchKernelGGL(kd_embed_fill<uint16_t>, dim3(blocks), dim3(kBlock), 0, stream, m,
-                         (uint16_t *)out);
-  }
-  if (n > 0) {
+  if (n == 0) {
+    hipLaunchKernelGGL(kd_embed_hist, dim3(fblocks), dim3(kBlock), 0, stream, SortKeys{}, 0, 0u, 0,
+                       (uint32_t *)nullptr, fill, (void *)out);
+  } else {
+    const EmbedPlan p = embed_plan(n, nkeys, D, (int)sizeof(T));
+    if (wsb < p.total || !ws)
+      return set_error(KD_ERR_WORKSPACE, "workspace too small: %zu < %zu", wsb, p.total);
     char *c = (char *)ws;
-    uint32_t *buf[4];
-    for (int i = 0; i < 4; ++i) buf[i] = (uint32_t *)(c + (size_t)i * p.pairs);
-    c += 4 * p.pairs;
+    uint2 *buf[2] = {(uint2 *)c, (uint2 *)(c + p.pairs)};
+    c += 2 * p.pairs;
     uint32_t *hist = (uint32_t *)c, *totals = hist + (size_t)kDigits * p.ntile;
+    uint32_t *kept = totals + kDigits;
     c += p.hist;
-    void *head = c, *tail = c + p.part;
+    A *head = (A *)c, *tail = (A *)(c + p.part);
     int *flags = (int *)(c + 2 * p.part);
     SortKeys s;
+    s.index = index;
+    s.pairs = nullptr;
+    s.kept = kept;
     s.n = (uint32_t)n;
     s.per_batch = batch > 1 ? (uint32_t)(n / batch) : 0u;
-    s.nkeys = (uint32_t)nkeys;
     s.rows = rows;
-    s.keys = s.toks = nullptr;
-    s.index = index;
     const uint32_t mask = (1u << p.bits) - 1u;
-    int cur = 0;
+    const unsigned nt = (unsigned)p.ntile;
     for (int q = 0; q < p.passes; ++q) {
       const int shift = q * p.bits;
-      hipLaunchKernelGGL(kd_embed_hist, dim3(p.ntile), dim3(kBlock), 0, stream, s, shift, mask,
-                         p.ntile, hist);
-      hipLaunchKernelGGL(kd_embed_scan, dim3(mask + 1), dim3(kBlock), 0, stream, p.ntile, hist,
-                         totals);
-      hipLaunchKernelGGL(kd_embed_scatter, dim3(p.ntile), dim3(kBlock), 0, stream, s, shift, p.bits,
-                         p.ntile, hist, totals, buf[2 * cur], buf[2 * cur + 1]);
+      const unsigned extra = q == 0 ? fblocks : 0u;  // the first launch clears the gradient too
+      if (p.ntile > 1)
+        hipLaunchKernelGGL(kd_embed_hist, dim3(nt + extra), dim3(kBlock), 0, stream, s, shift, mask,
+                           p.ntile, hist, fill, (void *)out);
+      if (p.ntile > kFewTiles)
+        hipLaunchKernelGGL(kd_embed_scan, dim3(mask + 1), dim3(kBlock), 0, stream, p.ntile, hist,
+                           totals);
+      hipLaunchKernelGGL(kd_embed_scatter, dim3(nt + (p.ntile == 1 ? extra : 0u)), dim3(kBlock), 0,
+                         stream, s, shift, p.bits, p.ntile, hist, totals,
+                         q == 0 ? kept : (uint32_t *)nullptr, buf[q & 1], fill, (void *)out);
       s.index = nullptr;
-      s.keys = buf[2 * cur];
-      s.toks = buf[2 * cur + 1];
-      cur ^= 1;
+      s.pairs = buf[q & 1];
     }
     SegArgs a;
-    a.n = (uint32_t)n;
-    a.nkeys = (uint32_t)nkeys;
+    a.kept = kept;
     a.D = D;
     a.glog = p.glog;
     a.per_group = p.per_group;
-    a.keys = s.keys;
-    a.toks = s.toks;
+    a.pairs = s.pairs;
     a.flags = flags;
-    if (vec)
-      embed_segments<T, V>(p, a, grad, (A)scale, out, head, tail, stream);
-    else
-      embed_segments<T, 1>(p, a, grad, (A)scale, out, head, tail, stream);
+    const dim3 grid((unsigned)p.nwg, (unsigned)p.gy);
+    hipLaunchKernelGGL(kd_embed_segments<T>, grid, dim3(kBlock), 0, stream, a, grad, (A)scale, out,
+                       head, tail);
+    if (p.nwg > 1)
+      hipLaunchKernelGGL(kd_embed_join<T>, grid, dim3(kBlock), 0, stream, a, p.nwg, (A)scale,
+                         (const A *)head, (const A *)tail, out);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
@@ -584,10 +605,11 @@ extern "C" {
 size_t kd_surface_embedding_workspace_size(int64_t num_indices, int64_t batch, int64_t rows,
                                            int channels, int element_size) {
   if (num_indices <= 0 || num_indices >= ((int64_t)1 << 31) || batch < 1 || rows < 1 ||
-      rows >= ((int64_t)1 << 31) || batch * rows >= ((int64_t)1 << 31) || channels < 1 ||
-      channels > kMaxChannels || (element_size != 2 && element_size != 4 && element_size != 8))
+      rows >= ((int64_t)1 << 31) || batch >= ((int64_t)1 << 31) ||
+      batch * rows >= ((int64_t)1 << 31) || channels < 1 || channels > kMaxChannels ||
+      (element_size != 2 && element_size != 4 && element_size != 8))
     return 0;
-  return embed_workspace(num_indices, batch * rows, channels, element_size);
+  return embed_plan(num_indices, batch * rows, channels, element_size).total;
 }
 
 #define KD_EMBED(SFX, T)                                                                          \

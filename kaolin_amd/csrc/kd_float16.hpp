@@ -29,9 +29,30 @@ __device__ __forceinline__ T from_wide(typename Wide<T>::type x) {
   return (T)x;  // to nearest, ties to even
 }
 
+// N elements at any element's address: 16-byte loads and stores here need no alignment.
 template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack {
+struct __attribute__((packed, aligned(sizeof(T)))) Pack {
   T v[N];
 };
+
+// the first `n` of N elements (n < N only at the end of a row)
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T *p, int n) {
+  if (n >= N) return *(const Pack<T, N> *)p;
+  Pack<T, N> x;
+#pragma unroll
+  for (int j = 0; j < N; ++j) x.v[j] = j < n ? p[j] : (T)0.f;
+  return x;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &x, int n) {
+  if (n >= N) {
+    *(Pack<T, N> *)p = x;
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < n) p[j] = x.v[j];
+  }
+}
 
 }  // namespace kd

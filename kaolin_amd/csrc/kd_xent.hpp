@@ -88,7 +88,9 @@ __device__ __forceinline__ void split3(float x, uint16_t &a, uint16_t &b, uint16
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kRowPad = 256;  // packed rows are padded with zeros to a multiple of this
-constexpr int kMapChunk = 2048;
+constexpr int kMapChunk = 2048;   // pixels listed at a time
+constexpr int kListChunks = 4;    // up to so many chunks one workgroup lists them all
+constexpr int kSumChunks = 4096;  // up to so many chunks a workgroup adds up the counts before its own
 
 // The work of one call.  Packed operands of a matrix M (rows padded to kRowPad, channels to DP),
 // in tiles of 32 rows, each tile NP planes, 16 bytes a lane:
@@ -110,6 +112,7 @@ struct Args {
   float *lse, *w;   // exponent of a probability but its logit, its complement negated (scaled)
   float *xn;        // squared sizes of the pixels' features
   uint32_t *emax;   // the largest squared size of the table's rows (its bits)
+  uint32_t *ticket; // workgroups that have added up their losses
   uint16_t *xs, *xt, *es;
   float *raw;       // (n, D): w (m - e_y)
   // scratch
@@ -122,12 +125,22 @@ struct Args {
   uint32_t *gmax;
 };
 
+// A launch of many workgroups is cut into rows of the grid: one dimension holds 2^32 threads.
+constexpr int64_t kGridRow = 1 << 20;
+inline dim3 grid_of(int64_t nblocks) {
+  const int64_t x = nblocks < kGridRow ? nblocks : kGridRow;
+  return dim3((unsigned)x, (unsigned)((nblocks + x - 1) / x));
+}
+__device__ __forceinline__ int64_t block_id() {
+  return (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+}
+
 // ------------------------------------------------------------------------------------------------
 // listing the pixels with a label
 // ------------------------------------------------------------------------------------------------
 static __global__ __launch_bounds__(kBlock) void kd_xent_count(int64_t n, int64_t V,
-                                                        const int64_t *__restrict__ labels,
-                                                        int *__restrict__ blk) {
+                                                               const int64_t *__restrict__ labels,
+                                                               int *__restrict__ blk) {
   __shared__ int s_c[kBlock / kWave];
   const int64_t b = (int64_t)blockIdx.x * kMapChunk;
   int c = 0;
@@ -142,9 +155,19 @@ static __global__ __launch_bounds__(kBlock) void kd_xent_count(int64_t n, int64_
   if (threadIdx.x == 0) blk[blockIdx.x] = s_c[0] + s_c[1] + s_c[2] + s_c[3];
 }
 
-static __global__ __launch_bounds__(kBlock) void kd_xent_scan(int nblk, int *__restrict__ blk,
-                                                       int *__restrict__ count,
-                                                       uint32_t *__restrict__ emax) {
+// The sum of the threads' values, in every thread.
+__device__ __forceinline__ int wg_total(int x, int *s_x) {
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) x += __shfl_xor(x, s);
+  if ((threadIdx.x & 63) == 0) s_x[threadIdx.x >> 6] = x;
+  __syncthreads();
+  const int t = s_x[0] + s_x[1] + s_x[2] + s_x[3];
+  __syncthreads();
+  return t;
+}
+
+// One workgroup: the chunks' counts become offsets (for more chunks than a workgroup adds up itself).
+static __global__ __launch_bounds__(kBlock) void kd_xent_scan(int nblk, int *__restrict__ blk) {
   __shared__ int s_w[kBlock / kWave];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int run = 0;
@@ -169,61 +192,108 @@ static __global__ __launch_bounds__(kBlock) void kd_xent_scan(int nblk, int *__r
     if (i < nblk) blk[i] = run + off + x - c;
     run += tot;
   }
-  if (threadIdx.x == 0) {
-    *count = run;
-    *emax = 0u;
-  }
 }
 
-static __global__ __launch_bounds__(kBlock) void kd_xent_map(int64_t n, int64_t V,
-                                                      const int64_t *__restrict__ labels,
-                                                      const int *__restrict__ blk,
-                                                      int *__restrict__ rowid,
-                                                      int *__restrict__ lab) {
+// Lists the pixels of `chunks` chunks a workgroup: blk holds the chunks' counts, or their offsets
+// (scanned), or is not needed (one workgroup lists all).  Losses of pixels without a label are 0.
+static __global__ __launch_bounds__(kBlock) void kd_xent_map(Args a, int chunks, bool scanned,
+                                                             const int64_t *__restrict__ labels,
+                                                             float *__restrict__ loss) {
   __shared__ int s_c[4];
-  const int64_t b = (int64_t)blockIdx.x * kMapChunk;
-  int run = blk[blockIdx.x];
-  for (int k = 0; k < kMapChunk / kBlock; ++k) {
-    const int64_t i = b + k * kBlock + threadIdx.x;
-    const int64_t y = i < n ? labels[i] : -1;
-    int total;
-    const int p = wg_compact(y >= 0 && y < V, s_c, total);
-    if (p >= 0) {
-      rowid[run + p] = (int)i;
-      lab[run + p] = (int)y;
+  int run = 0;
+  if (chunks == 1 && scanned) {
+    run = a.blk[blockIdx.x];
+  } else if (chunks == 1) {
+    int c = 0;
+    for (int k = threadIdx.x; k < (int)blockIdx.x; k += kBlock) c += a.blk[k];
+    run = wg_total(c, s_c);
+  }
+  for (int q = 0; q < chunks; ++q) {
+    const int64_t b = ((int64_t)blockIdx.x * chunks + q) * kMapChunk;
+    if (b >= a.n) break;
+    int64_t y[kMapChunk / kBlock];
+#pragma unroll
+    for (int k = 0; k < kMapChunk / kBlock; ++k) {
+      const int64_t i = b + k * kBlock + threadIdx.x;
+      y[k] = i < a.n ? labels[i] : -1;
     }
-    run += total;
+#pragma unroll
+    for (int k = 0; k < kMapChunk / kBlock; ++k) {
+      const int64_t i = b + k * kBlock + threadIdx.x;
+      int total;
+      const int p = wg_compact(y[k] >= 0 && y[k] < a.V, s_c, total);
+      if (p >= 0) {
+        a.rowid[run + p] = (int)i;
+        a.lab[run + p] = (int)y[k];
+      } else if (a.reduction == 0 && i < a.n) {
+        loss[i] = 0.f;
+      }
+      run += total;
+    }
+  }
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
+    *a.count = run;
+    *a.emax = 0u;
+    *a.ticket = 0u;
   }
 }
 
 // ------------------------------------------------------------------------------------------------
 // packing
 // ------------------------------------------------------------------------------------------------
+// A tile of 32 rows goes through LDS, 16 bytes a lane in and out.
 template <typename T, int DP>
 __global__ __launch_bounds__(kBlock) void kd_xent_pack(Args a, int xtiles,
                                                        const T *__restrict__ features,
                                                        const T *__restrict__ table) {
   using F = Form<T>;
-  constexpr int kPitch = DP + 4 / (int)sizeof(T);  // odd in words: columns spread over the banks
-  __shared__ T s_m[32 * kPitch];
-  const bool is_x = (int)blockIdx.x < xtiles;
-  const int tile = is_x ? (int)blockIdx.x : (int)blockIdx.x - xtiles;
+  constexpr int V = 16 / sizeof(T);
+  constexpr int kPitch = DP + V;  // rows 16 bytes apart over the banks
+  __shared__ __align__(16) T s_m[32 * kPitch];
+  const int64_t bid = block_id();
+  const bool is_x = bid < xtiles;
+  const int64_t tile = is_x ? bid : bid - xtiles;
+  if (tile >= a.vpad / 32 && !is_x) return;
   const int count = *a.count;
-  const int64_t r0 = (int64_t)tile * 32;
+  const int64_t r0 = tile * 32;
   if (is_x && r0 >= ((int64_t)count + kRowPad - 1) / kRowPad * kRowPad) return;
   const bool flip = is_x && a.scale < 0.f;
-  for (int e = threadIdx.x; e < 32 * DP; e += kBlock) {
-    const int r = e / DP, d = e % DP;
+#pragma unroll
+  for (int q = 0; q * kBlock < 32 * DP / V; ++q) {
+    const int e = q * kBlock + threadIdx.x, r = e / (DP / V), d = e % (DP / V) * V;
+    if (r >= 32) break;  // (whole waves)
     const int64_t i = r0 + r;
-    T x = (T)0.f;
+    Pack<T, V> x;
+#pragma unroll
+    for (int j = 0; j < V; ++j) x.v[j] = (T)0.f;
     if (d < a.D) {
       if (is_x) {
-        if (i < count) x = features[(int64_t)a.rowid[i] * a.D + d];
+        if (i < count) x = load_pack<T, V>(features + (int64_t)a.rowid[i] * a.D + d, a.D - d);
       } else if (i < a.V) {
-        x = table[i * a.D + d];
+        x = load_pack<T, V>(table + i * a.D + d, a.D - d);
       }
     }
-    s_m[r * kPitch + d] = flip ? (T)(-(float)x) : x;
+    float size = 0.f;  // the row's squared size: DP / V lanes hold it
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      size = fmaf((float)x.v[j], (float)x.v[j], size);
+      if (flip) x.v[j] = (T)(-(float)x.v[j]);
+    }
+    *(uint4 *)&s_m[r * kPitch + d] = __builtin_bit_cast(uint4, x);
+    constexpr int kLanes = DP / V < kWave ? DP / V : kWave;
+#pragma unroll
+    for (int k = kLanes / 2; k >= 1; k >>= 1) size += __shfl_xor(size, k);
+    if (is_x) {
+      if (d == 0) a.xn[i] = size;
+    } else {
+      uint32_t u = __float_as_uint(size);
+#pragma unroll
+      for (int k = 32; k >= kLanes; k >>= 1) u = max(u, (uint32_t)__shfl_xor((int)u, k));
+      // the look before saves all but the few atomics that raise it: one address, many tiles
+      if ((threadIdx.x & 63) == 0 &&
+          u > __hip_atomic_load(a.emax, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+        atomicMax(a.emax, u);
+    }
   }
   if (is_x && threadIdx.x < 32 && r0 + threadIdx.x >= count) {
     a.lab[r0 + threadIdx.x] = -1;
@@ -231,59 +301,39 @@ __global__ __launch_bounds__(kBlock) void kd_xent_pack(Args a, int xtiles,
     a.w[r0 + threadIdx.x] = 0.f;
   }
   __syncthreads();
-  {  // squared sizes: 8 lanes a row
-    const int r = threadIdx.x >> 3;
-    float q = 0.f;
-#pragma unroll
-    for (int k = 0; k < DP / 8; ++k) {
-      const int d = (threadIdx.x & 7) + 8 * k;
-      const float x = (float)s_m[r * kPitch + d];
-      q = fmaf(x, x, q);
-    }
-#pragma unroll
-    for (int k = 4; k >= 1; k >>= 1) q += __shfl_xor(q, k);
-    if (is_x) {
-      if ((threadIdx.x & 7) == 0) a.xn[r0 + r] = q;
-    } else {
-      uint32_t u = __float_as_uint(q);
-#pragma unroll
-      for (int k = 32; k >= 8; k >>= 1) u = max(u, (uint32_t)__shfl_xor((int)u, k));
-      // the look before saves all but the few atomics that raise it: one address, many tiles
-      if ((threadIdx.x & 63) == 0 && u > __hip_atomic_load(a.emax, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
-        atomicMax(a.emax, u);
-    }
-  }
   constexpr int kGroups = 32 * DP / 8;  // 16-byte groups per plane and layout
-  uint16_t *straight = (is_x ? a.xs : a.es) + (int64_t)tile * F::np * 32 * DP;
+  uint16_t *straight = (is_x ? a.xs : a.es) + tile * F::np * 32 * DP;
   uint16_t *transposed = is_x ? a.xt : a.et;
-  if (transposed) transposed += (int64_t)tile * F::np * 32 * DP;
-  for (int q = threadIdx.x; q < 2 * kGroups; q += kBlock) {
-    const bool tr = q >= kGroups;
-    if (tr && !transposed) break;
-    const int g = tr ? q - kGroups : q;
-    const int lane = g & 63, blkid = g >> 6;
+  auto put = [&](uint16_t *to, int g, const T *x) {
     Pack<uint16_t, 8> o[F::np];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      int r, d;
-      if (!tr) {
-        r = lane & 31;
-        d = 16 * blkid + 8 * (lane >> 5) + j;
-      } else {
-        constexpr int kT = DP / 32;
-        r = 16 * (blkid / kT) + 8 * (j >> 2) + 4 * (lane >> 5) + (j & 3);
-        d = 32 * (blkid % kT) + (lane & 31);
-      }
-      const T x = s_m[r * kPitch + d];
-      if constexpr (F::np == 1) {
-        o[0].v[j] = __builtin_bit_cast(uint16_t, x);
-      } else {
-        split3(x, o[0].v[j], o[1].v[j], o[2].v[j]);
-      }
+      if constexpr (F::np == 1)
+        o[0].v[j] = __builtin_bit_cast(uint16_t, x[j]);
+      else
+        split3(x[j], o[0].v[j], o[1].v[j], o[2].v[j]);
     }
 #pragma unroll
     for (int p = 0; p < F::np; ++p)
-      *(Pack<uint16_t, 8> *)((tr ? transposed : straight) + (int64_t)p * 32 * DP + g * 8) = o[p];
+      *(uint4 *)(to + (int64_t)p * 32 * DP + g * 8) = __builtin_bit_cast(uint4, o[p]);
+  };
+  for (int g = threadIdx.x; g < kGroups; g += kBlock) {
+    const int lane = g & 63, r = lane & 31, d = 16 * (g >> 6) + 8 * (lane >> 5);
+    T x[8];
+    *(uint4 *)x = *(const uint4 *)&s_m[r * kPitch + d];
+    if constexpr (sizeof(T) == 4) *(uint4 *)(x + 4) = *(const uint4 *)&s_m[r * kPitch + d + 4];
+    put(straight, g, x);
+  }
+  if (!transposed) return;
+  transposed += tile * F::np * 32 * DP;
+  for (int g = threadIdx.x; g < kGroups; g += kBlock) {
+    constexpr int kT = DP / 32;
+    const int lane = g & 63, blkid = g >> 6;
+    const int r = 16 * (blkid / kT) + 4 * (lane >> 5), d = 32 * (blkid % kT) + (lane & 31);
+    T x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = s_m[(r + 8 * (j >> 2) + (j & 3)) * kPitch + d];
+    put(transposed, g, x);
   }
 }
 
@@ -716,40 +766,49 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
 }
 
 // ------------------------------------------------------------------------------------------------
-// joining the parts: a wave per listed pixel
+// joining the parts: G lanes per listed pixel, four channels a lane at a time
 // ------------------------------------------------------------------------------------------------
-template <typename T>
+template <typename T, int G>
 __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__restrict__ features,
                                                           const T *__restrict__ table,
                                                           float *__restrict__ loss) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * (kBlock / kWave) + (threadIdx.x >> 6);
+  const int gl = threadIdx.x & (G - 1);
+  const int64_t r = block_id() * (kBlock / G) + threadIdx.x / G;
   if (r >= *a.count) return;
   const int64_t i = a.rowid[r], y = a.lab[r];
+  const int d = 4 * gl, left = a.D - d;  // (D <= 4 G)
+  Pack<T, 4> e;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) e.v[j] = (T)0.f;
   float z = 0.f;
-  for (int d = lane; d < a.D; d += kWave)
-    z = fmaf((float)features[i * a.D + d], (float)table[y * a.D + d], z);
+  if (left > 0) {
+    e = load_pack<T, 4>(table + y * a.D + d, left);
+    const Pack<T, 4> x = load_pack<T, 4>(features + i * a.D + d, left);
 #pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) z += __shfl_xor(z, s);
-  const float z2 = z * (a.scale * kLog2e);
+    for (int j = 0; j < 4; ++j) z = fmaf((float)x.v[j], (float)e.v[j], z);
+  }
   float m = -1e30f;
-  for (int s = lane; s < a.rsplit; s += kWave) m = fmaxf(m, a.pm[(int64_t)s * a.npad + r]);
+  for (int s = gl; s < a.rsplit; s += G) m = fmaxf(m, a.pm[(int64_t)s * a.npad + r]);
 #pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+  for (int s = G / 2; s >= 1; s >>= 1) {
+    z += __shfl_xor(z, s);
+    m = fmaxf(m, __shfl_xor(m, s));
+  }
+  const float z2 = z * (a.scale * kLog2e);
   float l = 0.f;
-  for (int s = lane; s < a.rsplit; s += kWave) {
+  for (int s = gl; s < a.rsplit; s += G) {
     const int64_t q = (int64_t)s * a.npad + r;
     l += a.pl[q] * __builtin_amdgcn_exp2f(a.pm[q] - m);
   }
 #pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) l += __shfl_xor(l, s);
+  for (int s = G / 2; s >= 1; s >>= 1) l += __shfl_xor(l, s);
   const float u = (m + log2f(l) - z2) * kLn2;  // -inf when the label is the only row
   const float t = expf(-fabsf(u));
   const float value = fmaxf(u, 0.f) + log1pf(t);
   const float w = u >= 0.f ? 1.f / (1.f + t) : t / (1.f + t);
   const float wn = u != u ? u : w;
   const float out = u != u ? u : value;
-  if (lane == 0) {
+  if (gl == 0) {
     a.lse[r] = Form<T>::shift_table - (z2 + out * kLog2e);
     a.w[r] = -wn * exp2f(Form<T>::shift_table);
     if (a.reduction == 0)
@@ -757,16 +816,18 @@ __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__res
     else
       a.lrow[r] = out;
   }
-  if (!a.raw) return;
+  if (!a.raw || left <= 0) return;
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  for (int d = lane; d < a.D; d += kWave) {
-    float o = 0.f;
-    for (int s = 0; s < a.rsplit; ++s) {
-      const int64_t q = (int64_t)s * a.npad + r;
-      o += a.po[q * a.dp + d] * __builtin_amdgcn_exp2f(a.pm[q] - m);
-    }
-    a.raw[i * a.D + d] = wn * (o * inv - (float)table[y * a.D + d]);
+  f32x4 o = (f32x4)(0.f);
+#pragma unroll 4
+  for (int s = 0; s < a.rsplit; ++s) {
+    const int64_t q = (int64_t)s * a.npad + r;
+    o += *(const f32x4 *)(a.po + q * a.dp + d) * __builtin_amdgcn_exp2f(a.pm[q] - m);
   }
+  Pack<float, 4> v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v.v[j] = wn * (o[j] * inv - (float)e.v[j]);
+  store_pack<float, 4>(a.raw + i * a.D + d, v, left);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -782,53 +843,69 @@ __device__ __forceinline__ double wg_sum(double x, double *s_x) {
   return s_x[0] + s_x[1] + s_x[2] + s_x[3];
 }
 
-static __global__ __launch_bounds__(kBlock) void kd_xent_sum(Args a) {
+// Each workgroup adds up its share; the one that finishes last adds up the shares, in their order.
+static __global__ __launch_bounds__(kBlock) void kd_xent_sum(Args a, float *__restrict__ loss) {
   __shared__ double s_x[kBlock / kWave];
+  __shared__ bool s_last;
   const int count = *a.count;
   double x = 0.0;
   for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < count;
-       i += (int64_t)kReduceBlocks * kBlock)
+       i += (int64_t)gridDim.x * kBlock)
     x += (double)a.lrow[i];
   x = wg_sum(x, s_x);
-  if (threadIdx.x == 0) a.part[blockIdx.x] = x;
-}
-
-static __global__ __launch_bounds__(kBlock) void kd_xent_finish(Args a, float *__restrict__ loss) {
-  __shared__ double s_x[kBlock / kWave];
-  const double x = wg_sum(a.part[threadIdx.x], s_x);
   if (threadIdx.x == 0) {
-    const int count = *a.count;
-    *loss = (float)(a.reduction == 1 ? x / (double)(count > 0 ? count : 1) : x);
+    a.part[blockIdx.x] = x;
+    __threadfence();
+    s_last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
   }
-}
-
-static __global__ __launch_bounds__(kBlock) void kd_xent_zero(int64_t n, float *__restrict__ p) {
-  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n;
-       i += (int64_t)gridDim.x * kBlock)
-    p[i] = 0.f;
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  double y = 0.0;
+  if (threadIdx.x < gridDim.x)
+    y = __hip_atomic_load(&a.part[threadIdx.x], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  y = wg_sum(y, s_x);
+  if (threadIdx.x == 0)
+    *loss = (float)(a.reduction == 1 ? y / (double)(count > 0 ? count : 1) : y);
 }
 
 // ------------------------------------------------------------------------------------------------
 // backward
 // ------------------------------------------------------------------------------------------------
-// the listed pixels' gradients of a loss per pixel, and the largest of their sizes (its bits as a
-// whole number: the order of the maxima does not matter)
-static __global__ __launch_bounds__(kBlock) void kd_xent_rowgrad(Args a, const float *__restrict__ grad) {
-  const int64_t r = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+// the listed pixels' gradients of a loss per pixel, and the largest of their sizes per workgroup
+constexpr int kGradChunk = 4096;
+
+static __global__ __launch_bounds__(kBlock) void kd_xent_rowgrad(Args a,
+                                                                 const float *__restrict__ grad) {
+  __shared__ uint32_t s_m[kBlock / kWave];
   const int count = *a.count;
-  float g = 0.f;
-  if (r < count) g = grad[a.rowid[r]];
-  if (r < a.npad) a.grow[r] = g;
-  uint32_t b = __float_as_uint(fabsf(g));
+  uint32_t top = 0;
+#pragma unroll 4
+  for (int k = 0; k < kGradChunk / kBlock; ++k) {
+    const int64_t r = (int64_t)blockIdx.x * kGradChunk + k * kBlock + threadIdx.x;
+    const float g = r < count ? grad[a.rowid[r]] : 0.f;
+    if (r < a.npad) a.grow[r] = g;
+    top = max(top, __float_as_uint(fabsf(g)));
+  }
 #pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) b = max(b, (uint32_t)__shfl_xor((int)b, s));
-  if ((threadIdx.x & 63) == 0 && b) atomicMax(a.gmax, b);
+  for (int s = 32; s >= 1; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
+  if ((threadIdx.x & 63) == 0) s_m[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) a.gmax[blockIdx.x] = max(max(s_m[0], s_m[1]), max(s_m[2], s_m[3]));
 }
 
 // the power of two that brings the largest gradient into [1, 2): the products' operands stay in
 // range whatever the incoming gradient's scale
-__device__ __forceinline__ float grad_unit(const uint32_t *gmax) {
-  const uint32_t e = *gmax >> 23;
+__device__ __forceinline__ float grad_unit(const Args &a) {
+  __shared__ uint32_t s_u[kBlock / kWave];
+  const int nblk = (int)((a.npad + kGradChunk - 1) / kGradChunk);
+  uint32_t top = 0;
+  for (int k = threadIdx.x; k < nblk; k += kBlock) top = max(top, a.gmax[k]);
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
+  if ((threadIdx.x & 63) == 0) s_u[threadIdx.x >> 6] = top;
+  __syncthreads();
+  const uint32_t e = max(max(s_u[0], s_u[1]), max(s_u[2], s_u[3])) >> 23;
   return e == 0 || e >= 254 ? 1.f : __uint_as_float((254u - e) << 23);
 }
 
@@ -918,7 +995,7 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, 2>::waves)) void kd_xent_table
   TableWalk<T, DP, ROWG> w;
   w.v0 = ((int)blockIdx.x * 4 + wave) * (32 * RB);
   w.c2 = a.c2;
-  w.unit = ROWG ? grad_unit(a.gmax) : 1.f;
+  w.unit = ROWG ? grad_unit(a) : 1.f;
   w.lunit = ROWG ? log2f(w.unit) : 0.f;  // a power of two: exact
   w.plse = a.lse;
   w.pw = a.w;
@@ -964,34 +1041,46 @@ __device__ __forceinline__ float grad_factor(const Args &a, const float *grad) {
   return g;
 }
 
+// The first `xblocks` workgroups scale dX, the others join the parts of dE: four channels a thread.
 template <typename T>
-__global__ __launch_bounds__(kBlock) void kd_xent_table_join(Args a, const float *__restrict__ grad,
-                                                             T *__restrict__ out) {
-  const int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  if (q >= (int64_t)a.V * a.D) return;
-  const int64_t v = q / a.D;
-  const int d = (int)(q - v * a.D);
-  float x = 0.f;
-  for (int s = 0; s < a.tsplit; ++s) x += a.pe[((int64_t)s * a.vpad + v) * a.dp + d];
-  const float f = a.reduction == 0 ? 1.f / grad_unit(a.gmax) : grad_factor(a, grad);
-  out[q] = (T)(x * exp2f(-Form<T>::shift_table) * fabsf(a.scale) * f);
-}
-
-template <typename T>
-__global__ __launch_bounds__(kBlock) void kd_xent_grad_features(Args a,
-                                                                const int64_t *__restrict__ labels,
-                                                                const float *__restrict__ grad,
-                                                                T *__restrict__ out) {
-  const int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  if (q >= a.n * a.D) return;
-  const int64_t i = q / a.D;
-  const int64_t y = labels[i];
-  T v = (T)0.f;
-  if (y >= 0 && y < a.V) {
-    const float g = a.reduction == 0 ? grad[i] : grad_factor(a, grad);
-    v = (T)(a.raw[q] * (a.scale * g));
+__global__ __launch_bounds__(kBlock) void kd_xent_grads(Args a, int64_t xblocks, int vpr,
+                                                        const int64_t *__restrict__ labels,
+                                                        const float *__restrict__ grad,
+                                                        T *__restrict__ gx, T *__restrict__ ge) {
+  const int64_t bid = block_id();
+  const bool is_x = bid < xblocks;
+  const int64_t q = (is_x ? bid : bid - xblocks) * kBlock + threadIdx.x;
+  const int64_t r = q <= 0xffffffffll ? (int64_t)((uint32_t)q / (uint32_t)vpr) : q / vpr;
+  const int d = (int)(q - r * vpr) * 4, left = a.D - d;
+  float f = 1.f;
+  if (!is_x && a.reduction == 0)
+    f = 1.f / grad_unit(a);  // (the workgroup as a whole)
+  else if (a.reduction != 0)
+    f = grad_factor(a, grad);
+  Pack<T, 4> o;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o.v[j] = (T)0.f;
+  if (is_x) {
+    if (r >= a.n) return;
+    const int64_t y = labels[r];
+    if (y >= 0 && y < a.V) {
+      if (a.reduction == 0) f = grad[r];
+      const Pack<float, 4> x = load_pack<float, 4>(a.raw + r * a.D + d, left);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o.v[j] = (T)(x.v[j] * (a.scale * f));
+    }
+    store_pack<T, 4>(gx + r * a.D + d, o, left);
+  } else {
+    if (r >= a.V) return;
+    f32x4 x = (f32x4)(0.f);
+#pragma unroll 4
+    for (int s = 0; s < a.tsplit; ++s)
+      x += *(const f32x4 *)(a.pe + ((int64_t)s * a.vpad + r) * a.dp + d);
+    const float g = exp2f(-Form<T>::shift_table) * fabsf(a.scale) * f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o.v[j] = (T)(x[j] * g);
+    store_pack<T, 4>(ge + r * a.D + d, o, left);
   }
-  out[q] = v;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1042,6 +1131,7 @@ inline size_t lay_state(Args &a, int np, bool need_x, bool need_e, void *base) {
   const size_t xe = (size_t)a.npad * a.dp * np, ee = (size_t)a.vpad * a.dp * np;
   a.count = s.take<int>(64);
   a.emax = s.take<uint32_t>(64);
+  a.ticket = s.take<uint32_t>(64);
   a.rowid = s.take<int>(a.npad);
   a.lab = s.take<int>(a.npad);
   a.lse = s.take<float>(a.npad);
@@ -1068,7 +1158,7 @@ inline size_t lay_forward(Args &a, int np, bool need_x, void *base) {
 
 inline size_t lay_backward(Args &a, bool need_e, void *base) {
   Space s{(char *)base, 0};
-  a.gmax = s.take<uint32_t>(64);
+  a.gmax = s.take<uint32_t>((size_t)((a.npad + kGradChunk - 1) / kGradChunk) + 1);
   a.grow = s.take<float>(a.npad);
   a.pe = need_e ? s.take<float>((size_t)a.tsplit * a.vpad * a.dp) : nullptr;
   return s.used;
@@ -1087,10 +1177,10 @@ inline int check(int64_t n, int64_t V, int D, double scale, int reduction) {
 }
 
 template <typename T, int DP>
-void launch_forward(const Args &a, bool need_x, const T *features, const T *table,
+void launch_forward(const Args &a, bool need_x, const T *features, const T *table, float *loss,
                     hipStream_t stream) {
   const int xtiles = (int)(a.npad / 32), etiles = a.vpad / 32;
-  hipLaunchKernelGGL((kd_xent_pack<T, DP>), dim3((unsigned)(xtiles + etiles)), dim3(kBlock), 0,
+  hipLaunchKernelGGL((kd_xent_pack<T, DP>), grid_of((int64_t)xtiles + etiles), dim3(kBlock), 0,
                      stream, a, xtiles, features, table);
   if (need_x) {
     constexpr int rows = Walk<T, DP, 1>::rows;
@@ -1101,6 +1191,9 @@ void launch_forward(const Args &a, bool need_x, const T *features, const T *tabl
     const dim3 grid((unsigned)((a.n + rows - 1) / rows), (unsigned)a.rsplit);
     hipLaunchKernelGGL((kd_xent_rows<T, DP, false>), grid, dim3(kBlock), 0, stream, a);
   }
+  constexpr int per = kBlock / (DP / 4);  // listed pixels a workgroup joins
+  hipLaunchKernelGGL((kd_xent_combine<T, DP / 4>), grid_of((a.n + per - 1) / per),
+                     dim3(kBlock), 0, stream, a, features, table, loss);
 }
 
 template <typename T, int DP>
@@ -1113,7 +1206,7 @@ void launch_table(const Args &a, hipStream_t stream) {
     hipLaunchKernelGGL((kd_xent_table<T, DP, false>), grid, dim3(kBlock), 0, stream, a);
 }
 
-inline unsigned blocks(int64_t n) { return (unsigned)((n + kBlock - 1) / kBlock); }
+inline int64_t blocks(int64_t n) { return (n + kBlock - 1) / kBlock; }
 
 template <typename T>
 int forward(int64_t n, int64_t V, int D, const T *features, const T *table, const int64_t *labels,
@@ -1130,30 +1223,27 @@ int forward(int64_t n, int64_t V, int D, const T *features, const T *table, cons
     return set_error(KD_ERR_WORKSPACE, "workspace too small: %zu < %zu or %zu < %zu", state_bytes,
                      ns, scratch_bytes, nw);
   ProfScope prof(K_XENT_FWD, stream);
-  if (reduction == 0 && n > 0)
-    hipLaunchKernelGGL(kd_xent_zero, dim3(std::min(blocks(n), 4096u)), dim3(kBlock), 0, stream, n,
-                       loss);
   const int nblk = (int)((n + kMapChunk - 1) / kMapChunk);
-  if (nblk > 0)
+  if (nblk <= kListChunks) {  // one workgroup lists them all in less time than two launches take
+    hipLaunchKernelGGL(kd_xent_map, dim3(1), dim3(kBlock), 0, stream, a, kListChunks, false, labels,
+                       loss);
+  } else {
     hipLaunchKernelGGL(kd_xent_count, dim3(nblk), dim3(kBlock), 0, stream, n, V, labels, a.blk);
-  hipLaunchKernelGGL(kd_xent_scan, dim3(1), dim3(kBlock), 0, stream, nblk, a.blk, a.count,
-                     a.emax);
+    const bool scan = nblk > kSumChunks;
+    if (scan) hipLaunchKernelGGL(kd_xent_scan, dim3(1), dim3(kBlock), 0, stream, nblk, a.blk);
+    hipLaunchKernelGGL(kd_xent_map, dim3(nblk), dim3(kBlock), 0, stream, a, 1, scan, labels, loss);
+  }
   if (n > 0) {
-    hipLaunchKernelGGL(kd_xent_map, dim3(nblk), dim3(kBlock), 0, stream, n, V, labels, a.blk,
-                       a.rowid, a.lab);
     switch (a.dp) {
-      case 32: launch_forward<T, 32>(a, need_x, features, table, stream); break;
-      case 64: launch_forward<T, 64>(a, need_x, features, table, stream); break;
-      case 128: launch_forward<T, 128>(a, need_x, features, table, stream); break;
-      default: launch_forward<T, 256>(a, need_x, features, table, stream); break;
+      case 32: launch_forward<T, 32>(a, need_x, features, table, loss, stream); break;
+      case 64: launch_forward<T, 64>(a, need_x, features, table, loss, stream); break;
+      case 128: launch_forward<T, 128>(a, need_x, features, table, loss, stream); break;
+      default: launch_forward<T, 256>(a, need_x, features, table, loss, stream); break;
     }
-    hipLaunchKernelGGL(kd_xent_combine<T>, dim3((unsigned)((n + 3) / 4)), dim3(kBlock), 0, stream,
-                       a, features, table, loss);
   }
-  if (reduction != 0) {
-    hipLaunchKernelGGL(kd_xent_sum, dim3(kReduceBlocks), dim3(kBlock), 0, stream, a);
-    hipLaunchKernelGGL(kd_xent_finish, dim3(1), dim3(kBlock), 0, stream, a, loss);
-  }
+  if (reduction != 0)
+    hipLaunchKernelGGL(kd_xent_sum, dim3(n > 16 * kBlock ? kReduceBlocks : 1), dim3(kBlock), 0,
+                       stream, a, loss);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return set_error(KD_ERR_LAUNCH, "surface_cross_entropy: %s", hipGetErrorString(e));
@@ -1177,25 +1267,23 @@ int backward(int64_t n, int64_t V, int D, const int64_t *labels, double scale, i
     return set_error(KD_ERR_WORKSPACE, "workspace too small: %zu < %zu or %zu < %zu", state_bytes,
                      ns, scratch_bytes, nw);
   ProfScope prof(K_XENT_BWD, stream);
-  if (gx && n > 0)
-    hipLaunchKernelGGL(kd_xent_grad_features<T>, dim3(blocks(n * D)), dim3(kBlock), 0, stream, a,
-                       labels, grad, gx);
   if (ge) {
-    if (reduction == 0) {
-      hipLaunchKernelGGL(kd_xent_zero, dim3(1), dim3(kBlock), 0, stream, (int64_t)64,
-                         (float *)a.gmax);
-      if (n > 0)
-        hipLaunchKernelGGL(kd_xent_rowgrad, dim3(blocks(a.npad)), dim3(kBlock), 0, stream, a, grad);
-    }
+    if (reduction == 0)
+      hipLaunchKernelGGL(kd_xent_rowgrad,
+                         dim3((unsigned)std::max<int64_t>((a.npad + kGradChunk - 1) / kGradChunk, 1)),
+                         dim3(kBlock), 0, stream, a, grad);
     switch (a.dp) {
       case 32: launch_table<T, 32>(a, stream); break;
       case 64: launch_table<T, 64>(a, stream); break;
       case 128: launch_table<T, 128>(a, stream); break;
       default: launch_table<T, 256>(a, stream); break;
     }
-    hipLaunchKernelGGL(kd_xent_table_join<T>, dim3(blocks((int64_t)V * D)), dim3(kBlock), 0, stream,
-                       a, grad, ge);
   }
+  const int vpr = (D + 3) / 4;
+  const int64_t xb = gx ? blocks(n * vpr) : 0, eb = ge ? blocks(V * vpr) : 0;
+  if (xb + eb > 0)
+    hipLaunchKernelGGL(kd_xent_grads<T>, grid_of(xb + eb), dim3(kBlock), 0, stream, a, xb, vpr, labels,
+                       grad, gx, ge);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return set_error(KD_ERR_LAUNCH, "surface_cross_entropy bwd: %s", hipGetErrorString(e));
