@@ -293,7 +293,7 @@ __global__ __launch_bounds__(kBlock) void kd_embed_segments(SegArgs a, const T *
                                                             typename Wide<T>::type *__restrict__ head,
                                                             typename Wide<T>::type *__restrict__ tail) {
   using A = typename Wide<T>::type;
-  constexpr int V = 16 / sizeof(T), U = 8;  // channels of a lane, gradient rows in flight
+  constexpr int V = 16 / sizeof(T), U = 4;  // channels of a lane, gradient rows in flight
   __shared__ A s_head[kBlock * V];
   __shared__ int s_kind[kBlock];
   const uint32_t n = *a.kept;

@@ -87,6 +87,7 @@ __device__ __forceinline__ void split3(float x, uint16_t &a, uint16_t &b, uint16
 }
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kSlots = 64, kSlotPad = 16;  // maxima of the table, 64 bytes apart
 constexpr int kRowPad = 256;  // packed rows are padded with zeros to a multiple of this
 constexpr int kMapChunk = 2048;   // pixels listed at a time
 constexpr int kListChunks = 4;    // up to so many chunks one workgroup lists them all
@@ -111,14 +112,14 @@ struct Args {
   int *rowid, *lab; // listed pixel -> pixel, its label
   float *lse, *w;   // exponent of a probability but its logit, its complement negated (scaled)
   float *xn;        // squared sizes of the pixels' features
-  uint32_t *emax;   // the largest squared size of the table's rows (its bits)
+  uint32_t *emax;   // the largest squared sizes of the table's rows (their bits), kSlots of them
   uint32_t *ticket; // workgroups that have added up their losses
   uint16_t *xs, *xt, *es;
   float *raw;       // (n, D): w (m - e_y)
   // scratch
   int *blk;
   uint16_t *et;
-  float *pm, *pl, *po;
+  float *pm, *pl, *pz, *po;  // a part's maximum, sum, label's logit (or -inf), weighted sum
   float *lrow;
   double *part;
   float *grow, *pe;
@@ -231,10 +232,12 @@ static __global__ __launch_bounds__(kBlock) void kd_xent_map(Args a, int chunks,
       run += total;
     }
   }
-  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
-    *a.count = run;
-    *a.emax = 0u;
-    *a.ticket = 0u;
+  if (blockIdx.x == gridDim.x - 1) {
+    if (threadIdx.x < kSlots) a.emax[threadIdx.x * kSlotPad] = 0u;
+    if (threadIdx.x == 0) {
+      *a.count = run;
+      *a.ticket = 0u;
+    }
   }
 }
 
@@ -250,6 +253,8 @@ __global__ __launch_bounds__(kBlock) void kd_xent_pack(Args a, int xtiles,
   constexpr int V = 16 / sizeof(T);
   constexpr int kPitch = DP + V;  // rows 16 bytes apart over the banks
   __shared__ __align__(16) T s_m[32 * kPitch];
+  __shared__ uint32_t s_top[kBlock / kWave];
+  uint32_t top = 0;
   const int64_t bid = block_id();
   const bool is_x = bid < xtiles;
   const int64_t tile = is_x ? bid : bid - xtiles;
@@ -286,14 +291,13 @@ __global__ __launch_bounds__(kBlock) void kd_xent_pack(Args a, int xtiles,
     if (is_x) {
       if (d == 0) a.xn[i] = size;
     } else {
-      uint32_t u = __float_as_uint(size);
-#pragma unroll
-      for (int k = 32; k >= kLanes; k >>= 1) u = max(u, (uint32_t)__shfl_xor((int)u, k));
-      // the look before saves all but the few atomics that raise it: one address, many tiles
-      if ((threadIdx.x & 63) == 0 &&
-          u > __hip_atomic_load(a.emax, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
-        atomicMax(a.emax, u);
+      top = max(top, __float_as_uint(size));
     }
+  }
+  if (!is_x) {  // one atomic a workgroup, spread over the slots: they would queue at one address
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, k));
+    if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = top;
   }
   if (is_x && threadIdx.x < 32 && r0 + threadIdx.x >= count) {
     a.lab[r0 + threadIdx.x] = -1;
@@ -301,6 +305,9 @@ __global__ __launch_bounds__(kBlock) void kd_xent_pack(Args a, int xtiles,
     a.w[r0 + threadIdx.x] = 0.f;
   }
   __syncthreads();
+  if (!is_x && threadIdx.x == 0)
+    atomicMax(a.emax + tile % kSlots * kSlotPad,
+              max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3])));
   constexpr int kGroups = 32 * DP / 8;  // 16-byte groups per plane and layout
   uint16_t *straight = (is_x ? a.xs : a.es) + tile * F::np * 32 * DP;
   uint16_t *transposed = is_x ? a.xt : a.et;
@@ -602,7 +609,7 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
   using H8 = typename F::H8;
   static constexpr int NP = B::NP, RB = B::RB, DT = B::DT;
   int lab[RB];
-  float m[RB], l[RB][2];
+  float m[RB], l[RB][2], zy[RB];
   int V;
   float c2;
 
@@ -620,6 +627,7 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int v = first + 8 * (i >> 2) + (i & 3);
+          zy[b] = v == lab[b] ? this->s[b][i] : zy[b];
           this->s[b][i] = v == lab[b] || v >= V ? -INFINITY : this->s[b][i];
         }
     }
@@ -702,7 +710,10 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
   w.c2 = a.c2;
   // |logit| <= |x| |e| scale, over the kRowPad rows about this wave's (so that the choice does not
   // depend on how many of them a wave holds); a NaN size takes the general way
-  const float size = a.c2 * sqrtf(__uint_as_float(*a.emax));
+  uint32_t big = a.emax[lane * kSlotPad];
+#pragma unroll
+  for (int k = 32; k >= 1; k >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, k));
+  const float size = a.c2 * sqrtf(__uint_as_float(big));
   bool safe = F::shift == 0.f;
 #pragma unroll
   for (int k = 0; k < kRowPad / kWave; ++k)
@@ -714,6 +725,7 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
     w.lab[b] = a.lab[row0 + 32 * b + (lane & 31)];
     w.m[b] = general ? -1e30f : 0.f;
     w.l[b][0] = w.l[b][1] = 0.f;
+    w.zy[b] = -INFINITY;
   }
   // tiles come in pairs, for the two buffers
   const int npair = (a.V + 63) / 64;
@@ -757,7 +769,9 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
     const int64_t r = part + row0 + 32 * b + (lane & 31);
     float l = w.l[b][0] + w.l[b][1];
     l += __shfl_xor(l, 32);
+    const float other = __shfl_xor(w.zy[b], 32);  // one of the halves has met the label, or none
     if (half == 0 && z == 0) {
+      a.pz[r] = w.zy[b] == -INFINITY ? other : w.zy[b];
       a.pm[r] = w.m[b] - F::shift;
       a.pl[r] = l;
     }
@@ -766,42 +780,54 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
 }
 
 // ------------------------------------------------------------------------------------------------
-// joining the parts: G lanes per listed pixel, four channels a lane at a time
+// joining the parts: G lanes per listed pixel; with RAW, four channels of dX a lane
 // ------------------------------------------------------------------------------------------------
-template <typename T, int G>
-__global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__restrict__ features,
-                                                          const T *__restrict__ table,
+constexpr int kFewParts = 16;
+
+template <typename T, int G, bool RAW>
+__global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__restrict__ table,
                                                           float *__restrict__ loss) {
   const int gl = threadIdx.x & (G - 1);
   const int64_t r = block_id() * (kBlock / G) + threadIdx.x / G;
   if (r >= *a.count) return;
-  const int64_t i = a.rowid[r], y = a.lab[r];
+  const int64_t i = a.rowid[r];
   const int d = 4 * gl, left = a.D - d;  // (D <= 4 G)
   Pack<T, 4> e;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) e.v[j] = (T)0.f;
-  float z = 0.f;
-  if (left > 0) {
-    e = load_pack<T, 4>(table + y * a.D + d, left);
-    const Pack<T, 4> x = load_pack<T, 4>(features + i * a.D + d, left);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) z = fmaf((float)x.v[j], (float)e.v[j], z);
+  f32x4 o = (f32x4)(0.f);
+  if (RAW && left > 0) {
+    e = load_pack<T, 4>(table + (int64_t)a.lab[r] * a.D + d, left);
+    if (a.rsplit == 1) o = *(const f32x4 *)(a.po + r * a.dp + d);
   }
-  float m = -1e30f;
-  for (int s = gl; s < a.rsplit; s += G) m = fmaxf(m, a.pm[(int64_t)s * a.npad + r]);
-#pragma unroll
-  for (int s = G / 2; s >= 1; s >>= 1) {
-    z += __shfl_xor(z, s);
-    m = fmaxf(m, __shfl_xor(m, s));
+  // few parts: every lane goes through them all; the order of the sum is the same whatever G
+  const bool few = a.rsplit < kFewParts;
+  const int s0 = few ? 0 : gl, ds = few ? 1 : G;
+  float m = -1e30f, z = -INFINITY;
+#pragma unroll 4
+  for (int s = s0; s < a.rsplit; s += ds) {
+    const int64_t q = (int64_t)s * a.npad + r;
+    const float part = a.pz[q];
+    m = fmaxf(m, a.pm[q]);
+    z = part == -INFINITY ? z : part;  // (a NaN stays)
   }
-  const float z2 = z * (a.scale * kLog2e);
+  if (!few) {
+#pragma unroll
+    for (int s = G / 2; s >= 1; s >>= 1) {
+      const float part = __shfl_xor(z, s);
+      m = fmaxf(m, __shfl_xor(m, s));
+      z = part == -INFINITY ? z : part;
+    }
+  }
+  const float z2 = z * (fabsf(a.scale) * kLog2e);
   float l = 0.f;
-  for (int s = gl; s < a.rsplit; s += G) {
+#pragma unroll 4
+  for (int s = s0; s < a.rsplit; s += ds) {
     const int64_t q = (int64_t)s * a.npad + r;
     l += a.pl[q] * __builtin_amdgcn_exp2f(a.pm[q] - m);
   }
+  if (!few) {
 #pragma unroll
-  for (int s = G / 2; s >= 1; s >>= 1) l += __shfl_xor(l, s);
+    for (int s = G / 2; s >= 1; s >>= 1) l += __shfl_xor(l, s);
+  }
   const float u = (m + log2f(l) - z2) * kLn2;  // -inf when the label is the only row
   const float t = expf(-fabsf(u));
   const float value = fmaxf(u, 0.f) + log1pf(t);
@@ -816,18 +842,21 @@ __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__res
     else
       a.lrow[r] = out;
   }
-  if (!a.raw || left <= 0) return;
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  f32x4 o = (f32x4)(0.f);
+  if constexpr (RAW) {
+    if (left <= 0) return;
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    if (a.rsplit > 1) {
 #pragma unroll 4
-  for (int s = 0; s < a.rsplit; ++s) {
-    const int64_t q = (int64_t)s * a.npad + r;
-    o += *(const f32x4 *)(a.po + q * a.dp + d) * __builtin_amdgcn_exp2f(a.pm[q] - m);
-  }
-  Pack<float, 4> v;
+      for (int s = 0; s < a.rsplit; ++s) {
+        const int64_t q = (int64_t)s * a.npad + r;
+        o += *(const f32x4 *)(a.po + q * a.dp + d) * __builtin_amdgcn_exp2f(a.pm[q] - m);
+      }
+    }
+    Pack<float, 4> v;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v.v[j] = wn * (o[j] * inv - (float)e.v[j]);
-  store_pack<float, 4>(a.raw + i * a.D + d, v, left);
+    for (int j = 0; j < 4; ++j) v.v[j] = wn * (o[j] * inv - (float)e.v[j]);
+    store_pack<float, 4>(a.raw + i * a.D + d, v, left);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1130,7 +1159,7 @@ inline size_t lay_state(Args &a, int np, bool need_x, bool need_e, void *base) {
   Space s{(char *)base, 0};
   const size_t xe = (size_t)a.npad * a.dp * np, ee = (size_t)a.vpad * a.dp * np;
   a.count = s.take<int>(64);
-  a.emax = s.take<uint32_t>(64);
+  a.emax = s.take<uint32_t>(kSlots * kSlotPad);
   a.ticket = s.take<uint32_t>(64);
   a.rowid = s.take<int>(a.npad);
   a.lab = s.take<int>(a.npad);
@@ -1150,6 +1179,7 @@ inline size_t lay_forward(Args &a, int np, bool need_x, void *base) {
   a.et = need_x ? s.take<uint16_t>((size_t)a.vpad * a.dp * np) : nullptr;
   a.pm = s.take<float>((size_t)a.rsplit * a.npad);
   a.pl = s.take<float>((size_t)a.rsplit * a.npad);
+  a.pz = s.take<float>((size_t)a.rsplit * a.npad);
   a.po = need_x ? s.take<float>((size_t)a.rsplit * a.npad * a.dp) : nullptr;
   a.lrow = s.take<float>(a.npad);
   a.part = s.take<double>(kReduceBlocks);
@@ -1191,9 +1221,17 @@ void launch_forward(const Args &a, bool need_x, const T *features, const T *tabl
     const dim3 grid((unsigned)((a.n + rows - 1) / rows), (unsigned)a.rsplit);
     hipLaunchKernelGGL((kd_xent_rows<T, DP, false>), grid, dim3(kBlock), 0, stream, a);
   }
-  constexpr int per = kBlock / (DP / 4);  // listed pixels a workgroup joins
-  hipLaunchKernelGGL((kd_xent_combine<T, DP / 4>), grid_of((a.n + per - 1) / per),
-                     dim3(kBlock), 0, stream, a, features, table, loss);
+  auto combine = [&](auto lanes, auto raw) {
+    constexpr int G = decltype(lanes)::value, per = kBlock / G;  // listed pixels a workgroup joins
+    hipLaunchKernelGGL((kd_xent_combine<T, G, decltype(raw)::value>),
+                       grid_of((a.n + per - 1) / per), dim3(kBlock), 0, stream, a, table, loss);
+  };
+  if (need_x)
+    combine(std::integral_constant<int, DP / 4>{}, std::true_type{});
+  else if (a.rsplit >= kFewParts)
+    combine(std::integral_constant<int, DP / 4>{}, std::false_type{});
+  else
+    combine(std::integral_constant<int, 1>{}, std::false_type{});
 }
 
 template <typename T, int DP>
