@@ -106,7 +106,6 @@ struct Args {
   float c2;         // |scale| log2(e)
   float scale;
   int reduction;    // 0 none, 1 mean, 2 sum
-  int rsplit, tsplit;
   // state kept from forward to backward
   int *count;       // pixels with a label
   int *rowid, *lab; // listed pixel -> pixel, its label
@@ -391,21 +390,102 @@ __device__ __forceinline__ void pack_pair(float p0, float p1, int i, uint4 *o) {
 }
 
 // How a walk is laid out (KIND 0: over the table, loss only; 1: over the table with dX; 2: over the
-// pixels, dE).  rb: blocks of 32 rows that a wave holds; two double the products per operand read from
-// LDS, the registers of wide or split operands allow one.  waves: per SIMD, at least; one where the
-// held operands, the sums and two blocks of logits need more than 256 registers.  cs: into how many
-// column ranges the sums are cut, over workgroups that each form the logits: two where the operands
-// of all columns would not fit LDS twice.
+// pixels, dE), for np planes and dp channels.
+// Blocks of 32 rows that a wave holds: two double the products per operand read from LDS, the
+// registers of wide or split operands allow one.
+constexpr int walk_blocks(int np, int dp, int kind) {
+  return np == 1 && (dp <= 64 || (dp == 128 && kind == 0)) ? 2 : 1;
+}
+// Waves per SIMD: one where the held operands, the sums and two blocks of logits need more than 256
+// registers.
+constexpr int walk_waves(int np, int dp, int kind) {
+  return (np == 1 ? dp == 256 && kind > 0 : dp >= (kind > 0 ? 128 : 256)) ? 1 : 2;
+}
+// Into how many column ranges the sums are cut, over workgroups that each form the logits: two where
+// the operands of all columns would not fit LDS twice.
+constexpr int walk_columns(int np, int dp, int kind) {
+  return np == 3 && dp == 256 && kind > 0 ? 2 : 1;
+}
+constexpr int walk_rows(int np, int dp, int kind) { return 128 * walk_blocks(np, dp, kind); }
+// Workgroups: as many as run at once on 256 compute units.
+constexpr int walk_workers(int np, int dp, int kind) {
+  return 256 * walk_waves(np, dp, kind) / walk_columns(np, dp, kind);
+}
+
 template <typename T, int DP, int KIND>
 struct Walk {
   static constexpr int np = Form<T>::np;
-  static constexpr int rb = np == 1 && (DP <= 64 || (DP == 128 && KIND == 0)) ? 2 : 1;
-  static constexpr int waves = (np == 1 ? DP == 256 && KIND > 0 : DP >= (KIND > 0 ? 128 : 256)) ? 1 : 2;
-  static constexpr int cs = np == 3 && DP == 256 && KIND > 0 ? 2 : 1;
-  static constexpr int rows = 4 * 32 * rb;             // held by a workgroup
+  static constexpr int rb = walk_blocks(np, DP, KIND);
+  static constexpr int waves = walk_waves(np, DP, KIND);
+  static constexpr int cs = walk_columns(np, DP, KIND);
+  static constexpr int rows = walk_rows(np, DP, KIND);  // held by a workgroup
+  static constexpr int workers = walk_workers(np, DP, KIND);
   static constexpr int tile_bytes = np * 32 * DP * 2;  // a tile's operands: a multiple of 1024
   static constexpr int sum_bytes = tile_bytes / cs;    // of the weighted sum
 };
+
+// How the work is dealt to the workgroups that run at once: `blocks` blocks of held rows, each walked
+// over `pairs` pairs of tiles.  Every workgroup takes the same number of whole blocks, all of them
+// walking in step so that they read the same tiles at the same time; the blocks that are left over
+// are dealt evenly by pairs, across their borders.  So no round is left half empty, with few blocks
+// as with many, and the count of pixels with a label need not be known on the host.
+// A block's parts (one, or those of the left-over deal) stand in consecutive slots.
+struct Deal {
+  int pairs, full, rem, nw;  // whole blocks a worker, blocks left over, workers that share those
+  int64_t units;
+  int workers;
+  __device__ __forceinline__ Deal(int64_t blocks, int pairs_, int workers_)
+      : pairs(pairs_), workers(workers_) {
+    full = (int)(blocks / workers);
+    rem = (int)(blocks - (int64_t)full * workers);
+    units = (int64_t)rem * pairs;
+    nw = (int)min((int64_t)workers, units);
+  }
+  __device__ __forceinline__ int64_t begin(int w) const { return units * w / nw; }
+  // the slots of a block's parts
+  __device__ __forceinline__ void parts(int64_t block, int64_t &slot, int &n) const {
+    const int64_t whole = (int64_t)full * workers;
+    if (block < whole) {
+      slot = block;
+      n = 1;
+    } else if (units == 0) {
+      slot = 0;
+      n = 0;
+    } else {
+      const int64_t t = block - whole;
+      const int64_t w0 = ((t * pairs + 1) * nw - 1) / units;
+      const int64_t w1 = ((t + 1) * pairs * nw - 1) / units;
+      slot = whole + w0 + t;
+      n = (int)(w1 - w0) + 1;
+    }
+  }
+  // calls f(block, first pair, last pair, slot) for worker w's share
+  template <typename F>
+  __device__ __forceinline__ void each(int w, F f) const {
+    int64_t u = 0, end = 0;
+    if (w < nw) {
+      u = begin(w);
+      end = begin(w + 1);
+    }
+    for (int k = 0;; ++k) {  // (one call: the walks are long)
+      int64_t block = (int64_t)k * workers + w, slot = block;
+      int p0 = 0, p1 = pairs;
+      if (k >= full) {
+        if (u >= end) break;
+        const int t = (int)(u / pairs);
+        p0 = (int)(u - (int64_t)t * pairs);
+        p1 = (int)min((int64_t)pairs, p0 + (end - u));
+        u += p1 - p0;
+        block = (int64_t)full * workers + t;
+        slot = block + w;
+      }
+      f(block, p0, p1, slot);
+    }
+  }
+};
+inline int64_t deal_slots(int64_t rows, int np, int dp, int kind) {
+  return rows / walk_rows(np, dp, kind) + walk_workers(np, dp, kind) + 1;
+}
 
 // The waves that share a SIMD take different priorities (by their slot): waves of the same priority
 // fall into step, all in their products and then all in their exponentials, and leave one of the two
@@ -702,81 +782,78 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
   __shared__ uint4 s_t0[SUM ? W::sum_bytes / 16 : 1], s_t1[SUM ? W::sum_bytes / 16 : 1];
   const int z = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int64_t row0 = ((int64_t)blockIdx.x * 4 + wave) * (32 * RB);
-  if ((int64_t)blockIdx.x * W::rows >= *a.count) return;
+  const Deal deal(((int64_t)*a.count + W::rows - 1) / W::rows, (a.V + 63) / 64, W::workers);
   stagger();
   RowsWalk<T, DP, SUM> w;
   w.V = a.V;
   w.c2 = a.c2;
-  // |logit| <= |x| |e| scale, over the kRowPad rows about this wave's (so that the choice does not
-  // depend on how many of them a wave holds); a NaN size takes the general way
   uint32_t big = a.emax[lane * kSlotPad];
 #pragma unroll
   for (int k = 32; k >= 1; k >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, k));
   const float size = a.c2 * sqrtf(__uint_as_float(big));
-  bool safe = F::shift == 0.f;
-#pragma unroll
-  for (int k = 0; k < kRowPad / kWave; ++k)
-    safe &= size * sqrtf(a.xn[row0 / kRowPad * kRowPad + k * kWave + lane]) < kSafeLogit;
-  const bool general = !__all(safe);
-  w.hold(a.xs, row0);
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    w.lab[b] = a.lab[row0 + 32 * b + (lane & 31)];
-    w.m[b] = general ? -1e30f : 0.f;
-    w.l[b][0] = w.l[b][1] = 0.f;
-    w.zy[b] = -INFINITY;
-  }
-  // tiles come in pairs, for the two buffers
-  const int npair = (a.V + 63) / 64;
-  const int t0 = (int)((int64_t)npair * blockIdx.y / gridDim.y) * 2;
-  const int t1 = (int)((int64_t)npair * (blockIdx.y + 1) / gridDim.y) * 2;
   const uint16_t *es = a.es, *et = a.et;
   constexpr int64_t kTile = kBytes / 2;
-  auto walk = [&](auto online) {
-    constexpr bool ONLINE = decltype(online)::value;
-    fetch<kBytes>(s_e0, es + t0 * kTile);
-    arrive();
-    fetch<kBytes>(s_e1, es + (t0 + 1) * kTile);
-    if constexpr (SUM) fetch_sum<W>(s_t1, et + t0 * kTile, z);  // (times zeros)
-    w.logits(s_e0);
-    w.template ready<ONLINE>(t0 * 32);
-    arrive();
-    for (int t = t0; t < t1; t += 2) {
-      const int t2 = min(t + 2, t1 - 1), t3 = min(t + 3, t1 - 1);  // behind the end: not used
-      fetch<kBytes>(s_e0, es + t2 * kTile);
-      if constexpr (SUM) fetch_sum<W>(s_t0, et + t * kTile, z);
-      w.template next<ONLINE>(s_e1, s_t1);
-      w.template ready<ONLINE>((t + 1) * 32);
-      arrive();
-      fetch<kBytes>(s_e1, es + t3 * kTile);
-      if constexpr (SUM) fetch_sum<W>(s_t1, et + (t + 1) * kTile, z);
-      w.template next<ONLINE>(s_e0, s_t0);
-      w.template ready<ONLINE>(t2 * 32);
-      arrive();
+  deal.each(blockIdx.x, [&](int64_t block, int p0, int p1, int64_t slot) {
+    const int64_t row0 = block * W::rows + wave * (32 * RB);
+    // |logit| <= |x| |e| scale, over the kRowPad rows about this wave's (so that the choice does not
+    // depend on how many of them a wave holds); a NaN size takes the general way
+    bool safe = F::shift == 0.f;
+#pragma unroll
+    for (int k = 0; k < kRowPad / kWave; ++k)
+      safe &= size * sqrtf(a.xn[row0 / kRowPad * kRowPad + k * kWave + lane]) < kSafeLogit;
+    const bool general = !__all(safe);
+    w.hold(a.xs, row0);
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      w.lab[b] = a.lab[row0 + 32 * b + (lane & 31)];
+      w.m[b] = general ? -1e30f : 0.f;
+      w.l[b][0] = w.l[b][1] = 0.f;
+      w.zy[b] = -INFINITY;
     }
-    if constexpr (SUM) w.add(s_t1);
-  };
-  if (t0 < t1) {
+    const int t0 = 2 * p0, t1 = 2 * p1;
+    auto walk = [&](auto online) {
+      constexpr bool ONLINE = decltype(online)::value;
+      fetch<kBytes>(s_e0, es + t0 * kTile);
+      arrive();
+      fetch<kBytes>(s_e1, es + (t0 + 1) * kTile);
+      if constexpr (SUM) fetch_sum<W>(s_t1, et + t0 * kTile, z);  // (times zeros)
+      w.logits(s_e0);
+      w.template ready<ONLINE>(t0 * 32);
+      arrive();
+      for (int t = t0; t < t1; t += 2) {
+        const int t2 = min(t + 2, t1 - 1), t3 = min(t + 3, t1 - 1);  // behind the end: not used
+        fetch<kBytes>(s_e0, es + t2 * kTile);
+        if constexpr (SUM) fetch_sum<W>(s_t0, et + t * kTile, z);
+        w.template next<ONLINE>(s_e1, s_t1);
+        w.template ready<ONLINE>((t + 1) * 32);
+        arrive();
+        fetch<kBytes>(s_e1, es + t3 * kTile);
+        if constexpr (SUM) fetch_sum<W>(s_t1, et + (t + 1) * kTile, z);
+        w.template next<ONLINE>(s_e0, s_t0);
+        w.template ready<ONLINE>(t2 * 32);
+        arrive();
+      }
+      if constexpr (SUM) w.add(s_t1);
+    };
     if (general)
       walk(std::true_type{});
     else
       walk(std::false_type{});
-  }
-  const int64_t part = (int64_t)blockIdx.y * a.npad;
+    const int64_t out = slot * W::rows + wave * (32 * RB);
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const int64_t r = part + row0 + 32 * b + (lane & 31);
-    float l = w.l[b][0] + w.l[b][1];
-    l += __shfl_xor(l, 32);
-    const float other = __shfl_xor(w.zy[b], 32);  // one of the halves has met the label, or none
-    if (half == 0 && z == 0) {
-      a.pz[r] = w.zy[b] == -INFINITY ? other : w.zy[b];
-      a.pm[r] = w.m[b] - F::shift;
-      a.pl[r] = l;
+    for (int b = 0; b < RB; ++b) {
+      const int64_t r = out + 32 * b + (lane & 31);
+      float l = w.l[b][0] + w.l[b][1];
+      l += __shfl_xor(l, 32);
+      const float other = __shfl_xor(w.zy[b], 32);  // one of the halves has met the label, or none
+      if (half == 0 && z == 0) {
+        a.pz[r] = w.zy[b] == -INFINITY ? other : w.zy[b];
+        a.pm[r] = w.m[b] - F::shift;
+        a.pl[r] = l;
+      }
     }
-  }
-  if constexpr (SUM) w.store(a.po, part + row0, z * (DP / W::cs));
+    if constexpr (SUM) w.store(a.po, out, z * (DP / W::cs));
+  });
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -784,27 +861,34 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
 // ------------------------------------------------------------------------------------------------
 constexpr int kFewParts = 16;
 
-template <typename T, int G, bool RAW>
+template <typename T, int DP, int G, bool RAW>
 __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__restrict__ table,
                                                           float *__restrict__ loss) {
   const int gl = threadIdx.x & (G - 1);
   const int64_t r = block_id() * (kBlock / G) + threadIdx.x / G;
-  if (r >= *a.count) return;
+  const int count = *a.count;
+  if (r >= count) return;
   const int64_t i = a.rowid[r];
+  using W = Walk<T, DP, RAW ? 1 : 0>;
+  int64_t slot;
+  int n;
+  Deal(((int64_t)count + W::rows - 1) / W::rows, (a.V + 63) / 64, W::workers)
+      .parts(r / W::rows, slot, n);
+  const int64_t first = slot * W::rows + r % W::rows;
   const int d = 4 * gl, left = a.D - d;  // (D <= 4 G)
   Pack<T, 4> e;
   f32x4 o = (f32x4)(0.f);
   if (RAW && left > 0) {
     e = load_pack<T, 4>(table + (int64_t)a.lab[r] * a.D + d, left);
-    if (a.rsplit == 1) o = *(const f32x4 *)(a.po + r * a.dp + d);
+    if (n == 1) o = *(const f32x4 *)(a.po + first * DP + d);
   }
-  // few parts: every lane goes through them all; the order of the sum is the same whatever G
-  const bool few = a.rsplit < kFewParts;
+  const bool few = n < kFewParts;  // every lane goes through them all
+
   const int s0 = few ? 0 : gl, ds = few ? 1 : G;
   float m = -1e30f, z = -INFINITY;
 #pragma unroll 4
-  for (int s = s0; s < a.rsplit; s += ds) {
-    const int64_t q = (int64_t)s * a.npad + r;
+  for (int s = s0; s < n; s += ds) {
+    const int64_t q = first + (int64_t)s * W::rows;
     const float part = a.pz[q];
     m = fmaxf(m, a.pm[q]);
     z = part == -INFINITY ? z : part;  // (a NaN stays)
@@ -820,8 +904,8 @@ __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__res
   const float z2 = z * (fabsf(a.scale) * kLog2e);
   float l = 0.f;
 #pragma unroll 4
-  for (int s = s0; s < a.rsplit; s += ds) {
-    const int64_t q = (int64_t)s * a.npad + r;
+  for (int s = s0; s < n; s += ds) {
+    const int64_t q = first + (int64_t)s * W::rows;
     l += a.pl[q] * __builtin_amdgcn_exp2f(a.pm[q] - m);
   }
   if (!few) {
@@ -845,11 +929,11 @@ __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__res
   if constexpr (RAW) {
     if (left <= 0) return;
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    if (a.rsplit > 1) {
+    if (n > 1) {
 #pragma unroll 4
-      for (int s = 0; s < a.rsplit; ++s) {
-        const int64_t q = (int64_t)s * a.npad + r;
-        o += *(const f32x4 *)(a.po + q * a.dp + d) * __builtin_amdgcn_exp2f(a.pm[q] - m);
+      for (int s = 0; s < n; ++s) {
+        const int64_t q = first + (int64_t)s * W::rows;
+        o += *(const f32x4 *)(a.po + q * DP + d) * __builtin_amdgcn_exp2f(a.pm[q] - m);
       }
     }
     Pack<float, 4> v;
@@ -1020,9 +1104,9 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, 2>::waves)) void kd_xent_table
   __shared__ uint4 s_t0[W::sum_bytes / 16], s_t1[W::sum_bytes / 16];
   const int z = blockIdx.z;
   const int wave = threadIdx.x >> 6;
+  const Deal deal((a.V + W::rows - 1) / W::rows, (int)(((int64_t)*a.count + 63) / 64), W::workers);
   stagger();
   TableWalk<T, DP, ROWG> w;
-  w.v0 = ((int)blockIdx.x * 4 + wave) * (32 * RB);
   w.c2 = a.c2;
   w.unit = ROWG ? grad_unit(a) : 1.f;
   w.lunit = ROWG ? log2f(w.unit) : 0.f;  // a power of two: exact
@@ -1030,34 +1114,35 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, 2>::waves)) void kd_xent_table
   w.pw = a.w;
   w.pg = a.grow;
   w.plab = a.lab;
-  w.hold(a.es, w.v0);
-  const int npair = (int)(((int64_t)*a.count + 63) / 64);
-  const int t0 = (int)((int64_t)npair * blockIdx.y / gridDim.y) * 2;
-  const int t1 = (int)((int64_t)npair * (blockIdx.y + 1) / gridDim.y) * 2;
   const uint16_t *xs = a.xs, *xt = a.xt;
   constexpr int64_t kTile = kBytes / 2;
-  if (t0 < t1) {
-    fetch<kBytes>(s_x0, xs + t0 * kTile);
-    w.rows(t0, w.lse, w.g, w.near);
-    arrive();
-    fetch<kBytes>(s_x1, xs + (t0 + 1) * kTile);
-    fetch_sum<W>(s_t1, xt + t0 * kTile, z);  // (times zeros)
-    w.logits(s_x0);
-    arrive();
-    for (int t = t0; t < t1; t += 2) {
-      const int t2 = min(t + 2, t1 - 1), t3 = min(t + 3, t1 - 1);  // behind the end: not used
-      fetch<kBytes>(s_x0, xs + t2 * kTile);
-      fetch_sum<W>(s_t0, xt + t * kTile, z);
-      w.next(s_x1, s_t1, t, t + 1);
+  deal.each(blockIdx.x, [&](int64_t block, int p0, int p1, int64_t slot) {
+    w.v0 = (int)(block * W::rows) + wave * (32 * RB);
+    w.hold(a.es, w.v0);
+    const int t0 = 2 * p0, t1 = 2 * p1;
+    if (t0 < t1) {
+      fetch<kBytes>(s_x0, xs + t0 * kTile);
+      w.rows(t0, w.lse, w.g, w.near);
       arrive();
-      fetch<kBytes>(s_x1, xs + t3 * kTile);
-      fetch_sum<W>(s_t1, xt + (t + 1) * kTile, z);
-      w.next(s_x0, s_t0, t + 1, t2);
+      fetch<kBytes>(s_x1, xs + (t0 + 1) * kTile);
+      fetch_sum<W>(s_t1, xt + t0 * kTile, z);  // (times zeros)
+      w.logits(s_x0);
       arrive();
+      for (int t = t0; t < t1; t += 2) {
+        const int t2 = min(t + 2, t1 - 1), t3 = min(t + 3, t1 - 1);  // behind the end: not used
+        fetch<kBytes>(s_x0, xs + t2 * kTile);
+        fetch_sum<W>(s_t0, xt + t * kTile, z);
+        w.next(s_x1, s_t1, t, t + 1);
+        arrive();
+        fetch<kBytes>(s_x1, xs + t3 * kTile);
+        fetch_sum<W>(s_t1, xt + (t + 1) * kTile, z);
+        w.next(s_x0, s_t0, t + 1, t2);
+        arrive();
+      }
+      w.add(s_t1);
     }
-    w.add(s_t1);
-  }
-  w.store(a.pe, (int64_t)blockIdx.y * a.vpad + w.v0, z * (DP / W::cs));
+    w.store(a.pe, slot * W::rows + wave * (32 * RB), z * (DP / W::cs));
+  });
 }
 
 // The gradient's common factor: the incoming scalar, over the count for the mean.
@@ -1071,7 +1156,7 @@ __device__ __forceinline__ float grad_factor(const Args &a, const float *grad) {
 }
 
 // The first `xblocks` workgroups scale dX, the others join the parts of dE: four channels a thread.
-template <typename T>
+template <typename T, int DP>
 __global__ __launch_bounds__(kBlock) void kd_xent_grads(Args a, int64_t xblocks, int vpr,
                                                         const int64_t *__restrict__ labels,
                                                         const float *__restrict__ grad,
@@ -1102,9 +1187,14 @@ __global__ __launch_bounds__(kBlock) void kd_xent_grads(Args a, int64_t xblocks,
   } else {
     if (r >= a.V) return;
     f32x4 x = (f32x4)(0.f);
-#pragma unroll 4
-    for (int s = 0; s < a.tsplit; ++s)
-      x += *(const f32x4 *)(a.pe + ((int64_t)s * a.vpad + r) * a.dp + d);
+    using W = Walk<T, DP, 2>;
+    int64_t slot;
+    int n;
+    Deal((a.V + W::rows - 1) / W::rows, (int)(((int64_t)*a.count + 63) / 64), W::workers)
+        .parts(r / W::rows, slot, n);
+    const float *part = a.pe + (slot * W::rows + r % W::rows) * DP + d;
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) x += *(const f32x4 *)(part + (int64_t)s * W::rows * DP);
     const float g = exp2f(-Form<T>::shift_table) * fabsf(a.scale) * f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) o.v[j] = (T)(x[j] * g);
@@ -1128,16 +1218,6 @@ struct Space {
   }
 };
 
-// rows a workgroup holds, and into how many parts the other matrix is cut so that the grid fills
-// the chip when there are few rows to hold
-inline int held_rows(int np, int dp) { return 128 * (np == 1 && dp <= 64 ? 2 : 1); }
-inline int parts(int64_t held, int per, int64_t walked) {
-  const int64_t gx = (held + per - 1) / per, tiles = (walked + 31) / 32;
-  int64_t s = (1024 + gx - 1) / (gx > 0 ? gx : 1);
-  if (s > tiles) s = tiles;
-  return (int)(s < 1 ? 1 : (s > 1024 ? 1024 : s));
-}
-
 inline Args shape(int64_t n, int64_t V, int D, int np, double scale, int reduction) {
   Args a = {};
   a.n = n;
@@ -1150,8 +1230,6 @@ inline Args shape(int64_t n, int64_t V, int D, int np, double scale, int reducti
   // never 0: a masked logit, -inf, stays -inf (a scale of 0 makes every logit next to 0 all the same)
   a.c2 = (float)std::max(fabs(scale) * 1.4426950408889634, 1e-30);
   a.reduction = reduction;
-  a.rsplit = parts(n, held_rows(np, a.dp), V);
-  a.tsplit = parts(V, held_rows(np, a.dp), n);
   return a;
 }
 
@@ -1177,20 +1255,24 @@ inline size_t lay_forward(Args &a, int np, bool need_x, void *base) {
   Space s{(char *)base, 0};
   a.blk = s.take<int>((size_t)((a.n + kMapChunk - 1) / kMapChunk));
   a.et = need_x ? s.take<uint16_t>((size_t)a.vpad * a.dp * np) : nullptr;
-  a.pm = s.take<float>((size_t)a.rsplit * a.npad);
-  a.pl = s.take<float>((size_t)a.rsplit * a.npad);
-  a.pz = s.take<float>((size_t)a.rsplit * a.npad);
-  a.po = need_x ? s.take<float>((size_t)a.rsplit * a.npad * a.dp) : nullptr;
+  const int kind = need_x ? 1 : 0;
+  const size_t part =
+      (size_t)deal_slots(a.npad, np, a.dp, kind) * (size_t)walk_rows(np, a.dp, kind);
+  a.pm = s.take<float>(part);
+  a.pl = s.take<float>(part);
+  a.pz = s.take<float>(part);
+  a.po = need_x ? s.take<float>(part * a.dp) : nullptr;
   a.lrow = s.take<float>(a.npad);
   a.part = s.take<double>(kReduceBlocks);
   return s.used;
 }
 
-inline size_t lay_backward(Args &a, bool need_e, void *base) {
+inline size_t lay_backward(Args &a, int np, bool need_e, void *base) {
   Space s{(char *)base, 0};
   a.gmax = s.take<uint32_t>((size_t)((a.npad + kGradChunk - 1) / kGradChunk) + 1);
   a.grow = s.take<float>(a.npad);
-  a.pe = need_e ? s.take<float>((size_t)a.tsplit * a.vpad * a.dp) : nullptr;
+  const size_t part = (size_t)deal_slots(a.vpad, np, a.dp, 2) * (size_t)walk_rows(np, a.dp, 2);
+  a.pe = need_e ? s.take<float>(part * a.dp) : nullptr;
   return s.used;
 }
 
@@ -1206,45 +1288,53 @@ inline int check(int64_t n, int64_t V, int D, double scale, int reduction) {
   return KD_OK;
 }
 
+template <typename T, int DP, int KIND>
+dim3 walk_grid() {
+  return dim3(Walk<T, DP, KIND>::workers, 1, Walk<T, DP, KIND>::cs);
+}
+
 template <typename T, int DP>
 void launch_forward(const Args &a, bool need_x, const T *features, const T *table, float *loss,
                     hipStream_t stream) {
   const int xtiles = (int)(a.npad / 32), etiles = a.vpad / 32;
   hipLaunchKernelGGL((kd_xent_pack<T, DP>), grid_of((int64_t)xtiles + etiles), dim3(kBlock), 0,
                      stream, a, xtiles, features, table);
-  if (need_x) {
-    constexpr int rows = Walk<T, DP, 1>::rows;
-    const dim3 grid((unsigned)((a.n + rows - 1) / rows), (unsigned)a.rsplit, Walk<T, DP, 1>::cs);
-    hipLaunchKernelGGL((kd_xent_rows<T, DP, true>), grid, dim3(kBlock), 0, stream, a);
-  } else {
-    constexpr int rows = Walk<T, DP, 0>::rows;
-    const dim3 grid((unsigned)((a.n + rows - 1) / rows), (unsigned)a.rsplit);
-    hipLaunchKernelGGL((kd_xent_rows<T, DP, false>), grid, dim3(kBlock), 0, stream, a);
-  }
+  if (need_x)
+    hipLaunchKernelGGL((kd_xent_rows<T, DP, true>), (walk_grid<T, DP, 1>()), dim3(kBlock), 0,
+                       stream, a);
+  else
+    hipLaunchKernelGGL((kd_xent_rows<T, DP, false>), (walk_grid<T, DP, 0>()), dim3(kBlock), 0,
+                       stream, a);
   auto combine = [&](auto lanes, auto raw) {
     constexpr int G = decltype(lanes)::value, per = kBlock / G;  // listed pixels a workgroup joins
-    hipLaunchKernelGGL((kd_xent_combine<T, G, decltype(raw)::value>),
+    hipLaunchKernelGGL((kd_xent_combine<T, DP, G, decltype(raw)::value>),
                        grid_of((a.n + per - 1) / per), dim3(kBlock), 0, stream, a, table, loss);
   };
   if (need_x)
     combine(std::integral_constant<int, DP / 4>{}, std::true_type{});
-  else if (a.rsplit >= kFewParts)
+  else if (a.npad / Walk<T, DP, 0>::rows * kFewParts <= Walk<T, DP, 0>::workers)  // many parts
     combine(std::integral_constant<int, DP / 4>{}, std::false_type{});
   else
     combine(std::integral_constant<int, 1>{}, std::false_type{});
 }
 
-template <typename T, int DP>
-void launch_table(const Args &a, hipStream_t stream) {
-  constexpr int rows = Walk<T, DP, 2>::rows;
-  const dim3 grid((unsigned)((a.V + rows - 1) / rows), (unsigned)a.tsplit, Walk<T, DP, 2>::cs);
-  if (a.reduction == 0)
-    hipLaunchKernelGGL((kd_xent_table<T, DP, true>), grid, dim3(kBlock), 0, stream, a);
-  else
-    hipLaunchKernelGGL((kd_xent_table<T, DP, false>), grid, dim3(kBlock), 0, stream, a);
-}
-
 inline int64_t blocks(int64_t n) { return (n + kBlock - 1) / kBlock; }
+
+template <typename T, int DP>
+void launch_backward(const Args &a, const int64_t *labels, const float *grad, T *gx, T *ge,
+                     hipStream_t stream) {
+  if (ge && a.reduction == 0)
+    hipLaunchKernelGGL((kd_xent_table<T, DP, true>), (walk_grid<T, DP, 2>()), dim3(kBlock), 0, stream,
+                       a);
+  else if (ge)
+    hipLaunchKernelGGL((kd_xent_table<T, DP, false>), (walk_grid<T, DP, 2>()), dim3(kBlock), 0,
+                       stream, a);
+  const int vpr = (a.D + 3) / 4;
+  const int64_t xb = gx ? blocks(a.n * vpr) : 0, eb = ge ? blocks((int64_t)a.V * vpr) : 0;
+  if (xb + eb > 0)
+    hipLaunchKernelGGL((kd_xent_grads<T, DP>), grid_of(xb + eb), dim3(kBlock), 0, stream, a, xb, vpr,
+                       labels, grad, gx, ge);
+}
 
 template <typename T>
 int forward(int64_t n, int64_t V, int D, const T *features, const T *table, const int64_t *labels,
@@ -1300,28 +1390,21 @@ int backward(int64_t n, int64_t V, int D, const int64_t *labels, double scale, i
                "surface_cross_entropy: a gradient that the forward call did not prepare");
   Args a = shape(n, V, D, Form<T>::np, scale, reduction);
   const size_t ns = lay_state(a, Form<T>::np, need_x, need_e, state);
-  const size_t nw = lay_backward(a, ge != nullptr, scratch);
+  const size_t nw = lay_backward(a, Form<T>::np, ge != nullptr, scratch);
   if (!state || state_bytes < ns || !scratch || scratch_bytes < nw)
     return set_error(KD_ERR_WORKSPACE, "workspace too small: %zu < %zu or %zu < %zu", state_bytes,
                      ns, scratch_bytes, nw);
   ProfScope prof(K_XENT_BWD, stream);
-  if (ge) {
-    if (reduction == 0)
-      hipLaunchKernelGGL(kd_xent_rowgrad,
-                         dim3((unsigned)std::max<int64_t>((a.npad + kGradChunk - 1) / kGradChunk, 1)),
-                         dim3(kBlock), 0, stream, a, grad);
-    switch (a.dp) {
-      case 32: launch_table<T, 32>(a, stream); break;
-      case 64: launch_table<T, 64>(a, stream); break;
-      case 128: launch_table<T, 128>(a, stream); break;
-      default: launch_table<T, 256>(a, stream); break;
-    }
+  if (ge && reduction == 0)
+    hipLaunchKernelGGL(kd_xent_rowgrad,
+                       dim3((unsigned)std::max<int64_t>((a.npad + kGradChunk - 1) / kGradChunk, 1)),
+                       dim3(kBlock), 0, stream, a, grad);
+  switch (a.dp) {
+    case 32: launch_backward<T, 32>(a, labels, grad, gx, ge, stream); break;
+    case 64: launch_backward<T, 64>(a, labels, grad, gx, ge, stream); break;
+    case 128: launch_backward<T, 128>(a, labels, grad, gx, ge, stream); break;
+    default: launch_backward<T, 256>(a, labels, grad, gx, ge, stream); break;
   }
-  const int vpr = (D + 3) / 4;
-  const int64_t xb = gx ? blocks(n * vpr) : 0, eb = ge ? blocks(V * vpr) : 0;
-  if (xb + eb > 0)
-    hipLaunchKernelGGL(kd_xent_grads<T>, grid_of(xb + eb), dim3(kBlock), 0, stream, a, xb, vpr, labels,
-                       grad, gx, ge);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return set_error(KD_ERR_LAUNCH, "surface_cross_entropy bwd: %s", hipGetErrorString(e));

@@ -143,8 +143,10 @@ def test_loss_and_gradients(dname, n, V, D, scale, reduction):
     assert (got[1][y < 0] == 0).all()
     again = _run(x, e, y, scale, reduction, grad)
     assert all(torch.equal(a, b) for a, b in zip(got, again))  # a fixed order of the sums
+    # without gradients the parts of a sum can be cut elsewhere: the same bounds, not the same bits
     from kaolin_amd.metrics.render import surface_cross_entropy
-    assert torch.equal(surface_cross_entropy(x, e, y, scale, reduction), got[0])
+    _check((surface_cross_entropy(x, e, y, scale, reduction), *got[1:]),
+           _reference(x, e, y, scale, reduction, grad))
 
 
 @pytest.mark.parametrize('dname', ['f32', 'f16', 'bf16'])
@@ -419,7 +421,7 @@ def test_correspondence_step(dname):
     # bf16 pixels are rounded (2^-8), which moves logits of size |2 x.e| and what follows from them
     u = torch.finfo(dt).eps
     bound = u * 2.0 * float((px[hit].detach().abs() @ t64.detach().abs().t()).max()) * 4 + 1e-4
-    assert abs(float(loss) - float(ref)) <= bound
+    assert abs(float(loss.detach()) - float(ref.detach())) <= bound
     scale = float(t64.grad.abs().max())
     assert float((table.grad.double() - t64.grad).abs().max()) <= bound * scale
     for p in (vert, vfeat, table):
