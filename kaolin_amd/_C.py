@@ -774,11 +774,12 @@ def _number(fname, name, x):
 
 def _launch(dev, name, *args):
     """The native call on the current stream of `dev`, which need not be the current device."""
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
     if torch.cuda.current_device() == dev.index:
-        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+        _lib.call(name, *args, stream)
     else:
         with torch.cuda.device(dev):
-            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+            _lib.call(name, *args, stream)
 
 
 def _bytes(nb, dev):

@@ -33,7 +33,9 @@ constexpr int kMaxChannels = 1 << 20;
 // ------------------------------------------------------------------------------------------------
 // forward
 // ------------------------------------------------------------------------------------------------
-template <typename T>
+// WHOLE: rows are whole 16-byte vectors, 16-byte aligned.  The output is written past the caches: it
+// is larger than they are where its time counts, and the table's rows are what they should hold.
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kBlock) void kd_embed_gather(
     int64_t n, uint32_t per_batch, int64_t rows, int D, int rows_per_block,
     const int64_t *__restrict__ index, const T *__restrict__ table, typename Wide<T>::type scale,
@@ -59,7 +61,7 @@ __global__ __launch_bounds__(kBlock) void kd_embed_gather(
       if (k[u] >= 0 && k[u] < rows) {
         const int64_t row =
             per_batch ? (int64_t)((uint32_t)(r0 + lr[u]) / per_batch) * rows + k[u] : k[u];
-        o[u] = load_pack<T, V>(table + row * D + c[u], D - (int)c[u]);
+        o[u] = load_pack<T, V>(table + row * D + c[u], WHOLE ? V : D - (int)c[u]);
       } else {
 #pragma unroll
         for (int j = 0; j < V; ++j) o[u].v[j] = (T)0.f;
@@ -73,7 +75,13 @@ __global__ __launch_bounds__(kBlock) void kd_embed_gather(
 #pragma unroll
         for (int j = 0; j < V; ++j) o[u].v[j] = from_wide<T>(to_wide(o[u].v[j]) * scale);
       }
-      store_pack<T, V>(out + (r0 + lr[u]) * D + c[u], o[u], D - (int)c[u]);
+      T *to = out + (r0 + lr[u]) * D + c[u];
+      if constexpr (WHOLE) {
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        __builtin_nontemporal_store(__builtin_bit_cast(u32x4, o[u]), (u32x4 *)to);
+      } else {
+        store_pack<T, V>(to, o[u], D - (int)c[u]);
+      }
     }
   }
 }
@@ -516,8 +524,12 @@ static int embed_forward(int64_t n, int64_t batch, int64_t rows, int D, const in
   const uint32_t pb = batch > 1 ? (uint32_t)(n / batch) : 0u;
   {
     ProfScope prof(K_EMBED_FWD, stream);
-    hipLaunchKernelGGL(kd_embed_gather<T>, dim3(grid), dim3(kBlock), 0, stream, n, pb, rows, D, rpb,
-                       index, table, (A)scale, out);
+    if (D % V == 0 && (((uintptr_t)table | (uintptr_t)out) & 15u) == 0)
+      hipLaunchKernelGGL((kd_embed_gather<T, true>), dim3(grid), dim3(kBlock), 0, stream, n, pb, rows,
+                         D, rpb, index, table, (A)scale, out);
+    else
+      hipLaunchKernelGGL((kd_embed_gather<T, false>), dim3(grid), dim3(kBlock), 0, stream, n, pb,
+                         rows, D, rpb, index, table, (A)scale, out);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(KD_ERR_LAUNCH, "surface_embedding: %s", hipGetErrorString(e));

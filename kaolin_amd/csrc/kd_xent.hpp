@@ -861,6 +861,19 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
 // ------------------------------------------------------------------------------------------------
 constexpr int kFewParts = 16;
 
+// A pixel's loss softplus(L' - z_y) from the maximum (log2) and the sum over the rows but its label's
+// and from the label's logit; lse: log2 of the whole sum, w: 1 - p_y.
+__device__ __forceinline__ float pixel_loss(float m, float l, float z, const Args &a, float &lse,
+                                            float &w) {
+  const float z2 = z * a.c2;
+  const float u = (m + log2f(l) - z2) * kLn2;  // -inf when the label is the only row
+  const float t = expf(-fabsf(u));
+  const float value = u != u ? u : fmaxf(u, 0.f) + log1pf(t);
+  w = u != u ? u : (u >= 0.f ? 1.f / (1.f + t) : t / (1.f + t));
+  lse = z2 + value * kLog2e;
+  return value;
+}
+
 template <typename T, int DP, int G, bool RAW>
 __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__restrict__ table,
                                                           float *__restrict__ loss) {
@@ -901,7 +914,6 @@ __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__res
       z = part == -INFINITY ? z : part;
     }
   }
-  const float z2 = z * (fabsf(a.scale) * kLog2e);
   float l = 0.f;
 #pragma unroll 4
   for (int s = s0; s < n; s += ds) {
@@ -912,14 +924,10 @@ __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__res
 #pragma unroll
     for (int s = G / 2; s >= 1; s >>= 1) l += __shfl_xor(l, s);
   }
-  const float u = (m + log2f(l) - z2) * kLn2;  // -inf when the label is the only row
-  const float t = expf(-fabsf(u));
-  const float value = fmaxf(u, 0.f) + log1pf(t);
-  const float w = u >= 0.f ? 1.f / (1.f + t) : t / (1.f + t);
-  const float wn = u != u ? u : w;
-  const float out = u != u ? u : value;
+  float lse, wn;
+  const float out = pixel_loss(m, l, z, a, lse, wn);
   if (gl == 0) {
-    a.lse[r] = Form<T>::shift_table - (z2 + out * kLog2e);
+    a.lse[r] = Form<T>::shift_table - lse;
     a.w[r] = -wn * exp2f(Form<T>::shift_table);
     if (a.reduction == 0)
       loss[i] = out;
@@ -941,6 +949,211 @@ __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__res
     for (int j = 0; j < 4; ++j) v.v[j] = wn * (o[j] * inv - (float)e.v[j]);
     store_pack<float, 4>(a.raw + i * a.D + d, v, left);
   }
+}
+
+// ------------------------------------------------------------------------------------------------
+// the loss of a few pixels
+// ------------------------------------------------------------------------------------------------
+// Up to kFewPixels pixels and no gradients (a query at a clicked pixel): the table is read once as it
+// stands, straight into the products' operands, and nothing is listed, packed or kept.  Each wave
+// takes tiles of 32 table rows in turn; the workgroup's parts are joined in LDS, all of them by a
+// second launch of one workgroup.  Bound by the table's bytes.
+constexpr int kFewPixels = 64, kFewWorkers = 512;
+
+// 8 channels of a row
+template <typename T>
+struct Chunk {
+  T x[8];
+  // `left` of them inside the row, no read behind it
+  __device__ __forceinline__ void load(const T *row, int left) {
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int k = 0; k < 8; k += V) {
+      const Pack<T, V> p = left > k ? load_pack<T, V>(row + k, left - k) : Pack<T, V>{};
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[k + j] = p.v[j];
+    }
+  }
+  // all 8, whatever they are
+  __device__ __forceinline__ void load_any(const T *p) {
+    const Pack<T, 8> v = *(const Pack<T, 8> *)p;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = v.v[j];
+  }
+  __device__ __forceinline__ void clear_behind(int left) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = j < left ? x[j] : (T)0.f;
+  }
+  __device__ __forceinline__ void operand(uint4 *o) const {
+    Pack<uint16_t, 8> u[Form<T>::np];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (Form<T>::np == 1)
+        u[0].v[j] = __builtin_bit_cast(uint16_t, x[j]);
+      else
+        split3(x[j], u[0].v[j], u[1].v[j], u[2].v[j]);
+    }
+#pragma unroll
+    for (int p = 0; p < Form<T>::np; ++p) o[p] = __builtin_bit_cast(uint4, u[p]);
+  }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kBlock) void kd_xent_few(Args a, const T *__restrict__ features,
+                                                      const T *__restrict__ table,
+                                                      const int64_t *__restrict__ labels) {
+  using F = Form<T>;
+  using H8 = typename F::H8;
+  constexpr int NP = F::np, KS = DP / 16, kTimes = NP == 3 ? 6 : 1;
+  constexpr int kChunk = NP == 3 ? (KS < 4 ? KS : 4) : (KS < 16 ? KS : 16);  // operands in flight
+  __shared__ float s_p[3][kBlock / kWave][32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int64_t i = (int64_t)blockIdx.y * 32 + (lane & 31);  // this lane's pixel
+  uint4 x[KS][NP];
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    const int d = 16 * k + 8 * half;
+    Chunk<T> f;
+    f.load(features + i * a.D + d, i < a.n ? a.D - d : 0);
+    if (a.scale < 0.f) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f.x[j] = (T)(-(float)f.x[j]);
+    }
+    f.operand(x[k]);
+  }
+  const int64_t y = i < a.n ? labels[i] : -1;
+  float m = -1e30f, l = 0.f, zy = -INFINITY;
+  const int ntile = (a.V + 31) / 32;
+  for (int t = blockIdx.x * (kBlock / kWave) + wave; t < ntile; t += gridDim.x * (kBlock / kWave)) {
+    const int64_t v0 = (int64_t)t * 32, v = v0 + (lane & 31);
+    f32x16 s = (f32x16)(0.f);
+    // all the tile's loads at once, with no branch between them: the chunks that cross a row's end
+    // read on into the next row, which the last tiles of the table have not
+    const bool inside = (v0 + 32) * a.D + 7 <= (int64_t)a.V * a.D;
+#pragma unroll
+    for (int c = 0; c < KS; c += kChunk) {
+      Chunk<T> e[kChunk];
+      if (inside) {
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k)
+          e[k].load_any(table + v * a.D + min(16 * (c + k) + 8 * half, a.D - 1));
+        if (a.D < 16 * (c + kChunk)) {
+#pragma unroll
+          for (int k = 0; k < kChunk; ++k) e[k].clear_behind(a.D - (16 * (c + k) + 8 * half));
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) {
+          const int d = 16 * (c + k) + 8 * half;
+          e[k].load(table + v * a.D + d, v < a.V ? a.D - d : 0);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kChunk; ++k) {
+        uint4 ew[NP];
+        H8 ea[NP], xb[NP];
+        e[k].operand(ew);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          ea[p] = __builtin_bit_cast(H8, ew[p]);
+          xb[p] = __builtin_bit_cast(H8, x[c + k][p]);
+        }
+#pragma unroll
+        for (int q = 0; q < kTimes; ++q) s = product<NP>(q, ea, xb, s);
+      }
+    }
+    if (v0 + 32 > a.V || __any((uint64_t)(y - v0) < 32u)) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int64_t r = v0 + 8 * (j >> 2) + 4 * half + (j & 3);
+        zy = r == y ? s[j] : zy;
+        s[j] = r == y || r >= a.V ? -INFINITY : s[j];
+      }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) top = fmaxf(top, s[j]);
+    top *= a.c2;
+    if (top > m) {  // (a lane by itself: the halves of a pixel are joined at the end)
+      l *= __builtin_amdgcn_exp2f(m - top);
+      m = top;
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sum += __builtin_amdgcn_exp2f(fmaf(s[j], a.c2, -m));
+    l += sum;
+  }
+  // the two halves, then the waves
+  {
+    const float mo = __shfl_xor(m, 32), lo = __shfl_xor(l, 32), zo = __shfl_xor(zy, 32);
+    const float mn = fmaxf(m, mo);
+    l = l * __builtin_amdgcn_exp2f(m - mn) + lo * __builtin_amdgcn_exp2f(mo - mn);
+    m = mn;
+    zy = zy == -INFINITY ? zo : zy;
+  }
+  if (half == 0) {
+    s_p[0][wave][lane] = m;
+    s_p[1][wave][lane] = l;
+    s_p[2][wave][lane] = zy;
+  }
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+#pragma unroll
+  for (int w = 1; w < kBlock / kWave; ++w) {
+    const float mo = s_p[0][w][lane], zo = s_p[2][w][lane];
+    const float mn = fmaxf(m, mo);
+    l = l * __builtin_amdgcn_exp2f(m - mn) + s_p[1][w][lane] * __builtin_amdgcn_exp2f(mo - mn);
+    m = mn;
+    zy = zy == -INFINITY ? zo : zy;
+  }
+  const int64_t q = (int64_t)blockIdx.x * kFewPixels + i;
+  a.pm[q] = m;
+  a.pl[q] = l;
+  a.pz[q] = zy;
+}
+
+static __global__ __launch_bounds__(1024) void kd_xent_few_join(Args a, int nparts,
+                                                                const int64_t *__restrict__ labels,
+                                                                float *__restrict__ loss) {
+  constexpr int kLanes = 1024 / kFewPixels;
+  __shared__ float s_m[kLanes][kFewPixels], s_l[kLanes][kFewPixels], s_z[kLanes][kFewPixels];
+  const int i = threadIdx.x % kFewPixels, j = threadIdx.x / kFewPixels;
+  float m = -1e30f, l = 0.f, z = -INFINITY;
+  if (i < a.n) {
+#pragma unroll 4
+    for (int p = j; p < nparts; p += kLanes) {
+      const int q = p * kFewPixels + i;
+      const float mo = a.pm[q], zo = a.pz[q], mn = fmaxf(m, mo);
+      l = l * __builtin_amdgcn_exp2f(m - mn) + a.pl[q] * __builtin_amdgcn_exp2f(mo - mn);
+      m = mn;
+      z = zo == -INFINITY ? z : zo;
+    }
+  }
+  s_m[j][i] = m;
+  s_l[j][i] = l;
+  s_z[j][i] = z;
+  __syncthreads();
+  if (j) return;  // one wave is left, a lane a pixel
+#pragma unroll
+  for (int k = 1; k < kLanes; ++k) {
+    const float mo = s_m[k][i], zo = s_z[k][i], mn = fmaxf(m, mo);
+    l = l * __builtin_amdgcn_exp2f(m - mn) + s_l[k][i] * __builtin_amdgcn_exp2f(mo - mn);
+    m = mn;
+    z = zo == -INFINITY ? z : zo;
+  }
+  const int64_t y = i < a.n ? labels[i] : -1;
+  const bool in = y >= 0 && y < a.V;
+  float lse, w;
+  const float out = in ? pixel_loss(m, l, z, a, lse, w) : 0.f;
+  if (a.reduction == 0) {
+    if (i < a.n) loss[i] = out;
+    return;
+  }
+  double sum = (double)out;
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) sum += __shfl_xor(sum, s);
+  const int count = __popcll(__ballot(in));
+  if (i == 0) *loss = (float)(a.reduction == 1 ? sum / (double)(count > 0 ? count : 1) : sum);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1294,6 +1507,15 @@ dim3 walk_grid() {
 }
 
 template <typename T, int DP>
+void launch_few(const Args &a, const T *features, const T *table, const int64_t *labels, float *loss,
+                hipStream_t stream) {
+  const int wgs = std::min((a.V + 127) / 128, kFewWorkers);
+  hipLaunchKernelGGL((kd_xent_few<T, DP>), dim3(wgs, (unsigned)((a.n + 31) / 32)), dim3(kBlock), 0,
+                     stream, a, features, table, labels);
+  hipLaunchKernelGGL(kd_xent_few_join, dim3(1), dim3(1024), 0, stream, a, wgs, labels, loss);
+}
+
+template <typename T, int DP>
 void launch_forward(const Args &a, bool need_x, const T *features, const T *table, float *loss,
                     hipStream_t stream) {
   const int xtiles = (int)(a.npad / 32), etiles = a.vpad / 32;
@@ -1351,6 +1573,18 @@ int forward(int64_t n, int64_t V, int D, const T *features, const T *table, cons
     return set_error(KD_ERR_WORKSPACE, "workspace too small: %zu < %zu or %zu < %zu", state_bytes,
                      ns, scratch_bytes, nw);
   ProfScope prof(K_XENT_FWD, stream);
+  if (n > 0 && n <= kFewPixels && !need_x && !need_e) {
+    switch (a.dp) {
+      case 32: launch_few<T, 32>(a, features, table, labels, loss, stream); break;
+      case 64: launch_few<T, 64>(a, features, table, labels, loss, stream); break;
+      case 128: launch_few<T, 128>(a, features, table, labels, loss, stream); break;
+      default: launch_few<T, 256>(a, features, table, labels, loss, stream); break;
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess)
+      return set_error(KD_ERR_LAUNCH, "surface_cross_entropy: %s", hipGetErrorString(e));
+    return KD_OK;
+  }
   const int nblk = (int)((n + kMapChunk - 1) / kMapChunk);
   if (nblk <= kListChunks) {  // one workgroup lists them all in less time than two launches take
     hipLaunchKernelGGL(kd_xent_map, dim3(1), dim3(kBlock), 0, stream, a, kListChunks, false, labels,

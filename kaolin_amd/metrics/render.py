@@ -68,15 +68,22 @@ class SurfaceCrossEntropyHip(Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_loss):
-        if grad_loss is None:
-            return (None,) * 5
-        labels, state = ctx.saved_tensors
-        gx, ge = _C.metrics.surface_xent_backward(
-            grad_loss, labels, ctx.shape, ctx.dtype, ctx.scale, ctx.reduction, state, *ctx.need,
-            *ctx.needs_input_grad[:2])
-        return gx, ge, None, None, None
+        # (the guard against second derivatives costs time that a plain backward need not spend)
+        return _guarded_grad(ctx, grad_loss) if torch.is_grad_enabled() else _grad(ctx, grad_loss)
+
+
+def _grad(ctx, grad_loss):
+    if grad_loss is None:
+        return (None,) * 5
+    labels, state = ctx.saved_tensors
+    gx, ge = _C.metrics.surface_xent_backward(
+        grad_loss, labels, ctx.shape, ctx.dtype, ctx.scale, ctx.reduction, state, *ctx.need,
+        *ctx.needs_input_grad[:2])
+    return gx, ge, None, None, None
+
+
+_guarded_grad = once_differentiable(_grad)
 
 
 def surface_cross_entropy(features, embeddings, labels, scale=1.0, reduction='mean'):

@@ -27,13 +27,20 @@ class SurfaceEmbeddingHip(Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_out):
-        if grad_out is None or not ctx.needs_input_grad[1]:
-            return None, None, None
-        index, = ctx.saved_tensors
-        return None, _C.render.mesh.surface_embedding_backward(grad_out, index, ctx.table_shape,
-                                                               ctx.scale), None
+        # (the guard against second derivatives costs time that a plain backward need not spend)
+        return _guarded_grad(ctx, grad_out) if torch.is_grad_enabled() else _grad(ctx, grad_out)
+
+
+def _grad(ctx, grad_out):
+    if grad_out is None:
+        return None, None, None
+    index, = ctx.saved_tensors
+    return None, _C.render.mesh.surface_embedding_backward(grad_out, index, ctx.table_shape,
+                                                           ctx.scale), None
+
+
+_guarded_grad = once_differentiable(_grad)
 
 
 def surface_embedding(index, embeddings, scale=1.0):

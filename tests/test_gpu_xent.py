@@ -150,6 +150,28 @@ def test_loss_and_gradients(dname, n, V, D, scale, reduction):
 
 
 @pytest.mark.parametrize('dname', ['f32', 'f16', 'bf16'])
+@pytest.mark.parametrize('reduction', ['mean', 'sum', 'none'])
+@pytest.mark.parametrize('n,V,D', [(1, 1, 1), (2, 33, 7), (31, 5000, 33), (32, 127, 64), (33, 129, 128),
+                                   (63, 70000, 20), (64, 2000, 250), (65, 2000, 40)])
+def test_losses_of_a_few_pixels(dname, reduction, n, V, D):
+    """Without gradients the table is read as it stands, up to 64 pixels; a table one element off any
+    alignment, a label of no row, NaN in its features."""
+    from kaolin_amd.metrics.render import surface_cross_entropy
+    x, e, y = _inputs(n, V, D, TYPES[dname], seed=n + D, background=0.0)
+    flat = torch.zeros(V * D + 1, device=DEV, dtype=e.dtype)
+    off = flat[1:].view(V, D)
+    off.copy_(e)
+    if n > 1:
+        y[n // 2] = V
+        x[n // 2] = math.nan
+    want = _reference(x, e, y, 9.0, reduction, _grad(reduction, (n,)))
+    for table in (e, off):
+        loss = surface_cross_entropy(x, table, y, 9.0, reduction)
+        assert ((loss.double() - want[0]).abs() <= want[1]).all()
+        assert torch.equal(loss, surface_cross_entropy(x, table, y, 9.0, reduction))
+
+
+@pytest.mark.parametrize('dname', ['f32', 'f16', 'bf16'])
 @pytest.mark.parametrize('spread,scale', [(0.02, 200.0), (0.0, 60.0), (8.0, 40.0)])
 def test_far_from_even(dname, spread, scale):
     """Trained (the label's probability next to 1: its complement must keep its digits) and far
