@@ -10,7 +10,7 @@
 // are looked at, writes n * D * sizeof(T).
 //
 // Backward: no atomics on values, so the result does not depend on timing.  The tokens that name a row
-// are sorted by key with a stable least-significant-digit radix sort (8 bits a pass, 8 bytes a token),
+// are sorted by key with a stable least-significant-digit radix sort (up to 10 bits a pass, 8 bytes a token),
 // so a row's tokens stand together in token order; then each group of G lanes (one row of the
 // gradient, 16 bytes a lane) walks a run of sorted tokens and adds their gradient rows in registers.
 // Runs that cross a group's border are joined in LDS by the group in which they begin, runs that cross
@@ -26,7 +26,8 @@ namespace kd {
 
 constexpr int kSortTile = 4096;             // tokens per sort workgroup (16 per thread)
 constexpr int kSortIters = kSortTile / kBlock;
-constexpr int kDigits = 256;
+constexpr int kMaxBits = 10;                // of a sort digit: 16-bit keys take two passes, 20-bit ones too
+constexpr int kDigits = 1 << kMaxBits;
 constexpr int kFewTiles = 64;               // up to so many tiles the sort needs no scan launch
 constexpr int kMaxChannels = 1 << 20;
 
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(kBlock) void kd_embed_hist(SortKeys s, int shift, u
     return;
   }
   __shared__ uint32_t cnt[kDigits];
-  cnt[threadIdx.x] = 0;
+  for (uint32_t d = threadIdx.x; d <= mask; d += kBlock) cnt[d] = 0;
   __syncthreads();
   const uint32_t base = blockIdx.x * (uint32_t)kSortTile, m = s.count();
   if (base < m) {
@@ -144,7 +145,8 @@ __global__ __launch_bounds__(kBlock) void kd_embed_hist(SortKeys s, int shift, u
     }
   }
   __syncthreads();
-  if (threadIdx.x <= mask) hist[(int64_t)threadIdx.x * ntile + blockIdx.x] = cnt[threadIdx.x];
+  for (uint32_t d = threadIdx.x; d <= mask; d += kBlock)
+    hist[(int64_t)d * ntile + blockIdx.x] = cnt[d];
 }
 
 // Inclusive sum over the workgroup's threads; total in every thread.
@@ -204,8 +206,10 @@ __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
   const uint32_t mask = (1u << bits) - 1u, m = s.count();
   if (blockIdx.x * (uint32_t)kSortTile >= m && blockIdx.x > 0) return;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (uint32_t d = threadIdx.x; d <= mask; d += kBlock) {
 #pragma unroll
-  for (int k = 0; k < kWaves; ++k) wcnt[k][threadIdx.x] = 0;
+    for (int k = 0; k < kWaves; ++k) wcnt[k][d] = 0;
+  }
   const uint32_t base = blockIdx.x * (uint32_t)kSortTile + w * (kSortTile / kWaves) + lane;
   uint2 kt[kSortIters];
   uint32_t rank[kSortIters], in = 0;
@@ -235,32 +239,43 @@ __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
   }
   __syncthreads();
   // where each digit begins among all tokens, and this tile's part of it
-  uint32_t all = 0, before = 0, tot;
-  if (threadIdx.x <= mask) {
+  // (a thread takes kDigits / kBlock digits in a row, as the sum over the digits needs)
+  constexpr int kPer = kDigits / kBlock;
+  uint32_t all[kPer], before[kPer], mine = 0, tot;
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    const uint32_t d = threadIdx.x * kPer + q;
+    all[q] = before[q] = 0;
+    if (d > mask) continue;
     if (ntile == 1) {
 #pragma unroll
-      for (int k = 0; k < kWaves; ++k) all += wcnt[k][threadIdx.x];
+      for (int k = 0; k < kWaves; ++k) all[q] += wcnt[k][d];
     } else if (ntile <= kFewTiles) {
-      const uint32_t *h = hist + (int64_t)threadIdx.x * ntile;
+      const uint32_t *h = hist + (int64_t)d * ntile;
 #pragma unroll 8
       for (int k = 0; k < ntile; ++k) {
         const uint32_t c = h[k];
-        before += k < (int)blockIdx.x ? c : 0u;
-        all += c;
+        before[q] += k < (int)blockIdx.x ? c : 0u;
+        all[q] += c;
       }
     } else {
-      all = totals[threadIdx.x];
-      before = hist[(int64_t)threadIdx.x * ntile + blockIdx.x];
+      all[q] = totals[d];
+      before[q] = hist[(int64_t)d * ntile + blockIdx.x];
     }
+    mine += all[q];
   }
-  const uint32_t begin = wg_scan(all, s_w, tot) - all;
+  uint32_t begin = wg_scan(mine, s_w, tot) - mine;
   if (blockIdx.x == 0 && threadIdx.x == 0 && kept) *kept = tot;
-  if (threadIdx.x <= mask) {
-    uint32_t off = begin + before;
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    const uint32_t d = threadIdx.x * kPer + q;
+    if (d > mask) continue;
+    uint32_t off = begin + before[q];
+    begin += all[q];
 #pragma unroll
     for (int k = 0; k < kWaves; ++k) {
-      const uint32_t c = wcnt[k][threadIdx.x];
-      wcnt[k][threadIdx.x] = off;
+      const uint32_t c = wcnt[k][d];
+      wcnt[k][d] = off;
       off += c;
     }
   }
@@ -411,9 +426,9 @@ __global__ __launch_bounds__(kBlock) void kd_embed_segments(SegArgs a, const T *
   }
 }
 
-// The runs that cross a workgroup's border: the workgroup in which such a run begins adds up its
-// own part and the heads of the workgroups behind it, split over the groups of lanes in a fixed
-// order.
+// The runs that cross a workgroup's border, each added up where it begins: a group of lanes takes one
+// border and joins the two sides; the few runs that go on through whole workgroups are left to all
+// groups together, one after the other, in a fixed order.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void kd_embed_join(SegArgs a, int nwg,
                                                         typename Wide<T>::type scale,
@@ -422,43 +437,67 @@ __global__ __launch_bounds__(kBlock) void kd_embed_join(SegArgs a, int nwg,
                                                         T *__restrict__ out) {
   using A = typename Wide<T>::type;
   constexpr int V = 16 / sizeof(T);
-  const int w = blockIdx.x;
-  if (!(a.flags[w] & kHasTail)) return;
   __shared__ int s_end;
+  __shared__ uint8_t s_long[kBlock];
   __shared__ A s_sum[kBlock * V];
   const int G = 1 << a.glog, NG = kBlock >> a.glog;
   const int g = threadIdx.x >> a.glog, gl = threadIdx.x & (G - 1);
-  if (threadIdx.x == 0) s_end = nwg;
-  __syncthreads();
-  // the first workgroup behind w through which the run does not go on
-  for (int b = w + 1; b < nwg; b += kBlock) {
-    const int q = b + threadIdx.x;
-    if (q < nwg && !(a.flags[q] & kThrough)) atomicMin(&s_end, q);
-    __syncthreads();
-    const bool found = s_end < nwg;
-    __syncthreads();
-    if (found) break;
-  }
-  const int last = min(s_end, nwg - 1);
   const int col = ((int)blockIdx.y * G + gl) * V;
   const int64_t wcol = (int64_t)gridDim.y * G * V;
-  A acc[V];
+  // a run that is open at the end of workgroup w goes on behind it: the position is inside
+  auto store = [&](int w, const A *acc) {
+    const uint64_t end = (uint64_t)(w + 1) * NG * a.per_group;
+    if (col < a.D) embed_store<T, V>(out, a.D, a.pairs[end - 1].x, col, acc, scale);
+  };
+  {
+    const int w = (int)blockIdx.x * NG + g;
+    bool far = false;
+    if (w < nwg - 1 && (a.flags[w] & kHasTail)) {
+      far = a.flags[w + 1] & kThrough;
+      if (!far) {
+        A acc[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) acc[j] = g == 0 ? tail[(int64_t)w * wcol + col + j] : (A)0;
-  for (int q = w + 1 + g; q <= last; q += NG) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) acc[j] += head[(int64_t)q * wcol + col + j];
-  }
-#pragma unroll
-  for (int j = 0; j < V; ++j) s_sum[threadIdx.x * V + j] = acc[j];
-  __syncthreads();
-  if (g == 0 && col < a.D) {
-    for (int q = 1; q < NG; ++q) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] += s_sum[((q << a.glog) + gl) * V + j];
+        for (int j = 0; j < V; ++j)
+          acc[j] = tail[(int64_t)w * wcol + col + j] + head[(int64_t)(w + 1) * wcol + col + j];
+        store(w, acc);
+      }
     }
-    const uint64_t end = (uint64_t)(w + 1) * NG * a.per_group;  // <= n: a run goes on behind it
-    embed_store<T, V>(out, a.D, a.pairs[end - 1].x, col, acc, scale);
+    if (gl == 0) s_long[g] = far;
+  }
+  __syncthreads();
+  for (int q0 = 0; q0 < NG; ++q0) {
+    if (!s_long[q0]) continue;  // (the same for the whole workgroup)
+    const int w = (int)blockIdx.x * NG + q0;
+    if (threadIdx.x == 0) s_end = nwg;
+    __syncthreads();
+    // the first workgroup behind w through which the run does not go on
+    for (int b = w + 1; b < nwg; b += kBlock) {
+      const int q = b + threadIdx.x;
+      if (q < nwg && !(a.flags[q] & kThrough)) atomicMin(&s_end, q);
+      __syncthreads();
+      const bool found = s_end < nwg;
+      __syncthreads();
+      if (found) break;
+    }
+    const int last = min(s_end, nwg - 1);
+    A acc[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = g == 0 ? tail[(int64_t)w * wcol + col + j] : (A)0;
+    for (int q = w + 1 + g; q <= last; q += NG) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] += head[(int64_t)q * wcol + col + j];
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) s_sum[threadIdx.x * V + j] = acc[j];
+    __syncthreads();
+    if (g == 0) {
+      for (int q = 1; q < NG; ++q) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] += s_sum[((q << a.glog) + gl) * V + j];
+      }
+      store(w, acc);
+    }
+    __syncthreads();
   }
 }
 
@@ -486,7 +525,7 @@ static EmbedPlan embed_plan(int64_t n, int64_t nkeys, int D, int esize) {
   p.ntile = (int)((n + kSortTile - 1) / kSortTile);
   int kb = 1;
   while (kb < 32 && ((nkeys - 1) >> kb) != 0) ++kb;  // keys 0 .. nkeys - 1
-  p.passes = (kb + 7) / 8;
+  p.passes = (kb + kMaxBits - 1) / kMaxBits;
   p.bits = (kb + p.passes - 1) / p.passes;
   const int asize = esize == 8 ? 8 : 4;
   p.pairs = up256(8 * (size_t)n);
@@ -599,8 +638,11 @@ static int embed_backward(int64_t n, int64_t batch, int64_t rows, int D, const i
     hipLaunchKernelGGL(kd_embed_segments<T>, grid, dim3(kBlock), 0, stream, a, grad, (A)scale, out,
                        head, tail);
     if (p.nwg > 1)
-      hipLaunchKernelGGL(kd_embed_join<T>, grid, dim3(kBlock), 0, stream, a, p.nwg, (A)scale,
-                         (const A *)head, (const A *)tail, out);
+      hipLaunchKernelGGL(kd_embed_join<T>,
+                         dim3((unsigned)((p.nwg + (kBlock >> p.glog) - 1) / (kBlock >> p.glog)),
+                              (unsigned)p.gy),
+                         dim3(kBlock), 0, stream, a, p.nwg, (A)scale, (const A *)head,
+                         (const A *)tail, out);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
