@@ -103,7 +103,7 @@ constexpr int kSumChunks = 4096;  // up to so many chunks a workgroup adds up th
 struct Args {
   int64_t n, npad;  // pixels, padded
   int V, vpad, D, dp;
-  float c2;         // |scale| log2(e)
+  float c2, c2l;    // |scale| log2(e), and what its rounding left
   float scale;
   int reduction;    // 0 none, 1 mean, 2 sum
   // state kept from forward to backward
@@ -346,7 +346,7 @@ __global__ __launch_bounds__(kBlock) void kd_xent_pack(Args a, int xtiles,
 // ------------------------------------------------------------------------------------------------
 // shared pieces of the two walks
 // ------------------------------------------------------------------------------------------------
-// acc += the i-th of the planes' products of a . b, the small ones first
+// acc += the i-th of the planes' products of a . b, the large one last
 template <int NP, typename H8>
 __device__ __forceinline__ f32x16 product(int i, const H8 *a, const H8 *b, f32x16 c) {
   if constexpr (NP == 1) {
@@ -355,6 +355,14 @@ __device__ __forceinline__ f32x16 product(int i, const H8 *a, const H8 *b, f32x1
     constexpr int ka[6] = {0, 2, 1, 0, 1, 0}, kb[6] = {2, 0, 1, 1, 0, 0};
     return mfma(a[ka[i]], b[kb[i]], c);
   }
+}
+
+// log2 of a term: the logit times the factor, in two parts for 32-bit data (a factor off by 2^-25
+// would be a bias that no averaging takes out), and an offset.
+template <typename T>
+__device__ __forceinline__ float exponent(float s, float c2, float c2l, float offset) {
+  if constexpr (sizeof(T) == 4) offset = fmaf(s, c2l, offset);
+  return fmaf(s, c2, offset);
 }
 
 // the upper halves of two words as one
@@ -575,15 +583,17 @@ struct Step {
   template <bool ADD, bool LOGITS, typename Between>
   __device__ __forceinline__ void products(const uint4 *straight, const uint4 *transposed,
                                            f32x16 *next, Between between) {
+    if constexpr (NP == 3) {
+      products3<ADD, LOGITS>(straight, transposed, next[0], between);
+      return;
+    }
     constexpr int kAdd = ADD ? 2 * DT : 0, kOps = kAdd + (LOGITS ? KS : 0);
-    constexpr int kAhead = NP == 3 ? 2 : RB == 2 ? 3 : 5, kTimes = NP == 3 ? 6 : 1;
+    constexpr int kAhead = RB == 2 ? 3 : 5;
     const int lane = threadIdx.x & 63;
-    H8 a[kOps][NP];
+    H8 a[kOps];
     auto load = [&](int n) {
-#pragma unroll
-      for (int p = 0; p < NP; ++p)
-        a[n][p] = n < kAdd ? *(const H8 *)&transposed[(p * 2 * DT + n) * 64 + lane]
-                           : *(const H8 *)&straight[(p * KS + n - kAdd) * 64 + lane];
+      a[n] = n < kAdd ? *(const H8 *)&transposed[n * 64 + lane]
+                      : *(const H8 *)&straight[(n - kAdd) * 64 + lane];
     };
 #pragma unroll
     for (int n = 0; n < (kAhead < kOps ? kAhead : kOps); ++n) load(n);
@@ -598,21 +608,101 @@ struct Step {
     for (int n = 0; n < kOps; ++n) {
       if (n + kAhead < kOps) load(n + kAhead);
 #pragma unroll
-      for (int i = 0; i < kTimes; ++i)
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
-          if (n < kAdd) {
-            H8 w[NP];
-#pragma unroll
-            for (int p = 0; p < NP; ++p) w[p] = __builtin_bit_cast(H8, q[b][n / DT][p]);
-            o[b][n % DT] = product<NP>(i, a[n], w, o[b][n % DT]);
-          } else {
-            next[b] = product<NP>(i, a[n], held[b][n - kAdd], next[b]);
-          }
-          between(done++);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+      for (int b = 0; b < RB; ++b) {
+        if (n < kAdd)
+          o[b][n % DT] = mfma(a[n], __builtin_bit_cast(H8, q[b][n / DT][0]), o[b][n % DT]);
+        else
+          next[b] = mfma(a[n], held[b][n - kAdd][0], next[b]);
+        between(done++);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
+  }
+
+  // The same for operands of three parts.  A product rounds its sum with every term, so the five small
+  // products of all terms go first, at 2^-8 of the sum's size, and then the large ones: as many
+  // roundings as a sum of 32-bit products has.  A tile's weighted sum is formed by itself and added as
+  // a whole, one rounding a tile.
+  template <bool ADD, bool LOGITS, typename Between>
+  __device__ __forceinline__ void products3(const uint4 *straight, const uint4 *transposed,
+                                            f32x16 &next, Between between) {
+    const int lane = threadIdx.x & 63;
+    constexpr int kAdd = ADD ? 2 * DT : 0;                    // groups of the weighted sum
+    constexpr int kSmall = LOGITS ? KS : 0;                   // groups of small products
+    constexpr int kLast = LOGITS ? (KS < 4 ? 1 : KS / 4) : 0;  // groups of large ones
+    constexpr int kPer = KS < 4 ? KS : 4;
+    constexpr int kGroups = kAdd + kSmall + kLast;
+    H8 a[2][4];  // a group's operands: three planes, or the first planes of kPer steps
+    H8 first;    // the first plane of the other row half
+    auto load = [&](int g) {
+      H8 *to = a[g & 1];
+      if (g < kAdd) {  // group 2 d + h
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+          to[p] = *(const H8 *)&transposed[((p * 2 + (g & 1)) * DT + g / 2) * 64 + lane];
+      } else if (g < kAdd + kSmall) {
+#pragma unroll
+        for (int p = 0; p < 3; ++p) to[p] = *(const H8 *)&straight[(p * KS + g - kAdd) * 64 + lane];
+      } else {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          to[j] = *(const H8 *)&straight[((g - kAdd - kSmall) * kPer + j) * 64 + lane];
+      }
+    };
+    load(0);
+    int done = 0;
+    auto slot = [&] {
+      between(done++);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    slot();
+    f32x16 tmp[2];
+    if constexpr (LOGITS) next = (f32x16)(0.f);
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      if (g + 1 < kGroups) load(g + 1);
+      const H8 *x = a[g & 1];
+      if (g < kAdd) {
+        const int d = g / 2, h = g & 1;
+        H8 w[3], w0;
+#pragma unroll
+        for (int p = 0; p < 3; ++p) w[p] = __builtin_bit_cast(H8, q[0][h][p]);
+        w0 = __builtin_bit_cast(H8, q[0][0][0]);
+        if (h == 0) {
+          tmp[d & 1] = (f32x16)(0.f);
+          first = x[0];
+        }
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+          tmp[d & 1] = product<3>(i, x, w, tmp[d & 1]);
+          slot();
+        }
+        if (h == 1) {
+          tmp[d & 1] = mfma(first, w0, tmp[d & 1]);
+          slot();
+          tmp[d & 1] = mfma(x[0], w[0], tmp[d & 1]);
+          slot();
+        }
+      } else if (g < kAdd + kSmall) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+          next = product<3>(i, x, held[0][g - kAdd], next);
+          slot();
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          next = mfma(x[j], held[0][(g - kAdd - kSmall) * kPer + j][0], next);
+          slot();
+        }
+      }
+      // the sum of the columns before, once its products are through
+      if (ADD && g >= 2 && g <= kAdd && g % 2 == 0) {
+        o[0][g / 2 - 1] += tmp[(g / 2 - 1) & 1];
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if constexpr (ADD && !LOGITS) o[0][DT - 1] += tmp[(DT - 1) & 1];
   }
 
   __device__ __forceinline__ void logits(const uint4 *straight) {
@@ -630,9 +720,14 @@ struct Step {
     constexpr int kPairs = RB * 8;
     f32x16 next[RB];
     uint4 fresh[RB][2][NP];
+    // split operands: behind the weighted sum, whose operands' registers the new ones take over
+    constexpr int kFirst = NP == 3 && SUM ? 12 * DT : 0;
     products<SUM, true>(straight, transposed, next, [&](int slot) {
+      if (slot < kFirst) return;
+      const int k0 = (slot - kFirst) * kPairs / (kSlots - kFirst);
+      const int k1 = (slot + 1 - kFirst) * kPairs / (kSlots - kFirst);
 #pragma unroll
-      for (int k = slot * kPairs / kSlots; k < (slot + 1) * kPairs / kSlots; ++k) {
+      for (int k = k0; k < k1; ++k) {
         const int b = k / 8, i = k % 8;
         float p0 = s[b][2 * i], p1 = s[b][2 * i + 1];
         pair(b, i, p0, p1);
@@ -679,8 +774,9 @@ struct Step {
 // the walk over the table
 // ------------------------------------------------------------------------------------------------
 // exp2 of logits up to this size needs no maximum: 2^60 a term leaves room for the sum and for the
-// smallest term, 2^-60, in 32 bits (and in bf16)
-constexpr float kSafeLogit = 60.f;
+// smallest term, 2^-60, in 32 bits (and in bf16), if the table's rows are no larger than 2^20 and the
+// largest no smaller than 2^-20.
+constexpr float kSafeLogit = 60.f, kSafeRow = 0x1p40f;  // (the latter squared)
 
 template <typename T, int DP, bool SUM>
 struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
@@ -691,7 +787,7 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
   int lab[RB];
   float m[RB], l[RB][2], zy[RB];
   int V;
-  float c2;
+  float c2, c2l;
 
   // the label's own column and the table's padding take no part
   __device__ __forceinline__ void mask(int v0) {
@@ -763,9 +859,14 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
   template <bool ONLINE>
   __device__ __forceinline__ void next(const uint4 *s_e, const uint4 *s_t) {
     B::step(s_e, s_t, [&](int b, int, float &p0, float &p1) {
-      const float shift = ONLINE ? F::shift - m[b] : 0.f;
-      p0 = __builtin_amdgcn_exp2f(ONLINE ? fmaf(p0, c2, shift) : p0 * c2);
-      p1 = __builtin_amdgcn_exp2f(ONLINE ? fmaf(p1, c2, shift) : p1 * c2);
+      if constexpr (ONLINE || sizeof(T) == 4) {
+        const float shift = ONLINE ? F::shift - m[b] : 0.f;
+        p0 = __builtin_amdgcn_exp2f(exponent<T>(p0, c2, c2l, shift));
+        p1 = __builtin_amdgcn_exp2f(exponent<T>(p1, c2, c2l, shift));
+      } else {
+        p0 = __builtin_amdgcn_exp2f(p0 * c2);
+        p1 = __builtin_amdgcn_exp2f(p1 * c2);
+      }
       l[b][0] += p0;
       l[b][1] += p1;
       asm volatile("" : "+v"(l[b][0]), "+v"(l[b][1]));  // (stays in its slot)
@@ -787,17 +888,19 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
   RowsWalk<T, DP, SUM> w;
   w.V = a.V;
   w.c2 = a.c2;
+  w.c2l = a.c2l;
   uint32_t big = a.emax[lane * kSlotPad];
 #pragma unroll
   for (int k = 32; k >= 1; k >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, k));
-  const float size = a.c2 * sqrtf(__uint_as_float(big));
+  const float size2 = __uint_as_float(big), size = a.c2 * sqrtf(size2);
+  const bool fits = F::shift == 0.f && size2 < kSafeRow && size2 > 1.f / kSafeRow;
   const uint16_t *es = a.es, *et = a.et;
   constexpr int64_t kTile = kBytes / 2;
   deal.each(blockIdx.x, [&](int64_t block, int p0, int p1, int64_t slot) {
     const int64_t row0 = block * W::rows + wave * (32 * RB);
     // |logit| <= |x| |e| scale, over the kRowPad rows about this wave's (so that the choice does not
     // depend on how many of them a wave holds); a NaN size takes the general way
-    bool safe = F::shift == 0.f;
+    bool safe = fits;
 #pragma unroll
     for (int k = 0; k < kRowPad / kWave; ++k)
       safe &= size * sqrtf(a.xn[row0 / kRowPad * kRowPad + k * kWave + lane]) < kSafeLogit;
@@ -866,7 +969,13 @@ constexpr int kFewParts = 16;
 __device__ __forceinline__ float pixel_loss(float m, float l, float z, const Args &a, float &lse,
                                             float &w) {
   const float z2 = z * a.c2;
-  const float u = (m + log2f(l) - z2) * kLn2;  // -inf when the label is the only row
+  // log2 of the sum less z_y, both near the whole number m + k: the difference is formed where it is
+  // small (m is a whole number), the sum's logarithm next to 1 if the loss is neither large nor small
+  const float k = fminf(fmaxf(rintf(z2 - m), -1e9f), 1e9f);
+  const float d = fmaf(z, a.c2, -(m + k)) + z * a.c2l;
+  const float fits = fminf(fmaxf(k, -40.f), 40.f);  // (sums reach from 2^-60 to 2^91)
+  const float g = log2f(l * __builtin_amdgcn_exp2f(-fits)) - (k - fits);
+  const float u = (g - d) * kLn2;  // -inf when the label is the only row
   const float t = expf(-fabsf(u));
   const float value = u != u ? u : fmaxf(u, 0.f) + log1pf(t);
   w = u != u ? u : (u >= 0.f ? 1.f / (1.f + t) : t / (1.f + t));
@@ -1026,7 +1135,7 @@ __global__ __launch_bounds__(kBlock) void kd_xent_few(Args a, const T *__restric
   const int ntile = (a.V + 31) / 32;
   for (int t = blockIdx.x * (kBlock / kWave) + wave; t < ntile; t += gridDim.x * (kBlock / kWave)) {
     const int64_t v0 = (int64_t)t * 32, v = v0 + (lane & 31);
-    f32x16 s = (f32x16)(0.f);
+    f32x16 s = (f32x16)(0.f), low = (f32x16)(0.f);
     // all the tile's loads at once, with no branch between them: the chunks that cross a row's end
     // read on into the next row, which the last tiles of the table have not
     const bool inside = (v0 + 32) * a.D + 7 <= (int64_t)a.V * a.D;
@@ -1058,10 +1167,13 @@ __global__ __launch_bounds__(kBlock) void kd_xent_few(Args a, const T *__restric
           ea[p] = __builtin_bit_cast(H8, ew[p]);
           xb[p] = __builtin_bit_cast(H8, x[c + k][p]);
         }
+        // (the small products by themselves: see products3)
 #pragma unroll
-        for (int q = 0; q < kTimes; ++q) s = product<NP>(q, ea, xb, s);
+        for (int q = 0; q < kTimes - 1; ++q) low = product<NP>(q, ea, xb, low);
+        s = product<NP>(kTimes - 1, ea, xb, s);
       }
     }
+    if constexpr (NP == 3) s += low;
     if (v0 + 32 > a.V || __any((uint64_t)(y - v0) < 32u)) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -1073,14 +1185,14 @@ __global__ __launch_bounds__(kBlock) void kd_xent_few(Args a, const T *__restric
     float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 16; ++j) top = fmaxf(top, s[j]);
-    top *= a.c2;
+    top = ceilf(top * a.c2);  // (whole numbers: see pixel_loss)
     if (top > m) {  // (a lane by itself: the halves of a pixel are joined at the end)
       l *= __builtin_amdgcn_exp2f(m - top);
       m = top;
     }
     float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) sum += __builtin_amdgcn_exp2f(fmaf(s[j], a.c2, -m));
+    for (int j = 0; j < 16; ++j) sum += __builtin_amdgcn_exp2f(exponent<T>(s[j], a.c2, a.c2l, -m));
     l += sum;
   }
   // the two halves, then the waves
@@ -1243,7 +1355,7 @@ struct TableWalk : Step<T, DP, 2> {
   using F = Form<T>;
   static constexpr int NP = B::NP, RB = B::RB;
   int v0, near;  // near: this lane's pixel's label
-  float c2, unit, lunit;
+  float c2, c2l, unit, lunit;
   f32x4 lse[4], g[ROWG ? 4 : 1];
   const float *plse, *pw, *pg;
   const int *plab;
@@ -1264,12 +1376,16 @@ struct TableWalk : Step<T, DP, 2> {
     const int lane = threadIdx.x & 63, half = lane >> 5;
     f32x4 l1[4], g1[ROWG ? 4 : 1];
     int near1;
-    rows(t1, l1, g1, near1);
+    // one step ahead; where registers are short, in the step itself, whose exponentials come late
+    if constexpr (NP == 1)
+      rows(t1, l1, g1, near1);
+    else
+      rows(t, lse, g, near);
     B::step(s_x, s_t, [&](int, int i, float &p0, float &p1) {
       const f32x4 l = lse[i / 2];
       const int j = 2 * (i & 1);
-      p0 = __builtin_amdgcn_exp2f(fmaf(p0, c2, ROWG ? l[j] + lunit : l[j]));
-      p1 = __builtin_amdgcn_exp2f(fmaf(p1, c2, ROWG ? l[j + 1] + lunit : l[j + 1]));
+      p0 = __builtin_amdgcn_exp2f(exponent<T>(p0, c2, c2l, ROWG ? l[j] + lunit : l[j]));
+      p1 = __builtin_amdgcn_exp2f(exponent<T>(p1, c2, c2l, ROWG ? l[j + 1] + lunit : l[j + 1]));
       if (ROWG) {
         p0 *= g[i / 2][j];
         p1 *= g[i / 2][j + 1];
@@ -1300,11 +1416,13 @@ struct TableWalk : Step<T, DP, 2> {
             }
         }
     }
-    near = near1;
+    if constexpr (NP == 1) {
+      near = near1;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      lse[i] = l1[i];
-      if (ROWG) g[i] = g1[i];
+      for (int i = 0; i < 4; ++i) {
+        lse[i] = l1[i];
+        if (ROWG) g[i] = g1[i];
+      }
     }
   }
 };
@@ -1321,6 +1439,7 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, 2>::waves)) void kd_xent_table
   stagger();
   TableWalk<T, DP, ROWG> w;
   w.c2 = a.c2;
+  w.c2l = a.c2l;
   w.unit = ROWG ? grad_unit(a) : 1.f;
   w.lunit = ROWG ? log2f(w.unit) : 0.f;  // a power of two: exact
   w.plse = a.lse;
@@ -1335,7 +1454,7 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, 2>::waves)) void kd_xent_table
     const int t0 = 2 * p0, t1 = 2 * p1;
     if (t0 < t1) {
       fetch<kBytes>(s_x0, xs + t0 * kTile);
-      w.rows(t0, w.lse, w.g, w.near);
+      if constexpr (W::np == 1) w.rows(t0, w.lse, w.g, w.near);
       arrive();
       fetch<kBytes>(s_x1, xs + (t0 + 1) * kTile);
       fetch_sum<W>(s_t1, xt + t0 * kTile, z);  // (times zeros)
@@ -1441,7 +1560,10 @@ inline Args shape(int64_t n, int64_t V, int D, int np, double scale, int reducti
   a.dp = padded_channels(D);
   a.scale = (float)scale;
   // never 0: a masked logit, -inf, stays -inf (a scale of 0 makes every logit next to 0 all the same)
-  a.c2 = (float)std::max(fabs(scale) * 1.4426950408889634, 1e-30);
+  const double c2 = std::max(fabs(scale) * 1.4426950408889634, 1e-30);
+  a.c2 = (float)c2;
+  if ((double)a.c2 > c2) a.c2 = nextafterf(a.c2, 0.f);
+  a.c2l = std::max((float)(c2 - (double)a.c2), 1.2e-38f);  // positive too, for the same reason
   a.reduction = reduction;
   return a;
 }

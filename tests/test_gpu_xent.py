@@ -182,6 +182,60 @@ def test_far_from_even(dname, spread, scale):
     _check(got, _reference(x, e, y, scale, 'none', grad))
 
 
+@pytest.mark.parametrize('dname,size', [('f32', 1e-18), ('f32', 1e18), ('bf16', 1e-18),
+                                        ('bf16', 1e18), ('f32', 1e-8), ('bf16', 1e8)])
+def test_tables_of_any_size(dname, size):
+    """Ordinary logits of very small and very large rows: no part of a sum may leave the range."""
+    x, e, y = _inputs(300, 200, 40, TYPES[dname], seed=15)
+    x, e = (x.float() / size).to(x.dtype), (e.float() * size).to(e.dtype)
+    grad = _grad('none', (300,))
+    got = _run(x, e, y, 6.0, 'none', grad)
+    _check(got, _reference(x, e, y, 6.0, 'none', grad))
+    assert (got[1][y >= 0] != 0).any() and (got[2] != 0).any()
+
+
+@pytest.mark.parametrize('dname,n,V,D', [('bf16', 290000, 70, 16), ('bf16', 140000, 33, 100),
+                                         ('f32', 150000, 40, 8), ('f32', 70000, 20, 129),
+                                         ('f16', 70000, 50, 250), ('f16', 300, 140000, 8),
+                                         ('f32', 260, 70000, 33), ('bf16', 100, 70000, 200)])
+def test_more_blocks_than_workgroups(dname, n, V, D):
+    """Whole blocks of held rows in turn and the rest cut across their borders, on both sides."""
+    x, e, y = _inputs(n, V, D, TYPES[dname], seed=16, background=0.05)
+    grad = _grad('none', (n,))
+    _check(_run(x, e, y, 8.0, 'none', grad), _reference(x, e, y, 8.0, 'none', grad))
+
+
+def test_backward_twice():
+    """The forward's state is only read: a second backward gives the same."""
+    from kaolin_amd.metrics.render import surface_cross_entropy
+    x, e, y = _inputs(700, 300, 48, torch.bfloat16, seed=17)
+    x, e = x.requires_grad_(True), e.requires_grad_(True)
+    grad = _grad('none', (700,))
+    loss = surface_cross_entropy(x, e, y, 5.0, 'none')
+    a = torch.autograd.grad(loss, [x, e], grad, retain_graph=True)
+    torch.autograd.grad(loss, [x, e], grad * 1e-3, retain_graph=True)
+    b = torch.autograd.grad(loss, [x, e], grad)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_two_streams_at_once():
+    """Calls in flight on two streams share nothing."""
+    sets = [(_inputs(6000, 3000, 64, torch.bfloat16, seed=18), 9.0),
+            (_inputs(5000, 4000, 32, torch.float32, seed=19), 7.0)]
+    one = torch.tensor(1.0, device=DEV)
+    want = [_run(*a, s, 'mean', one) for a, s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for rep in range(3):
+        for st, (a, s) in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(_run(*a, s, 'mean', one))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(p, q) for p, q in zip(g, want[i % 2]))
+
+
 def test_large_logits_move_the_maximum():
     """Rows of rising size: the running maximum moves in almost every block of the table."""
     x, e, y = _inputs(200, 3001, 48, torch.bfloat16, seed=4)
