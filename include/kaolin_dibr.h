@@ -663,7 +663,8 @@ int kd_deftet_sparse_render_backward_f64(int batch, int64_t num_pixels, int64_t 
  * looked up in its own table.  The backward writes every row of grad_embeddings (batch, rows, D):
  * scale * the sum of its indices' rows of grad_out (n, D), added in a fixed order (no atomics).
  * Limits: n < 2^31, batch * rows < 2^31, D <= 2^20.  The pointers are f32, f64, f16 or bf16 data
- * by the suffix; element_size is 4, 8 or 2.
+ * by the suffix, aligned to an element; element_size is 4, 8 or 2.  The workspace is aligned to 256
+ * bytes.
  * ------------------------------------------------------------------------------------------- */
 size_t kd_surface_embedding_workspace_size(int64_t num_indices, int64_t batch, int64_t rows,
                                            int channels, int element_size);
@@ -706,7 +707,7 @@ int kd_surface_embedding_backward_bf16(int64_t num_indices, int64_t batch, int64
  * only read by the backward, `scratch` is free after each call.  The backward takes the loss's
  * gradient (a scalar, or (n) for reduction 0; fp32, device) and writes grad_features (n, D) and
  * grad_embeddings (rows, D); NULL skips one.  Limits: 1 <= D <= 256, 1 <= rows < 2^31 - 256,
- * n < 2^31 - 256, |scale| < 1e30.
+ * n < 2^31 - 256, |scale| < 1e30.  state and scratch are aligned to 256 bytes, data to an element.
  * ------------------------------------------------------------------------------------------- */
 size_t kd_surface_xent_state_size(int64_t num_pixels, int64_t rows, int channels,
                                   int element_size, int need_features, int need_embeddings);

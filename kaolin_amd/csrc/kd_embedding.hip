@@ -595,6 +595,8 @@ static int embed_backward(int64_t n, int64_t batch, int64_t rows, int D, const i
     const EmbedPlan p = embed_plan(n, nkeys, D, (int)sizeof(T));
     if (wsb < p.total || !ws)
       return set_error(KD_ERR_WORKSPACE, "workspace too small: %zu < %zu", wsb, p.total);
+    KD_CHECK_ARG(((uintptr_t)ws & 255u) == 0,
+                 "surface_embedding: the workspace must be aligned to 256 bytes");
     char *c = (char *)ws;
     uint2 *buf[2] = {(uint2 *)c, (uint2 *)(c + p.pairs)};
     c += 2 * p.pairs;

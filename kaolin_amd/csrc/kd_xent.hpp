@@ -1694,6 +1694,8 @@ int forward(int64_t n, int64_t V, int D, const T *features, const T *table, cons
   if (!state || state_bytes < ns || !scratch || scratch_bytes < nw)
     return set_error(KD_ERR_WORKSPACE, "workspace too small: %zu < %zu or %zu < %zu", state_bytes,
                      ns, scratch_bytes, nw);
+  KD_CHECK_ARG((((uintptr_t)state | (uintptr_t)scratch) & 255u) == 0,
+               "surface_cross_entropy: state and scratch must be aligned to 256 bytes");
   ProfScope prof(K_XENT_FWD, stream);
   if (n > 0 && n <= kFewPixels && !need_x && !need_e) {
     switch (a.dp) {
@@ -1750,6 +1752,8 @@ int backward(int64_t n, int64_t V, int D, const int64_t *labels, double scale, i
   if (!state || state_bytes < ns || !scratch || scratch_bytes < nw)
     return set_error(KD_ERR_WORKSPACE, "workspace too small: %zu < %zu or %zu < %zu", state_bytes,
                      ns, scratch_bytes, nw);
+  KD_CHECK_ARG((((uintptr_t)state | (uintptr_t)scratch) & 255u) == 0,
+               "surface_cross_entropy: state and scratch must be aligned to 256 bytes");
   ProfScope prof(K_XENT_BWD, stream);
   if (ge && reduction == 0)
     hipLaunchKernelGGL(kd_xent_rowgrad,

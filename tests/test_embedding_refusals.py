@@ -96,6 +96,10 @@ def test_native_calls_refuse_before_they_launch():
                                               1 << 30, None), b'workspace'),
             ('kd_surface_xent_forward_bf16', (8, 5, 16, p, p, p, 1.0, 1, 1, 1, p, p, 1 << 30, p,
                                               64, None), b'workspace'),
+            ('kd_surface_xent_forward_bf16', (8, 5, 16, p, p, p, 1.0, 1, 1, 1, p, p + 16, 1 << 30, p,
+                                              1 << 30, None), b'aligned'),
+            ('kd_surface_embedding_backward_f16', (8, 1, 5, 4, p, p, 1.0, p, p + 16, 1 << 30, None),
+             b'aligned'),
             ('kd_surface_xent_backward_f32', (8, 5, 16, p, 1.0, 1, 0, 1, p, p, p, p, 1 << 30, p,
                                               1 << 30, None), b'did not prepare'),
             ('kd_surface_xent_backward_f32', (8, 5, 16, p, 1.0, 1, 1, 1, None, p, p, p, 1 << 30, p,
