@@ -820,22 +820,29 @@ def surface_embedding_forward(index, embeddings, scale):
     return out
 
 
-def surface_embedding_backward(grad_out, index, shape, scale):
-    """The gradient of a table of `shape`: scale * the sum of the rows of grad_out (..., D) that
-    each table row was looked up for, added in the indices' order."""
-    fn = 'surface_embedding_backward'
-    dev = _check_same_gpu(fn, grad_out=grad_out, index=index)
-    sfx = _sfx16(grad_out, fn)
-    n, B, N, D, scale = _embedding_args(fn, index, shape, scale)
-    _check_size(fn, 'grad_out', grad_out, (*index.shape, D))
-    index, grad_out = index.contiguous(), grad_out.contiguous()
-    grad = torch.empty(tuple(shape), device=dev, dtype=grad_out.dtype)
+def surface_embedding_plan(index, embeddings, scale):
+    """What surface_embedding_backward needs for the gradient of `embeddings`, checked once: the
+    forward's arguments, the table's shape and the workspace's size."""
+    fn = 'surface_embedding'
+    dev = _check_same_gpu(fn, index=index, embeddings=embeddings)
+    sfx = _sfx16(embeddings, fn)
+    n, B, N, D, scale = _embedding_args(fn, index, embeddings.shape, scale)
+    nb = int(_lib.load().kd_surface_embedding_workspace_size(n, B, N, D,
+                                                             embeddings.element_size()))
+    return (f'kd_surface_embedding_backward_{sfx}', dev, embeddings.shape, embeddings.dtype,
+            (n, B, N, D), scale, nb)
+
+
+def surface_embedding_backward(grad_out, index, plan):
+    """The gradient of the plan's table: scale * the sum of the rows of grad_out (..., D) that each
+    table row was looked up for, added in the indices' order."""
+    name, dev, shape, dtype, sizes, scale, nb = plan
+    grad = torch.empty(shape, device=dev, dtype=dtype)
     if grad.numel():
-        nb = int(_lib.load().kd_surface_embedding_workspace_size(n, B, N, D,
-                                                                 grad_out.element_size()))
+        index, grad_out = index.contiguous(), grad_out.contiguous()
         ws = _bytes(nb, dev)
-        _launch(dev, f'kd_surface_embedding_backward_{sfx}', n, B, N, D, _ptr(index),
-                _ptr(grad_out), scale, _ptr(grad), _ptr(ws), nb)
+        _launch(dev, name, *sizes, index.data_ptr(), grad_out.data_ptr(), scale, grad.data_ptr(),
+                ws.data_ptr(), nb)
     return grad
 
 
@@ -1074,6 +1081,7 @@ render = types.SimpleNamespace(mesh=types.SimpleNamespace(
     deftet_sparse_render_forward_cuda=deftet_sparse_render_forward_cuda,
     deftet_sparse_render_backward_cuda=deftet_sparse_render_backward_cuda,
     surface_embedding_forward=surface_embedding_forward,
+    surface_embedding_plan=surface_embedding_plan,
     surface_embedding_backward=surface_embedding_backward,
 ))
 metrics = types.SimpleNamespace(mask_iou_forward=mask_iou_forward,

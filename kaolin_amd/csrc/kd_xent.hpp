@@ -370,8 +370,8 @@ __device__ __forceinline__ uint32_t upper2(uint32_t lo, uint32_t hi) {
   return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
 }
 
-// Two probabilities of a lane as elements 2 i and 2 i + 1 of an operand (its words, plane by plane).
-template <typename T>
+// Two probabilities of a lane as elements 2 i and 2 i + 1 of an operand (its words, part by part).
+template <typename T, int PP>
 __device__ __forceinline__ void pack_pair(float p0, float p1, int i, uint4 *o) {
   using H = typename Form<T>::H;
   if constexpr (Form<T>::np == 1) {
@@ -380,6 +380,12 @@ __device__ __forceinline__ void pack_pair(float p0, float p1, int i, uint4 *o) {
     v[0] = (H)p0;
     v[1] = (H)p1;
     ((uint32_t *)o)[i] = __builtin_bit_cast(uint32_t, v);
+    if constexpr (PP == 2) {
+      h2 r;
+      r[0] = (H)(p0 - (float)v[0]);
+      r[1] = (H)(p1 - (float)v[1]);
+      ((uint32_t *)&o[1])[i] = __builtin_bit_cast(uint32_t, r);
+    }
   } else {
     uint32_t u[3][2];
 #pragma unroll
@@ -414,6 +420,13 @@ constexpr int walk_waves(int np, int dp, int kind) {
 constexpr int walk_columns(int np, int dp, int kind) {
   return np == 3 && dp == 256 && kind > 0 ? 2 : 1;
 }
+// Parts of a probability in its product with the table's rows or the pixels' features.  Rounded once
+// to bf16 or fp16 (half a step, 2^-9 or 2^-12 of the probability, which averages out over rows that
+// differ), the error stays whole where few channels make the rows alike: one channel and tens of rows
+// had gradients 2e-3 to 4e-3 off in bf16, where one rounding of the result is 1.7e-3.  Up to 32
+// channels the products are the smaller part of the work (512 x 512 pixels, 64 channels: the logits and
+// the sum are as long as the exponentials), so there a second part carries what the first left out.
+constexpr int walk_parts(int np, int dp) { return np == 3 ? 3 : (dp == 32 ? 2 : 1); }
 constexpr int walk_rows(int np, int dp, int kind) { return 128 * walk_blocks(np, dp, kind); }
 // Workgroups: as many as run at once on 256 compute units.
 constexpr int walk_workers(int np, int dp, int kind) {
@@ -426,6 +439,7 @@ struct Walk {
   static constexpr int rb = walk_blocks(np, DP, KIND);
   static constexpr int waves = walk_waves(np, DP, KIND);
   static constexpr int cs = walk_columns(np, DP, KIND);
+  static constexpr int pp = walk_parts(np, DP);
   static constexpr int rows = walk_rows(np, DP, KIND);  // held by a workgroup
   static constexpr int workers = walk_workers(np, DP, KIND);
   static constexpr int tile_bytes = np * 32 * DP * 2;  // a tile's operands: a multiple of 1024
@@ -550,11 +564,11 @@ struct Step {
   using H8 = typename F::H8;
   using W = Walk<T, DP, KIND>;
   static constexpr bool SUM = KIND > 0;
-  static constexpr int NP = F::np, RB = W::rb, KS = DP / 16, DT = DP / 32 / W::cs;
+  static constexpr int NP = F::np, RB = W::rb, PP = W::pp, KS = DP / 16, DT = DP / 32 / W::cs;
   H8 held[RB][KS][NP];
   f32x16 s[RB];
   f32x16 o[SUM ? RB : 1][SUM ? DT : 1];
-  uint4 q[RB][2][NP];
+  uint4 q[RB][2][PP];
 
   __device__ __forceinline__ void hold(const uint16_t *packed, int64_t row0) {
     const int lane = threadIdx.x & 63;
@@ -573,7 +587,7 @@ struct Step {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int p = 0; p < NP; ++p) q[b][h][p] = make_uint4(0, 0, 0, 0);
+        for (int p = 0; p < PP; ++p) q[b][h][p] = make_uint4(0, 0, 0, 0);
     }
   }
 
@@ -608,13 +622,17 @@ struct Step {
     for (int n = 0; n < kOps; ++n) {
       if (n + kAhead < kOps) load(n + kAhead);
 #pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        if (n < kAdd)
-          o[b][n % DT] = mfma(a[n], __builtin_bit_cast(H8, q[b][n / DT][0]), o[b][n % DT]);
-        else
-          next[b] = mfma(a[n], held[b][n - kAdd][0], next[b]);
-        between(done++);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int p = PP - 1; p >= 0; --p) {  // (the small part first)
+        if (n >= kAdd && p > 0) continue;
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+          if (n < kAdd)
+            o[b][n % DT] = mfma(a[n], __builtin_bit_cast(H8, q[b][n / DT][p]), o[b][n % DT]);
+          else
+            next[b] = mfma(a[n], held[b][n - kAdd][0], next[b]);
+          between(done++);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
   }
@@ -716,10 +734,11 @@ struct Step {
   // pair(b, i, z0, z1): the probabilities 2 i and 2 i + 1 of block b in place of their logits
   template <typename Pair>
   __device__ __forceinline__ void step(const uint4 *straight, const uint4 *transposed, Pair pair) {
-    constexpr int kSlots = (NP == 3 ? 6 : 1) * RB * (KS + (SUM ? 2 * DT : 0)) + 1;
+    constexpr int kSlots =
+        NP == 3 ? 6 * (KS + (SUM ? 2 * DT : 0)) + 1 : RB * (KS + (SUM ? 2 * DT * PP : 0)) + 1;
     constexpr int kPairs = RB * 8;
     f32x16 next[RB];
-    uint4 fresh[RB][2][NP];
+    uint4 fresh[RB][2][PP];
     // split operands: behind the weighted sum, whose operands' registers the new ones take over
     constexpr int kFirst = NP == 3 && SUM ? 12 * DT : 0;
     products<SUM, true>(straight, transposed, next, [&](int slot) {
@@ -732,10 +751,10 @@ struct Step {
         float p0 = s[b][2 * i], p1 = s[b][2 * i + 1];
         pair(b, i, p0, p1);
         if constexpr (SUM) {
-          pack_pair<T>(p0, p1, i & 3, fresh[b][i >> 2]);
+          pack_pair<T, PP>(p0, p1, i & 3, fresh[b][i >> 2]);
           // (stays in its slot: the compiler would move it behind the products)
 #pragma unroll
-          for (int p = 0; p < NP; ++p)
+          for (int p = 0; p < PP; ++p)
             asm volatile("" : "+v"(((uint32_t *)&fresh[b][i >> 2][p])[i & 3]));
         }
       }
@@ -747,7 +766,7 @@ struct Step {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int p = 0; p < NP; ++p) q[b][h][p] = fresh[b][h][p];
+          for (int p = 0; p < PP; ++p) q[b][h][p] = fresh[b][h][p];
       }
     }
   }
@@ -783,7 +802,7 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
   using B = Step<T, DP, SUM ? 1 : 0>;
   using F = Form<T>;
   using H8 = typename F::H8;
-  static constexpr int NP = B::NP, RB = B::RB, DT = B::DT;
+  static constexpr int RB = B::RB, DT = B::DT, PP = B::PP;
   int lab[RB];
   float m[RB], l[RB][2], zy[RB];
   int V;
@@ -839,7 +858,7 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int p = 0; p < NP; ++p)
+            for (int p = 0; p < PP; ++p)
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
                 typename F::H *e = (typename F::H *)&this->q[b][h][p] + j;
@@ -1353,7 +1372,7 @@ template <typename T, int DP, bool ROWG>
 struct TableWalk : Step<T, DP, 2> {
   using B = Step<T, DP, 2>;
   using F = Form<T>;
-  static constexpr int NP = B::NP, RB = B::RB;
+  static constexpr int NP = B::NP, RB = B::RB, PP = B::PP;
   int v0, near;  // near: this lane's pixel's label
   float c2, c2l, unit, lunit;
   f32x4 lse[4], g[ROWG ? 4 : 1];
@@ -1403,14 +1422,16 @@ struct TableWalk : Step<T, DP, 2> {
           const int y = plab[k] - v0 - (lane & 31);
           const float neg = ROWG ? pw[k] * (pg[k] * unit) : pw[k];
           uint16_t part[3] = {0, 0, 0};
-          if constexpr (NP == 1)
-            part[0] = __builtin_bit_cast(uint16_t, (typename F::H)neg);
-          else
+          if constexpr (NP == 1) {
+            const typename F::H large = (typename F::H)neg;
+            part[0] = __builtin_bit_cast(uint16_t, large);
+            part[1] = __builtin_bit_cast(uint16_t, (typename F::H)(neg - (float)large));
+          } else
             split3(neg, part[0], part[1], part[2]);
 #pragma unroll
           for (int b = 0; b < RB; ++b)
 #pragma unroll
-            for (int p = 0; p < NP; ++p) {
+            for (int p = 0; p < PP; ++p) {
               uint16_t *e = (uint16_t *)&this->q[b][h][p] + j;
               *e = y == 32 * b ? part[p] : *e;
             }

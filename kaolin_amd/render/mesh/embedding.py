@@ -22,7 +22,7 @@ class SurfaceEmbeddingHip(Function):
     def forward(ctx, index, embeddings, scale):
         out = _C.render.mesh.surface_embedding_forward(index, embeddings, scale)
         ctx.save_for_backward(index)
-        ctx.table_shape, ctx.scale = embeddings.shape, scale
+        ctx.plan = _C.render.mesh.surface_embedding_plan(index, embeddings, scale)
         ctx.set_materialize_grads(False)
         return out
 
@@ -36,8 +36,7 @@ def _grad(ctx, grad_out):
     if grad_out is None:
         return None, None, None
     index, = ctx.saved_tensors
-    return None, _C.render.mesh.surface_embedding_backward(grad_out, index, ctx.table_shape,
-                                                           ctx.scale), None
+    return None, _C.render.mesh.surface_embedding_backward(grad_out, index, ctx.plan), None
 
 
 _guarded_grad = once_differentiable(_grad)
