@@ -22,7 +22,7 @@
 // 16-bit data multiply exactly into 32-bit sums.  The probabilities enter their product with the
 // table (or the features) rounded to the data's type, at most 2^-8 (bf16) or 2^-11 (fp16, scaled so that
 // small ones stay normal) of each term, like the operands themselves; the sums L' use the
-// unrounded values.  32-bit data are split by truncation into three bf16 parts (8 + 8 + 8 bits, the
+// unrounded values.  32-bit data are split into three bf16 parts (8 + 8 + 8 bits, the
 // whole significand) and multiplied as the six products above 2^-24: the fp32 matrix instructions
 // run at 1/16 of the bf16 rate, six bf16 products at 1/6.
 #pragma once
@@ -76,17 +76,23 @@ __device__ __forceinline__ f32x16 mfma(bfloat8 a, bfloat8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// x as three bf16 by truncation (exact: 8 + 8 + 8 significand bits)
+// x as three bf16, each the nearest to what is left (exact: what the first two leave, at most 2^-18 x,
+// has 8 bits).  Parts by truncation would all have the sign of x, and so would the three small
+// products that are not formed: 4e-8 of every logit, a gradient of the table 8e-7 off where rounded
+// parts leave 4e-9 (60,000 pixels, 59 rows, 3 channels, scale 24).
 __device__ __forceinline__ void split3(float x, uint16_t &a, uint16_t &b, uint16_t &c) {
-  const uint32_t u = __float_as_uint(x);
-  a = (uint16_t)(u >> 16);
-  const float r = x - __uint_as_float(u & 0xffff0000u);
-  const uint32_t v = __float_as_uint(r);
-  b = (uint16_t)(v >> 16);
-  c = (uint16_t)(__float_as_uint(r - __uint_as_float(v & 0xffff0000u)) >> 16);
+  const uint32_t cut = __float_as_uint(x) & 0xffff0000u;  // (the nearest to these is infinite)
+  const bfloat_t h =
+      fabsf(x) < 0x1.ffp127f ? (bfloat_t)x : __builtin_bit_cast(bfloat_t, (uint16_t)(cut >> 16));
+  const float r = x - (float)h;
+  const bfloat_t m = (bfloat_t)r;
+  a = __builtin_bit_cast(uint16_t, h);
+  b = __builtin_bit_cast(uint16_t, m);
+  c = __builtin_bit_cast(uint16_t, (bfloat_t)(r - (float)m));
 }
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.9259629e-8f;
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kSlots = 64, kSlotPad = 16;  // maxima of the table, 64 bytes apart
 constexpr int kRowPad = 256;  // packed rows are padded with zeros to a multiple of this
 constexpr int kMapChunk = 2048;   // pixels listed at a time
@@ -387,6 +393,8 @@ __device__ __forceinline__ void pack_pair(float p0, float p1, int i, uint4 *o) {
       ((uint32_t *)&o[1])[i] = __builtin_bit_cast(uint32_t, r);
     }
   } else {
+    // (by truncation, which is cheaper: the other operand's parts are rounded, so what is left out has
+    // either sign all the same)
     uint32_t u[3][2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -804,7 +812,7 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
   using H8 = typename F::H8;
   static constexpr int RB = B::RB, DT = B::DT, PP = B::PP;
   int lab[RB];
-  float m[RB], l[RB][2], zy[RB];
+  float m[RB], l[RB][2], zy[RB];  // l: two sums, of which the sum of the probabilities is the sum
   int V;
   float c2, c2l;
 
@@ -877,6 +885,7 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
 
   template <bool ONLINE>
   __device__ __forceinline__ void next(const uint4 *s_e, const uint4 *s_t) {
+    float t[RB][2] = {};  // the tile's sums
     B::step(s_e, s_t, [&](int b, int, float &p0, float &p1) {
       if constexpr (ONLINE || sizeof(T) == 4) {
         const float shift = ONLINE ? F::shift - m[b] : 0.f;
@@ -886,10 +895,21 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
         p0 = __builtin_amdgcn_exp2f(p0 * c2);
         p1 = __builtin_amdgcn_exp2f(p1 * c2);
       }
-      l[b][0] += p0;
-      l[b][1] += p1;
-      asm volatile("" : "+v"(l[b][0]), "+v"(l[b][1]));  // (stays in its slot)
+      float(&sum)[2] = sizeof(T) == 4 ? t[b] : l[b];
+      sum[0] += p0;
+      sum[1] += p1;
+      asm volatile("" : "+v"(sum[0]), "+v"(sum[1]));  // (stays in its slot)
     });
+    // 32-bit data: a walk of 150,000 rows is 40,000 additions a lane, whose roundings would leave 3e-6
+    // of the sum; l[b][1] holds what the last one lost
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        const float y = l[b][1] + (t[b][0] + t[b][1]), sum = l[b][0] + y;
+        l[b][1] = y - (sum - l[b][0]);
+        l[b][0] = sum;
+      }
+    }
   }
 };
 
@@ -998,7 +1018,7 @@ __device__ __forceinline__ float pixel_loss(float m, float l, float z, const Arg
   const float t = expf(-fabsf(u));
   const float value = u != u ? u : fmaxf(u, 0.f) + log1pf(t);
   w = u != u ? u : (u >= 0.f ? 1.f / (1.f + t) : t / (1.f + t));
-  lse = z2 + value * kLog2e;
+  lse = fmaf(z, a.c2, fmaf(z, a.c2l, fmaf(value, kLog2e, value * kLog2eLow)));
   return value;
 }
 
