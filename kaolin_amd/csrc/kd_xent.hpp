@@ -812,7 +812,7 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
   using H8 = typename F::H8;
   static constexpr int RB = B::RB, DT = B::DT, PP = B::PP;
   int lab[RB];
-  float m[RB], l[RB][2], zy[RB];  // l: two sums, of which the sum of the probabilities is the sum
+  float m[RB], l[RB][2], t[RB][2], zy[RB];  // l + t: the sum of the probabilities in four terms
   int V;
   float c2, c2l;
 
@@ -858,6 +858,8 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
         m[b] = mn;
         l[b][0] *= f;
         l[b][1] *= f;
+        t[b][0] *= f;
+        t[b][1] *= f;
         if constexpr (SUM) {
 #pragma unroll
           for (int d = 0; d < DT; ++d)
@@ -883,9 +885,27 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
     if constexpr (ONLINE) raise();
   }
 
+  // The sums of the last tiles (one of 32-bit data, two of 16-bit data) to those before: a walk of
+  // 150,000 rows would be 40,000 additions a lane, whose roundings leave 3e-6 of the sum.  With 32-bit
+  // data l[b][1] holds what the last addition lost; with 16-bit data that takes 1.5 % of the time, and
+  // a rounding every 16 probabilities is little beside the operands'.
+  __device__ __forceinline__ void fold() {
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      if constexpr (sizeof(T) == 4) {
+        const float y = l[b][1] + (t[b][0] + t[b][1]), sum = l[b][0] + y;
+        l[b][1] = y - (sum - l[b][0]);
+        l[b][0] = sum;
+      } else {
+        l[b][0] += t[b][0];
+        l[b][1] += t[b][1];
+      }
+      t[b][0] = t[b][1] = 0.f;
+    }
+  }
+
   template <bool ONLINE>
   __device__ __forceinline__ void next(const uint4 *s_e, const uint4 *s_t) {
-    float t[RB][2] = {};  // the tile's sums
     B::step(s_e, s_t, [&](int b, int, float &p0, float &p1) {
       if constexpr (ONLINE || sizeof(T) == 4) {
         const float shift = ONLINE ? F::shift - m[b] : 0.f;
@@ -895,21 +915,11 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
         p0 = __builtin_amdgcn_exp2f(p0 * c2);
         p1 = __builtin_amdgcn_exp2f(p1 * c2);
       }
-      float(&sum)[2] = sizeof(T) == 4 ? t[b] : l[b];
-      sum[0] += p0;
-      sum[1] += p1;
-      asm volatile("" : "+v"(sum[0]), "+v"(sum[1]));  // (stays in its slot)
+      t[b][0] += p0;
+      t[b][1] += p1;
+      asm volatile("" : "+v"(t[b][0]), "+v"(t[b][1]));  // (stays in its slot)
     });
-    // 32-bit data: a walk of 150,000 rows is 40,000 additions a lane, whose roundings would leave 3e-6
-    // of the sum; l[b][1] holds what the last one lost
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        const float y = l[b][1] + (t[b][0] + t[b][1]), sum = l[b][0] + y;
-        l[b][1] = y - (sum - l[b][0]);
-        l[b][0] = sum;
-      }
-    }
+    if constexpr (sizeof(T) == 4) fold();
   }
 };
 
@@ -949,7 +959,7 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
     for (int b = 0; b < RB; ++b) {
       w.lab[b] = a.lab[row0 + 32 * b + (lane & 31)];
       w.m[b] = general ? -1e30f : 0.f;
-      w.l[b][0] = w.l[b][1] = 0.f;
+      w.l[b][0] = w.l[b][1] = w.t[b][0] = w.t[b][1] = 0.f;
       w.zy[b] = -INFINITY;
     }
     const int t0 = 2 * p0, t1 = 2 * p1;
@@ -972,6 +982,7 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
         fetch<kBytes>(s_e1, es + t3 * kTile);
         if constexpr (SUM) fetch_sum<W>(s_t1, et + (t + 1) * kTile, z);
         w.template next<ONLINE>(s_e0, s_t0);
+        if constexpr (sizeof(T) == 2) w.fold();
         w.template ready<ONLINE>(t2 * 32);
         arrive();
       }
@@ -1603,8 +1614,9 @@ inline Args shape(int64_t n, int64_t V, int D, int np, double scale, int reducti
   // never 0: a masked logit, -inf, stays -inf (a scale of 0 makes every logit next to 0 all the same)
   const double c2 = std::max(fabs(scale) * 1.4426950408889634, 1e-30);
   a.c2 = (float)c2;
-  if ((double)a.c2 > c2) a.c2 = nextafterf(a.c2, 0.f);
-  a.c2l = std::max((float)(c2 - (double)a.c2), 1.2e-38f);  // positive too, for the same reason
+  if (np == 3 && (double)a.c2 > c2) a.c2 = nextafterf(a.c2, 0.f);
+  // positive too, for the same reason; 16-bit data are multiplied by c2 alone, all of them
+  a.c2l = np == 3 ? std::max((float)(c2 - (double)a.c2), 1.2e-38f) : 1.2e-38f;
   a.reduction = reduction;
   return a;
 }

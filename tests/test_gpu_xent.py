@@ -205,6 +205,27 @@ def test_more_blocks_than_workgroups(dname, n, V, D):
     _check(_run(x, e, y, 8.0, 'none', grad), _reference(x, e, y, 8.0, 'none', grad))
 
 
+@pytest.mark.parametrize('dname', ['f32', 'f16', 'bf16'])
+@pytest.mark.parametrize('train', [False, True])
+def test_long_sums(dname, train):
+    """A table of like rows, more pixels than workgroups hold: the loss is log V, and adding up like
+    terms one by one rounds every time the same way.  In steps of 2^-24: 16 + 3 for the terms of one or
+    two tiles, V / 64 for the tiles (16-bit data; 32-bit data carry what is lost: 3), 256 for the parts
+    of a walk, 4 for the exponential, 16 for a logit's product with its factor (below 8 in log2, twice),
+    and the loss's own 4 roundings."""
+    from kaolin_amd.metrics.render import surface_cross_entropy
+    V, n = 100001, 140000
+    dt = TYPES[dname]
+    e = torch.tensor([0.75, -0.5, 0.375], device=DEV, dtype=dt).repeat(V, 1)
+    x = torch.tensor([0.875, -0.625, 0.3125], device=DEV, dtype=dt).repeat(n, 1)
+    y = torch.arange(n, device=DEV) % V
+    x.requires_grad_(train)
+    loss = surface_cross_entropy(x, e, y, 3.7, 'none').detach().double()
+    want = math.log(V)
+    steps = 19 + (3 if dname == 'f32' else V / 64) + 256 + 4 + 16 + 4 * want
+    assert (loss - want).abs().max() <= steps * 2.0 ** -24
+
+
 def test_backward_twice():
     """The forward's state is only read: a second backward gives the same."""
     from kaolin_amd.metrics.render import surface_cross_entropy
