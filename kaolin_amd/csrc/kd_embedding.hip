@@ -10,11 +10,11 @@
 // are looked at, writes n * D * sizeof(T).
 //
 // Backward: no atomics on values, so the result does not depend on timing.  The tokens that name a row
-// are sorted by key with a stable least-significant-digit radix sort (up to 10 bits a pass, 8 bytes a token),
-// so a row's tokens stand together in token order; then each group of G lanes (one row of the
+// are sorted by key with a stable least-significant-digit radix sort (up to 10 bits a pass, 8 bytes a
+// token), so a row's tokens stand together in token order; then each group of G lanes (one row of the
 // gradient, 16 bytes a lane) walks a run of sorted tokens and adds their gradient rows in registers.
 // Runs that cross a group's border are joined in LDS by the group in which they begin, runs that cross
-// a workgroup's border by a second launch.  The split of the walk over groups goes by position and
+// a workgroup's border by the last workgroup or, where they are many, by a second launch.  The split of the walk over groups goes by position and
 // not by key, so one face that fills the image costs no more than any other.
 #include "kd_capi.hpp"
 #include "kd_common.hpp"
@@ -29,6 +29,8 @@ constexpr int kSortIters = kSortTile / kBlock;
 constexpr int kMaxBits = 10;                // of a sort digit: 16-bit keys take two passes, 20-bit ones too
 constexpr int kDigits = 1 << kMaxBits;
 constexpr int kFewTiles = 64;               // up to so many tiles the sort needs no scan launch
+constexpr int kSortOne = 16384;             // up to so many tokens one workgroup sorts in one launch
+constexpr int kJoinRounds = 4;              // up to so many rounds the last workgroup joins the borders
 constexpr int kMaxChannels = 1 << 20;
 
 // ------------------------------------------------------------------------------------------------
@@ -116,9 +118,9 @@ struct SortKeys {
 __device__ __forceinline__ void embed_fill(uint32_t block, uint32_t nblocks, int64_t bytes,
                                            void *p) {
   const int64_t head = min(bytes, (int64_t)((16 - ((uintptr_t)p & 15)) & 15));
-  const int64_t body = (bytes - head) / 16, i0 = (int64_t)block * kBlock + threadIdx.x;
+  const int64_t body = (bytes - head) / 16, i0 = (int64_t)block * blockDim.x + threadIdx.x;
   uint4 *q = (uint4 *)((char *)p + head);
-  for (int64_t i = i0; i < body; i += (int64_t)nblocks * kBlock) q[i] = make_uint4(0, 0, 0, 0);
+  for (int64_t i = i0; i < body; i += (int64_t)nblocks * blockDim.x) q[i] = make_uint4(0, 0, 0, 0);
   if (block == 0) {  // the two ends, 2 bytes at a time
     uint16_t *a = (uint16_t *)p, *z = (uint16_t *)(q + body);
     const int na = (int)(head / 2), nz = (int)((bytes - head - body * 16) / 2);
@@ -151,7 +153,8 @@ __global__ __launch_bounds__(kBlock) void kd_embed_hist(SortKeys s, int shift, u
     hist[(int64_t)d * ntile + blockIdx.x] = cnt[d];
 }
 
-// Inclusive sum over the workgroup's threads; total in every thread.
+// Inclusive sum over the workgroup's N threads; total in every thread.
+template <int N = kBlock>
 __device__ __forceinline__ uint32_t wg_scan(uint32_t x, uint32_t *s_w, uint32_t &total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
@@ -164,7 +167,7 @@ __device__ __forceinline__ uint32_t wg_scan(uint32_t x, uint32_t *s_w, uint32_t 
   uint32_t off = 0;
   total = 0;
 #pragma unroll
-  for (int k = 0; k < kBlock / kWave; ++k) {
+  for (int k = 0; k < N / kWave; ++k) {
     if (k < w) off += s_w[k];
     total += s_w[k];
   }
@@ -189,22 +192,45 @@ __global__ __launch_bounds__(kBlock) void kd_embed_scan(int ntile, uint32_t *__r
   if (threadIdx.x == 0) totals[blockIdx.x] = run;
 }
 
+// A wave's rank of its ITERS x 64 consecutive tokens (kt, those of `in`), 64 at a time: the lanes that hold
+// the same digit are found with one ballot per digit bit, a lane's rank is the number of lower ones among
+// them plus the wave's count of that digit so far.  The order within a digit is the tokens' order: stable.
+template <int ITERS>
+__device__ __forceinline__ void embed_rank(const uint2 (&kt)[ITERS], uint32_t in, int iters, int shift,
+                                           int bits, uint32_t *cnt, uint32_t (&rank)[ITERS]) {
+  const uint32_t mask = (1u << bits) - 1u;
+#pragma unroll
+  for (int it = 0; it < ITERS; ++it) {
+    if (it < iters) {
+      const bool have = (in >> it) & 1u;
+      const uint32_t d = (kt[it].x >> shift) & mask;
+      uint64_t same = __ballot(have);
+      for (int b = 0; b < bits; ++b) {
+        const uint64_t set = __ballot((d >> b) & 1u);
+        same &= ((d >> b) & 1u) ? set : ~set;
+      }
+      const int below = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32),
+                                                  __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
+      uint32_t r = 0;
+      if (have) {
+        r = cnt[d];
+        rank[it] = r + below;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (have && below == 0) cnt[d] = r + (uint32_t)__popcll(same);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+  }
+}
+
 // Bound by latency and the scattered 8-byte writes: 4,217,024 tokens that name one of 50,000 rows, of
 // 8,388,608, 29 us a pass (two passes) behind 16 us of counting, 2,097,152 tokens 15 and 8 us.
-// Each wave ranks its 1024 consecutive tokens 64 at a time: the lanes that hold the same digit are
-// found with one ballot per digit bit, a lane's rank is the number of lower ones among them plus
-// the wave's count of that digit so far.  The order within a digit is the tokens' order: stable.
 // Where the tiles are few (kFewTiles) each workgroup adds up the tiles' counts itself, a thread a
-// digit, and a single tile counts its own: the launches cost more than the work there.
+// digit: a launch costs more than that.
 __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
     SortKeys s, int shift, int bits, int ntile, const uint32_t *__restrict__ hist,
-    const uint32_t *__restrict__ totals, uint32_t *__restrict__ kept, uint2 *__restrict__ out,
-    int64_t fill_bytes, void *fill) {
+    const uint32_t *__restrict__ totals, uint32_t *__restrict__ kept, uint2 *__restrict__ out) {
   constexpr int kWaves = kBlock / kWave;
-  if ((int)blockIdx.x >= ntile) {
-    embed_fill(blockIdx.x - ntile, gridDim.x - ntile, fill_bytes, fill);
-    return;
-  }
   __shared__ uint32_t wcnt[kWaves][kDigits];
   __shared__ uint32_t s_w[kWaves];
   const uint32_t mask = (1u << bits) - 1u, m = s.count();
@@ -221,26 +247,7 @@ __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
   for (int it = 0; it < kSortIters; ++it)
     if (s.get(base + it * kWave, m, kt[it])) in |= 1u << it;
   __syncthreads();
-#pragma unroll
-  for (int it = 0; it < kSortIters; ++it) {
-    const bool have = (in >> it) & 1u;
-    const uint32_t d = (kt[it].x >> shift) & mask;
-    uint64_t same = __ballot(have);
-    for (int b = 0; b < bits; ++b) {
-      const uint64_t set = __ballot((d >> b) & 1u);
-      same &= ((d >> b) & 1u) ? set : ~set;
-    }
-    const int below = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32),
-                                                __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
-    uint32_t r = 0;
-    if (have) {
-      r = wcnt[w][d];
-      rank[it] = r + below;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (have && below == 0) wcnt[w][d] = r + (uint32_t)__popcll(same);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  }
+  embed_rank<kSortIters>(kt, in, kSortIters, shift, bits, wcnt[w], rank);
   __syncthreads();
   // where each digit begins among all tokens, and this tile's part of it
   // (a thread takes kDigits / kBlock digits in a row, as the sum over the digits needs)
@@ -251,10 +258,7 @@ __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
     const uint32_t d = threadIdx.x * kPer + q;
     all[q] = before[q] = 0;
     if (d > mask) continue;
-    if (ntile == 1) {
-#pragma unroll
-      for (int k = 0; k < kWaves; ++k) all[q] += wcnt[k][d];
-    } else if (ntile <= kFewTiles) {
+    if (ntile <= kFewTiles) {
       const uint32_t *h = hist + (int64_t)d * ntile;
 #pragma unroll 8
       for (int k = 0; k < ntile; ++k) {
@@ -269,7 +273,10 @@ __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
     mine += all[q];
   }
   uint32_t begin = wg_scan(mine, s_w, tot) - mine;
-  if (blockIdx.x == 0 && threadIdx.x == 0 && kept) *kept = tot;
+  if (blockIdx.x == 0 && threadIdx.x == 0 && kept) {
+    kept[0] = tot;
+    kept[1] = 0;
+  }
 #pragma unroll
   for (int q = 0; q < kPer; ++q) {
     const uint32_t d = threadIdx.x * kPer + q;
@@ -289,6 +296,71 @@ __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
     if ((in >> it) & 1u) out[wcnt[w][(kt[it].x >> shift) & mask] + rank[it]] = kt[it];
 }
 
+// All passes for few tokens in one workgroup, in the place of two launches a pass (bound by the latency
+// of its loads, ranks and stores: 9,680 tokens and 6,335 rows 22 us against 39 us for the four launches,
+// 16,000 tokens 43 us against 43).  The blocks behind the first clear the gradient.
+constexpr int kOneThreads = 1024, kOneIters = kSortOne / kOneThreads;
+static_assert(kOneThreads == kDigits, "a thread a digit");
+__global__ __launch_bounds__(kOneThreads) void kd_embed_sort(SortKeys s, int bits, int passes,
+                                                             uint32_t *kept, uint2 *even, uint2 *odd,
+                                                             int64_t fill_bytes, void *fill) {
+  if (blockIdx.x > 0) {
+    embed_fill(blockIdx.x - 1, gridDim.x - 1, fill_bytes, fill);
+    return;
+  }
+  constexpr int kWaves = kOneThreads / kWave;
+  __shared__ uint32_t wcnt[kWaves][kDigits];
+  __shared__ uint32_t s_w[kWaves];
+  const uint32_t mask = (1u << bits) - 1u, d = threadIdx.x;
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  uint32_t m = s.n;
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * bits, iters = (int)((m + kOneThreads - 1) / kOneThreads);
+    if (d <= mask) {
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) wcnt[k][d] = 0;
+    }
+    const uint32_t base = (uint32_t)(w * iters * kWave + lane);
+    uint2 kt[kOneIters];
+    uint32_t rank[kOneIters], in = 0;
+#pragma unroll
+    for (int it = 0; it < kOneIters; ++it) {
+      if (it < iters && s.get(base + it * kWave, m, kt[it])) in |= 1u << it;
+    }
+    __syncthreads();
+    embed_rank<kOneIters>(kt, in, iters, shift, bits, wcnt[w], rank);
+    __syncthreads();
+    uint32_t mine = 0, tot;
+    if (d <= mask) {
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) mine += wcnt[k][d];
+    }
+    uint32_t off = wg_scan<kOneThreads>(mine, s_w, tot) - mine;
+    if (d <= mask) {
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) {
+        const uint32_t c = wcnt[k][d];
+        wcnt[k][d] = off;
+        off += c;
+      }
+    }
+    __syncthreads();
+    uint2 *out = pass & 1 ? odd : even;
+#pragma unroll
+    for (int it = 0; it < kOneIters; ++it) {
+      if ((in >> it) & 1u) out[wcnt[w][(kt[it].x >> shift) & mask] + rank[it]] = kt[it];
+    }
+    m = tot;
+    s.index = nullptr;
+    s.pairs = out;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    kept[0] = m;
+    kept[1] = 0;
+  }
+}
+
 // ------------------------------------------------------------------------------------------------
 // sums over the runs of equal keys
 // ------------------------------------------------------------------------------------------------
@@ -299,7 +371,7 @@ constexpr int kHasTail = 2;   // the last run goes on behind this range
 constexpr int kThrough = 4;   // one run covers the range and both borders (its sum is the head's)
 
 struct SegArgs {
-  const uint32_t *kept;    // sorted tokens
+  uint32_t *kept;          // sorted tokens; behind it the workgroups that are done
   int D, glog, per_group;  // lanes per gradient row (log2), sorted tokens per group
   const uint2 *pairs;
   int *flags;              // per workgroup
@@ -316,11 +388,10 @@ __device__ __forceinline__ void embed_store(T *out, int D, uint32_t key, int col
 }
 
 template <typename T>
-__global__ __launch_bounds__(kBlock) void kd_embed_segments(SegArgs a, const T *__restrict__ grad,
-                                                            typename Wide<T>::type scale,
-                                                            T *__restrict__ out,
-                                                            typename Wide<T>::type *__restrict__ head,
-                                                            typename Wide<T>::type *__restrict__ tail) {
+__device__ __forceinline__ void embed_segments(const SegArgs &a, const T *__restrict__ grad,
+                                               typename Wide<T>::type scale, T *out,
+                                               typename Wide<T>::type *head,
+                                               typename Wide<T>::type *tail) {
   using A = typename Wide<T>::type;
   constexpr int V = 16 / sizeof(T), U = 4;  // channels of a lane, gradient rows in flight
   __shared__ A s_head[kBlock * V];
@@ -436,11 +507,10 @@ __global__ __launch_bounds__(kBlock) void kd_embed_segments(SegArgs a, const T *
 // border and joins the two sides; the few runs that go on through whole workgroups are left to all
 // groups together, one after the other, in a fixed order.
 template <typename T>
-__global__ __launch_bounds__(kBlock) void kd_embed_join(SegArgs a, int nwg,
-                                                        typename Wide<T>::type scale,
-                                                        const typename Wide<T>::type *__restrict__ head,
-                                                        const typename Wide<T>::type *__restrict__ tail,
-                                                        T *__restrict__ out) {
+__device__ __forceinline__ void embed_join(const SegArgs &a, int bx, int by, int gy, int nwg,
+                                           typename Wide<T>::type scale,
+                                           const typename Wide<T>::type *head,
+                                           const typename Wide<T>::type *tail, T *out) {
   using A = typename Wide<T>::type;
   constexpr int V = 16 / sizeof(T);
   __shared__ int s_end;
@@ -448,15 +518,15 @@ __global__ __launch_bounds__(kBlock) void kd_embed_join(SegArgs a, int nwg,
   __shared__ A s_sum[kBlock * V];
   const int G = 1 << a.glog, NG = kBlock >> a.glog;
   const int g = threadIdx.x >> a.glog, gl = threadIdx.x & (G - 1);
-  const int col = ((int)blockIdx.y * G + gl) * V;
-  const int64_t wcol = (int64_t)gridDim.y * G * V;
+  const int col = (by * G + gl) * V;
+  const int64_t wcol = (int64_t)gy * G * V;
   // a run that is open at the end of workgroup w goes on behind it: the position is inside
   auto store = [&](int w, const A *acc) {
     const uint64_t end = (uint64_t)(w + 1) * NG * a.per_group;
     if (col < a.D) embed_store<T, V>(out, a.D, a.pairs[end - 1].x, col, acc, scale);
   };
   {
-    const int w = (int)blockIdx.x * NG + g;
+    const int w = bx * NG + g;
     bool far = false;
     if (w < nwg - 1 && (a.flags[w] & kHasTail)) {
       far = a.flags[w + 1] & kThrough;
@@ -473,7 +543,7 @@ __global__ __launch_bounds__(kBlock) void kd_embed_join(SegArgs a, int nwg,
   __syncthreads();
   for (int q0 = 0; q0 < NG; ++q0) {
     if (!s_long[q0]) continue;  // (the same for the whole workgroup)
-    const int w = (int)blockIdx.x * NG + q0;
+    const int w = bx * NG + q0;
     if (threadIdx.x == 0) s_end = nwg;
     __syncthreads();
     // the first workgroup behind w through which the run does not go on
@@ -507,6 +577,41 @@ __global__ __launch_bounds__(kBlock) void kd_embed_join(SegArgs a, int nwg,
   }
 }
 
+template <typename T>
+__global__ __launch_bounds__(kBlock) void kd_embed_join(SegArgs a, int nwg,
+                                                        typename Wide<T>::type scale,
+                                                        const typename Wide<T>::type *__restrict__ head,
+                                                        const typename Wide<T>::type *__restrict__ tail,
+                                                        T *__restrict__ out) {
+  embed_join<T>(a, (int)blockIdx.x, (int)blockIdx.y, (int)gridDim.y, nwg, scale, head, tail, out);
+}
+
+// JOIN: the workgroup that is done last joins the borders of all, while they are few rounds of its
+// groups.  Its time is that of a second launch (4,000 tokens 18.5 us against 8.7 and 8.6), without the
+// launch.
+template <typename T, bool JOIN>
+__global__ __launch_bounds__(kBlock) void kd_embed_segments(SegArgs a, const T *__restrict__ grad,
+                                                            typename Wide<T>::type scale, T *out,
+                                                            typename Wide<T>::type *head,
+                                                            typename Wide<T>::type *tail) {
+  embed_segments<T>(a, grad, scale, out, head, tail);
+  if constexpr (JOIN) {
+    __shared__ bool s_last;
+    const int nwg = (int)gridDim.x, gy = (int)gridDim.y, per = kBlock >> a.glog;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) s_last = atomicAdd(a.kept + 1, 1u) == gridDim.x * gridDim.y - 1;
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    for (int y = 0; y < gy; ++y)
+      for (int x = 0; x * per < nwg; ++x) {
+        embed_join<T>(a, x, y, gy, nwg, scale, head, tail, out);
+        __syncthreads();
+      }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------
 // host
 // ------------------------------------------------------------------------------------------------
@@ -535,7 +640,7 @@ static EmbedPlan embed_plan(int64_t n, int64_t nkeys, int D, int esize) {
   p.bits = (kb + p.passes - 1) / p.passes;
   const int asize = esize == 8 ? 8 : 4;
   p.pairs = up256(8 * (size_t)n);
-  p.hist = up256(4 * (size_t)kDigits * (size_t)p.ntile + 4 * kDigits + 4);
+  p.hist = up256(4 * (size_t)kDigits * (size_t)p.ntile + 4 * kDigits + 8);
   p.part = up256((size_t)p.nwg * (size_t)p.gy * (size_t)(V << p.glog) * (size_t)asize);
   p.flags = up256(4 * (size_t)p.nwg);
   p.total = 2 * p.pairs + p.hist + 2 * p.part + p.flags;
@@ -618,22 +723,27 @@ static int embed_backward(int64_t n, int64_t batch, int64_t rows, int D, const i
     s.n = (uint32_t)n;
     s.per_batch = batch > 1 ? (uint32_t)(n / batch) : 0u;
     s.rows = rows;
-    const uint32_t mask = (1u << p.bits) - 1u;
-    const unsigned nt = (unsigned)p.ntile;
-    for (int q = 0; q < p.passes; ++q) {
-      const int shift = q * p.bits;
-      const unsigned extra = q == 0 ? fblocks : 0u;  // the first launch clears the gradient too
-      if (p.ntile > 1)
+    if (n <= kSortOne) {
+      hipLaunchKernelGGL(kd_embed_sort, dim3(1 + (unsigned)std::min<int64_t>(fblocks, 512)),
+                         dim3(kOneThreads), 0, stream, s, p.bits, p.passes, kept, buf[0], buf[1], fill,
+                         (void *)out);
+      s.pairs = buf[(p.passes - 1) & 1];
+    } else {
+      const uint32_t mask = (1u << p.bits) - 1u;
+      const unsigned nt = (unsigned)p.ntile;
+      for (int q = 0; q < p.passes; ++q) {
+        const int shift = q * p.bits;
+        const unsigned extra = q == 0 ? fblocks : 0u;  // the first launch clears the gradient too
         hipLaunchKernelGGL(kd_embed_hist, dim3(nt + extra), dim3(kBlock), 0, stream, s, shift, mask,
                            p.ntile, hist, fill, (void *)out);
-      if (p.ntile > kFewTiles)
-        hipLaunchKernelGGL(kd_embed_scan, dim3(mask + 1), dim3(kBlock), 0, stream, p.ntile, hist,
-                           totals);
-      hipLaunchKernelGGL(kd_embed_scatter, dim3(nt + (p.ntile == 1 ? extra : 0u)), dim3(kBlock), 0,
-                         stream, s, shift, p.bits, p.ntile, hist, totals,
-                         q == 0 ? kept : (uint32_t *)nullptr, buf[q & 1], fill, (void *)out);
-      s.index = nullptr;
-      s.pairs = buf[q & 1];
+        if (p.ntile > kFewTiles)
+          hipLaunchKernelGGL(kd_embed_scan, dim3(mask + 1), dim3(kBlock), 0, stream, p.ntile, hist,
+                             totals);
+        hipLaunchKernelGGL(kd_embed_scatter, dim3(nt), dim3(kBlock), 0, stream, s, shift, p.bits,
+                           p.ntile, hist, totals, q == 0 ? kept : (uint32_t *)nullptr, buf[q & 1]);
+        s.index = nullptr;
+        s.pairs = buf[q & 1];
+      }
     }
     SegArgs a;
     a.kept = kept;
@@ -643,14 +753,18 @@ static int embed_backward(int64_t n, int64_t batch, int64_t rows, int D, const i
     a.pairs = s.pairs;
     a.flags = flags;
     const dim3 grid((unsigned)p.nwg, (unsigned)p.gy);
-    hipLaunchKernelGGL(kd_embed_segments<T>, grid, dim3(kBlock), 0, stream, a, grad, (A)scale, out,
-                       head, tail);
-    if (p.nwg > 1)
-      hipLaunchKernelGGL(kd_embed_join<T>,
-                         dim3((unsigned)((p.nwg + (kBlock >> p.glog) - 1) / (kBlock >> p.glog)),
-                              (unsigned)p.gy),
-                         dim3(kBlock), 0, stream, a, p.nwg, (A)scale, (const A *)head,
-                         (const A *)tail, out);
+    const int per = kBlock >> p.glog;
+    if (p.nwg > 1 && p.gy * ((p.nwg + per - 1) / per) <= kJoinRounds) {
+      hipLaunchKernelGGL((kd_embed_segments<T, true>), grid, dim3(kBlock), 0, stream, a, grad, (A)scale,
+                         out, head, tail);
+    } else {
+      hipLaunchKernelGGL((kd_embed_segments<T, false>), grid, dim3(kBlock), 0, stream, a, grad,
+                         (A)scale, out, head, tail);
+      if (p.nwg > 1)
+        hipLaunchKernelGGL(kd_embed_join<T>, dim3((unsigned)((p.nwg + per - 1) / per), (unsigned)p.gy),
+                           dim3(kBlock), 0, stream, a, p.nwg, (A)scale, (const A *)head,
+                           (const A *)tail, out);
+    }
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)

@@ -123,6 +123,24 @@ def test_lookup_and_gradient(dname, kind, n, N, D, scale):
     assert torch.equal(out, out2) and torch.equal(ge, ge2)  # a fixed order of the sums
 
 
+@pytest.mark.parametrize('kind', ['random', 'one', 'runs', 'wild'])
+@pytest.mark.parametrize('n,N,D', [(2, 1024, 40), (1023, 1025, 3), (1024, 1, 9), (1025, 3000, 300),
+                                   (8191, 1024, 16), (16383, 40000, 8), (16384, 1025, 33),
+                                   (16384, 2, 600), (16385, 1024, 8), (16385, 30000, 1)])
+def test_around_the_sort_s_sizes(kind, n, N, D):
+    """One workgroup's tokens and a token more, a digit's keys and one more, borders joined by the last
+    workgroup and by a launch of their own."""
+    gen = torch.Generator().manual_seed(n + N)
+    index = _index(kind, n, N, gen).to(DEV)
+    table = torch.randn(N, D, generator=gen).to(DEV)
+    grad = torch.randn(n, D, generator=gen).to(DEV)
+    out, ge = _run(index, table, 1.0, grad)
+    ref, rg, mag, cnt = _reference(index, table, 1.0, grad)
+    _check_out(out, ref)
+    _check_grad(ge, rg, mag, cnt)
+    assert torch.equal(ge, _run(index, table, 1.0, grad)[1])
+
+
 @pytest.mark.parametrize('shape,N,D', [((3, 20, 30), 50, 16), ((2, 7), 9, 5), ((1, 4, 4), 6, 8),
                                        ((5, 0), 4, 3)])
 def test_table_per_batch_entry(shape, N, D):
