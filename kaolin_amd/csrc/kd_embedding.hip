@@ -14,23 +14,24 @@
 // token), so a row's tokens stand together in token order; then each group of G lanes (one row of the
 // gradient, 16 bytes a lane) walks a run of sorted tokens and adds their gradient rows in registers.
 // Runs that cross a group's border are joined in LDS by the group in which they begin, runs that cross
-// a workgroup's border by the last workgroup or, where they are many, by a second launch.  The split of the walk over groups goes by position and
-// not by key, so one face that fills the image costs no more than any other.
+// a workgroup's border by a second launch or, where the workgroups are few, by the last one.  The split
+// of the walk over groups goes by position and not by key, so one face that fills the image costs no
+// more than any other.
 #include "kd_capi.hpp"
 #include "kd_common.hpp"
 #include "kd_float16.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace kd {
 
-constexpr int kSortTile = 4096;             // tokens per sort workgroup (16 per thread)
-constexpr int kSortIters = kSortTile / kBlock;
 constexpr int kMaxBits = 10;                // of a sort digit: 16-bit keys take two passes, 20-bit ones too
 constexpr int kDigits = 1 << kMaxBits;
-constexpr int kFewTiles = 64;               // up to so many tiles the sort needs no scan launch
+constexpr int kFewCounts = 32768;           // up to so many counts (tiles x digits) need no scan launch
 constexpr int kSortOne = 16384;             // up to so many tokens one workgroup sorts in one launch
-constexpr int kJoinRounds = 4;              // up to so many rounds the last workgroup joins the borders
+constexpr int kJoinHere = 32;               // up to so many workgroups the last one joins the borders
+constexpr int kJoinRounds = 4;              // (in so many rounds of its groups)
 constexpr int kMaxChannels = 1 << 20;
 
 // ------------------------------------------------------------------------------------------------
@@ -129,9 +130,17 @@ __device__ __forceinline__ void embed_fill(uint32_t block, uint32_t nblocks, int
   }
 }
 
+// Tokens a thread takes in a tile of kBlock times as many.  Small tiles fill the chip and shorten the
+// chain of ranks in a workgroup, large ones leave fewer counts to sum and longer runs to write.  Both
+// passes of 262,144 tokens take 31 us with 4 tokens a thread and 50 with 16, of 600,000 46, 46 and 58
+// with 4, 8 and 16, of 2,097,152 57, 51 and 58, of 8,388,608 153, 121 and 120.
+inline int sort_iters(int64_t n) { return n <= (1 << 19) ? 4 : n <= (1 << 22) ? 8 : 16; }
+
 // Per tile the count of each digit; the blocks behind the tiles clear the gradient.
+// few: a tile's counts stand together, else a digit's.
+template <int ITERS>
 __global__ __launch_bounds__(kBlock) void kd_embed_hist(SortKeys s, int shift, uint32_t mask,
-                                                        int ntile, uint32_t *__restrict__ hist,
+                                                        int ntile, bool few, uint32_t *__restrict__ hist,
                                                         int64_t fill_bytes, void *fill) {
   if ((int)blockIdx.x >= ntile) {
     embed_fill(blockIdx.x - ntile, gridDim.x - ntile, fill_bytes, fill);
@@ -140,17 +149,17 @@ __global__ __launch_bounds__(kBlock) void kd_embed_hist(SortKeys s, int shift, u
   __shared__ uint32_t cnt[kDigits];
   for (uint32_t d = threadIdx.x; d <= mask; d += kBlock) cnt[d] = 0;
   __syncthreads();
-  const uint32_t base = blockIdx.x * (uint32_t)kSortTile, m = s.count();
+  const uint32_t base = blockIdx.x * (uint32_t)(ITERS * kBlock), m = s.count();
   if (base < m) {
-#pragma unroll 8
-    for (int it = 0; it < kSortIters; ++it) {
+#pragma unroll
+    for (int it = 0; it < ITERS; ++it) {
       uint2 kt;
       if (s.get(base + it * kBlock + threadIdx.x, m, kt)) atomicAdd(&cnt[(kt.x >> shift) & mask], 1u);
     }
   }
   __syncthreads();
   for (uint32_t d = threadIdx.x; d <= mask; d += kBlock)
-    hist[(int64_t)d * ntile + blockIdx.x] = cnt[d];
+    hist[few ? (int64_t)blockIdx.x * (mask + 1) + d : (int64_t)d * ntile + blockIdx.x] = cnt[d];
 }
 
 // Inclusive sum over the workgroup's N threads; total in every thread.
@@ -223,31 +232,49 @@ __device__ __forceinline__ void embed_rank(const uint2 (&kt)[ITERS], uint32_t in
   }
 }
 
-// Bound by latency and the scattered 8-byte writes: 4,217,024 tokens that name one of 50,000 rows, of
-// 8,388,608, 29 us a pass (two passes) behind 16 us of counting, 2,097,152 tokens 15 and 8 us.
-// Where the tiles are few (kFewTiles) each workgroup adds up the tiles' counts itself, a thread a
-// digit: a launch costs more than that.
+// Bound by latency and the scattered 8-byte writes: of 8,388,608 tokens the 4,217,024 that name one of
+// 50,000 rows are written in 45 us, and in the second pass in 27 us, behind 16 us of counting; of
+// 2,097,152 in 14 and 12 us behind 8.
+// few: each workgroup adds up all tiles' counts itself, 16 bytes a thread and a share of the tiles: both
+// passes of 262,144 tokens take 31 us in four launches against 26 in six, a call whose launches are its
+// time 104 us against 109.
+template <int ITERS>
 __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
-    SortKeys s, int shift, int bits, int ntile, const uint32_t *__restrict__ hist,
+    SortKeys s, int shift, int bits, int ntile, bool few, const uint32_t *__restrict__ hist,
     const uint32_t *__restrict__ totals, uint32_t *__restrict__ kept, uint2 *__restrict__ out) {
   constexpr int kWaves = kBlock / kWave;
   __shared__ uint32_t wcnt[kWaves][kDigits];
+  __shared__ uint4 s_all[kBlock], s_before[kBlock];
   __shared__ uint32_t s_w[kWaves];
   const uint32_t mask = (1u << bits) - 1u, m = s.count();
-  if (blockIdx.x * (uint32_t)kSortTile >= m && blockIdx.x > 0) return;
+  if (blockIdx.x * (uint32_t)(ITERS * kBlock) >= m && blockIdx.x > 0) return;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   for (uint32_t d = threadIdx.x; d <= mask; d += kBlock) {
 #pragma unroll
     for (int k = 0; k < kWaves; ++k) wcnt[k][d] = 0;
   }
-  const uint32_t base = blockIdx.x * (uint32_t)kSortTile + w * (kSortTile / kWaves) + lane;
-  uint2 kt[kSortIters];
-  uint32_t rank[kSortIters], in = 0;
+  const uint32_t base = blockIdx.x * (uint32_t)(ITERS * kBlock) + w * (ITERS * kWave) + lane;
+  uint2 kt[ITERS];
+  uint32_t rank[ITERS], in = 0;
 #pragma unroll
-  for (int it = 0; it < kSortIters; ++it)
+  for (int it = 0; it < ITERS; ++it)
     if (s.get(base + it * kWave, m, kt[it])) in |= 1u << it;
+  const int quads = (int)(mask + 1) / 4, shares = kBlock / quads;  // (two bits or more)
+  if (few) {
+    uint4 all = make_uint4(0, 0, 0, 0), before = all;
+#pragma unroll 8
+    for (int k = (int)threadIdx.x / quads; k < ntile; k += shares) {
+      const uint4 c = ((const uint4 *)hist)[k * quads + (int)threadIdx.x % quads];
+      const bool b = k < (int)blockIdx.x;
+      all.x += c.x, all.y += c.y, all.z += c.z, all.w += c.w;
+      before.x += b ? c.x : 0u, before.y += b ? c.y : 0u;
+      before.z += b ? c.z : 0u, before.w += b ? c.w : 0u;
+    }
+    s_all[threadIdx.x] = all;
+    s_before[threadIdx.x] = before;
+  }
   __syncthreads();
-  embed_rank<kSortIters>(kt, in, kSortIters, shift, bits, wcnt[w], rank);
+  embed_rank<ITERS>(kt, in, ITERS, shift, bits, wcnt[w], rank);
   __syncthreads();
   // where each digit begins among all tokens, and this tile's part of it
   // (a thread takes kDigits / kBlock digits in a row, as the sum over the digits needs)
@@ -258,13 +285,10 @@ __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
     const uint32_t d = threadIdx.x * kPer + q;
     all[q] = before[q] = 0;
     if (d > mask) continue;
-    if (ntile <= kFewTiles) {
-      const uint32_t *h = hist + (int64_t)d * ntile;
-#pragma unroll 8
-      for (int k = 0; k < ntile; ++k) {
-        const uint32_t c = h[k];
-        before[q] += k < (int)blockIdx.x ? c : 0u;
-        all[q] += c;
+    if (few) {
+      for (int k = 0; k < shares; ++k) {
+        all[q] += ((const uint32_t *)s_all)[k * (int)(mask + 1) + d];
+        before[q] += ((const uint32_t *)s_before)[k * (int)(mask + 1) + d];
       }
     } else {
       all[q] = totals[d];
@@ -292,7 +316,7 @@ __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
   }
   __syncthreads();
 #pragma unroll
-  for (int it = 0; it < kSortIters; ++it)
+  for (int it = 0; it < ITERS; ++it)
     if ((in >> it) & 1u) out[wcnt[w][(kt[it].x >> shift) & mask] + rank[it]] = kt[it];
 }
 
@@ -586,9 +610,9 @@ __global__ __launch_bounds__(kBlock) void kd_embed_join(SegArgs a, int nwg,
   embed_join<T>(a, (int)blockIdx.x, (int)blockIdx.y, (int)gridDim.y, nwg, scale, head, tail, out);
 }
 
-// JOIN: the workgroup that is done last joins the borders of all, while they are few rounds of its
-// groups.  Its time is that of a second launch (4,000 tokens 18.5 us against 8.7 and 8.6), without the
-// launch.
+// JOIN: the workgroup that is done last joins the borders of all, where there are few workgroups: the
+// time is that of a second launch (4,000 tokens 18.5 us against 8.7 and 8.6), without the launch.  Each
+// workgroup's fence costs 0.2 us, one after the other: with 196 of them 44 us against 11.
 template <typename T, bool JOIN>
 __global__ __launch_bounds__(kBlock) void kd_embed_segments(SegArgs a, const T *__restrict__ grad,
                                                             typename Wide<T>::type scale, T *out,
@@ -616,7 +640,7 @@ __global__ __launch_bounds__(kBlock) void kd_embed_segments(SegArgs a, const T *
 // host
 // ------------------------------------------------------------------------------------------------
 struct EmbedPlan {
-  int glog, gy, per_group, nwg, ntile, passes, bits;
+  int glog, gy, per_group, nwg, iters, ntile, passes, bits;
   size_t pairs, hist, part, flags, total;  // workspace parts in bytes
 };
 
@@ -633,11 +657,12 @@ static EmbedPlan embed_plan(int64_t n, int64_t nkeys, int D, int esize) {
   p.per_group = 64;
   while (p.per_group > 8 && (n + ng * p.per_group - 1) / (ng * p.per_group) < 4096) p.per_group >>= 1;
   p.nwg = (int)((n + ng * p.per_group - 1) / (ng * p.per_group));
-  p.ntile = (int)((n + kSortTile - 1) / kSortTile);
+  p.iters = sort_iters(n);
+  p.ntile = (int)((n + p.iters * kBlock - 1) / (p.iters * kBlock));
   int kb = 1;
   while (kb < 32 && ((nkeys - 1) >> kb) != 0) ++kb;  // keys 0 .. nkeys - 1
   p.passes = (kb + kMaxBits - 1) / kMaxBits;
-  p.bits = (kb + p.passes - 1) / p.passes;
+  p.bits = std::max((kb + p.passes - 1) / p.passes, 2);
   const int asize = esize == 8 ? 8 : 4;
   p.pairs = up256(8 * (size_t)n);
   p.hist = up256(4 * (size_t)kDigits * (size_t)p.ntile + 4 * kDigits + 8);
@@ -700,8 +725,8 @@ static int embed_backward(int64_t n, int64_t batch, int64_t rows, int D, const i
   const unsigned fblocks = (unsigned)std::min<int64_t>((fill / 16 + kBlock) / kBlock, 2048);
   ProfScope prof(K_EMBED_BWD, stream);
   if (n == 0) {
-    hipLaunchKernelGGL(kd_embed_hist, dim3(fblocks), dim3(kBlock), 0, stream, SortKeys{}, 0, 0u, 0,
-                       (uint32_t *)nullptr, fill, (void *)out);
+    hipLaunchKernelGGL(kd_embed_hist<4>, dim3(fblocks), dim3(kBlock), 0, stream, SortKeys{}, 0, 0u, 0,
+                       false, (uint32_t *)nullptr, fill, (void *)out);
   } else {
     const EmbedPlan p = embed_plan(n, nkeys, D, (int)sizeof(T));
     if (wsb < p.total || !ws)
@@ -731,16 +756,27 @@ static int embed_backward(int64_t n, int64_t batch, int64_t rows, int D, const i
     } else {
       const uint32_t mask = (1u << p.bits) - 1u;
       const unsigned nt = (unsigned)p.ntile;
+      const bool few = (int64_t)p.ntile * (mask + 1) <= kFewCounts;
       for (int q = 0; q < p.passes; ++q) {
         const int shift = q * p.bits;
         const unsigned extra = q == 0 ? fblocks : 0u;  // the first launch clears the gradient too
-        hipLaunchKernelGGL(kd_embed_hist, dim3(nt + extra), dim3(kBlock), 0, stream, s, shift, mask,
-                           p.ntile, hist, fill, (void *)out);
-        if (p.ntile > kFewTiles)
-          hipLaunchKernelGGL(kd_embed_scan, dim3(mask + 1), dim3(kBlock), 0, stream, p.ntile, hist,
-                             totals);
-        hipLaunchKernelGGL(kd_embed_scatter, dim3(nt), dim3(kBlock), 0, stream, s, shift, p.bits,
-                           p.ntile, hist, totals, q == 0 ? kept : (uint32_t *)nullptr, buf[q & 1]);
+        uint32_t *first = q == 0 ? kept : nullptr;
+        auto pass = [&](auto iters) {
+          constexpr int I = decltype(iters)::value;
+          hipLaunchKernelGGL(kd_embed_hist<I>, dim3(nt + extra), dim3(kBlock), 0, stream, s, shift, mask,
+                             p.ntile, few, hist, fill, (void *)out);
+          if (!few)
+            hipLaunchKernelGGL(kd_embed_scan, dim3(mask + 1), dim3(kBlock), 0, stream, p.ntile, hist,
+                               totals);
+          hipLaunchKernelGGL(kd_embed_scatter<I>, dim3(nt), dim3(kBlock), 0, stream, s, shift, p.bits,
+                             p.ntile, few, hist, totals, first, buf[q & 1]);
+        };
+        if (p.iters == 4)
+          pass(std::integral_constant<int, 4>{});
+        else if (p.iters == 8)
+          pass(std::integral_constant<int, 8>{});
+        else
+          pass(std::integral_constant<int, 16>{});
         s.index = nullptr;
         s.pairs = buf[q & 1];
       }
@@ -754,7 +790,7 @@ static int embed_backward(int64_t n, int64_t batch, int64_t rows, int D, const i
     a.flags = flags;
     const dim3 grid((unsigned)p.nwg, (unsigned)p.gy);
     const int per = kBlock >> p.glog;
-    if (p.nwg > 1 && p.gy * ((p.nwg + per - 1) / per) <= kJoinRounds) {
+    if (p.nwg > 1 && p.nwg <= kJoinHere && p.gy * ((p.nwg + per - 1) / per) <= kJoinRounds) {
       hipLaunchKernelGGL((kd_embed_segments<T, true>), grid, dim3(kBlock), 0, stream, a, grad, (A)scale,
                          out, head, tail);
     } else {
