@@ -418,19 +418,19 @@ __device__ __forceinline__ void pack_pair(float p0, float p1, int i, uint4 *o) {
 
 // How a walk is laid out (KIND 0: over the table, loss only; 1: over the table with dX; 2: over the
 // pixels, dE), for np planes and dp channels.
-// Blocks of 32 rows that a wave holds.  Every operand read from LDS feeds one product per block; with one
-// block a product, 32 clocks on each of four SIMDs, takes all that LDS delivers (4 x 1 KiB), so 16-bit
-// data take two wherever the registers hold them, down to one wave a SIMD: dE of 527,000 pixels and
-// 10,000 rows at 128 channels 2.98 -> 2.87 ms, losses at 256 channels 2.41 -> 2.26 ms.  Not where
-// the second wave, whose exponentials go beside the first one's products, is worth more: dX at 128
-// channels 0.64 ms for 132,000 pixels against 0.69 with two blocks (2.73 against 2.69 for 527,000).
+// Blocks of 32 rows that a wave holds.  Every operand read from LDS feeds one product per block; with
+// one block a product, 32 clocks on each of four SIMDs, takes all that LDS delivers (4 x 1 KiB), so
+// 16-bit data take two where two waves a SIMD have the registers: losses at 256 channels of 527,000
+// pixels and 10,000 rows 2.43 -> 2.07 ms (33,000 and 2,000: 47 and 48 us).  Not the sums at 128
+// channels, where two blocks leave one wave a SIMD: dE of 527,000 pixels 2.98 -> 2.87 ms, but of 33,000
+// pixels and 2,000 rows 55 -> 65 us, dX of 132,000 0.64 -> 0.69 ms.
 constexpr int walk_blocks(int np, int dp, int kind) {
-  return np == 1 && (dp <= 64 || (dp == 128 && kind != 1) || (dp == 256 && kind == 0)) ? 2 : 1;
+  return np == 1 && (dp <= 64 || kind == 0) ? 2 : 1;
 }
 // Waves per SIMD: one where the held operands, the sums and the blocks of logits need more than 256
 // registers.
 constexpr int walk_waves(int np, int dp, int kind) {
-  return (np == 1 ? dp == 256 || (dp == 128 && kind == 2) : dp >= (kind > 0 ? 128 : 256)) ? 1 : 2;
+  return (np == 1 ? dp == 256 && kind > 0 : dp >= (kind > 0 ? 128 : 256)) ? 1 : 2;
 }
 // Into how many column ranges the sums are cut, over workgroups that each form the logits: two where
 // the operands of all columns would not fit LDS twice.
