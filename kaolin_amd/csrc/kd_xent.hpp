@@ -1378,17 +1378,24 @@ static __global__ __launch_bounds__(kBlock) void kd_xent_sum(Args a, float *__re
 // ------------------------------------------------------------------------------------------------
 // backward
 // ------------------------------------------------------------------------------------------------
-// the listed pixels' gradients of a loss per pixel, and the largest of their sizes per workgroup
-constexpr int kGradChunk = 4096;
+// The listed pixels' gradients of a loss per pixel, and the largest of their sizes per workgroup of
+// grad_steps() x kBlock pixels: few in a row are short of latency (26,000 pixels 5 us with 4 against 12
+// with 16), many leave fewer sizes to look through.
+__host__ __device__ inline int grad_steps(int64_t npad) { return npad <= (1 << 20) ? 4 : 16; }
+__host__ __device__ inline int grad_blocks(int64_t npad) {
+  const int64_t chunk = (int64_t)grad_steps(npad) * kBlock;
+  return (int)((npad + chunk - 1) / chunk);
+}
 
 static __global__ __launch_bounds__(kBlock) void kd_xent_rowgrad(Args a,
                                                                  const float *__restrict__ grad) {
   __shared__ uint32_t s_m[kBlock / kWave];
   const int count = *a.count;
+  const int steps = grad_steps(a.npad);
   uint32_t top = 0;
 #pragma unroll 4
-  for (int k = 0; k < kGradChunk / kBlock; ++k) {
-    const int64_t r = (int64_t)blockIdx.x * kGradChunk + k * kBlock + threadIdx.x;
+  for (int k = 0; k < steps; ++k) {
+    const int64_t r = ((int64_t)blockIdx.x * steps + k) * kBlock + threadIdx.x;
     const float g = r < count ? grad[a.rowid[r]] : 0.f;
     if (r < a.npad) a.grow[r] = g;
     top = max(top, __float_as_uint(fabsf(g)));
@@ -1404,7 +1411,7 @@ static __global__ __launch_bounds__(kBlock) void kd_xent_rowgrad(Args a,
 // range whatever the incoming gradient's scale
 __device__ __forceinline__ float grad_unit(const Args &a) {
   __shared__ uint32_t s_u[kBlock / kWave];
-  const int nblk = (int)((a.npad + kGradChunk - 1) / kGradChunk);
+  const int nblk = grad_blocks(a.npad);
   uint32_t top = 0;
   for (int k = threadIdx.x; k < nblk; k += kBlock) top = max(top, a.gmax[k]);
 #pragma unroll
@@ -1680,7 +1687,7 @@ inline size_t lay_forward(Args &a, int np, bool need_x, void *base) {
 
 inline size_t lay_backward(Args &a, int np, bool need_e, void *base) {
   Space s{(char *)base, 0};
-  a.gmax = s.take<uint32_t>((size_t)((a.npad + kGradChunk - 1) / kGradChunk) + 1);
+  a.gmax = s.take<uint32_t>((size_t)grad_blocks(a.npad) + 1);
   a.grow = s.take<float>(a.npad);
   const size_t part = (size_t)deal_slots(a.vpad, np, a.dp, 2) * (size_t)walk_rows(np, a.dp, 2);
   a.pe = need_e ? s.take<float>(part * a.dp) : nullptr;
@@ -1833,7 +1840,7 @@ int backward(int64_t n, int64_t V, int D, const int64_t *labels, double scale, i
   ProfScope prof(K_XENT_BWD, stream);
   if (ge && reduction == 0)
     hipLaunchKernelGGL(kd_xent_rowgrad,
-                       dim3((unsigned)std::max<int64_t>((a.npad + kGradChunk - 1) / kGradChunk, 1)),
+                       dim3((unsigned)std::max(grad_blocks(a.npad), 1)),
                        dim3(kBlock), 0, stream, a, grad);
   switch (a.dp) {
     case 32: launch_backward<T, 32>(a, labels, grad, gx, ge, stream); break;
