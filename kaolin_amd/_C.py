@@ -805,32 +805,25 @@ def _embedding_args(fn, index, shape, scale):
     return index.numel(), max(batch, 1), rows, D, _number(fn, 'scale', scale)
 
 
-def surface_embedding_forward(index, embeddings, scale):
-    """index (...) int64, embeddings (N, D) or (B, N, D) with index (B, ...) -> (..., D):
-    scale * embeddings[index], 0 where the index lies outside [0, N)."""
+def surface_embedding_forward(index, embeddings, scale, need_embeddings=False):
+    """index (...) int64, embeddings (N, D) or (B, N, D) with index (B, ...) -> (out, plan): out
+    (..., D) is scale * embeddings[index], 0 where the index lies outside [0, N); plan is what
+    surface_embedding_backward needs, or None unless asked for."""
     fn = 'surface_embedding'
     dev = _check_same_gpu(fn, index=index, embeddings=embeddings)
-    sfx = _sfx16(embeddings, fn)
-    n, B, N, D, scale = _embedding_args(fn, index, embeddings.shape, scale)
+    sfx, shape, plan = _sfx16(embeddings, fn), embeddings.shape, None
+    n, B, N, D, scale = _embedding_args(fn, index, shape, scale)
     index, embeddings = index.contiguous(), embeddings.contiguous()
     out = torch.empty((*index.shape, D), device=dev, dtype=embeddings.dtype)
     if out.numel():
-        _launch(dev, f'kd_surface_embedding_forward_{sfx}', n, B, N, D, _ptr(index),
-                _ptr(embeddings), scale, _ptr(out))
-    return out
-
-
-def surface_embedding_plan(index, embeddings, scale):
-    """What surface_embedding_backward needs for the gradient of `embeddings`, checked once: the
-    forward's arguments, the table's shape and the workspace's size."""
-    fn = 'surface_embedding'
-    dev = _check_same_gpu(fn, index=index, embeddings=embeddings)
-    sfx = _sfx16(embeddings, fn)
-    n, B, N, D, scale = _embedding_args(fn, index, embeddings.shape, scale)
-    nb = int(_lib.load().kd_surface_embedding_workspace_size(n, B, N, D,
-                                                             embeddings.element_size()))
-    return (f'kd_surface_embedding_backward_{sfx}', dev, embeddings.shape, embeddings.dtype,
-            (n, B, N, D), scale, nb)
+        _launch(dev, f'kd_surface_embedding_forward_{sfx}', n, B, N, D, index.data_ptr(),
+                embeddings.data_ptr(), scale, out.data_ptr())
+    if need_embeddings:
+        nb = int(_lib.load().kd_surface_embedding_workspace_size(n, B, N, D,
+                                                                 embeddings.element_size()))
+        plan = (f'kd_surface_embedding_backward_{sfx}', dev, shape, embeddings.dtype,
+                (n, B, N, D), scale, nb)
+    return out, plan
 
 
 def surface_embedding_backward(grad_out, index, plan):
@@ -1081,7 +1074,6 @@ render = types.SimpleNamespace(mesh=types.SimpleNamespace(
     deftet_sparse_render_forward_cuda=deftet_sparse_render_forward_cuda,
     deftet_sparse_render_backward_cuda=deftet_sparse_render_backward_cuda,
     surface_embedding_forward=surface_embedding_forward,
-    surface_embedding_plan=surface_embedding_plan,
     surface_embedding_backward=surface_embedding_backward,
 ))
 metrics = types.SimpleNamespace(mask_iou_forward=mask_iou_forward,

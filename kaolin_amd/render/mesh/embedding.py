@@ -20,9 +20,8 @@ class SurfaceEmbeddingHip(Function):
 
     @staticmethod
     def forward(ctx, index, embeddings, scale):
-        out = _C.render.mesh.surface_embedding_forward(index, embeddings, scale)
+        out, ctx.plan = _C.render.mesh.surface_embedding_forward(index, embeddings, scale, True)
         ctx.save_for_backward(index)
-        ctx.plan = _C.render.mesh.surface_embedding_plan(index, embeddings, scale)
         ctx.set_materialize_grads(False)
         return out
 
@@ -63,5 +62,5 @@ def surface_embedding(index, embeddings, scale=1.0):
         to it once, and the gradient's sums are held in 32 bits (64 for float64).
     """
     if not torch.is_grad_enabled() or not embeddings.requires_grad:
-        return _C.render.mesh.surface_embedding_forward(index, embeddings, scale)
+        return _C.render.mesh.surface_embedding_forward(index, embeddings, scale)[0]
     return SurfaceEmbeddingHip.apply(index, embeddings, scale)
