@@ -582,19 +582,27 @@ struct Step {
   using W = Walk<T, DP, KIND>;
   static constexpr bool SUM = KIND > 0;
   static constexpr int NP = F::np, RB = W::rb, PP = W::pp, KS = DP / 16, DT = DP / 32 / W::cs;
-  H8 held[RB][KS][NP];
+  // Three parts of 256 channels and their sums do not fit the registers: the held rows' second and third
+  // parts, which three of six products take, are read again for every tile, by the vector cache, which
+  // is free for them (held, 500 bytes a lane are spilled: 27,000 pixels x 56,506 rows of 235 channels take
+  // 48.9 ms for both gradients, with two parts held 37.6, with one 30.7).
+  static constexpr bool kLean = NP == 3 && DP == 256 && SUM;
+  static constexpr int HP = kLean ? 1 : NP;
+  H8 held[RB][KS][HP];
+  const uint16_t *low;
   f32x16 s[RB];
   f32x16 o[SUM ? RB : 1][SUM ? DT : 1];
   uint4 q[RB][2][PP];
 
   __device__ __forceinline__ void hold(const uint16_t *packed, int64_t row0) {
     const int lane = threadIdx.x & 63;
+    low = packed + ((row0 >> 5) * NP + HP) * KS * 512 + lane * 8;
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
-        for (int p = 0; p < NP; ++p)
+        for (int p = 0; p < HP; ++p)
           held[b][k][p] =
               *(const H8 *)(packed + ((((row0 >> 5) + b) * NP + p) * KS + k) * 512 + lane * 8);
       if constexpr (SUM) {
@@ -669,6 +677,9 @@ struct Step {
     constexpr int kGroups = kAdd + kSmall + kLast;
     H8 a[2][4];  // a group's operands: three planes, or the first planes of kPer steps
     H8 first;    // the first plane of the other row half
+    H8 rest[2][kLean ? NP - HP : 1];
+    const uint16_t *again = low;
+    if constexpr (kLean) asm volatile("" : "+v"(again));  // (not read once before the walk)
     auto load = [&](int g) {
       H8 *to = a[g & 1];
       if (g < kAdd) {  // group 2 d + h
@@ -678,6 +689,11 @@ struct Step {
       } else if (g < kAdd + kSmall) {
 #pragma unroll
         for (int p = 0; p < 3; ++p) to[p] = *(const H8 *)&straight[(p * KS + g - kAdd) * 64 + lane];
+        if constexpr (kLean) {
+#pragma unroll
+          for (int p = HP; p < 3; ++p)
+            rest[g & 1][p - HP] = *(const H8 *)(again + ((p - HP) * KS + g - kAdd) * 512);
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < kPer; ++j)
@@ -719,9 +735,16 @@ struct Step {
           slot();
         }
       } else if (g < kAdd + kSmall) {
+        H8 y[3];
+#pragma unroll
+        for (int p = 0; p < HP; ++p) y[p] = held[0][g - kAdd][p];
+        if constexpr (kLean) {
+#pragma unroll
+          for (int p = HP; p < 3; ++p) y[p] = rest[g & 1][p - HP];
+        }
 #pragma unroll
         for (int i = 0; i < 5; ++i) {
-          next = product<3>(i, x, held[0][g - kAdd], next);
+          next = product<3>(i, x, y, next);
           slot();
         }
       } else {
