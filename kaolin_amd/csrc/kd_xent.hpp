@@ -585,7 +585,7 @@ struct Step {
   // Three parts of 256 channels and their sums do not fit the registers: the held rows' second and third
   // parts, which three of six products take, are read again for every tile, by the vector cache, which
   // is free for them (held, 500 bytes a lane are spilled: 27,000 pixels x 56,506 rows of 235 channels take
-  // 48.9 ms for both gradients, with two parts held 37.6, with one 30.7).
+  // 48.9 ms for both gradients, with two parts held 37.6, with one 28.3).
   static constexpr bool kLean = NP == 3 && DP == 256 && SUM;
   static constexpr int HP = kLean ? 1 : NP;
   H8 held[RB][KS][HP];
@@ -677,7 +677,9 @@ struct Step {
     constexpr int kGroups = kAdd + kSmall + kLast;
     H8 a[2][4];  // a group's operands: three planes, or the first planes of kPer steps
     H8 first;    // the first plane of the other row half
-    H8 rest[2][kLean ? NP - HP : 1];
+    // groups that the parts read again are ahead: 500 clocks, as a load from L2 takes (0: 10 % slower)
+    constexpr int kDeep = 2, kRing = kDeep + 2;
+    H8 rest[kLean ? kRing : 1][kLean ? NP - HP : 1];
     const uint16_t *again = low;
     if constexpr (kLean) asm volatile("" : "+v"(again));  // (not read once before the walk)
     auto load = [&](int g) {
@@ -689,18 +691,23 @@ struct Step {
       } else if (g < kAdd + kSmall) {
 #pragma unroll
         for (int p = 0; p < 3; ++p) to[p] = *(const H8 *)&straight[(p * KS + g - kAdd) * 64 + lane];
-        if constexpr (kLean) {
-#pragma unroll
-          for (int p = HP; p < 3; ++p)
-            rest[g & 1][p - HP] = *(const H8 *)(again + ((p - HP) * KS + g - kAdd) * 512);
-        }
       } else {
 #pragma unroll
         for (int j = 0; j < kPer; ++j)
           to[j] = *(const H8 *)&straight[((g - kAdd - kSmall) * kPer + j) * 64 + lane];
       }
     };
+    auto read_again = [&](int k) {
+      if constexpr (kLean) {
+        if (k < 0 || k >= kSmall) return;
+#pragma unroll
+        for (int p = HP; p < 3; ++p)
+          rest[k % kRing][p - HP] = *(const H8 *)(again + ((p - HP) * KS + k) * 512);
+      }
+    };
     load(0);
+#pragma unroll
+    for (int k = 0; k <= kDeep - kAdd; ++k) read_again(k);
     int done = 0;
     auto slot = [&] {
       between(done++);
@@ -712,6 +719,7 @@ struct Step {
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       if (g + 1 < kGroups) load(g + 1);
+      read_again(g + 1 + kDeep - kAdd);
       const H8 *x = a[g & 1];
       if (g < kAdd) {
         const int d = g / 2, h = g & 1;
@@ -740,7 +748,7 @@ struct Step {
         for (int p = 0; p < HP; ++p) y[p] = held[0][g - kAdd][p];
         if constexpr (kLean) {
 #pragma unroll
-          for (int p = HP; p < 3; ++p) y[p] = rest[g & 1][p - HP];
+          for (int p = HP; p < 3; ++p) y[p] = rest[(g - kAdd) % kRing][p - HP];
         }
 #pragma unroll
         for (int i = 0; i < 5; ++i) {
