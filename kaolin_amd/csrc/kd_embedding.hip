@@ -236,7 +236,7 @@ __device__ __forceinline__ void embed_rank(const uint2 (&kt)[ITERS], uint32_t in
 // 50,000 rows are written in 45 us, and in the second pass in 27 us, behind 16 us of counting; of
 // 2,097,152 in 14 and 12 us behind 8.
 // few: each workgroup adds up all tiles' counts itself, 16 bytes a thread and a share of the tiles: both
-// passes of 262,144 tokens take 31 us in four launches against 26 in six, a call whose launches are its
+// passes of 262,144 tokens take 30 us in four launches against 26 in six, a call whose launches are its
 // time 104 us against 109.
 template <int ITERS>
 __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
@@ -272,6 +272,15 @@ __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
     }
     s_all[threadIdx.x] = all;
     s_before[threadIdx.x] = before;
+    for (int h = shares / 2; h >= 1; h >>= 1) {
+      __syncthreads();
+      if ((int)threadIdx.x < h * quads) {
+        const uint4 c = s_all[threadIdx.x + h * quads], b = s_before[threadIdx.x + h * quads];
+        uint4 &x = s_all[threadIdx.x], &y = s_before[threadIdx.x];
+        x.x += c.x, x.y += c.y, x.z += c.z, x.w += c.w;
+        y.x += b.x, y.y += b.y, y.z += b.z, y.w += b.w;
+      }
+    }
   }
   __syncthreads();
   embed_rank<ITERS>(kt, in, ITERS, shift, bits, wcnt[w], rank);
@@ -286,10 +295,8 @@ __global__ __launch_bounds__(kBlock) void kd_embed_scatter(
     all[q] = before[q] = 0;
     if (d > mask) continue;
     if (few) {
-      for (int k = 0; k < shares; ++k) {
-        all[q] += ((const uint32_t *)s_all)[k * (int)(mask + 1) + d];
-        before[q] += ((const uint32_t *)s_before)[k * (int)(mask + 1) + d];
-      }
+      all[q] = ((const uint32_t *)s_all)[d];
+      before[q] = ((const uint32_t *)s_before)[d];
     } else {
       all[q] = totals[d];
       before[q] = hist[(int64_t)d * ntile + blockIdx.x];
@@ -549,9 +556,9 @@ __device__ __forceinline__ void embed_join(const SegArgs &a, int bx, int by, int
     const uint64_t end = (uint64_t)(w + 1) * NG * a.per_group;
     if (col < a.D) embed_store<T, V>(out, a.D, a.pairs[end - 1].x, col, acc, scale);
   };
+  bool far = false;
   {
     const int w = bx * NG + g;
-    bool far = false;
     if (w < nwg - 1 && (a.flags[w] & kHasTail)) {
       far = a.flags[w + 1] & kThrough;
       if (!far) {
@@ -564,7 +571,7 @@ __device__ __forceinline__ void embed_join(const SegArgs &a, int bx, int by, int
     }
     if (gl == 0) s_long[g] = far;
   }
-  __syncthreads();
+  if (!__syncthreads_or(far)) return;
   for (int q0 = 0; q0 < NG; ++q0) {
     if (!s_long[q0]) continue;  // (the same for the whole workgroup)
     const int w = bx * NG + q0;
