@@ -1438,8 +1438,9 @@ static __global__ __launch_bounds__(kBlock) void kd_xent_rowgrad(Args a,
   if (threadIdx.x == 0) a.gmax[blockIdx.x] = max(max(s_m[0], s_m[1]), max(s_m[2], s_m[3]));
 }
 
-// the power of two that brings the largest gradient into [1, 2): the products' operands stay in
-// range whatever the incoming gradient's scale
+// The power of two that brings the largest gradient into [1, 2): the products' operands stay in
+// range whatever the incoming gradient's scale.  No larger than 2^112, so that its inverse and 2^14
+// times it are normal numbers; gradients below 2^-112 are then less than 1.
 __device__ __forceinline__ float grad_unit(const Args &a) {
   __shared__ uint32_t s_u[kBlock / kWave];
   const int nblk = grad_blocks(a.npad);
@@ -1450,7 +1451,8 @@ __device__ __forceinline__ float grad_unit(const Args &a) {
   if ((threadIdx.x & 63) == 0) s_u[threadIdx.x >> 6] = top;
   __syncthreads();
   const uint32_t e = max(max(s_u[0], s_u[1]), max(s_u[2], s_u[3])) >> 23;
-  return e == 0 || e >= 254 ? 1.f : __uint_as_float((254u - e) << 23);
+  if (e == 255) return 1.f;  // infinite or NaN
+  return e == 254 ? 0x1p-127f : __uint_as_float(min(254u - e, 239u) << 23);
 }
 
 // The walk over the pixels: kd_xent_rows with the sides exchanged, the logits formed a second time
@@ -1466,7 +1468,7 @@ struct TableWalk : Step<T, DP, 2> {
   using F = Form<T>;
   static constexpr int NP = B::NP, RB = B::RB, PP = B::PP;
   int v0, near;  // near: this lane's pixel's label
-  float c2, c2l, unit, lunit;
+  float c2, c2l, unit;
   f32x4 lse[4], g[ROWG ? 4 : 1];
   const float *plse, *pw, *pg;
   const int *plab;
@@ -1477,7 +1479,8 @@ struct TableWalk : Step<T, DP, 2> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       l[i] = *(const f32x4 *)(plse + r + 8 * i + 4 * (lane >> 5));
-      if (ROWG) gr[i] = *(const f32x4 *)(pg + r + 8 * i + 4 * (lane >> 5));
+      // (before the probabilities: unit times one of them can leave the range where g is small)
+      if (ROWG) gr[i] = *(const f32x4 *)(pg + r + 8 * i + 4 * (lane >> 5)) * unit;
     }
     y = plab[r + (lane & 31)];
   }
@@ -1495,8 +1498,8 @@ struct TableWalk : Step<T, DP, 2> {
     B::step(s_x, s_t, [&](int, int i, float &p0, float &p1) {
       const f32x4 l = lse[i / 2];
       const int j = 2 * (i & 1);
-      p0 = __builtin_amdgcn_exp2f(exponent<T>(p0, c2, c2l, ROWG ? l[j] + lunit : l[j]));
-      p1 = __builtin_amdgcn_exp2f(exponent<T>(p1, c2, c2l, ROWG ? l[j + 1] + lunit : l[j + 1]));
+      p0 = __builtin_amdgcn_exp2f(exponent<T>(p0, c2, c2l, l[j]));
+      p1 = __builtin_amdgcn_exp2f(exponent<T>(p1, c2, c2l, l[j + 1]));
       if (ROWG) {
         p0 *= g[i / 2][j];
         p1 *= g[i / 2][j + 1];
@@ -1554,7 +1557,6 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, 2>::waves)) void kd_xent_table
   w.c2 = a.c2;
   w.c2l = a.c2l;
   w.unit = ROWG ? grad_unit(a) : 1.f;
-  w.lunit = ROWG ? log2f(w.unit) : 0.f;  // a power of two: exact
   w.plse = a.lse;
   w.pw = a.w;
   w.pg = a.grow;
