@@ -288,7 +288,8 @@ __global__ __launch_bounds__(kBlock) void kd_xent_pack(Args a, int xtiles,
         x = load_pack<T, V>(table + i * a.D + d, a.D - d);
       }
     }
-    float size = 0.f;  // the row's squared size: DP / V lanes hold it
+    // the row's squared size (DP / V lanes hold it), no less than it is where the squares leave the range
+    float size = 0x1p-100f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       size = fmaf((float)x.v[j], (float)x.v[j], size);

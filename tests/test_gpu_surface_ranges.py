@@ -5,6 +5,8 @@ import math
 import pytest
 import torch
 
+from test_gpu_xent import _check, _reference
+
 pytestmark = pytest.mark.gpu
 
 DEV = 'cuda'
@@ -44,3 +46,27 @@ def test_incoming_gradients_scale_the_result(dname, power):
         near = (a.double() - want.double()).abs() <= _subnormal_step(dt)
         assert (near | (a == want)).all(), float(a.float().abs().max())
         assert not torch.isnan(a).any()
+
+
+@pytest.mark.parametrize('dname', ['f32', 'bf16'])
+def test_features_whose_squares_vanish(dname):
+    """Features of 1e-23, whose squares are 0 in 32 bits, and a scale of 1e22: logits of some hundred,
+    whose exponentials need the running maximum."""
+    dt = TYPES[dname]
+    g = torch.Generator().manual_seed(21)
+    n, V, D = 300, 50, 256
+    x = torch.where(torch.rand(n, D, generator=g) < 0.5, -1e-23, 1e-23).to(DEV, dt)
+    e = (torch.randn(V, D, generator=g) * 100).to(DEV, dt)
+    y = torch.randint(0, V, (n,), generator=g).to(DEV)
+    grad = torch.rand(n, generator=g).to(DEV) + 0.25
+    want = list(_reference(x, e, y, 1e22, 'none', grad))
+    assert 300 < float(want[0].max()) < 2000
+    # A probability below 2^-126 is subnormal or 0 in 32 bits, off by at most that, and so is 1 - p of a
+    # label whose logit is some 100 above the others: times |g| scale |e| (or |x|) a term.  The bounds of
+    # _reference leave 1e-37 for it, which is for scales next to 1.
+    gs = 2.0 ** -126 * 1e22 * grad.double()
+    want[3] = want[3] + 2 * gs[:, None] * e.double().abs().sum(0)
+    want[5] = want[5] + 2 * gs @ x.double().abs()
+    got = _run(x, e, y, 1e22, 'none', grad)
+    assert all(torch.isfinite(t).all() for t in got)
+    _check(got, want)
