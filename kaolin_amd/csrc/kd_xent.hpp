@@ -32,6 +32,8 @@
 #include "kd_common.hpp"
 #include "kd_float16.hpp"
 
+#include <cfloat>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -40,6 +42,7 @@ namespace xent {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef half_t half8 __attribute__((ext_vector_type(8)));
 typedef bfloat_t bfloat8 __attribute__((ext_vector_type(8)));
 
@@ -92,7 +95,7 @@ __device__ __forceinline__ void split3(float x, uint16_t &a, uint16_t &b, uint16
   c = __builtin_bit_cast(uint16_t, (bfloat_t)(r - (float)m));
 }
 
-constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.9259629e-8f;
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kSlots = 64, kSlotPad = 16;  // maxima of the table, 64 bytes apart
 constexpr int kRowPad = 256;  // packed rows are padded with zeros to a multiple of this
@@ -116,9 +119,11 @@ struct Args {
   // state kept from forward to backward
   int *count;       // pixels with a label
   int *rowid, *lab; // listed pixel -> pixel, its label
-  float *lse, *w;   // exponent of a probability but its logit, its complement negated (scaled)
+  int *far;         // 1: logits beyond kFar
+  float *lse, *rl;  // exponent of a probability but its logit, factor of the exponential
+  float *w;         // its complement negated (scaled)
   float *xn;        // squared sizes of the pixels' features
-  uint32_t *emax;   // the largest squared sizes of the table's rows (their bits), kSlots of them
+  uint32_t *emax, *xmax;  // the largest squared sizes of rows and pixels (their bits), kSlots of each
   uint32_t *ticket; // workgroups that have added up their losses
   uint16_t *xs, *xt, *es;
   float *raw;       // (n, D): w (m - e_y)
@@ -128,7 +133,7 @@ struct Args {
   float *pm, *pl, *pz, *po;  // a part's maximum, sum, label's logit (or -inf), weighted sum
   float *lrow;
   double *part;
-  float *grow, *pe;
+  float *grow, *gfac, *pe;  // a pixel's incoming gradient, and times its factor
   uint32_t *gmax;
 };
 
@@ -241,9 +246,10 @@ static __global__ __launch_bounds__(kBlock) void kd_xent_map(Args a, int chunks,
     }
   }
   if (blockIdx.x == gridDim.x - 1) {
-    if (threadIdx.x < kSlots) a.emax[threadIdx.x * kSlotPad] = 0u;
+    if (threadIdx.x < kSlots) a.emax[threadIdx.x * kSlotPad] = a.xmax[threadIdx.x * kSlotPad] = 0u;
     if (threadIdx.x == 0) {
       *a.count = run;
+      *a.far = 0;
       *a.ticket = 0u;
     }
   }
@@ -262,6 +268,7 @@ __global__ __launch_bounds__(kBlock) void kd_xent_pack(Args a, int xtiles,
   using F = Form<T>;
   constexpr int V = 16 / sizeof(T);
   constexpr int kPitch = DP + V;  // rows 16 bytes apart over the banks
+  constexpr int kLanes = DP / V < kWave ? DP / V : kWave;  // that hold a row
   __shared__ __align__(16) T s_m[32 * kPitch];
   __shared__ uint32_t s_top[kBlock / kWave];
   uint32_t top = 0;
@@ -296,28 +303,23 @@ __global__ __launch_bounds__(kBlock) void kd_xent_pack(Args a, int xtiles,
       if (flip) x.v[j] = (T)(-(float)x.v[j]);
     }
     *(uint4 *)&s_m[r * kPitch + d] = __builtin_bit_cast(uint4, x);
-    constexpr int kLanes = DP / V < kWave ? DP / V : kWave;
 #pragma unroll
     for (int k = kLanes / 2; k >= 1; k >>= 1) size += __shfl_xor(size, k);
-    if (is_x) {
-      if (d == 0) a.xn[i] = size;
-    } else {
-      top = max(top, __float_as_uint(size));
-    }
+    if (is_x && d == 0) a.xn[i] = size;
+    top = max(top, __float_as_uint(size));
   }
-  if (!is_x) {  // one atomic a workgroup, spread over the slots: they would queue at one address
 #pragma unroll
-    for (int k = 32; k >= 1; k >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, k));
-    if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = top;
-  }
+  for (int k = 32; k >= kLanes; k >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, k));
+  if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = top;
   if (is_x && threadIdx.x < 32 && r0 + threadIdx.x >= count) {
     a.lab[r0 + threadIdx.x] = -1;
     a.lse[r0 + threadIdx.x] = -INFINITY;  // its probabilities are 0
+    a.rl[r0 + threadIdx.x] = 0.f;
     a.w[r0 + threadIdx.x] = 0.f;
   }
   __syncthreads();
-  if (!is_x && threadIdx.x == 0)
-    atomicMax(a.emax + tile % kSlots * kSlotPad,
+  if (threadIdx.x == 0)  // spread over the slots: they would queue at one address
+    atomicMax((is_x ? a.xmax : a.emax) + tile % kSlots * kSlotPad,
               max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3])));
   constexpr int kGroups = 32 * DP / 8;  // 16-byte groups per plane and layout
   uint16_t *straight = (is_x ? a.xs : a.es) + tile * F::np * 32 * DP;
@@ -358,23 +360,48 @@ __global__ __launch_bounds__(kBlock) void kd_xent_pack(Args a, int xtiles,
 // ------------------------------------------------------------------------------------------------
 // shared pieces of the two walks
 // ------------------------------------------------------------------------------------------------
-// acc += the i-th of the planes' products of a . b, the large one last
-template <int NP, typename H8>
+// acc += the i-th of the planes' products of a . b, the large one last.  SWAP: the order that the same
+// product has with a and b exchanged, so that the logits of both walks have the same roundings.
+template <int NP, bool SWAP = false, typename H8>
 __device__ __forceinline__ f32x16 product(int i, const H8 *a, const H8 *b, f32x16 c) {
   if constexpr (NP == 1) {
     return mfma(a[0], b[0], c);
   } else {
     constexpr int ka[6] = {0, 2, 1, 0, 1, 0}, kb[6] = {2, 0, 1, 1, 0, 0};
-    return mfma(a[ka[i]], b[kb[i]], c);
+    return mfma(a[SWAP ? kb[i] : ka[i]], b[SWAP ? ka[i] : kb[i]], c);
   }
 }
 
 // log2 of a term: the logit times the factor, in two parts for 32-bit data (a factor off by 2^-25
-// would be a bias that no averaging takes out), and an offset.
+// would be a bias that no averaging takes out), and an offset (first, where the sum becomes small).
 template <typename T>
 __device__ __forceinline__ float exponent(float s, float c2, float c2l, float offset) {
-  if constexpr (sizeof(T) == 4) offset = fmaf(s, c2l, offset);
-  return fmaf(s, c2, offset);
+  const float e = fmaf(s, c2, offset);
+  if constexpr (sizeof(T) == 4) return fmaf(s, c2l, e);
+  return e;
+}
+
+// Logits that may be larger than this (in log2, by the largest sizes of the pixels and the rows) take
+// walks of their own, tile by tile, in which a term's log2 is the logit times the factor, rounded, the
+// same number in both walks.  In the others that product is not rounded: an offset of its size is off by
+// half a step of it, which an exponential turns into 2^-25 of the logit, relative.  In 16 bits, whose
+// other walks hold the offset log2 of the sum in one number, that is 2^-15 here, an eighth of a step of
+// fp16; without a limit fp16 and bf16 gradients were 0.8 % off at logits of 8e4, 32-bit ones too, all of
+// them wrong at 1e7 and not finite at 1e9.  With 32-bit data the offset is two numbers, a whole one
+// (exact up to 2^24) and a factor of the exponential.
+// Measured (loss; loss and both gradients), bounded / with the running maximum / large logits: bf16, 64
+// channels, 263,576 pixels x 50,000 rows 2.4 / 2.7 / 3.4 ms; 7.2 / 7.8 / 10.2 ms; 256 channels, 131,788 x
+// 10,000 0.63 / 0.67 / 0.71; 3.2 / 3.4 / 4.7; fp16, 64 channels, 131,072 x 10,000 0.41 / 0.39 / 0.47; 0.91 /
+// 0.91 / 1.28; fp32, 64 channels, 131,712 x 10,000 0.86 / 0.87 / 0.90; 3.56 / 3.65 / 3.55.
+template <typename T>
+constexpr float kFar = sizeof(T) == 4 ? 0x1p22f : 0x1p10f;
+
+// the largest of a kind of sizes, squared (NaN if there is one: its bits are above infinity's)
+__device__ __forceinline__ float largest(const uint32_t *slots) {
+  uint32_t big = slots[(threadIdx.x & 63) * kSlotPad];
+#pragma unroll
+  for (int k = 32; k >= 1; k >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, k));
+  return __uint_as_float(big);
 }
 
 // the upper halves of two words as one
@@ -753,7 +780,7 @@ struct Step {
         }
 #pragma unroll
         for (int i = 0; i < 5; ++i) {
-          next = product<3>(i, x, y, next);
+          next = product<3, KIND == 2>(i, x, y, next);
           slot();
         }
       } else {
@@ -926,6 +953,29 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
     if constexpr (ONLINE) raise();
   }
 
+  // a tile of large logits (see kFar), with no other's work beside it.  The power of two by which
+  // probabilities are scaled in the products stays out of the maximum, which may be too large for it.
+  __device__ __forceinline__ void far_tile(const uint4 *s_e, const uint4 *s_t, int v0) {
+    B::logits(s_e);
+    mask(v0);
+    raise();
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p0 = __builtin_amdgcn_exp2f(this->s[b][2 * i] * c2 - m[b]);
+        const float p1 = __builtin_amdgcn_exp2f(this->s[b][2 * i + 1] * c2 - m[b]);
+        t[b][0] += p0;
+        t[b][1] += p1;
+        if constexpr (SUM) {
+          constexpr float f = F::shift == 0.f ? 1.f : 0x1p10f;
+          pack_pair<T, PP>(p0 * f, p1 * f, i & 3, this->q[b][i >> 2]);
+        }
+      }
+    fold();
+    if constexpr (SUM) B::add(s_t);
+  }
+
   // The sums of the last tiles (one of 32-bit data, two of 16-bit data) to those before: a walk of
   // 150,000 rows would be 40,000 additions a lane, whose roundings leave 3e-6 of the sum.  With 32-bit
   // data l[b][1] holds what the last addition lost; with 16-bit data that takes 1.5 % of the time, and
@@ -981,79 +1031,104 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const Deal deal(((int64_t)*a.count + W::rows - 1) / W::rows, (a.V + 63) / 64, W::workers);
   stagger();
-  RowsWalk<T, DP, SUM> w;
-  w.V = a.V;
-  w.c2 = a.c2;
-  w.c2l = a.c2l;
-  uint32_t big = a.emax[lane * kSlotPad];
-#pragma unroll
-  for (int k = 32; k >= 1; k >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, k));
-  const float size2 = __uint_as_float(big), size = a.c2 * sqrtf(size2);
+  const float size2 = largest(a.emax), size = a.c2 * sqrtf(size2);
   const bool fits = F::shift == 0.f && size2 < kSafeRow && size2 > 1.f / kSafeRow;
+  const bool far = !(size * sqrtf(largest(a.xmax)) < kFar<T>);  // (a NaN too)
+  if (far && blockIdx.x == 0 && z == 0 && threadIdx.x == 0) *a.far = 1;
   const uint16_t *es = a.es, *et = a.et;
   constexpr int64_t kTile = kBytes / 2;
-  deal.each(blockIdx.x, [&](int64_t block, int p0, int p1, int64_t slot) {
-    const int64_t row0 = block * W::rows + wave * (32 * RB);
-    // |logit| <= |x| |e| scale, over the kRowPad rows about this wave's (so that the choice does not
-    // depend on how many of them a wave holds); a NaN size takes the general way
-    bool safe = fits;
+  // (the whole share in one way, so that the registers of one are not those of the other)
+  auto share = [&](auto is_far) {
+    constexpr bool FAR = decltype(is_far)::value;
+    RowsWalk<T, DP, SUM> w;
+    w.V = a.V;
+    w.c2 = a.c2;
+    w.c2l = a.c2l;
+    deal.each(blockIdx.x, [&](int64_t block, int p0, int p1, int64_t slot) {
+      const int64_t row0 = block * W::rows + wave * (32 * RB);
+      bool general = true;
+      if constexpr (!FAR) {
+        // |logit| <= |x| |e| scale, over the kRowPad rows about this wave's (so that the choice does not
+        // depend on how many of them a wave holds); a NaN size takes the general way
+        bool safe = fits;
 #pragma unroll
-    for (int k = 0; k < kRowPad / kWave; ++k)
-      safe &= size * sqrtf(a.xn[row0 / kRowPad * kRowPad + k * kWave + lane]) < kSafeLogit;
-    const bool general = !__all(safe);
-    w.hold(a.xs, row0);
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      w.lab[b] = a.lab[row0 + 32 * b + (lane & 31)];
-      w.m[b] = general ? -1e30f : 0.f;
-      w.l[b][0] = w.l[b][1] = w.t[b][0] = w.t[b][1] = 0.f;
-      w.zy[b] = -INFINITY;
-    }
-    const int t0 = 2 * p0, t1 = 2 * p1;
-    auto walk = [&](auto online) {
-      constexpr bool ONLINE = decltype(online)::value;
-      fetch<kBytes>(s_e0, es + t0 * kTile);
-      arrive();
-      fetch<kBytes>(s_e1, es + (t0 + 1) * kTile);
-      if constexpr (SUM) fetch_sum<W>(s_t1, et + t0 * kTile, z);  // (times zeros)
-      w.logits(s_e0);
-      w.template ready<ONLINE>(t0 * 32);
-      arrive();
-      for (int t = t0; t < t1; t += 2) {
-        const int t2 = min(t + 2, t1 - 1), t3 = min(t + 3, t1 - 1);  // behind the end: not used
-        fetch<kBytes>(s_e0, es + t2 * kTile);
-        if constexpr (SUM) fetch_sum<W>(s_t0, et + t * kTile, z);
-        w.template next<ONLINE>(s_e1, s_t1);
-        w.template ready<ONLINE>((t + 1) * 32);
-        arrive();
-        fetch<kBytes>(s_e1, es + t3 * kTile);
-        if constexpr (SUM) fetch_sum<W>(s_t1, et + (t + 1) * kTile, z);
-        w.template next<ONLINE>(s_e0, s_t0);
-        if constexpr (sizeof(T) == 2) w.fold();
-        w.template ready<ONLINE>(t2 * 32);
-        arrive();
+        for (int k = 0; k < kRowPad / kWave; ++k)
+          safe &= size * sqrtf(a.xn[row0 / kRowPad * kRowPad + k * kWave + lane]) < kSafeLogit;
+        general = !__all(safe);
       }
-      if constexpr (SUM) w.add(s_t1);
-    };
-    if (general)
-      walk(std::true_type{});
-    else
-      walk(std::false_type{});
-    const int64_t out = slot * W::rows + wave * (32 * RB);
+      w.hold(a.xs, row0);
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      const int64_t r = out + 32 * b + (lane & 31);
-      float l = w.l[b][0] + w.l[b][1];
-      l += __shfl_xor(l, 32);
-      const float other = __shfl_xor(w.zy[b], 32);  // one of the halves has met the label, or none
-      if (half == 0 && z == 0) {
-        a.pz[r] = w.zy[b] == -INFINITY ? other : w.zy[b];
-        a.pm[r] = w.m[b] - F::shift;
-        a.pl[r] = l;
+      for (int b = 0; b < RB; ++b) {
+        w.lab[b] = a.lab[row0 + 32 * b + (lane & 31)];
+        w.m[b] = general ? -FLT_MAX : 0.f;
+        w.l[b][0] = w.l[b][1] = w.t[b][0] = w.t[b][1] = 0.f;
+        w.zy[b] = -INFINITY;
       }
-    }
-    if constexpr (SUM) w.store(a.po, out, z * (DP / W::cs));
-  });
+      const int t0 = 2 * p0, t1 = 2 * p1;
+      auto walk = [&](auto online) {
+        constexpr bool ONLINE = decltype(online)::value;
+        fetch<kBytes>(s_e0, es + t0 * kTile);
+        arrive();
+        fetch<kBytes>(s_e1, es + (t0 + 1) * kTile);
+        if constexpr (SUM) fetch_sum<W>(s_t1, et + t0 * kTile, z);  // (times zeros)
+        w.logits(s_e0);
+        w.template ready<ONLINE>(t0 * 32);
+        arrive();
+        for (int t = t0; t < t1; t += 2) {
+          const int t2 = min(t + 2, t1 - 1), t3 = min(t + 3, t1 - 1);  // behind the end: not used
+          fetch<kBytes>(s_e0, es + t2 * kTile);
+          if constexpr (SUM) fetch_sum<W>(s_t0, et + t * kTile, z);
+          w.template next<ONLINE>(s_e1, s_t1);
+          w.template ready<ONLINE>((t + 1) * 32);
+          arrive();
+          fetch<kBytes>(s_e1, es + t3 * kTile);
+          if constexpr (SUM) fetch_sum<W>(s_t1, et + (t + 1) * kTile, z);
+          w.template next<ONLINE>(s_e0, s_t0);
+          if constexpr (sizeof(T) == 2) w.fold();
+          w.template ready<ONLINE>(t2 * 32);
+          arrive();
+        }
+        if constexpr (SUM) w.add(s_t1);
+      };
+      if constexpr (FAR) {
+        for (int t = t0; t < t1; ++t) {
+          fetch<kBytes>(s_e0, es + t * kTile);
+          if constexpr (SUM) fetch_sum<W>(s_t0, et + t * kTile, z);
+          arrive();
+          w.far_tile(s_e0, s_t0, t * 32);
+          __syncthreads();
+        }
+        if constexpr (SUM && F::shift != 0.f) {
+#pragma unroll
+          for (int b = 0; b < RB; ++b)
+#pragma unroll
+            for (int d = 0; d < RowsWalk<T, DP, SUM>::DT; ++d) w.o[b][d] *= 0x1p-10f;
+        }
+      } else if (general) {
+        walk(std::true_type{});
+      } else {
+        walk(std::false_type{});
+      }
+      const int64_t out = slot * W::rows + wave * (32 * RB);
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        const int64_t r = out + 32 * b + (lane & 31);
+        float l = w.l[b][0] + w.l[b][1];
+        l += __shfl_xor(l, 32);
+        const float other = __shfl_xor(w.zy[b], 32);  // one of the halves has met the label, or none
+        if (half == 0 && z == 0) {
+          a.pz[r] = w.zy[b] == -INFINITY ? other : w.zy[b];
+          a.pm[r] = FAR ? w.m[b] : w.m[b] - F::shift;
+          a.pl[r] = l;
+        }
+      }
+      if constexpr (SUM) w.store(a.po, out, z * (DP / W::cs));
+    });
+  };
+  if (far)
+    share(std::true_type{});
+  else
+    share(std::false_type{});
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1064,22 +1139,27 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
 constexpr int kFewParts = 16;
 
 // A pixel's loss softplus(L' - z_y) from the maximum (log2) and the sum over the rows but its label's
-// and from the label's logit; lse: log2 of the whole sum, w: 1 - p_y.
-__device__ __forceinline__ float pixel_loss(float m, float l, float z, const Args &a, float &lse,
-                                            float &w) {
+// and from the label's logit; w: 1 - p_y, base + rest: log2 of the whole sum (far: see kFar), base a
+// whole number and the larger of the two sides, so that rest is small.
+__device__ __forceinline__ float pixel_loss(float m, float l, float z, bool far, const Args &a,
+                                            float &w, float &base, float &rest) {
   const float z2 = z * a.c2;
   // log2 of the sum less z_y, both near the whole number m + k: the difference is formed where it is
   // small (m is a whole number), the sum's logarithm next to 1 if the loss is neither large nor small
-  const float k = fminf(fmaxf(rintf(z2 - m), -1e9f), 1e9f);
-  const float d = fmaf(z, a.c2, -(m + k)) + z * a.c2l;
+  float k = fminf(fmaxf(rintf(z2 - m), -1e9f), 1e9f);
+  const float mk = m + k;
+  if (far) k = mk - m;  // (as far as m + k was rounded)
+  const float d = far ? z2 - mk : fmaf(z, a.c2, -mk) + z * a.c2l;
   const float fits = fminf(fmaxf(k, -40.f), 40.f);  // (sums reach from 2^-60 to 2^91)
-  const float g = log2f(l * __builtin_amdgcn_exp2f(-fits)) - (k - fits);
-  const float u = (g - d) * kLn2;  // -inf when the label is the only row
-  const float t = expf(-fabsf(u));
-  const float value = u != u ? u : fmaxf(u, 0.f) + log1pf(t);
-  w = u != u ? u : (u >= 0.f ? 1.f / (1.f + t) : t / (1.f + t));
-  lse = fmaf(z, a.c2, fmaf(z, a.c2l, fmaf(value, kLog2e, value * kLog2eLow)));
-  return value;
+  const float part = log2f(l * __builtin_amdgcn_exp2f(-fits)), g = part - (k - fits);
+  float u = (g - d) * kLn2;  // -inf when the label is the only row
+  if (z2 == INFINITY) u = NAN;  // as infinity less infinity
+  const float t = expf(-fabsf(u)), more = log1pf(t);
+  const bool others = u > 0.f;
+  w = u != u ? u : (others ? 1.f : t) / (1.f + t);
+  base = others ? m : far ? z2 : mk;
+  rest = fmaf(more, kLog2e, others ? part + fits : far ? 0.f : d);
+  return u != u ? u : fmaxf(u, 0.f) + more;
 }
 
 template <typename T, int DP, int G, bool RAW>
@@ -1106,7 +1186,7 @@ __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__res
   const bool few = n < kFewParts;  // every lane goes through them all
 
   const int s0 = few ? 0 : gl, ds = few ? 1 : G;
-  float m = -1e30f, z = -INFINITY;
+  float m = -FLT_MAX, z = -INFINITY;
 #pragma unroll 4
   for (int s = s0; s < n; s += ds) {
     const int64_t q = first + (int64_t)s * W::rows;
@@ -1132,10 +1212,20 @@ __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__res
 #pragma unroll
     for (int s = G / 2; s >= 1; s >>= 1) l += __shfl_xor(l, s);
   }
-  float lse, wn;
-  const float out = pixel_loss(m, l, z, a, lse, wn);
+  float wn, base, rest;
+  const bool far = *a.far;
+  const float out = pixel_loss(m, l, z, far, a, wn, base, rest);
   if (gl == 0) {
-    a.lse[r] = Form<T>::shift_table - lse;
+    if (far) {
+      a.rl[r] = exp2f(-rest);
+    } else if (sizeof(T) == 4) {
+      const float whole = floorf(rest);
+      base += whole;
+      a.rl[r] = exp2f(whole - rest);
+    } else {
+      base += rest - Form<T>::shift_table;  // (no factor)
+    }
+    a.lse[r] = -base;
     a.w[r] = -wn * exp2f(Form<T>::shift_table);
     if (a.reduction == 0)
       loss[i] = out;
@@ -1231,7 +1321,7 @@ __global__ __launch_bounds__(kBlock) void kd_xent_few(Args a, const T *__restric
     f.operand(x[k]);
   }
   const int64_t y = i < a.n ? labels[i] : -1;
-  float m = -1e30f, l = 0.f, zy = -INFINITY;
+  float m = -FLT_MAX, l = 0.f, zy = -INFINITY;
   const int ntile = (a.V + 31) / 32;
   for (int t = blockIdx.x * (kBlock / kWave) + wave; t < ntile; t += gridDim.x * (kBlock / kWave)) {
     const int64_t v0 = (int64_t)t * 32, v = v0 + (lane & 31);
@@ -1291,8 +1381,10 @@ __global__ __launch_bounds__(kBlock) void kd_xent_few(Args a, const T *__restric
       m = top;
     }
     float sum = 0.f;
+    const bool far = !(fabsf(m) < kFar<T>);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) sum += __builtin_amdgcn_exp2f(exponent<T>(s[j], a.c2, a.c2l, -m));
+    for (int j = 0; j < 16; ++j)
+      sum += __builtin_amdgcn_exp2f(far ? s[j] * a.c2 - m : exponent<T>(s[j], a.c2, a.c2l, -m));
     l += sum;
   }
   // the two halves, then the waves
@@ -1324,13 +1416,14 @@ __global__ __launch_bounds__(kBlock) void kd_xent_few(Args a, const T *__restric
   a.pz[q] = zy;
 }
 
-static __global__ __launch_bounds__(1024) void kd_xent_few_join(Args a, int nparts,
+template <typename T>
+__global__ __launch_bounds__(1024) void kd_xent_few_join(Args a, int nparts,
                                                                 const int64_t *__restrict__ labels,
                                                                 float *__restrict__ loss) {
   constexpr int kLanes = 1024 / kFewPixels;
   __shared__ float s_m[kLanes][kFewPixels], s_l[kLanes][kFewPixels], s_z[kLanes][kFewPixels];
   const int i = threadIdx.x % kFewPixels, j = threadIdx.x / kFewPixels;
-  float m = -1e30f, l = 0.f, z = -INFINITY;
+  float m = -FLT_MAX, l = 0.f, z = -INFINITY;
   if (i < a.n) {
 #pragma unroll 4
     for (int p = j; p < nparts; p += kLanes) {
@@ -1355,8 +1448,9 @@ static __global__ __launch_bounds__(1024) void kd_xent_few_join(Args a, int npar
   }
   const int64_t y = i < a.n ? labels[i] : -1;
   const bool in = y >= 0 && y < a.V;
-  float lse, w;
-  const float out = in ? pixel_loss(m, l, z, a, lse, w) : 0.f;
+  const bool far = !(fmaxf(fabsf(m), fabsf(z * a.c2)) < kFar<T>);
+  float w, base, rest;
+  const float out = in ? pixel_loss(m, l, z, far, a, w, base, rest) : 0.f;
   if (a.reduction == 0) {
     if (i < a.n) loss[i] = out;
     return;
@@ -1419,7 +1513,8 @@ __host__ __device__ inline int grad_blocks(int64_t npad) {
   return (int)((npad + chunk - 1) / chunk);
 }
 
-static __global__ __launch_bounds__(kBlock) void kd_xent_rowgrad(Args a,
+// factors: of 32-bit data, the others have them only with large logits
+static __global__ __launch_bounds__(kBlock) void kd_xent_rowgrad(Args a, bool factors,
                                                                  const float *__restrict__ grad) {
   __shared__ uint32_t s_m[kBlock / kWave];
   const int count = *a.count;
@@ -1429,7 +1524,10 @@ static __global__ __launch_bounds__(kBlock) void kd_xent_rowgrad(Args a,
   for (int k = 0; k < steps; ++k) {
     const int64_t r = ((int64_t)blockIdx.x * steps + k) * kBlock + threadIdx.x;
     const float g = r < count ? grad[a.rowid[r]] : 0.f;
-    if (r < a.npad) a.grow[r] = g;
+    if (r < a.npad) {
+      a.grow[r] = g;
+      if (factors || *a.far) a.gfac[r] = r < count ? g * a.rl[r] : 0.f;
+    }
     top = max(top, __float_as_uint(fabsf(g)));
   }
 #pragma unroll
@@ -1468,45 +1566,115 @@ struct TableWalk : Step<T, DP, 2> {
   using B = Step<T, DP, 2>;
   using F = Form<T>;
   static constexpr int NP = B::NP, RB = B::RB, PP = B::PP;
+  static constexpr bool FAC = ROWG || sizeof(T) == 4;  // exponentials have a factor
   int v0, near;  // near: this lane's pixel's label
   float c2, c2l, unit;
-  f32x4 lse[4], g[ROWG ? 4 : 1];
-  const float *plse, *pw, *pg;
+  f32x4 lse[NP == 1 ? 4 : 1], g[NP == 1 && FAC ? 4 : 1];
+  const float *plse, *pw, *pg, *pf;  // pg: incoming gradients, pf: factors
   const int *plab;
 
-  __device__ __forceinline__ void rows(int t, f32x4 *l, f32x4 *gr, int &y) {
+  // the exponents and factors of a lane's pixels 8 i + 4 (lane / 32) + k .., of those of a tile
+  template <typename VEC>
+  __device__ __forceinline__ void rows(const float *tile_lse, const float *tile_f, int i, int k, VEC &l,
+                                       VEC &f) {
+    const int r = 8 * i + 4 * ((threadIdx.x & 63) >> 5) + k;
+    l = *(const VEC *)(tile_lse + r);
+    if (FAC) f = *(const VEC *)(tile_f + r);
+    // (before the probabilities: unit times one of them can leave the range where g is small)
+    if (ROWG) f *= unit;
+  }
+  // 32-bit data: tile t's by way of LDS, 64 x 4 bytes
+  __device__ __forceinline__ void fetch_rows(float *s_r, int t) {
     const int lane = threadIdx.x & 63;
-    const int64_t r = (int64_t)t * 32;
+    if (NP == 1 || threadIdx.x >= kWave) return;
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) void *)((lane < 32 ? plse : pf - 32) +
+                                                         (int64_t)t * 32 + lane),
+        (__attribute__((address_space(3))) void *)s_r, 4, 0, 0);
+  }
+  __device__ __forceinline__ int label(int t) { return plab[(int64_t)t * 32 + (threadIdx.x & 31)]; }
+
+  // 16-bit data: what the next step needs
+  __device__ __forceinline__ void ahead(int t, f32x4 *l, f32x4 *f, int &y) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      l[i] = *(const f32x4 *)(plse + r + 8 * i + 4 * (lane >> 5));
-      // (before the probabilities: unit times one of them can leave the range where g is small)
-      if (ROWG) gr[i] = *(const f32x4 *)(pg + r + 8 * i + 4 * (lane >> 5)) * unit;
-    }
-    y = plab[r + (lane & 31)];
+    for (int i = 0; i < 4; ++i)
+      rows(plse + (int64_t)t * 32, pf + (int64_t)t * 32, i, 0, l[i], f[FAC ? i : 0]);
+    y = label(t);
   }
 
-  // tile t is stepped over, t1 the next one's values
-  __device__ __forceinline__ void next(const uint4 *s_x, const uint4 *s_t, int t, int t1) {
-    const int lane = threadIdx.x & 63, half = lane >> 5;
-    f32x4 l1[4], g1[ROWG ? 4 : 1];
+  // tile t is stepped over (s_r: its exponents and factors), t1 the next one's values
+  __device__ __forceinline__ void next(const uint4 *s_x, const uint4 *s_t, const float *s_r, int t,
+                                       int t1) {
+    f32x4 l1[NP == 1 ? 4 : 1], g1[NP == 1 && FAC ? 4 : 1];
+    f32x2 l2[2], g2[2];
     int near1;
-    // one step ahead; where registers are short, in the step itself, whose exponentials come late
-    if constexpr (NP == 1)
-      rows(t1, l1, g1, near1);
-    else
-      rows(t, lse, g, near);
+    // one step ahead; where registers are short, from LDS, one pair ahead
+    if constexpr (NP == 1) {
+      ahead(t1, l1, g1, near1);
+    } else {
+      rows(s_r, s_r + 32, 0, 0, l2[0], g2[0]);
+      near = label(t);
+    }
     B::step(s_x, s_t, [&](int, int i, float &p0, float &p1) {
-      const f32x4 l = lse[i / 2];
-      const int j = 2 * (i & 1);
-      p0 = __builtin_amdgcn_exp2f(exponent<T>(p0, c2, c2l, l[j]));
-      p1 = __builtin_amdgcn_exp2f(exponent<T>(p1, c2, c2l, l[j + 1]));
-      if (ROWG) {
-        p0 *= g[i / 2][j];
-        p1 *= g[i / 2][j + 1];
+      f32x2 l, f = {1.f, 1.f};
+      if constexpr (NP == 1) {
+        const int j = 2 * (i & 1);
+        l[0] = lse[i / 2][j], l[1] = lse[i / 2][j + 1];
+        if (FAC) f[0] = g[i / 2][j], f[1] = g[i / 2][j + 1];
+      } else {
+        if (i < 7) rows(s_r, s_r + 32, (i + 1) / 2, 2 * ((i + 1) & 1), l2[(i + 1) & 1], g2[(i + 1) & 1]);
+        l = l2[i & 1];
+        f = g2[i & 1];
+      }
+      p0 = __builtin_amdgcn_exp2f(exponent<T>(p0, c2, c2l, l[0]));
+      p1 = __builtin_amdgcn_exp2f(exponent<T>(p1, c2, c2l, l[1]));
+      if (FAC) {
+        p0 *= f[0];
+        p1 *= f[1];
       }
     });
-    // pixels labelled with these rows: p - 1 = -(1 - p) in the place of p
+    labelled(t);
+    if constexpr (NP == 1) {
+      near = near1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lse[i] = l1[i];
+        if (FAC) g[i] = g1[i];
+      }
+    }
+  }
+
+  // a tile of large logits (see kFar), with no other's work beside it
+  __device__ __forceinline__ void far_tile(const uint4 *s_x, const uint4 *s_t, int t) {
+    const int lane = threadIdx.x & 63;
+    near = label(t);
+    B::logits(s_x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t r = (int64_t)t * 32 + 8 * i + 4 * (lane >> 5);
+      const f32x4 l = *(const f32x4 *)(plse + r);
+      f32x4 f = *(const f32x4 *)(pf + r) * unit;
+      if constexpr (F::shift_table != 0.f) f *= 0x1p14f;
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          float p[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            p[k] = __builtin_amdgcn_exp2f(this->s[b][4 * i + j + k] * c2 + l[j + k]) * f[j + k];
+            if (l[j + k] == -INFINITY) p[k] = 0.f;  // (padding, whatever the row holds)
+          }
+          pack_pair<T, PP>(p[0], p[1], 2 * (i & 1) + j / 2, this->q[b][i >> 1]);
+        }
+    }
+    labelled(t);
+    B::add(s_t);
+  }
+
+  // pixels of tile t labelled with these rows: p - 1 = -(1 - p) in the place of p
+  __device__ __forceinline__ void labelled(int t) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
     if (__any((uint32_t)(near - v0) < 32u * RB)) {
       int64_t r = (int64_t)t * 32 + 4 * half;
       asm volatile("" : "+v"(r));  // its sums stay in here and out of the loop's registers
@@ -1533,14 +1701,6 @@ struct TableWalk : Step<T, DP, 2> {
             }
         }
     }
-    if constexpr (NP == 1) {
-      near = near1;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        lse[i] = l1[i];
-        if (ROWG) g[i] = g1[i];
-      }
-    }
   }
 };
 
@@ -1550,47 +1710,69 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, 2>::waves)) void kd_xent_table
   constexpr int RB = W::rb, kBytes = W::tile_bytes;
   __shared__ uint4 s_x0[kBytes / 16], s_x1[kBytes / 16];
   __shared__ uint4 s_t0[W::sum_bytes / 16], s_t1[W::sum_bytes / 16];
+  __shared__ float s_r0[W::np == 1 ? 1 : kWave], s_r1[W::np == 1 ? 1 : kWave];
   const int z = blockIdx.z;
   const int wave = threadIdx.x >> 6;
   const Deal deal((a.V + W::rows - 1) / W::rows, (int)(((int64_t)*a.count + 63) / 64), W::workers);
   stagger();
-  TableWalk<T, DP, ROWG> w;
-  w.c2 = a.c2;
-  w.c2l = a.c2l;
-  w.unit = ROWG ? grad_unit(a) : 1.f;
-  w.plse = a.lse;
-  w.pw = a.w;
-  w.pg = a.grow;
-  w.plab = a.lab;
+  const float unit = ROWG ? grad_unit(a) : 1.f;
+  const bool far = *a.far;
   const uint16_t *xs = a.xs, *xt = a.xt;
   constexpr int64_t kTile = kBytes / 2;
-  deal.each(blockIdx.x, [&](int64_t block, int p0, int p1, int64_t slot) {
-    w.v0 = (int)(block * W::rows) + wave * (32 * RB);
-    w.hold(a.es, w.v0);
-    const int t0 = 2 * p0, t1 = 2 * p1;
-    if (t0 < t1) {
-      fetch<kBytes>(s_x0, xs + t0 * kTile);
-      if constexpr (W::np == 1) w.rows(t0, w.lse, w.g, w.near);
-      arrive();
-      fetch<kBytes>(s_x1, xs + (t0 + 1) * kTile);
-      fetch_sum<W>(s_t1, xt + t0 * kTile, z);  // (times zeros)
-      w.logits(s_x0);
-      arrive();
-      for (int t = t0; t < t1; t += 2) {
-        const int t2 = min(t + 2, t1 - 1), t3 = min(t + 3, t1 - 1);  // behind the end: not used
-        fetch<kBytes>(s_x0, xs + t2 * kTile);
-        fetch_sum<W>(s_t0, xt + t * kTile, z);
-        w.next(s_x1, s_t1, t, t + 1);
+  auto share = [&](auto is_far) {  // (see kd_xent_rows)
+    constexpr bool FAR = decltype(is_far)::value;
+    TableWalk<T, DP, ROWG> w;
+    w.c2 = a.c2;
+    w.c2l = a.c2l;
+    w.unit = unit;
+    w.plse = a.lse;
+    w.pw = a.w;
+    w.pg = a.grow;
+    w.pf = !ROWG ? a.rl : FAR || sizeof(T) == 4 ? a.gfac : a.grow;
+    w.plab = a.lab;
+    deal.each(blockIdx.x, [&](int64_t block, int p0, int p1, int64_t slot) {
+      w.v0 = (int)(block * W::rows) + wave * (32 * RB);
+      w.hold(a.es, w.v0);
+      const int t0 = 2 * p0, t1 = 2 * p1;
+      if constexpr (FAR) {
+        for (int t = t0; t < t1; ++t) {
+          fetch<kBytes>(s_x0, xs + t * kTile);
+          fetch_sum<W>(s_t0, xt + t * kTile, z);
+          arrive();
+          w.far_tile(s_x0, s_t0, t);
+          __syncthreads();
+        }
+      } else if (t0 < t1) {
+        fetch<kBytes>(s_x0, xs + t0 * kTile);
+        if constexpr (W::np == 1) w.ahead(t0, w.lse, w.g, w.near);
+        w.fetch_rows(s_r0, t0);
         arrive();
-        fetch<kBytes>(s_x1, xs + t3 * kTile);
-        fetch_sum<W>(s_t1, xt + (t + 1) * kTile, z);
-        w.next(s_x0, s_t0, t + 1, t2);
+        fetch<kBytes>(s_x1, xs + (t0 + 1) * kTile);
+        fetch_sum<W>(s_t1, xt + t0 * kTile, z);  // (times zeros)
+        w.logits(s_x0);
         arrive();
+        for (int t = t0; t < t1; t += 2) {
+          const int t2 = min(t + 2, t1 - 1), t3 = min(t + 3, t1 - 1);  // behind the end: not used
+          fetch<kBytes>(s_x0, xs + t2 * kTile);
+          fetch_sum<W>(s_t0, xt + t * kTile, z);
+          w.fetch_rows(s_r1, t + 1);
+          w.next(s_x1, s_t1, s_r0, t, t + 1);
+          arrive();
+          fetch<kBytes>(s_x1, xs + t3 * kTile);
+          fetch_sum<W>(s_t1, xt + (t + 1) * kTile, z);
+          w.fetch_rows(s_r0, t2);
+          w.next(s_x0, s_t0, s_r1, t + 1, t2);
+          arrive();
+        }
+        w.add(s_t1);
       }
-      w.add(s_t1);
-    }
-    w.store(a.pe, slot * W::rows + wave * (32 * RB), z * (DP / W::cs));
-  });
+      w.store(a.pe, slot * W::rows + wave * (32 * RB), z * (DP / W::cs));
+    });
+  };
+  if (far)
+    share(std::true_type{});
+  else
+    share(std::false_type{});
 }
 
 // The gradient's common factor: the incoming scalar, over the count for the mean.
@@ -1689,11 +1871,14 @@ inline size_t lay_state(Args &a, int np, bool need_x, bool need_e, void *base) {
   Space s{(char *)base, 0};
   const size_t xe = (size_t)a.npad * a.dp * np, ee = (size_t)a.vpad * a.dp * np;
   a.count = s.take<int>(64);
+  a.far = s.take<int>(64);
   a.emax = s.take<uint32_t>(kSlots * kSlotPad);
+  a.xmax = s.take<uint32_t>(kSlots * kSlotPad);
   a.ticket = s.take<uint32_t>(64);
   a.rowid = s.take<int>(a.npad);
   a.lab = s.take<int>(a.npad);
   a.lse = s.take<float>(a.npad);
+  a.rl = s.take<float>(a.npad);
   a.w = s.take<float>(a.npad);
   a.xn = s.take<float>(a.npad);
   a.xs = s.take<uint16_t>(xe);
@@ -1723,6 +1908,7 @@ inline size_t lay_backward(Args &a, int np, bool need_e, void *base) {
   Space s{(char *)base, 0};
   a.gmax = s.take<uint32_t>((size_t)grad_blocks(a.npad) + 1);
   a.grow = s.take<float>(a.npad);
+  a.gfac = s.take<float>(a.npad);
   const size_t part = (size_t)deal_slots(a.vpad, np, a.dp, 2) * (size_t)walk_rows(np, a.dp, 2);
   a.pe = need_e ? s.take<float>(part * a.dp) : nullptr;
   return s.used;
@@ -1751,7 +1937,7 @@ void launch_few(const Args &a, const T *features, const T *table, const int64_t 
   const int wgs = std::min((a.V + 127) / 128, kFewWorkers);
   hipLaunchKernelGGL((kd_xent_few<T, DP>), dim3(wgs, (unsigned)((a.n + 31) / 32)), dim3(kBlock), 0,
                      stream, a, features, table, labels);
-  hipLaunchKernelGGL(kd_xent_few_join, dim3(1), dim3(1024), 0, stream, a, wgs, labels, loss);
+  hipLaunchKernelGGL(kd_xent_few_join<T>, dim3(1), dim3(1024), 0, stream, a, wgs, labels, loss);
 }
 
 template <typename T, int DP>
@@ -1875,7 +2061,7 @@ int backward(int64_t n, int64_t V, int D, const int64_t *labels, double scale, i
   if (ge && reduction == 0)
     hipLaunchKernelGGL(kd_xent_rowgrad,
                        dim3((unsigned)std::max(grad_blocks(a.npad), 1)),
-                       dim3(kBlock), 0, stream, a, grad);
+                       dim3(kBlock), 0, stream, a, sizeof(T) == 4, grad);
   switch (a.dp) {
     case 32: launch_backward<T, 32>(a, labels, grad, gx, ge, stream); break;
     case 64: launch_backward<T, 64>(a, labels, grad, gx, ge, stream); break;

@@ -70,3 +70,109 @@ def test_features_whose_squares_vanish(dname):
     got = _run(x, e, y, 1e22, 'none', grad)
     assert all(torch.isfinite(t).all() for t in got)
     _check(got, want)
+
+
+LARGE = [(dname, D, size) for dname in ('f32', 'f16', 'bf16') for D in (16, 64, 130, 256)
+         for size in (10.0, 300.0, 1e4, 1e9, 1e16) if dname != 'f16' or size < 1e4]
+
+
+@pytest.mark.parametrize('dname,D,size', LARGE)
+def test_large_logits_choose_one_row(dname, D, size):
+    """Logits of 1e3 to 1e33 in pixels whose largest logit is so far above the others that their
+    probabilities are below exp(-50), V of them below `rest`: the loss is the difference of two logits, the gradients are those of a
+    choice.  A logit is off by dz (see test_gpu_xent), a probability of 1 by its rounding and that of an
+    exponential near 0, 2^-21 in all, and the sums are of exact terms."""
+    from kaolin_amd.metrics.render import surface_cross_entropy
+    dt, scale = TYPES[dname], 0.75
+    g = torch.Generator().manual_seed(22)
+    n, V = 700, 150
+    x = (torch.randn(n, D, generator=g) * size).to(DEV, dt)
+    e = (torch.randn(V, D, generator=g) * size).to(DEV, dt)
+    y = torch.randint(0, V, (n,), generator=g).to(DEV)
+    grad = ((torch.rand(n, generator=g) + 0.25) / 1024).to(DEV)
+    z = scale * (x.double() @ e.double().t())
+    dz = ((6 if dname == 'f32' else 1) * D + 8) * 2.0 ** -24 * scale * (
+        x.double().abs() @ e.double().abs().t()).amax(1)
+    top, best = z.topk(2, 1)
+    clear = top[:, 0] - top[:, 1] > 2 * dz + 50
+    assert clear.sum() > 20
+    y = torch.where(clear, y, -1)
+    y[:40] = torch.where(clear[:40], best[:40, 0], -1)  # some of them right
+    u = torch.finfo(dt).eps / 2
+    ok = (y >= 0).double()
+    want = ok * (top[:, 0] - z[torch.arange(n, device=DEV), y.clamp(min=0)])
+    gs = grad.double() * scale * ok
+    hot = torch.zeros(n, V, dtype=torch.float64, device=DEV)
+    hot[torch.arange(n, device=DEV), best[:, 0]] += 1
+    hot[torch.arange(n, device=DEV), y.clamp(min=0)] -= 1
+    gx = gs[:, None] * (hot @ e.double())
+    ge = (hot * gs[:, None]).t() @ x.double()
+    up = u if dname != 'f32' else 2.0 ** -23
+    small = 2.0 ** -25 if dname == 'f16' else 1e-37
+    # what the other rows add: to the loss, and to a gradient times the largest element
+    rest = V * math.exp(-50)
+    tx = (up + 2.0 ** -21) * gs[:, None] * (hot.abs() @ e.double().abs()) + u * gx.abs() + small \
+        + rest * gs[:, None] * e.double().abs().max()
+    te = (up + (n + 32) * 2.0 ** -24) * (hot.abs() * gs[:, None]).t() @ x.double().abs() \
+        + u * ge.abs() + small + rest * gs.sum() * x.double().abs().max()
+    loss, dx, de = _run(x, e, y, scale, 'none', grad)
+    for out in (loss, surface_cross_entropy(x, e, y, scale, 'none')):
+        assert ((out.double() - want).abs() <= 2 * dz + 8 * 2.0 ** -24 * want + rest).all()
+    assert ((dx.double() - gx).abs() <= tx).all(), float(((dx.double() - gx).abs() - tx).max())
+    assert ((de.double() - ge).abs() <= te).all(), float(((de.double() - ge).abs() - te).max())
+    # the sum's gradients, whose kernels differ
+    one = torch.tensor(2.0 ** -10, device=DEV)
+    want_e = _run(x, e, y, scale, 'none', one.expand(n).contiguous())
+    got = _run(x, e, y, scale, 'sum', one)
+    terms = 2.0 ** -10 * scale * (hot.abs() * ok[:, None]).t() @ x.double().abs()
+    tol = 2 * (up + (n + 32) * 2.0 ** -24) * terms + 2 * u * want_e[2].double().abs() + small \
+        + rest * 2.0 ** -10 * n * x.double().abs().max()
+    assert ((got[2].double() - want_e[2].double()).abs() <= tol).all()
+
+
+@pytest.mark.parametrize('reduction', ['none', 'sum'])
+@pytest.mark.parametrize('size', [1.0, 6.0, 40.0, 300.0, 3000.0])
+@pytest.mark.parametrize('dname', ['f32', 'f16', 'bf16'])
+def test_probabilities_add_up_to_one(dname, size, reduction):
+    """With a feature that is 1 in every pixel the rows' gradients of that channel add up to
+    scale sum_i g_i (sum_v p_iv - 1) = 0, whatever the logits' size: both walks have to form the same
+    logits.  A probability p is off by its exponent's rounding, p (|log2 p| + 8) 2^-24, which is at
+    most 2^-20 for all of a pixel's together (p |log2 p| < 0.54, 200 rows), the sum's by
+    (V + 16) 2^-24, an operand's rounding by u_p; a row's sum by (n + 8) 2^-24 and u."""
+    dt, scale = TYPES[dname], 1.0
+    g = torch.Generator().manual_seed(23)
+    n, V, D = 900, 200, 48
+    x = (torch.randn(n, D, generator=g) * size).to(DEV, dt)
+    e = (torch.randn(V, D, generator=g) * size).to(DEV, dt)
+    x[:, 0] = 1
+    y = torch.randint(0, V, (n,), generator=g).to(DEV)
+    y[:300] = (x[:300].float() @ e.float().t()).argmax(1)
+    grad = (torch.rand(n, generator=g) + 0.25).to(DEV) if reduction == 'none' else \
+        torch.tensor(0.75, device=DEV)
+    _, _, de = _run(x, e, y, scale, reduction, grad)
+    gs = float(grad.double().expand(n).sum()) * scale
+    u = torch.finfo(dt).eps / 2
+    up = u if dname != 'f32' else 2.0 ** -22
+    col = de[:, 0].double()
+    # 16 bits: the offset of a walk of logits up to 2^10 is one number, 2^-15 of the probability
+    offset = 0.0 if dname == 'f32' else 2.0 ** -15
+    bound = 2 * gs * (2.0 ** -20 + (V + 16 + n + 8) * 2.0 ** -24 + up + offset) + u * float(col.abs().sum())
+    if dname == 'f16':
+        bound += V * 2.0 ** -25
+    assert abs(float(col.sum())) <= bound, (float(col.sum()), bound)
+    assert float(col.abs().max()) > 0
+
+
+@pytest.mark.parametrize('n', [10, 100])
+def test_all_logits_below_any_ordinary_number(n):
+    """Logits of -1e33 to -1e31: no maximum may begin above them."""
+    from kaolin_amd.metrics.render import surface_cross_entropy
+    g = torch.Generator().manual_seed(24)
+    x = torch.full((n, 16), 1e18, device=DEV)
+    e = -torch.rand(20, 16, generator=g).to(DEV) * 1e14
+    y = torch.randint(0, 20, (n,), generator=g).to(DEV)
+    z = x.double() @ e.double().t()
+    want = z.amax(1) - z[torch.arange(n, device=DEV), y]
+    dz = (6 * 16 + 8) * 2.0 ** -24 * z.abs().amax(1)
+    got = surface_cross_entropy(x, e, y, 1.0, 'none')
+    assert ((got.double() - want).abs() <= 2 * dz).all() and (got.double().amax() > 1e31)
