@@ -803,6 +803,24 @@ struct Step {
     products<false, true>(straight, straight, s, [](int) {});
   }
 
+  // Operands of three parts: an infinite element's second and third parts are NaN, and so are its
+  // logits.  The products of the first parts alone give the infinity (or NaN) that they are.
+  __device__ __forceinline__ void infinities(const uint4 *straight) {
+    if constexpr (NP == 3) {
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) odd |= !(fabsf(s[0][i]) < INFINITY);
+      if (!__any(odd)) return;
+      const int lane = threadIdx.x & 63;
+      f32x16 large = (f32x16)(0.f);
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        large = mfma(*(const H8 *)&straight[k * 64 + lane], held[0][k][0], large);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[0][i] = fabsf(s[0][i]) < INFINITY ? s[0][i] : large[i];
+    }
+  }
+
   __device__ __forceinline__ void add(const uint4 *transposed) {
     products<true, false>(transposed, transposed, s, [](int) {});
   }
@@ -957,6 +975,7 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
   // probabilities are scaled in the products stays out of the maximum, which may be too large for it.
   __device__ __forceinline__ void far_tile(const uint4 *s_e, const uint4 *s_t, int v0) {
     B::logits(s_e);
+    B::infinities(s_e);
     mask(v0);
     raise();
 #pragma unroll
@@ -1157,7 +1176,7 @@ __device__ __forceinline__ float pixel_loss(float m, float l, float z, bool far,
   const float t = expf(-fabsf(u)), more = log1pf(t);
   const bool others = u > 0.f;
   w = u != u ? u : (others ? 1.f : t) / (1.f + t);
-  base = others ? m : far ? z2 : mk;
+  base = u != u ? u : others ? m : far ? z2 : mk;  // (never infinite, as that of padding is)
   rest = fmaf(more, kLog2e, others ? part + fits : far ? 0.f : d);
   return u != u ? u : fmaxf(u, 0.f) + more;
 }
@@ -1363,7 +1382,11 @@ __global__ __launch_bounds__(kBlock) void kd_xent_few(Args a, const T *__restric
         s = product<NP>(kTimes - 1, ea, xb, s);
       }
     }
-    if constexpr (NP == 3) s += low;
+    if constexpr (NP == 3) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)  // (an infinite element's small products are NaN)
+        s[j] = fabsf(s[j]) < INFINITY ? s[j] + low[j] : s[j];
+    }
     if (v0 + 32 > a.V || __any((uint64_t)(y - v0) < 32u)) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -1649,6 +1672,7 @@ struct TableWalk : Step<T, DP, 2> {
     const int lane = threadIdx.x & 63;
     near = label(t);
     B::logits(s_x);
+    B::infinities(s_x);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int64_t r = (int64_t)t * 32 + 8 * i + 4 * (lane >> 5);

@@ -176,3 +176,53 @@ def test_all_logits_below_any_ordinary_number(n):
     dz = (6 * 16 + 8) * 2.0 ** -24 * z.abs().amax(1)
     got = surface_cross_entropy(x, e, y, 1.0, 'none')
     assert ((got.double() - want).abs() <= 2 * dz).all() and (got.double().amax() > 1e31)
+
+
+@pytest.mark.parametrize('n', [20, 300])
+@pytest.mark.parametrize('where', ['row', 'label', 'positive', 'pixel', 'all rows'])
+@pytest.mark.parametrize('dname', ['f32', 'f16', 'bf16'])
+def test_infinite_elements(dname, where, n):
+    """An infinite element of the table or of a pixel: losses and gradients are finite, infinite and NaN
+    where those of the formulas in 64 bits are (a row whose logits are all minus infinity takes no part),
+    and the finite ones are right: probabilities off by 2^-18 (logits below 2^4), rounded to u."""
+    from kaolin_amd.metrics.render import surface_cross_entropy
+    dt = TYPES[dname]
+    g = torch.Generator().manual_seed(25)
+    V, D, bad = 40, 24, 17
+    x = (torch.rand(n, D, generator=g) * 0.5 + 0.1).to(DEV, dt)
+    e = (torch.randn(V, D, generator=g) * 0.5).to(DEV, dt)
+    y = torch.randint(0, V - 1, (n,), generator=g).to(DEV)
+    y = torch.where(y >= bad, y + 1, y)  # no label is the bad row
+    if where in ('row', 'label', 'positive'):
+        e[bad, 3] = math.inf if where == 'positive' else -math.inf
+        if where == 'label':
+            y[5:8] = bad
+    else:
+        if where == 'all rows':
+            e[:, 3] = e[:, 3].abs() + 0.125
+        x[7, 3] = -math.inf
+    grad = (torch.rand(n, generator=g) + 0.25).to(DEV)
+    x64, e64 = x.double().requires_grad_(True), e.double().requires_grad_(True)
+    want = torch.nn.functional.cross_entropy(x64 @ e64.t(), y, reduction='none')
+    wx, we = torch.autograd.grad(want, [x64, e64], grad.double())
+    u = torch.finfo(dt).eps / 2
+    cap = lambda t: torch.where(torch.isfinite(t), t, torch.zeros_like(t)).abs().double()  # noqa: E731
+    gsum = grad.double().sum()
+    sizes = (2.0 ** -18 + 0 * want, (2 * u + 2.0 ** -18) * 2 * grad.double()[:, None] * cap(e).amax(0),
+             (2 * u + 2.0 ** -18) * 2 * gsum * cap(x).amax() + 0 * we)
+    loss, dx, de = _run(x, e, y, 1.0, 'none', grad)
+    if where == 'label':
+        # The walk leaves a label's own row out of the weighted sum as 0 times it, and 0 times infinity is
+        # NaN: where the label's row is infinite (and the loss too) an infinity of dX is NaN here.
+        assert not torch.isfinite(dx[5:8, 3]).any() and not torch.isfinite(wx[5:8, 3]).any()
+        dx[5:8, 3], wx[5:8, 3] = 0, 0
+    for got, ref, size in zip((loss, dx, de), (want.detach(), wx, we), sizes):
+        assert torch.equal(torch.isnan(got), torch.isnan(ref)), where
+        assert torch.equal(torch.isinf(got), torch.isinf(ref)), where
+        fin = torch.isfinite(ref)
+        assert ((got.double() - ref).abs()[fin] <= (size + 2 * u * ref.abs())[fin]).all()
+    few = surface_cross_entropy(x, e, y, 1.0, 'none')
+    assert torch.equal(torch.isnan(few), torch.isnan(want))
+    assert torch.equal(torch.isinf(few), torch.isinf(want))
+    fin = torch.isfinite(want)
+    assert ((few.double() - want).abs()[fin] <= 2.0 ** -18).all()
