@@ -13,9 +13,9 @@ logits are never stored.
 """
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from .. import _C
+from .._derivatives import first_only
 
 __all__ = ['mask_iou', 'surface_cross_entropy']
 
@@ -69,8 +69,11 @@ class SurfaceCrossEntropyHip(Function):
 
     @staticmethod
     def backward(ctx, grad_loss):
-        # (the guard against second derivatives costs time that a plain backward need not spend)
-        return _guarded_grad(ctx, grad_loss) if torch.is_grad_enabled() else _grad(ctx, grad_loss)
+        if not torch.is_grad_enabled():
+            return _grad(ctx, grad_loss)
+        with torch.no_grad():
+            grads = _grad(ctx, grad_loss)
+        return first_only('surface_cross_entropy', grads)
 
 
 def _grad(ctx, grad_loss):
@@ -81,9 +84,6 @@ def _grad(ctx, grad_loss):
         grad_loss, labels, ctx.shape, ctx.dtype, ctx.scale, ctx.reduction, state, *ctx.need,
         *ctx.needs_input_grad[:2])
     return gx, ge, None, None, None
-
-
-_guarded_grad = once_differentiable(_grad)
 
 
 def surface_cross_entropy(features, embeddings, labels, scale=1.0, reduction='mean'):
@@ -106,7 +106,7 @@ def surface_cross_entropy(features, embeddings, labels, scale=1.0, reduction='me
     Returns:
         (torch.Tensor): the loss, float32.  Gradients come in the inputs' type; logits, sums and
         the loss are held in 32 bits.  16-bit probabilities enter the gradients' products rounded
-        to the inputs' type.
+        to the inputs' type.  Second derivatives raise a RuntimeError.
     """
     if not torch.is_grad_enabled() or not (features.requires_grad or embeddings.requires_grad):
         return _C.metrics.surface_xent_forward(features, embeddings, labels, scale, reduction)[0]

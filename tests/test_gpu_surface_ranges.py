@@ -226,3 +226,27 @@ def test_infinite_elements(dname, where, n):
     assert torch.equal(torch.isinf(few), torch.isinf(want))
     fin = torch.isfinite(want)
     assert ((few.double() - want).abs()[fin] <= 2.0 ** -18).all()
+
+
+@pytest.mark.parametrize('which', ['features', 'embeddings', 'both'])
+def test_second_derivatives_raise(which):
+    """A gradient that enters a loss again raises, also where that loss has another term with a graph."""
+    from kaolin_amd.metrics.render import surface_cross_entropy
+    g = torch.Generator().manual_seed(26)
+    x, e = torch.randn(20, 8, generator=g).to(DEV), torch.randn(10, 8, generator=g).to(DEV)
+    y = torch.randint(0, 10, (20,), generator=g).to(DEV)
+    leaves = [t.requires_grad_(True) for t, w in ((x, 'features'), (e, 'embeddings'))
+              if which in (w, 'both')]
+    for weight in (1.0, torch.tensor(2.0, device=DEV, requires_grad=True)):
+        loss = surface_cross_entropy(x, e, y) * weight
+        grads = torch.autograd.grad(loss, leaves, create_graph=True)
+        plain = torch.autograd.grad(surface_cross_entropy(x, e, y) * weight, leaves)
+        assert all(torch.equal(a, b) for a, b in zip(grads, plain))
+        for a in grads:
+            with pytest.raises(RuntimeError, match='second derivatives'):
+                (loss + a.pow(2).sum()).backward(retain_graph=True)
+    # a recorded backward by itself is no error
+    x.grad = e.grad = None
+    surface_cross_entropy(x, e, y).backward(create_graph=True)
+    assert all(t.grad is not None for t in leaves)
+    x.grad = e.grad = None
