@@ -1,8 +1,16 @@
 """What an autograd function without second derivatives or a forward mode has to refuse."""
 import torch
 from torch.autograd import Function
+from torch.autograd.forward_ad import unpack_dual
 
-__all__ = ['first_only']
+__all__ = ['first_only', 'has_tangent']
+
+
+def has_tangent(*tensors):
+    """Whether one of them is dual (torch.autograd.forward_ad).  Such a tensor need not require a
+    gradient, and its data can be read like any other's: an operator that leaves autograd out would
+    give a result without a tangent."""
+    return any(unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _FirstOnly(Function):

@@ -15,7 +15,7 @@ import torch
 from torch.autograd import Function
 
 from .. import _C
-from .._derivatives import first_only
+from .._derivatives import first_only, has_tangent
 
 __all__ = ['mask_iou', 'surface_cross_entropy']
 
@@ -79,6 +79,8 @@ class SurfaceCrossEntropyHip(Function):
 def _grad(ctx, grad_loss):
     if grad_loss is None:
         return (None,) * 5
+    if has_tangent(grad_loss):
+        raise NotImplementedError('surface_cross_entropy: no forward mode')
     labels, state = ctx.saved_tensors
     gx, ge = _C.metrics.surface_xent_backward(
         grad_loss, labels, ctx.shape, ctx.dtype, ctx.scale, ctx.reduction, state, *ctx.need,
@@ -106,8 +108,10 @@ def surface_cross_entropy(features, embeddings, labels, scale=1.0, reduction='me
     Returns:
         (torch.Tensor): the loss, float32.  Gradients come in the inputs' type; logits, sums and
         the loss are held in 32 bits.  16-bit probabilities enter the gradients' products rounded
-        to the inputs' type.  Second derivatives raise a RuntimeError.
+        to the inputs' type.  Second derivatives raise a RuntimeError,
+        forward mode a NotImplementedError.
     """
-    if not torch.is_grad_enabled() or not (features.requires_grad or embeddings.requires_grad):
+    if not (torch.is_grad_enabled() and (features.requires_grad or embeddings.requires_grad)) \
+            and not has_tangent(features, embeddings):
         return _C.metrics.surface_xent_forward(features, embeddings, labels, scale, reduction)[0]
     return SurfaceCrossEntropyHip.apply(features, embeddings, labels, scale, reduction)

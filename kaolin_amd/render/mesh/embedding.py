@@ -11,6 +11,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from ... import _C
+from ..._derivatives import has_tangent
 
 __all__ = ['surface_embedding']
 
@@ -34,6 +35,8 @@ class SurfaceEmbeddingHip(Function):
 def _grad(ctx, grad_out):
     if grad_out is None:
         return None, None, None
+    if has_tangent(grad_out):
+        raise NotImplementedError('surface_embedding: no forward mode')
     index, = ctx.saved_tensors
     return None, _C.render.mesh.surface_embedding_backward(grad_out, index, ctx.plan), None
 
@@ -59,8 +62,9 @@ def surface_embedding(index, embeddings, scale=1.0):
 
     Returns:
         (torch.Tensor): (\*index.shape, num_channels), in embeddings' type; products are rounded
-        to it once, and the gradient's sums are held in 32 bits (64 for float64).
+        to it once, and the gradient's sums are held in 32 bits (64 for float64).  Forward mode
+        raises a NotImplementedError.
     """
-    if not torch.is_grad_enabled() or not embeddings.requires_grad:
+    if not (torch.is_grad_enabled() and embeddings.requires_grad) and not has_tangent(embeddings):
         return _C.render.mesh.surface_embedding_forward(index, embeddings, scale)[0]
     return SurfaceEmbeddingHip.apply(index, embeddings, scale)

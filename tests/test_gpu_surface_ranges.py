@@ -250,3 +250,30 @@ def test_second_derivatives_raise(which):
     surface_cross_entropy(x, e, y).backward(create_graph=True)
     assert all(t.grad is not None for t in leaves)
     x.grad = e.grad = None
+
+
+@pytest.mark.parametrize('grad_mode', [True, False])
+def test_tangents_raise(grad_mode):
+    """Forward mode is refused, not dropped: dual features, tables and incoming gradients."""
+    import torch.autograd.forward_ad as fw
+    from kaolin_amd.metrics.render import surface_cross_entropy
+    from kaolin_amd.render.mesh import surface_embedding
+    g = torch.Generator().manual_seed(27)
+    x, e = torch.randn(20, 8, generator=g).to(DEV), torch.randn(10, 8, generator=g).to(DEV)
+    y = torch.randint(0, 10, (20,), generator=g).to(DEV)
+    with fw.dual_level(), torch.set_grad_enabled(grad_mode):
+        dual = fw.make_dual
+        for call in (lambda: surface_cross_entropy(dual(x, x), e, y),
+                     lambda: surface_cross_entropy(x, dual(e, e), y),
+                     lambda: surface_embedding(y, dual(e, e))):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert torch.equal(surface_embedding(y, e), e[y])
+        if not grad_mode:
+            return
+        table = e.clone().requires_grad_(True)
+        weight = dual(torch.ones(20, 8, device=DEV), torch.ones(20, 8, device=DEV))
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(surface_embedding(y, table), table, weight)
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(surface_cross_entropy(x, table, y, 1.0, 'none'), table, weight[:, 0])

@@ -35,3 +35,15 @@ def test_none_stays_none():
     out = first_only('x', (None, a, None))
     assert out[0] is None and out[2] is None and torch.equal(out[1], a)
     assert first_only('x', (None, None)) == (None, None)
+
+
+def test_tangents_are_seen():
+    import torch.autograd.forward_ad as fw
+    from kaolin_amd._derivatives import has_tangent
+    a = torch.ones(3)
+    assert not has_tangent(a)
+    with fw.dual_level():
+        assert has_tangent(a, fw.make_dual(a, a))
+        assert not has_tangent(a)
+        with torch.no_grad():
+            assert has_tangent(fw.make_dual(a, a))
