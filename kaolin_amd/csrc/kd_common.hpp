@@ -470,6 +470,16 @@ __device__ __forceinline__ int wg_compact(bool pred, int *s_cnt, int &total) {
   return pred ? off + mbcnt(m) : -1;
 }
 
+// A launch of many workgroups is cut into rows of the grid: one dimension holds 2^32 threads.
+constexpr int64_t kGridRow = 1 << 20;
+inline dim3 grid_of(int64_t nblocks) {
+  const int64_t x = nblocks < kGridRow ? nblocks : kGridRow;
+  return dim3((unsigned)x, (unsigned)((nblocks + x - 1) / x));
+}
+__device__ __forceinline__ int64_t block_id() {
+  return (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+}
+
 // ------------------------------------------------------------------------------------------
 // coarse-bin geometry shared by host and device
 // ------------------------------------------------------------------------------------------

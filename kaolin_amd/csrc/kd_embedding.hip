@@ -48,7 +48,8 @@ __global__ __launch_bounds__(kBlock) void kd_embed_gather(
     T *__restrict__ out) {
   constexpr int V = 16 / sizeof(T);
   constexpr int U = 4;  // in flight per thread: the index, then the row, then the store
-  const int64_t r0 = (int64_t)blockIdx.x * rows_per_block;
+  const int64_t r0 = block_id() * rows_per_block;
+  if (r0 >= n) return;
   const uint32_t nrow = (uint32_t)min((int64_t)rows_per_block, n - r0);
   const uint32_t vpr = (uint32_t)(D + V - 1) / V, total = nrow * vpr;
   for (uint32_t v0 = threadIdx.x; v0 < total; v0 += U * kBlock) {
@@ -702,15 +703,15 @@ static int embed_forward(int64_t n, int64_t batch, int64_t rows, int D, const in
   using A = typename Wide<T>::type;
   constexpr int V = 16 / (int)sizeof(T);
   const int rpb = std::max(1, kBlock * 4 / ((D + V - 1) / V));
-  const unsigned grid = (unsigned)((n + rpb - 1) / rpb);
+  const dim3 grid = grid_of((n + rpb - 1) / rpb);
   const uint32_t pb = batch > 1 ? (uint32_t)(n / batch) : 0u;
   {
     ProfScope prof(K_EMBED_FWD, stream);
     if (D % V == 0 && (((uintptr_t)table | (uintptr_t)out) & 15u) == 0)
-      hipLaunchKernelGGL((kd_embed_gather<T, true>), dim3(grid), dim3(kBlock), 0, stream, n, pb, rows,
+      hipLaunchKernelGGL((kd_embed_gather<T, true>), grid, dim3(kBlock), 0, stream, n, pb, rows,
                          D, rpb, index, table, (A)scale, out);
     else
-      hipLaunchKernelGGL((kd_embed_gather<T, false>), dim3(grid), dim3(kBlock), 0, stream, n, pb,
+      hipLaunchKernelGGL((kd_embed_gather<T, false>), grid, dim3(kBlock), 0, stream, n, pb,
                          rows, D, rpb, index, table, (A)scale, out);
   }
   const hipError_t e = hipGetLastError();
