@@ -1881,8 +1881,14 @@ inline Args shape(int64_t n, int64_t V, int D, int np, double scale, int reducti
   return a;
 }
 
+// Few enough pixels, and no gradients: see kd_xent_few, which needs no state and a part a workgroup.
+inline bool few_pixels(const Args &a, bool need_x, bool need_e) {
+  return a.n > 0 && a.n <= kFewPixels && !need_x && !need_e;
+}
+
 inline size_t lay_state(Args &a, int np, bool need_x, bool need_e, void *base) {
   Space s{(char *)base, 0};
+  if (few_pixels(a, need_x, need_e)) return 1;
   const size_t xe = (size_t)a.npad * a.dp * np, ee = (size_t)a.vpad * a.dp * np;
   a.count = s.take<int>(64);
   a.far = s.take<int>(64);
@@ -1902,8 +1908,12 @@ inline size_t lay_state(Args &a, int np, bool need_x, bool need_e, void *base) {
   return s.used;
 }
 
-inline size_t lay_forward(Args &a, int np, bool need_x, void *base) {
+inline size_t lay_forward(Args &a, int np, bool need_x, bool need_e, void *base) {
   Space s{(char *)base, 0};
+  if (few_pixels(a, need_x, need_e)) {
+    for (float **p : {&a.pm, &a.pl, &a.pz}) *p = s.take<float>(kFewWorkers * kFewPixels);
+    return s.used;
+  }
   a.blk = s.take<int>((size_t)((a.n + kMapChunk - 1) / kMapChunk));
   a.et = need_x ? s.take<uint16_t>((size_t)a.vpad * a.dp * np) : nullptr;
   const int kind = need_x ? 1 : 0;
@@ -2007,14 +2017,14 @@ int forward(int64_t n, int64_t V, int D, const T *features, const T *table, cons
   KD_CHECK_ARG(table && (n == 0 || (features && labels)), "surface_cross_entropy: NULL input");
   Args a = shape(n, V, D, Form<T>::np, scale, reduction);
   const size_t ns = lay_state(a, Form<T>::np, need_x, need_e, state);
-  const size_t nw = lay_forward(a, Form<T>::np, need_x, scratch);
+  const size_t nw = lay_forward(a, Form<T>::np, need_x, need_e, scratch);
   if (!state || state_bytes < ns || !scratch || scratch_bytes < nw)
     return set_error(KD_ERR_WORKSPACE, "workspace too small: %zu < %zu or %zu < %zu", state_bytes,
                      ns, scratch_bytes, nw);
   KD_CHECK_ARG((((uintptr_t)state | (uintptr_t)scratch) & 255u) == 0,
                "surface_cross_entropy: state and scratch must be aligned to 256 bytes");
   ProfScope prof(K_XENT_FWD, stream);
-  if (n > 0 && n <= kFewPixels && !need_x && !need_e) {
+  if (few_pixels(a, need_x, need_e)) {
     switch (a.dp) {
       case 32: launch_few<T, 32>(a, features, table, labels, loss, stream); break;
       case 64: launch_few<T, 64>(a, features, table, labels, loss, stream); break;

@@ -24,7 +24,7 @@ size_t kd_surface_xent_scratch_size(int64_t n, int64_t rows, int channels, int e
   const int np = element_size == 4 ? 3 : 1;
   kd::xent::Args a = kd::xent::shape(n, rows, channels, np, 1.0, 0);
   return backward ? kd::xent::lay_backward(a, np, need_embeddings, nullptr)
-                  : kd::xent::lay_forward(a, np, need_features, nullptr);
+                  : kd::xent::lay_forward(a, np, need_features, need_embeddings, nullptr);
 }
 
 }  // extern "C"
