@@ -67,3 +67,47 @@ def test_choices_by_size(dname, kind, n, N, D):
     _check_out(out, ref)
     _check_grad(ge, rg, mag, cnt)
     assert torch.equal(ge, _run(index, table, 1.5, grad)[1])
+
+
+@pytest.mark.parametrize('dname', ['f32', 'f16', 'bf16'])
+def test_both_gradients_of_one_table(dname):
+    """A rendered image plus the lookup at its face_idx against the same table: the table's gradient is
+    the loss's and the lookup's, added.  From the pixels as they are (rounded), with the bounds of the
+    single operators: te and tx of the cross entropy (see test_gpu_xent), tx added up over a row's
+    pixels, a rounding u of each of the two gradients and of their sum, m 2^-24 for a sum of m terms."""
+    from test_gpu_xent import _reference as xent_reference
+    from kaolin_amd import workloads
+    from kaolin_amd.metrics.render import surface_cross_entropy
+    from kaolin_amd.render.mesh import dibr_rasterization, prepare_vertices, surface_embedding
+    dt, D, scale = TYPES[dname], 12, 2.0
+    s = workloads.sphere_views(20, 26, 64, 64, 2, DEV)
+    g = torch.Generator().manual_seed(14)
+    faces, F = s['faces'], s['faces'].shape[0]
+    vfeat = torch.randn(s['vertices'].shape[0], D, generator=g).to(DEV)
+    table = torch.randn(F, D, generator=g).to(DEV, dt).requires_grad_(True)
+    fvc, fvi, nrm = prepare_vertices(s['vertices'].unsqueeze(0), faces, s['proj'],
+                                     camera_transform=s['cam'])
+    feats = surface_embedding(faces, vfeat, 0.5).unsqueeze(0).expand(2, -1, -1, -1)
+    image, _, face_idx = dibr_rasterization(64, 64, fvc[..., 2], fvi, feats, nrm[..., 2])
+    rendered = surface_embedding(face_idx, table)
+    pixels = image.to(dt) + rendered
+    px = pixels.detach().requires_grad_(True)
+    weight = torch.tensor(64.0, device=DEV)  # (fp16 gradients well above its smallest numbers)
+    loss = surface_cross_entropy(pixels, table, face_idx, scale)
+    loss.backward(weight)
+    y = face_idx.reshape(-1)
+    want_loss, tl, gx, tx, ge, te = xent_reference(px.reshape(-1, D), table, y, scale, 'mean', weight)
+    hit = y >= 0
+    add = lambda t: torch.zeros(F, D, dtype=torch.float64, device=DEV).index_add_(  # noqa: E731
+        0, y[hit], t[hit].double())
+    u = torch.finfo(dt).eps / 2
+    m = torch.bincount(y[hit], minlength=F).double()[:, None]
+    look = add(gx)
+    tol = te + add(tx) + (m + 2) * 2.0 ** -24 * add(gx.abs()) + u * (look.abs() + add(tx)) \
+        + u * (ge + look).abs() * 1.02 + (2.0 ** -25 if dname == 'f16' else 0.0)
+    assert abs(float(loss.detach()) - float(want_loss)) <= float(tl)
+    got = table.grad.double()
+    assert ((got - ge - look).abs() <= tol).all(), float(((got - ge - look).abs() - tol).max())
+    # neither part, nor nothing, would pass
+    for part in (ge, look, ge + look):
+        assert (part.abs() > 4 * tol).float().mean() > 0.2
