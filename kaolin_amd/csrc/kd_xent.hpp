@@ -22,7 +22,10 @@
 // 16-bit data multiply exactly into 32-bit sums.  The probabilities enter their product with the
 // table (or the features) rounded to the data's type, at most 2^-8 (bf16) or 2^-11 (fp16, scaled so
 // that small ones stay normal) of each term, like the operands themselves (up to 32 channels in two
-// parts, see walk_parts); the sums L' use the unrounded values.  32-bit data are split into three
+// parts, see walk_parts); the sums L' use the unrounded values, the weights of dX's mean add up to 1
+// as they are rounded (see walk_norm).  What dE keeps of it: where thousands of pixels have the same
+// probabilities to 2^-9 (an untrained table, logits of 1e-3), a part that all features have in common is
+// off by up to 2^-9 of it.  32-bit data are split into three
 // bf16 parts (8 + 8 + 8 bits, the whole significand) and multiplied as the six products above 2^-24:
 // the fp32 matrix instructions run at 1/16 of the bf16 rate, six bf16 products at 1/6.
 // Losses are 32-bit numbers for every type, gradients of the data's type, rounded once.
@@ -80,6 +83,13 @@ __device__ __forceinline__ f32x16 mfma(bfloat8 a, bfloat8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
+__device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(bfloat8 a, bfloat8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
 // x as three bf16, each the nearest to what is left (exact: what the first two leave, at most 2^-18 x,
 // has 8 bits).  Parts by truncation would all have the sign of x, and so would the three small
 // products that are not formed: 4e-8 of every logit, a gradient of the table 8e-7 off where rounded
@@ -131,6 +141,7 @@ struct Args {
   int *blk;
   uint16_t *et;
   float *pm, *pl, *pz, *po;  // a part's maximum, sum, label's logit (or -inf), weighted sum
+  float *pq;                 // and the sum of the probabilities as they enter the weighted sum
   float *lrow;
   double *part;
   float *grow, *gfac, *pe;  // a pixel's incoming gradient, and times its factor
@@ -462,6 +473,15 @@ constexpr int walk_columns(int np, int dp, int kind) {
 // channels, where the exponentials take longer than the products, a second part carries what the first
 // left out.
 constexpr int walk_parts(int np, int dp) { return np == 3 ? 3 : (dp == 32 ? 2 : 1); }
+// The weighted sum's weights are the rounded probabilities over their own sum: over the sum of the
+// unrounded ones they would not add up to 1, and a direction that all likely rows have in common would be
+// off by 2^-9 of it, many times the differences that the gradient is made of (8 rows whose common part is
+// 30 times their spread: 1.7e-2 of the gradient in bf16, 1.8e-3 with this, where one rounding of the
+// result is 1.7e-3).  Two products of 16 x 16 x 32 a block and tile: 1.6 % of a call of 263,576 pixels x
+// 50,000 rows x 64 channels with both gradients.
+constexpr bool walk_norm(int np, int kind) {
+  return kind == 1 && np == 1;
+}
 constexpr int walk_rows(int np, int dp, int kind) { return 128 * walk_blocks(np, dp, kind); }
 // Workgroups: as many as run at once on 256 compute units.
 constexpr int walk_workers(int np, int dp, int kind) {
@@ -475,6 +495,7 @@ struct Walk {
   static constexpr int waves = walk_waves(np, DP, KIND);
   static constexpr int cs = walk_columns(np, DP, KIND);
   static constexpr int pp = walk_parts(np, DP);
+  static constexpr bool norm = walk_norm(np, KIND);
   static constexpr int rows = walk_rows(np, DP, KIND);  // held by a workgroup
   static constexpr int workers = walk_workers(np, DP, KIND);
   static constexpr int tile_bytes = np * 32 * DP * 2;  // a tile's operands: a multiple of 1024
@@ -611,6 +632,13 @@ struct Step {
   f32x16 s[RB];
   f32x16 o[SUM ? RB : 1][SUM ? DT : 1];
   uint4 q[RB][2][PP];
+  // The sums of q (see walk_norm), by the matrix pipe: the operand of a 32 x 32 x 16 product, 32 pixels in
+  // two halves of the lanes, taken as one of 16 x 16 x 32 has pixels c and c + 16 in the even and odd
+  // groups of 16 lanes.  Rows of ones and zeros keep them apart, and lane l gets pixel l % 32's sum.
+  // (finite values only: 0 times another pixel's NaN)
+  static constexpr bool NORM = W::norm;
+  f32x4 sum_q[NORM ? RB : 1];
+  H8 pick;
 
   __device__ __forceinline__ void hold(const uint16_t *packed, int64_t row0) {
     const int lane = threadIdx.x & 63;
@@ -631,6 +659,12 @@ struct Step {
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int p = 0; p < PP; ++p) q[b][h][p] = make_uint4(0, 0, 0, 0);
+      if constexpr (NORM) sum_q[b] = (f32x4)(0.f);
+    }
+    if constexpr (NORM) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        pick[j] = ((lane >> 2) & 1) == ((lane >> 4) & 1) ? (typename F::H)1.f : (typename F::H)0.f;
     }
   }
 
@@ -664,6 +698,15 @@ struct Step {
 #pragma unroll
     for (int n = 0; n < kOps; ++n) {
       if (n + kAhead < kOps) load(n + kAhead);
+      if constexpr (NORM) {
+        if (n < kAdd && n % DT == 0) {
+#pragma unroll
+          for (int b = 0; b < RB; ++b)
+#pragma unroll
+            for (int p = PP - 1; p >= 0; --p)
+              sum_q[b] = mfma16(pick, __builtin_bit_cast(H8, q[b][n / DT][p]), sum_q[b]);
+        }
+      }
 #pragma unroll
       for (int p = PP - 1; p >= 0; --p) {  // (the small part first)
         if (n >= kAdd && p > 0) continue;
@@ -889,6 +932,7 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
   static constexpr int RB = B::RB, DT = B::DT, PP = B::PP;
   int lab[RB];
   float m[RB], l[RB][2], t[RB][2], zy[RB];  // l + t: the sum of the probabilities in four terms
+  float far_q[RB];                          // a lane's part of the sum of q, of a walk of large logits
   int V;
   float c2, c2l;
 
@@ -936,6 +980,8 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
         l[b][1] *= f;
         t[b][0] *= f;
         t[b][1] *= f;
+        far_q[b] *= f;
+        if constexpr (B::NORM) this->sum_q[b] *= f;
         if constexpr (SUM) {
 #pragma unroll
           for (int d = 0; d < DT; ++d)
@@ -979,6 +1025,13 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
         if constexpr (SUM) {
           constexpr float f = F::shift == 0.f ? 1.f : 0x1p10f;
           pack_pair<T, PP>(p0 * f, p1 * f, i & 3, this->q[b][i >> 2]);
+          if constexpr (B::NORM) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float p = (k ? p1 : p0) * f, large = (float)(typename F::H)p;
+              far_q[b] += PP == 1 ? large : large + (float)(typename F::H)(p - large);
+            }
+          }
         }
       }
     fold();
@@ -1070,7 +1123,7 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
       for (int b = 0; b < RB; ++b) {
         w.lab[b] = a.lab[row0 + 32 * b + (lane & 31)];
         w.m[b] = general ? -FLT_MAX : 0.f;
-        w.l[b][0] = w.l[b][1] = w.t[b][0] = w.t[b][1] = 0.f;
+        w.l[b][0] = w.l[b][1] = w.t[b][0] = w.t[b][1] = w.far_q[b] = 0.f;
         w.zy[b] = -INFINITY;
       }
       const int t0 = 2 * p0, t1 = 2 * p1;
@@ -1125,7 +1178,13 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
         float l = w.l[b][0] + w.l[b][1];
         l += __shfl_xor(l, 32);
         const float other = __shfl_xor(w.zy[b], 32);  // one of the halves has met the label, or none
+        float q = 0.f;
+        if constexpr (W::norm) {
+          q = w.sum_q[b][0];
+          if constexpr (FAR) q = (w.far_q[b] + __shfl_xor(w.far_q[b], 32)) * (F::shift != 0.f ? 0x1p-10f : 1.f);
+        }
         if (half == 0 && z == 0) {
+          if constexpr (W::norm) a.pq[r] = q;
           a.pz[r] = w.zy[b] == -INFINITY ? other : w.zy[b];
           a.pm[r] = FAR ? w.m[b] : w.m[b] - F::shift;
           a.pl[r] = l;
@@ -1211,16 +1270,22 @@ __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__res
       z = part == -INFINITY ? z : part;
     }
   }
-  float l = 0.f;
+  float l = 0.f, lq = 0.f;  // (lq: see walk_norm)
 #pragma unroll 4
   for (int s = s0; s < n; s += ds) {
     const int64_t q = first + (int64_t)s * W::rows;
-    l += a.pl[q] * __builtin_amdgcn_exp2f(a.pm[q] - m);
+    const float f = __builtin_amdgcn_exp2f(a.pm[q] - m);
+    l += a.pl[q] * f;
+    if constexpr (W::norm) lq += a.pq[q] * f;
   }
   if (!few) {
 #pragma unroll
-    for (int s = G / 2; s >= 1; s >>= 1) l += __shfl_xor(l, s);
+    for (int s = G / 2; s >= 1; s >>= 1) {
+      l += __shfl_xor(l, s);
+      if constexpr (W::norm) lq += __shfl_xor(lq, s);
+    }
   }
+  if constexpr (!W::norm) lq = l;
   float wn, base, rest;
   const bool far = *a.far;
   const float out = pixel_loss(m, l, z, far, a, wn, base, rest);
@@ -1243,7 +1308,7 @@ __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__res
   }
   if constexpr (RAW) {
     if (left <= 0) return;
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    const float inv = lq > 0.f ? 1.f / lq : (lq == 0.f ? 0.f : lq);
     if (n > 1) {
 #pragma unroll 4
       for (int s = 0; s < n; ++s) {
@@ -1922,6 +1987,7 @@ inline size_t lay_forward(Args &a, int np, bool need_x, bool need_e, void *base)
   a.pm = s.take<float>(part);
   a.pl = s.take<float>(part);
   a.pz = s.take<float>(part);
+  a.pq = walk_norm(np, kind) ? s.take<float>(part) : nullptr;
   a.po = need_x ? s.take<float>(part * a.dp) : nullptr;
   a.lrow = s.take<float>(a.npad);
   a.part = s.take<double>(kReduceBlocks);

@@ -277,3 +277,38 @@ def test_tangents_raise(grad_mode):
             torch.autograd.grad(surface_embedding(y, table), table, weight)
         with pytest.raises(NotImplementedError):
             torch.autograd.grad(surface_cross_entropy(x, table, y, 1.0, 'none'), table, weight[:, 0])
+
+
+@pytest.mark.parametrize('D', [20, 64, 100, 256])
+@pytest.mark.parametrize('V', [8, 300])
+@pytest.mark.parametrize('size', [0.3, 300.0])
+@pytest.mark.parametrize('dname', ['f32', 'f16', 'bf16'])
+def test_rows_that_are_alike(dname, size, V, D):
+    """Rows with a common part of 30 times their differences (a smooth table: neighbouring faces): dX is
+    made of the differences, so the weights of the rows have to add up to 1.  With probabilities off by
+    rho = 2 du + u_p, the weighted mean of e_v - e_y is off by 2 rho times that of |e_v - e_y|, and the
+    sums of whole rows in 32 bits by (V / 8 + 32) 2^-24 of the largest element."""
+    dt = TYPES[dname]
+    g = torch.Generator().manual_seed(28)
+    n = 500
+    x = (torch.randn(n, D, generator=g) * size / 3 / D ** 0.5).to(DEV, dt)
+    e = ((torch.randn(V, D, generator=g) * 0.1 + 3 * torch.randn(1, D, generator=g))).to(DEV, dt)
+    y = torch.randint(0, V, (n,), generator=g).to(DEV)
+    grad = (torch.rand(n, generator=g) + 0.25).to(DEV)
+    x64, e64 = x.double().requires_grad_(True), e.double()
+    want = torch.nn.functional.cross_entropy(x64 @ e64.t(), y, reduction='none')
+    gx, = torch.autograd.grad(want, x64, grad.double())
+    p = torch.softmax(x64.detach() @ e64.t(), 1)
+    apart = torch.stack([(p[i, :, None] * (e64 - e64[y[i]]).abs()).sum(0) for i in range(n)])
+    dz = ((6 if dname == 'f32' else 1) * D + 8) * 2.0 ** -24 * (
+        x.double().abs() @ e64.abs().t()).amax(1)
+    u = torch.finfo(dt).eps / 2
+    rho = 2 * (3 * dz + (V + 16) * 2.0 ** -24) + (u if dname != 'f32' else 2.0 ** -23)
+    if dname != 'f32':
+        rho = rho + 2.0 ** -35 * V  # (fp16: terms below its normal range; small beside u in bf16)
+    tol = grad.double()[:, None] * (2 * rho[:, None] * apart
+                                    + (V / 8 + 32) * 2.0 ** -24 * e64.abs().max()) + u * gx.abs() * 1.01
+    if dname == 'f16':
+        tol = tol + 2.0 ** -25
+    got = _run(x, e, y, 1.0, 'none', grad)[1]
+    assert ((got.double() - gx).abs() <= tol).all(), float(((got.double() - gx).abs() / tol).max())
