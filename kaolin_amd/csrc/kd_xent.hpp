@@ -386,16 +386,16 @@ __device__ __forceinline__ float exponent(float s, float c2, float c2l, float of
 // walks of their own, tile by tile, in which a term's log2 is the logit times the factor, rounded, the
 // same number in both walks.  In the others that product is not rounded: an offset of its size is off by
 // half a step of it, which an exponential turns into 2^-25 of the logit, relative.  In 16 bits, whose
-// other walks hold the offset log2 of the sum in one number, that is 2^-15 here, an eighth of a step of
-// fp16; without a limit fp16 and bf16 gradients were 0.8 % off at logits of 8e4, 32-bit ones too, all of
-// them wrong at 1e7 and not finite at 1e9.  With 32-bit data the offset is two numbers, a whole one
-// (exact up to 2^24) and a factor of the exponential.
+// other walks hold the offset log2 of the sum in one number, that is 2^-15 here for fp16 and 2^-13 for
+// bf16, a sixteenth of half a step each; without a limit all types' gradients were 0.8 % off at logits of
+// 8e4, wrong at 1e7 and not finite at 1e9.  With 32-bit data the offset is two numbers, a whole one (exact
+// up to 2^24) and a factor of the exponential.
 // Measured (loss; loss and both gradients), bounded / with the running maximum / large logits: bf16, 64
 // channels, 263,576 pixels x 50,000 rows 2.4 / 2.7 / 3.4 ms; 7.2 / 7.8 / 10.2 ms; 256 channels, 131,788 x
 // 10,000 0.63 / 0.67 / 0.71; 3.2 / 3.4 / 4.7; fp16, 64 channels, 131,072 x 10,000 0.41 / 0.39 / 0.47; 0.91 /
 // 0.91 / 1.28; fp32, 64 channels, 131,712 x 10,000 0.86 / 0.87 / 0.90; 3.56 / 3.65 / 3.55.
 template <typename T>
-constexpr float kFar = sizeof(T) == 4 ? 0x1p22f : 0x1p10f;
+constexpr float kFar = std::is_same_v<T, float> ? 0x1p22f : std::is_same_v<T, half_t> ? 0x1p10f : 0x1p12f;
 
 // the largest of a kind of sizes, squared (NaN if there is one: its bits are above infinity's)
 __device__ __forceinline__ float largest(const uint32_t *slots) {

@@ -154,8 +154,8 @@ def test_probabilities_add_up_to_one(dname, size, reduction):
     u = torch.finfo(dt).eps / 2
     up = u if dname != 'f32' else 2.0 ** -22
     col = de[:, 0].double()
-    # 16 bits: the offset of a walk of logits up to 2^10 is one number, 2^-15 of the probability
-    offset = 0.0 if dname == 'f32' else 2.0 ** -15
+    # 16 bits: the offset of a walk of logits up to 2^10 (fp16) or 2^12 is one number, off by 2^-25 of it
+    offset = {'f32': 0.0, 'f16': 2.0 ** -15, 'bf16': 2.0 ** -13}[dname]
     bound = 2 * gs * (2.0 ** -20 + (V + 16 + n + 8) * 2.0 ** -24 + up + offset) + u * float(col.abs().sum())
     if dname == 'f16':
         bound += V * 2.0 ** -25
