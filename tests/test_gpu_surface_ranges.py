@@ -312,3 +312,51 @@ def test_rows_that_are_alike(dname, size, V, D):
         tol = tol + 2.0 ** -25
     got = _run(x, e, y, 1.0, 'none', grad)[1]
     assert ((got.double() - gx).abs() <= tol).all(), float(((got.double() - gx).abs() / tol).max())
+
+
+@pytest.mark.parametrize('dname', ['f32', 'f16', 'bf16'])
+def test_a_captured_step_follows_its_inputs(dname):
+    """The walk is chosen on the device: a captured step replayed on bounded, unbounded, large and
+    infinite logits in turn, with eager work between, gives what an eager call gives."""
+    dt = TYPES[dname]
+    g = torch.Generator().manual_seed(29)
+    n, V, D = 700, 90, 40
+    base_x, base_e = torch.randn(n, D, generator=g).to(DEV), torch.randn(V, D, generator=g).to(DEV)
+    y = torch.randint(-1, V, (n,), generator=g).to(DEV)
+    grad = (torch.rand(n, generator=g) + 0.25).to(DEV)
+    x, e = base_x.to(dt), base_e.to(dt)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        _run(x, e, y, 0.5, 'none', grad)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = _run(x, e, y, 0.5, 'none', grad)
+    for size in (1.0, 200.0, 0.1, 20.0, math.inf, 1.0, 200.0):
+        x.copy_(base_x * (size if math.isfinite(size) else 1.0))
+        e.copy_(base_e * (size if math.isfinite(size) else 1.0))
+        if not math.isfinite(size):
+            e[V - 1, 0] = -math.inf
+        for o in outs:
+            o.fill_(7.0)
+        graph.replay()
+        eager = _run(x, e, y, 0.5, 'none', grad)
+        for a, b in zip(outs, eager):
+            assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(
+                torch.nan_to_num(a), torch.nan_to_num(b)), size
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize('size', [1.0, 1e3])
+@pytest.mark.parametrize('dname', ['f32', 'f16', 'bf16'])
+def test_a_table_of_one_row(dname, size):
+    """Nothing to choose: no loss and no gradient, whatever the logit."""
+    from kaolin_amd.metrics.render import surface_cross_entropy
+    g = torch.Generator().manual_seed(30)
+    x = (torch.randn(90, 33, generator=g) * size).to(DEV, TYPES[dname])
+    e = (torch.randn(1, 33, generator=g) * size).to(DEV, TYPES[dname])
+    y = torch.randint(-1, 2, (90,), generator=g).to(DEV)
+    for out in (*_run(x, e, y, 2.0, 'none', torch.ones(90, device=DEV)),
+                surface_cross_entropy(x[:50], e, y[:50], 2.0, 'none')):
+        assert (out == 0).all()
