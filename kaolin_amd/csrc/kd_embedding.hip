@@ -39,8 +39,9 @@ constexpr int kMaxChannels = 1 << 20;
 // ------------------------------------------------------------------------------------------------
 // WHOLE: rows are whole 16-byte vectors, 16-byte aligned.  The output is written past the caches: it
 // is larger than they are where its time counts, and the table's rows are what they should hold.  Bound
-// by the bytes written: 2,097,152 tokens of 64 channels in bf16 (268 MB out, 17 MB of indices) 47 us,
-// 6 TB/s; 8,388,608 of 32 channels in fp16 135 us, 4.5 TB/s.
+// by the bytes written: 2,097,152 tokens of 64 channels in bf16 (268 MB out, 17 MB of indices) 51 us,
+// 5.6 TB/s; 8,388,608 of 32 channels in fp16 136 us, 4.4 TB/s (averages of six calls, as all times of one
+// kernel here).
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kBlock) void kd_embed_gather(
     int64_t n, uint32_t per_batch, int64_t rows, int D, int rows_per_block,
@@ -234,8 +235,8 @@ __device__ __forceinline__ void embed_rank(const uint2 (&kt)[ITERS], uint32_t in
 }
 
 // Bound by latency and the scattered 8-byte writes: of 8,388,608 tokens the 4,217,024 that name one of
-// 50,000 rows are written in 45 us, and in the second pass in 27 us, behind 16 us of counting; of
-// 2,097,152 in 14 and 12 us behind 8.
+// 50,000 rows are written in 47 us, and in the second pass in 28 us, behind 17 us of counting; of
+// 2,097,152 in 15 and 12 us behind 8.5.
 // few: each workgroup adds up all tiles' counts itself, 16 bytes a thread and a share of the tiles: both
 // passes of 262,144 tokens take 30 us in four launches against 26 in six, a call whose launches are its
 // time 104 us against 109.
@@ -397,7 +398,7 @@ __global__ __launch_bounds__(kOneThreads) void kd_embed_sort(SortKeys s, int bit
 // sums over the runs of equal keys
 // ------------------------------------------------------------------------------------------------
 // Bound by the gathered gradient rows, which are as long as a memory access or shorter: 1,054,304 rows
-// of 128 bytes 47 us, 3 TB/s; 4,217,024 rows of 64 bytes 122 us, 2.5 TB/s.
+// of 128 bytes 50 us, 2.9 TB/s; 4,217,024 rows of 64 bytes 124 us, 2.5 TB/s.
 constexpr int kHasHead = 1;   // the first run began before this range
 constexpr int kHasTail = 2;   // the last run goes on behind this range
 constexpr int kThrough = 4;   // one run covers the range and both borders (its sum is the head's)

@@ -21,12 +21,11 @@
 //
 // 16-bit data multiply exactly into 32-bit sums.  The probabilities enter their product with the
 // table (or the features) rounded to the data's type, at most 2^-8 (bf16) or 2^-11 (fp16, scaled so
-// that small ones stay normal) of each term, like the operands themselves (up to 32 channels in two
-// parts, see walk_parts); the sums L' use the unrounded values, the weights of dX's mean add up to 1
-// as they are rounded (see walk_norm).  What dE keeps of it: where thousands of pixels have the same
-// probabilities to 2^-9 (an untrained table, logits of 1e-3), a part that all features have in common is
-// off by up to 2^-9 of it.  32-bit data are split into three
-// bf16 parts (8 + 8 + 8 bits, the whole significand) and multiplied as the six products above 2^-24:
+// that small ones stay normal) of each term, like the operands themselves (up to 32 channels and
+// for few rows in two parts, see walk_parts); the sums L' use the unrounded values, the weights of dX's mean add up to 1
+// as they are rounded (see walk_norm).  What dE keeps of it, with more rows than kFewRows: where
+// thousands of pixels have the same probabilities to 2^-9 (an untrained table, logits of 1e-3), a part that
+// all features have in common is off by up to 2^-9 of it.  32-bit data are split into three bf16 parts (8 + 8 + 8 bits, the whole significand) and multiplied as the six products above 2^-24:
 // the fp32 matrix instructions run at 1/16 of the bf16 rate, six bf16 products at 1/6.
 // Losses are 32-bit numbers for every type, gradients of the data's type, rounded once.
 #pragma once
@@ -208,7 +207,8 @@ static __global__ __launch_bounds__(kBlock) void kd_xent_scan(int nblk, int *__r
 }
 
 // The pixels without a label cost a walk as much as the others, so the walks take a list (in order) of
-// those with one; counts and list read the labels twice: 2,097,152 in 6.5 and 7.5 us, 2.4 TB/s.
+// those with one; counts and list read the labels twice: 2,097,152 in 6.9 and 7.7 us, 2.4 TB/s
+// (averages of six calls, as all times of one kernel here).
 // Lists the pixels of `chunks` chunks a workgroup: blk holds the chunks' counts, or their offsets
 // (scanned), or is not needed (one workgroup lists all).  Losses of pixels without a label are 0.
 static __global__ __launch_bounds__(kBlock) void kd_xent_map(Args a, int chunks, bool scanned,
@@ -261,7 +261,7 @@ static __global__ __launch_bounds__(kBlock) void kd_xent_map(Args a, int chunks,
 // ------------------------------------------------------------------------------------------------
 // A tile of 32 rows goes through LDS, 16 bytes a lane in and out.  Once per call, so that the walks,
 // which read every tile hundreds of times, copy it as it is.  Bound by bytes: 1,054,304 pixels and 50,000
-// rows of 128 channels in bf16 121 us, 4.7 TB/s.
+// rows of 128 channels in bf16 125 us, 4.5 TB/s.
 template <typename T, int DP>
 __global__ __launch_bounds__(kBlock) void kd_xent_pack(Args a, int xtiles,
                                                        const T *__restrict__ features,
@@ -391,9 +391,9 @@ __device__ __forceinline__ float exponent(float s, float c2, float c2l, float of
 // 8e4, wrong at 1e7 and not finite at 1e9.  With 32-bit data the offset is two numbers, a whole one (exact
 // up to 2^24) and a factor of the exponential.
 // Measured (loss; loss and both gradients), bounded / with the running maximum / large logits: bf16, 64
-// channels, 263,576 pixels x 50,000 rows 2.4 / 2.7 / 3.4 ms; 7.2 / 7.8 / 10.2 ms; 256 channels, 131,788 x
-// 10,000 0.63 / 0.67 / 0.71; 3.2 / 3.4 / 4.7; fp16, 64 channels, 131,072 x 10,000 0.41 / 0.39 / 0.47; 0.91 /
-// 0.91 / 1.28; fp32, 64 channels, 131,712 x 10,000 0.86 / 0.87 / 0.90; 3.56 / 3.65 / 3.55.
+// channels, 263,576 pixels x 50,000 rows 2.4 / 2.7 / 3.4 ms; 7.1 / 7.7 / 11.3 ms; 256 channels, 131,788 x
+// 10,000 0.65 / 0.68 / 0.72; 3.2 / 3.4 / 4.8; fp16, 64 channels, 131,072 x 10,000 0.40 / 0.40 / 0.47; 0.95 /
+// 0.92 / 1.42; fp32, 64 channels, 131,712 x 10,000 0.87 / 0.89 / 0.97; 3.52 / 3.65 / 3.54.
 template <typename T>
 constexpr float kFar = std::is_same_v<T, float> ? 0x1p22f : std::is_same_v<T, half_t> ? 0x1p10f : 0x1p12f;
 
@@ -446,7 +446,7 @@ __device__ __forceinline__ void pack_pair(float p0, float p1, int i, uint4 *o) {
 }
 
 // How a walk is laid out (KIND 0: over the table, loss only; 1: over the table with dX; 2: over the
-// pixels, dE), for np planes and dp channels.
+// pixels, dE; 3: the same for few rows, see walk_parts), for np planes and dp channels.
 // Blocks of 32 rows that a wave holds.  Every operand read from LDS feeds one product per block; with
 // one block a product, 32 clocks on each of four SIMDs, takes all that LDS delivers (4 x 1 KiB), so
 // 16-bit data take two where two waves a SIMD have the registers: losses at 256 channels of 527,000
@@ -454,7 +454,7 @@ __device__ __forceinline__ void pack_pair(float p0, float p1, int i, uint4 *o) {
 // channels, where two blocks leave one wave a SIMD: dE of 527,000 pixels 2.98 -> 2.87 ms, but of 33,000
 // pixels and 2,000 rows 55 -> 65 us, dX of 132,000 0.64 -> 0.69 ms.
 constexpr int walk_blocks(int np, int dp, int kind) {
-  return np == 1 && (dp <= 64 || kind == 0) ? 2 : 1;
+  return np == 1 && kind != 3 && (dp <= 64 || kind == 0) ? 2 : 1;
 }
 // Waves per SIMD: one where the held operands, the sums and the blocks of logits need more than 256
 // registers.
@@ -472,7 +472,15 @@ constexpr int walk_columns(int np, int dp, int kind) {
 // had gradients 2e-3 to 4e-3 off in bf16, where one rounding of the result is 1.7e-3.  Up to 32
 // channels, where the exponentials take longer than the products, a second part carries what the first
 // left out.
-constexpr int walk_parts(int np, int dp) { return np == 3 ? 3 : (dp == 32 ? 2 : 1); }
+// Tables of few rows too, for dE: an error that is the same for many pixels stays whole there, as each row
+// has many of them (100,000 pixels that are alike, 8 rows, bf16: 7.7e-2 of the gradient, 1.6e-3 in two
+// parts), and the time of such a call is in the pixels' bytes: 500,000 pixels of 64 channels, both
+// gradients, 10 rows 349 -> 341 us, 100 rows 373 -> 371, but 300 rows 444 -> 485 and 1,000 662 -> 804.
+constexpr int kFewRows = 256;
+constexpr int walk_parts(int np, int dp, int kind) {
+  return np == 3 ? 3 : (dp == 32 || kind == 3 ? 2 : 1);
+}
+constexpr int walk_table(int np, int dp, int V) { return np == 1 && dp > 32 && V <= kFewRows ? 3 : 2; }
 // The weighted sum's weights are the rounded probabilities over their own sum: over the sum of the
 // unrounded ones they would not add up to 1, and a direction that all likely rows have in common would be
 // off by 2^-9 of it, many times the differences that the gradient is made of (8 rows whose common part is
@@ -494,7 +502,7 @@ struct Walk {
   static constexpr int rb = walk_blocks(np, DP, KIND);
   static constexpr int waves = walk_waves(np, DP, KIND);
   static constexpr int cs = walk_columns(np, DP, KIND);
-  static constexpr int pp = walk_parts(np, DP);
+  static constexpr int pp = walk_parts(np, DP, KIND);
   static constexpr bool norm = walk_norm(np, KIND);
   static constexpr int rows = walk_rows(np, DP, KIND);  // held by a workgroup
   static constexpr int workers = walk_workers(np, DP, KIND);
@@ -813,7 +821,7 @@ struct Step {
         }
 #pragma unroll
         for (int i = 0; i < 5; ++i) {
-          next = product<3, KIND == 2>(i, x, y, next);
+          next = product<3, (KIND >= 2)>(i, x, y, next);
           slot();
         }
       } else {
@@ -1077,11 +1085,11 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
 };
 
 // Bound by the matrix pipe, with the exponentials (16 a lane and 32 x 32 logits, 8 clocks each) partly
-// beside it.  Measured: 64 channels, bf16, 263,576 pixels x 50,000 rows with dX: 3.4 ms, 1.0 PFLOP/s;
-// 128 channels, losses of 1,054,304 pixels: 12.3 ms, 1.1 PFLOP/s (a bf16 library product of 8192^3
-// reaches 1.17); 256 channels, 131,788 x 10,000 with dX: 1.5 ms, 0.92 PFLOP/s, where one block of
-// rows a wave waits for LDS; fp32, 64 channels, 131,712 x 10,000: 1.7 ms, 0.20 PFLOP/s counted once,
-// 1.2 of bf16 products (a fp32 library product reaches 0.13).
+// beside it.  Measured: 64 channels, bf16, 263,576 pixels x 50,000 rows with dX: 3.74 ms, 0.90 PFLOP/s;
+// 128 channels, losses of 1,054,304 pixels: 12.4 ms, 1.09 PFLOP/s (a bf16 library product of 8192^3
+// reaches 1.17); 256 channels, 131,788 x 10,000 with dX: 1.60 ms, 0.85 PFLOP/s, where one block of
+// rows a wave waits for LDS; fp32, 64 channels, 131,712 x 10,000: 1.79 ms, 0.19 PFLOP/s counted once,
+// 1.1 of bf16 products (a fp32 library product reaches 0.13).
 template <typename T, int DP, bool SUM>
 __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_xent_rows(Args a) {
   using F = Form<T>;
@@ -1203,7 +1211,7 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_
 // joining the parts: G lanes per listed pixel; with RAW, four channels of dX a lane
 // ------------------------------------------------------------------------------------------------
 // Bound by the bytes of the parts' sums (32 bits) and of dX before its gradient: 131,788 pixels of 256
-// channels 94 us, 2.9 TB/s, in the time of 3 ms.
+// channels 100 us, 2.7 TB/s, in the time of 3 ms.
 constexpr int kFewParts = 16;
 
 // A pixel's loss softplus(L' - z_y) from the maximum (log2) and the sum over the rows but its label's
@@ -1330,7 +1338,7 @@ __global__ __launch_bounds__(kBlock) void kd_xent_combine(Args a, const T *__res
 // stands, straight into the products' operands, and nothing is listed, packed or kept.  Each wave
 // takes tiles of 32 table rows in turn; the workgroup's parts are joined in LDS, all of them by a
 // second launch of one workgroup.  Bound by the table's bytes: one pixel, 200,000 rows of 256
-// channels in bf16 28.5 us, 3.6 TB/s, and 7 us for the join.
+// channels in bf16 29.4 us, 3.5 TB/s, and 8 us for the join.
 constexpr int kFewPixels = 64, kFewWorkers = 512;
 
 // 8 channels of a row
@@ -1634,14 +1642,14 @@ __device__ __forceinline__ float grad_unit(const Args &a) {
 
 // The walk over the pixels: kd_xent_rows with the sides exchanged, the logits formed a second time
 // (2 n V D more operations; kept, they would be n V values written and read, 26 GB at the sizes below
-// in 16 bits, 10 ms).  Bound as there.  Measured: 64 channels, bf16, 263,576 pixels x 50,000 rows 3.2 ms,
-// 1.04 PFLOP/s; 256 channels, 131,788 x 10,000 1.7 ms, 0.79 PFLOP/s; fp32, 64 channels, 131,712 x
-// 10,000 1.84 ms.
-// A lane's 16 pixels of a tile are 8 i + 4 (lane / 32) + j: their exponents
-// (and gradients) are read one step ahead.
-template <typename T, int DP, bool ROWG>
-struct TableWalk : Step<T, DP, 2> {
-  using B = Step<T, DP, 2>;
+// in 16 bits, 10 ms).  Bound as there.  Measured: 64 channels, bf16, 263,576 pixels x 50,000 rows 3.38 ms,
+// 1.00 PFLOP/s; 256 channels, 131,788 x 10,000 1.78 ms, 0.76 PFLOP/s; fp32, 64 channels, 131,712 x
+// 10,000 1.89 ms.
+// A lane's 16 pixels of a tile are 8 i + 4 (lane / 32) + j: their exponents (and factors) are read one step
+// ahead, of 32-bit data by way of LDS and a pair at a time (held in registers they cost 6 to 11 %).
+template <typename T, int DP, bool ROWG, int KIND>
+struct TableWalk : Step<T, DP, KIND> {
+  using B = Step<T, DP, KIND>;
   using F = Form<T>;
   static constexpr int NP = B::NP, RB = B::RB, PP = B::PP;
   static constexpr bool FAC = ROWG || sizeof(T) == 4;  // exponentials have a factor
@@ -1783,9 +1791,9 @@ struct TableWalk : Step<T, DP, 2> {
   }
 };
 
-template <typename T, int DP, bool ROWG>
-__global__ __launch_bounds__(kBlock, (Walk<T, DP, 2>::waves)) void kd_xent_table(Args a) {
-  using W = Walk<T, DP, 2>;
+template <typename T, int DP, bool ROWG, int KIND>
+__global__ __launch_bounds__(kBlock, (Walk<T, DP, KIND>::waves)) void kd_xent_table(Args a) {
+  using W = Walk<T, DP, KIND>;
   constexpr int RB = W::rb, kBytes = W::tile_bytes;
   __shared__ uint4 s_x0[kBytes / 16], s_x1[kBytes / 16];
   __shared__ uint4 s_t0[W::sum_bytes / 16], s_t1[W::sum_bytes / 16];
@@ -1800,7 +1808,7 @@ __global__ __launch_bounds__(kBlock, (Walk<T, DP, 2>::waves)) void kd_xent_table
   constexpr int64_t kTile = kBytes / 2;
   auto share = [&](auto is_far) {  // (see kd_xent_rows)
     constexpr bool FAR = decltype(is_far)::value;
-    TableWalk<T, DP, ROWG> w;
+    TableWalk<T, DP, ROWG, KIND> w;
     w.c2 = a.c2;
     w.c2l = a.c2l;
     w.unit = unit;
@@ -1865,7 +1873,7 @@ __device__ __forceinline__ float grad_factor(const Args &a, const float *grad) {
 }
 
 // The first `xblocks` workgroups scale dX, the others join the parts of dE: four channels a thread.
-template <typename T, int DP>
+template <typename T, int DP, int KIND>
 __global__ __launch_bounds__(kBlock) void kd_xent_grads(Args a, int64_t xblocks, int vpr,
                                                         const int64_t *__restrict__ labels,
                                                         const float *__restrict__ grad,
@@ -1896,7 +1904,7 @@ __global__ __launch_bounds__(kBlock) void kd_xent_grads(Args a, int64_t xblocks,
   } else {
     if (r >= a.V) return;
     f32x4 x = (f32x4)(0.f);
-    using W = Walk<T, DP, 2>;
+    using W = Walk<T, DP, KIND>;
     int64_t slot;
     int n;
     Deal((a.V + W::rows - 1) / W::rows, (int)(((int64_t)*a.count + 63) / 64), W::workers)
@@ -1999,7 +2007,9 @@ inline size_t lay_backward(Args &a, int np, bool need_e, void *base) {
   a.gmax = s.take<uint32_t>((size_t)grad_blocks(a.npad) + 1);
   a.grow = s.take<float>(a.npad);
   a.gfac = s.take<float>(a.npad);
-  const size_t part = (size_t)deal_slots(a.vpad, np, a.dp, 2) * (size_t)walk_rows(np, a.dp, 2);
+  const int kind = walk_table(np, a.dp, a.V);
+  const size_t part =
+      (size_t)deal_slots(a.vpad, np, a.dp, kind) * (size_t)walk_rows(np, a.dp, kind);
   a.pe = need_e ? s.take<float>(part * a.dp) : nullptr;
   return s.used;
 }
@@ -2057,20 +2067,32 @@ void launch_forward(const Args &a, bool need_x, const T *features, const T *tabl
 
 inline int64_t blocks(int64_t n) { return (n + kBlock - 1) / kBlock; }
 
-template <typename T, int DP>
-void launch_backward(const Args &a, const int64_t *labels, const float *grad, T *gx, T *ge,
-                     hipStream_t stream) {
+template <typename T, int DP, int KIND>
+void launch_table(const Args &a, const int64_t *labels, const float *grad, T *gx, T *ge,
+                  hipStream_t stream) {
   if (ge && a.reduction == 0)
-    hipLaunchKernelGGL((kd_xent_table<T, DP, true>), (walk_grid<T, DP, 2>()), dim3(kBlock), 0, stream,
-                       a);
+    hipLaunchKernelGGL((kd_xent_table<T, DP, true, KIND>), (walk_grid<T, DP, KIND>()), dim3(kBlock), 0,
+                       stream, a);
   else if (ge)
-    hipLaunchKernelGGL((kd_xent_table<T, DP, false>), (walk_grid<T, DP, 2>()), dim3(kBlock), 0,
+    hipLaunchKernelGGL((kd_xent_table<T, DP, false, KIND>), (walk_grid<T, DP, KIND>()), dim3(kBlock), 0,
                        stream, a);
   const int vpr = (a.D + 3) / 4;
   const int64_t xb = gx ? blocks(a.n * vpr) : 0, eb = ge ? blocks((int64_t)a.V * vpr) : 0;
   if (xb + eb > 0)
-    hipLaunchKernelGGL((kd_xent_grads<T, DP>), grid_of(xb + eb), dim3(kBlock), 0, stream, a, xb, vpr,
-                       labels, grad, gx, ge);
+    hipLaunchKernelGGL((kd_xent_grads<T, DP, KIND>), grid_of(xb + eb), dim3(kBlock), 0, stream, a, xb,
+                       vpr, labels, grad, gx, ge);
+}
+
+template <typename T, int DP>
+void launch_backward(const Args &a, const int64_t *labels, const float *grad, T *gx, T *ge,
+                     hipStream_t stream) {
+  if constexpr (walk_table(Form<T>::np, DP, 1) == 3) {
+    if (walk_table(Form<T>::np, DP, a.V) == 3) {
+      launch_table<T, DP, 3>(a, labels, grad, gx, ge, stream);
+      return;
+    }
+  }
+  launch_table<T, DP, 2>(a, labels, grad, gx, ge, stream);
 }
 
 template <typename T>

@@ -360,3 +360,40 @@ def test_a_table_of_one_row(dname, size):
     for out in (*_run(x, e, y, 2.0, 'none', torch.ones(90, device=DEV)),
                 surface_cross_entropy(x[:50], e, y[:50], 2.0, 'none')):
         assert (out == 0).all()
+
+
+@pytest.mark.parametrize('V', [8, 200])
+@pytest.mark.parametrize('D', [40, 128, 200])
+@pytest.mark.parametrize('reduction', ['none', 'sum'])
+@pytest.mark.parametrize('dname', ['f32', 'f16', 'bf16'])
+def test_pixels_that_are_alike(dname, reduction, D, V):
+    """An untrained table of few rows and features with a common part c of 10 times their spread: every
+    pixel has next to the same probabilities, and labels as often as those say, so dE is what is left of
+    large sums.  A row's sum over the pixels of (p - p^) x_i is off by the probabilities' error in two
+    parts, u^2 at most and for the label's term too (32 bits: 2^-23), du of a probability relative, the
+    same for all pixels, and the sum's own roundings, (n / 16 + 32) 2^-24 of its terms and their number's
+    parts; rounded to u."""
+    dt = TYPES[dname]
+    g = torch.Generator().manual_seed(31)
+    n = 40000
+    x = (torch.randn(n, D, generator=g) + 10 * torch.randn(1, D, generator=g)).to(DEV, dt)
+    e = (torch.randn(V, D, generator=g) * 1e-4).to(DEV, dt)
+    y = (torch.arange(n) % V).to(DEV)
+    grad = torch.ones(n, device=DEV) if reduction == 'none' else torch.tensor(1.0, device=DEV)
+    x64, e64 = x.double(), e.double().requires_grad_(True)
+    want = torch.nn.functional.cross_entropy(x64 @ e64.t(), y, reduction='sum')
+    ge, = torch.autograd.grad(want, e64)
+    z = x64 @ e64.detach().t()
+    p = torch.softmax(z, 1)
+    p[torch.arange(n, device=DEV), y] = 1 - p[torch.arange(n, device=DEV), y]
+    terms = p.t() @ x64.abs()
+    u = torch.finfo(dt).eps / 2
+    two = u * u if dname != 'f32' else 2.0 ** -23
+    dz = ((6 if dname == 'f32' else 1) * D + 8) * 2.0 ** -24 * float(
+        (x64.abs() @ e64.detach().abs().t()).max())
+    # a probability's own error: its logit's, the log sum's (V terms) and an exponential's, in 32 bits
+    du = 2 * (3 * dz + (V + 16) * 2.0 ** -24)
+    tol = (2 * two + du + (n / 16 + 32) * 2.0 ** -24) * terms + u * ge.abs() * 1.01 + (
+        2.0 ** -25 if dname == 'f16' else 0.0)
+    got = _run(x, e, y, 1.0, reduction, grad)[2]
+    assert ((got.double() - ge).abs() <= tol).all(), float(((got.double() - ge).abs() / tol).max())
