@@ -208,7 +208,8 @@ static __global__ __launch_bounds__(kBlock) void kd_xent_scan(int nblk, int *__r
 
 // The pixels without a label cost a walk as much as the others, so the walks take a list (in order) of
 // those with one; counts and list read the labels twice: 2,097,152 in 6.9 and 7.7 us, 2.4 TB/s
-// (averages of six calls, as all times of one kernel here).
+// (averages of six calls, as all times of one kernel here; cards and their
+// clocks differ by up to 6 %).
 // Lists the pixels of `chunks` chunks a workgroup: blk holds the chunks' counts, or their offsets
 // (scanned), or is not needed (one workgroup lists all).  Losses of pixels without a label are 0.
 static __global__ __launch_bounds__(kBlock) void kd_xent_map(Args a, int chunks, bool scanned,
@@ -1085,10 +1086,10 @@ struct RowsWalk : Step<T, DP, SUM ? 1 : 0> {
 };
 
 // Bound by the matrix pipe, with the exponentials (16 a lane and 32 x 32 logits, 8 clocks each) partly
-// beside it.  Measured: 64 channels, bf16, 263,576 pixels x 50,000 rows with dX: 3.74 ms, 0.90 PFLOP/s;
-// 128 channels, losses of 1,054,304 pixels: 12.4 ms, 1.09 PFLOP/s (a bf16 library product of 8192^3
-// reaches 1.17); 256 channels, 131,788 x 10,000 with dX: 1.60 ms, 0.85 PFLOP/s, where one block of
-// rows a wave waits for LDS; fp32, 64 channels, 131,712 x 10,000: 1.79 ms, 0.19 PFLOP/s counted once,
+// beside it.  Measured: 64 channels, bf16, 263,576 pixels x 50,000 rows with dX: 3.81 ms, 0.89 PFLOP/s;
+// 128 channels, losses of 1,054,304 pixels: 12.7 ms, 1.06 PFLOP/s (a bf16 library product of 8192^3
+// reaches 1.17); 256 channels, 131,788 x 10,000 with dX: 1.61 ms, 0.84 PFLOP/s, where one block of
+// rows a wave waits for LDS; fp32, 64 channels, 131,712 x 10,000: 1.83 ms, 0.18 PFLOP/s counted once,
 // 1.1 of bf16 products (a fp32 library product reaches 0.13).
 template <typename T, int DP, bool SUM>
 __global__ __launch_bounds__(kBlock, (Walk<T, DP, SUM ? 1 : 0>::waves)) void kd_xent_rows(Args a) {
@@ -1642,9 +1643,9 @@ __device__ __forceinline__ float grad_unit(const Args &a) {
 
 // The walk over the pixels: kd_xent_rows with the sides exchanged, the logits formed a second time
 // (2 n V D more operations; kept, they would be n V values written and read, 26 GB at the sizes below
-// in 16 bits, 10 ms).  Bound as there.  Measured: 64 channels, bf16, 263,576 pixels x 50,000 rows 3.38 ms,
-// 1.00 PFLOP/s; 256 channels, 131,788 x 10,000 1.78 ms, 0.76 PFLOP/s; fp32, 64 channels, 131,712 x
-// 10,000 1.89 ms.
+// in 16 bits, 10 ms).  Bound as there.  Measured: 64 channels, bf16, 263,576 pixels x 50,000 rows 3.43 ms,
+// 0.98 PFLOP/s; 256 channels, 131,788 x 10,000 1.79 ms, 0.75 PFLOP/s; fp32, 64 channels, 131,712 x
+// 10,000 1.95 ms.
 // A lane's 16 pixels of a tile are 8 i + 4 (lane / 32) + j: their exponents (and factors) are read one step
 // ahead, of 32-bit data by way of LDS and a pair at a time (held in registers they cost 6 to 11 %).
 template <typename T, int DP, bool ROWG, int KIND>
