@@ -764,9 +764,12 @@ def _check_index(fname, name, t):
 
 
 def _number(fname, name, x):
-    if isinstance(x, torch.Tensor) or isinstance(x, bool):
-        raise RuntimeError(f'{fname}: {name} must be a number, got {type(x).__name__}')
-    x = float(x)
+    try:
+        if isinstance(x, (torch.Tensor, bool, str, bytes)):
+            raise TypeError
+        x = float(x)
+    except (TypeError, ValueError, OverflowError):
+        raise RuntimeError(f'{fname}: {name} must be a number, got {type(x).__name__}') from None
     if not math.isfinite(x) or abs(x) >= 1e30:
         raise RuntimeError(f'{fname}: {name} must be finite and below 1e30, got {x}')
     return x
